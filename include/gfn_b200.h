@@ -39,6 +39,9 @@ enum {
   GFN_ERR_RESOURCES = 5,   /* no launch plan fits the device (shared memory) */
 };
 
+/* Element types of the operators that take more than float32. */
+enum { GFN_F32 = 0, GFN_BF16 = 1, GFN_F16 = 2 };
+
 /* Device error bits recorded by kernels. */
 enum {
   GFN_DEVERR_MBAR_TIMEOUT = 1, /* a bounded wait for a bulk copy gave up */
@@ -469,6 +472,29 @@ int gfn_parallel_scan_noalloc(const float* a, const float* x, float* y, int batc
  * [batch, seq_len, 3*dim]: v_seq, x_seq [batch, seq_len, dim]. */
 int gfn_parallel_layer_scan(const float* z, float* x_seq, float* v_seq, int batch, int seq_len,
                             int dim, int heads, float base_dt, gfn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm over the last dimension, y = (x - mean) rstd weight + bias, and
+ * its backward pass (the nn.LayerNorm of gfn/model.py:113 and
+ * gfn/layers/parallel.py:27, which the reference leaves to torch).
+ * x [rows][dim] of `dtype` with x_row_stride elements between rows (inner
+ * stride 1); weight, bias [dim] of `weight_dtype` (GFN_F32 or `dtype`), each
+ * may be NULL; y [rows][dim] contiguous.  stats [rows][2] float receives
+ * (mean, rstd) for the backward pass, or is NULL.  Arithmetic is float32.
+ * The backward takes the forward's stats and writes dx [rows][dim]
+ * (contiguous) and the sums dweight, dbias [dim] of `weight_dtype`; each may
+ * be NULL.  Its workspace (needed for dweight or dbias) holds
+ * gfn_layer_norm_backward_workspace_floats(); sums run in a fixed order.  No
+ * alignment beyond the element type's is needed; 16-byte aligned rows take
+ * 128-bit accesses. */
+int gfn_layer_norm_forward(const void* x, long long x_row_stride, const void* weight, const void* bias,
+                           int dtype, int weight_dtype, long long rows, int dim, float eps, void* y,
+                           float* stats, gfn_stream_t stream);
+long long gfn_layer_norm_backward_workspace_floats(long long rows, int dim);
+int gfn_layer_norm_backward(const void* x, long long x_row_stride, const void* dy, long long dy_row_stride,
+                            const void* weight, const float* stats, int dtype, int weight_dtype,
+                            long long rows, int dim, void* dx, void* dweight, void* dbias, float* workspace,
+                            long long workspace_floats, gfn_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * FunctionalEmbedding, mode 'binary', coord_dim 16, hidden 64, 2 hidden

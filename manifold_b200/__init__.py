@@ -19,6 +19,7 @@ from .integrators import INTEGRATOR_CLASSES as INTEGRATORS
 from .embeddings import FunctionalEmbedding, ImplicitEmbedding, SineLayer
 from .scan import parallel_scan
 from .losses import CrossEntropyLoss, cross_entropy
+from .norm import LayerNorm, layer_norm
 from . import cuda
 
 __all__ = ["CrossEntropyLoss", "cross_entropy", "GFN", "Manifold", "GLayer", "MLayer", "ParallelMLayer", "RiemannianGating",
@@ -27,4 +28,4 @@ __all__ = ["CrossEntropyLoss", "cross_entropy", "GFN", "Manifold", "GLayer", "ML
            "SymplecticIntegrator", "VerletIntegrator", "YoshidaIntegrator", "ForestRuthIntegrator",
            "OmelyanIntegrator",
            "FunctionalEmbedding", "ImplicitEmbedding", "SineLayer", "ImplicitReadout",
-           "parallel_scan", "GfnError", "INTEGRATORS"]
+           "parallel_scan", "LayerNorm", "layer_norm", "GfnError", "INTEGRATORS"]

@@ -73,6 +73,9 @@ _SIGS = {
     "gfn_leapfrog_step_backward_workspace_floats": [_i, _i, _i, _i, _i],
     "gfn_leapfrog_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
                               _p, _i, _i, _i, _f, _p, _i, _i, _i, _f, _f, _p, _ll, _p],
+    "gfn_layer_norm_forward": [_p, _ll, _p, _p, _i, _i, _ll, _i, _f, _p, _p, _p],
+    "gfn_layer_norm_backward_workspace_floats": [_ll, _i],
+    "gfn_layer_norm_backward": [_p, _ll, _p, _ll, _p, _p, _i, _i, _ll, _i, _p, _p, _p, _p, _ll, _p],
 }
 _RESTYPES = {
     "gfn_status_string": ctypes.c_char_p,
@@ -86,6 +89,7 @@ _RESTYPES = {
     "gfn_leapfrog_layered_workspace_floats": ctypes.c_longlong,
     "gfn_christoffel_backward_workspace_floats": ctypes.c_longlong,
     "gfn_leapfrog_step_backward_workspace_floats": ctypes.c_longlong,
+    "gfn_layer_norm_backward_workspace_floats": ctypes.c_longlong,
 }
 
 EXPORTED = tuple(_SIGS)
@@ -143,6 +147,36 @@ def device_error(reset=True, device=None):
     call("gfn_get_device_error", ctypes.byref(bits), 1 if reset else 0,
          stream_of(device) if device is not None else torch.cuda.current_stream().cuda_stream)
     return bits.value
+
+
+# the C ABI's element type codes
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def dtype_code(t, name):
+    code = DTYPES.get(t.dtype)
+    if code is None:
+        raise GfnError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def call_on(t, name, *args):
+    """`call` on tensor t's device, with that device's current stream as the
+    last argument (the device is made current when it is not)."""
+    dev = t.device
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream_of(dev))
+
+
+def same_device(what, first, *others):
+    """Every operand on one CUDA device."""
+    require_cuda(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise GfnError(f"{what}: operands on {first.device} and {t.device}")
 
 
 def require_cuda(*tensors):
