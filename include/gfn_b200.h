@@ -497,6 +497,70 @@ int gfn_layer_norm_backward(const void* x, long long x_row_stride, const void* d
                             long long workspace_floats, gfn_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Gated scan h_t = a_t h_{t-1} + x_t from h0 over the length axis, and its
+ * backward pass (the training form of gfn/scan.py:11-104, which starts from
+ * zero and has float32 operands only).
+ * a, x [batch][length][dim] of `dtype`, inner stride 1, batch and step
+ * strides in elements (0 allowed: a broadcast operand); a NULL: a == 1.
+ * h0 [batch][dim] float or NULL (zero).  h contiguous, of `dtype`; h_last
+ * [batch][dim] float or NULL; states (NULL for inference) of
+ * gfn_gated_scan_states_floats() floats keeps what the backward needs.
+ * Backward: dh (strided as x) and dh_last (float) may be NULL (zero); da, dx
+ * (contiguous) and dh0 may be NULL.  Length 0 passes the state through.
+ * States are float32.  `workspace` of gfn_gated_scan_workspace_bytes(),
+ * 16-byte aligned, serves both passes of both scans; calls that run at the
+ * same time need one each. */
+long long gfn_gated_scan_states_floats(int batch, int length, int dim);
+long long gfn_gated_scan_workspace_bytes(int batch, int length, int dim);
+int gfn_gated_scan_forward(const void* a, long long a_batch_stride, long long a_step_stride, const void* x,
+                           long long x_batch_stride, long long x_step_stride, const float* h0, int dtype,
+                           int batch, int length, int dim, void* h, float* h_last, float* states,
+                           void* workspace, long long workspace_bytes, gfn_stream_t stream);
+int gfn_gated_scan_backward(const void* a, long long a_batch_stride, long long a_step_stride, const void* x,
+                            long long x_batch_stride, long long x_step_stride, const float* states,
+                            const void* dh, long long dh_batch_stride, long long dh_step_stride,
+                            const float* dh_last, int dtype, int batch, int length, int dim, void* da, void* dx,
+                            float* dh0, void* workspace, long long workspace_bytes, gfn_stream_t stream);
+
+/* The scan layer's recurrence (gfn_parallel_layer_scan) with a carried state
+ * and a backward pass.  z [batch][length][3 dim]; v0, x0 [batch][dim] or NULL
+ * (zero); x_last, v_last [batch][dim] or NULL; states as above (NULL for
+ * inference).  Backward: gx, gv [batch][length][dim] and gx_last, gv_last
+ * [batch][dim] may be NULL (zero); dz [batch][length][3 dim]; dx0, dv0 may be
+ * NULL.  Any dim; everything contiguous float32. */
+int gfn_layer_scan_forward(const float* z, const float* v0, const float* x0, int batch, int length, int dim,
+                           int heads, float base_dt, float* x_seq, float* v_seq, float* x_last, float* v_last,
+                           float* states, void* workspace, long long workspace_bytes, gfn_stream_t stream);
+int gfn_layer_scan_backward(const float* z, const float* states, const float* gx, const float* gv,
+                            const float* gx_last, const float* gv_last, int batch, int length, int dim, int heads,
+                            float base_dt, float* dz, float* dx0, float* dv0, void* workspace,
+                            long long workspace_bytes, gfn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Logits before sampling, in one pass (the reference samples from bare
+ * logits, gfn/model.py:404-469): for token j of a row,
+ *   s = x > 0 ? x / repetition : x * repetition   where the history holds j
+ *   s -= frequency * count + presence             where count > 0
+ *   out = (s + bias) / temperature, -inf where `allowed` has bit j clear.
+ * tokens [batch][history] int64 (row stride in elements); the first
+ * lengths[row] of them count (NULL: all; clamped to [0, history]), and those
+ * after prompt_lengths[row] (NULL: 0) make up `count`.  A token outside
+ * [0, vocab) is skipped and sets GFN_DEVERR_BAD_TOKEN.  Each parameter is one
+ * number, or one per row when its _rows pointer is given.  bias [vocab]
+ * float with row stride (0: shared by the rows) or NULL; allowed: 32-bit
+ * words, bit i of word w for token 32 w + i, row stride in words (0: shared)
+ * or NULL.  logits of `dtype` with a row stride; out [batch][vocab]
+ * contiguous of `dtype`, may be the logits' own buffer when those are
+ * contiguous.  A row whose mask leaves nothing is all -inf. */
+int gfn_process_logits(const void* logits, long long logits_row_stride, int dtype, int batch, int vocab,
+                       const long long* tokens, long long tokens_row_stride, int history, const long long* lengths,
+                       const long long* prompt_lengths, float repetition, const float* repetition_rows,
+                       float frequency, const float* frequency_rows, float presence, const float* presence_rows,
+                       float temperature, const float* temperature_rows, const float* bias,
+                       long long bias_row_stride, const void* allowed, long long allowed_row_stride, void* out,
+                       gfn_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * FunctionalEmbedding, mode 'binary', coord_dim 16, hidden 64, 2 hidden
  * SIREN layers (gfn/embeddings.py:121-206): ids [n] -> forces [n, dim],
  * float32 (out_f32) or bfloat16 (out_bf16, raw uint16 storage).

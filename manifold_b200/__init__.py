@@ -17,9 +17,10 @@ from .integrators import (DormandPrinceIntegrator, EulerIntegrator, ForestRuthIn
                           SymplecticIntegrator, VerletIntegrator, YoshidaIntegrator)
 from .integrators import INTEGRATOR_CLASSES as INTEGRATORS
 from .embeddings import FunctionalEmbedding, ImplicitEmbedding, SineLayer
-from .scan import parallel_scan
+from .scan import gated_scan, parallel_scan
 from .losses import CrossEntropyLoss, cross_entropy
 from .norm import LayerNorm, layer_norm
+from .sampling import pack_token_mask, process_logits
 from . import cuda
 
 __all__ = ["CrossEntropyLoss", "cross_entropy", "GFN", "Manifold", "GLayer", "MLayer", "ParallelMLayer", "RiemannianGating",
@@ -28,4 +29,5 @@ __all__ = ["CrossEntropyLoss", "cross_entropy", "GFN", "Manifold", "GLayer", "ML
            "SymplecticIntegrator", "VerletIntegrator", "YoshidaIntegrator", "ForestRuthIntegrator",
            "OmelyanIntegrator",
            "FunctionalEmbedding", "ImplicitEmbedding", "SineLayer", "ImplicitReadout",
-           "parallel_scan", "LayerNorm", "layer_norm", "GfnError", "INTEGRATORS"]
+           "parallel_scan", "gated_scan", "LayerNorm", "layer_norm", "process_logits",
+           "pack_token_mask", "GfnError", "INTEGRATORS"]

@@ -76,6 +76,15 @@ _SIGS = {
     "gfn_layer_norm_forward": [_p, _ll, _p, _p, _i, _i, _ll, _i, _f, _p, _p, _p],
     "gfn_layer_norm_backward_workspace_floats": [_ll, _i],
     "gfn_layer_norm_backward": [_p, _ll, _p, _ll, _p, _p, _i, _i, _ll, _i, _p, _p, _p, _p, _ll, _p],
+    "gfn_gated_scan_states_floats": [_i, _i, _i],
+    "gfn_gated_scan_workspace_bytes": [_i, _i, _i],
+    "gfn_gated_scan_forward": [_p, _ll, _ll, _p, _ll, _ll, _p, _i, _i, _i, _i, _p, _p, _p, _p, _ll, _p],
+    "gfn_gated_scan_backward": [_p, _ll, _ll, _p, _ll, _ll, _p, _p, _ll, _ll, _p, _i, _i, _i, _i, _p, _p, _p, _p,
+                                _ll, _p],
+    "gfn_layer_scan_forward": [_p, _p, _p, _i, _i, _i, _i, _f, _p, _p, _p, _p, _p, _p, _ll, _p],
+    "gfn_layer_scan_backward": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _p, _p, _p, _p, _ll, _p],
+    "gfn_process_logits": [_p, _ll, _i, _i, _i, _p, _ll, _i, _p, _p, _f, _p, _f, _p, _f, _p, _f, _p, _p, _ll, _p,
+                           _ll, _p, _p],
 }
 _RESTYPES = {
     "gfn_status_string": ctypes.c_char_p,
@@ -90,6 +99,8 @@ _RESTYPES = {
     "gfn_christoffel_backward_workspace_floats": ctypes.c_longlong,
     "gfn_leapfrog_step_backward_workspace_floats": ctypes.c_longlong,
     "gfn_layer_norm_backward_workspace_floats": ctypes.c_longlong,
+    "gfn_gated_scan_states_floats": ctypes.c_longlong,
+    "gfn_gated_scan_workspace_bytes": ctypes.c_longlong,
 }
 
 EXPORTED = tuple(_SIGS)

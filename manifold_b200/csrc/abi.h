@@ -31,5 +31,7 @@ int make_layout(int d, int H, int r, int NL, Layout* L);
 cudaError_t error_word_layered(int* v, int reset, cudaStream_t s);
 cudaError_t error_word_probe(int* v, int reset, cudaStream_t s);
 cudaError_t error_word_readout(int* v, int reset, cudaStream_t s);
+cudaError_t error_word_logits(int* v, int reset, cudaStream_t s);
+cudaError_t error_word_gated_scan(int* v, int reset, cudaStream_t s);
 
 }  // namespace gfn_abi

@@ -449,10 +449,18 @@ def parallel_scan_fused(a, x, workspace=True):
     return y
 
 
-def parallel_layer_scan(z, heads, base_dt=0.1):
+def parallel_layer_scan(z, heads, base_dt=0.1, state=None, return_state=False):
     """ParallelMLayer recurrence from z = [zA | zdt | zB] ([B, L, 3D]).
-    Returns (x_seq, v_seq)."""
+    Returns (x_seq, v_seq).
+
+    state: (v, x), each [B, D] float32, where the sequence continues from
+    (None: zero); with return_state the result is (x_seq, v_seq, (v, x)), the
+    state after the last step.  Differentiable in z and the state.  Calls with
+    a state, return_state or a gradient split the length axis when the columns
+    alone do not fill the GPU, and take any dim."""
     require_cuda(z)
+    if state is not None or return_state or _grad_wanted(z):
+        return _layer_scan(z, heads, base_dt, state, return_state)
     z = _f32c(z, "z")
     B, L, D3 = z.shape
     D = D3 // 3
@@ -461,6 +469,58 @@ def parallel_layer_scan(z, heads, base_dt=0.1):
     call("gfn_parallel_layer_scan", ptr(z), ptr(x_seq), ptr(v_seq), B, L, D, int(heads),
          float(base_dt), _stream(z))
     return x_seq, v_seq
+
+
+def _layer_scan(z, heads, base_dt, state, return_state):
+    v0, x0 = (None, None) if state is None else state
+    _lib.same_device("parallel_layer_scan", z, v0, x0)
+    z = _f32c(z, "z")
+    if z.dim() != 3 or z.shape[2] % 3:
+        raise GfnError(f"parallel_layer_scan: z must be [batch, length, 3 dim], got {tuple(z.shape)}")
+    for name, t in (("v", v0), ("x", x0)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (z.shape[0], z.shape[2] // 3)):
+            raise GfnError(f"parallel_layer_scan: state {name} must be float32 [{z.shape[0]}, {z.shape[2] // 3}], "
+                           f"got {t.dtype} {tuple(t.shape)}")
+    if _grad_wanted(z, v0, x0):
+        from .autograd import LayerScanFn
+        xs, vs, vl, xl = LayerScanFn.apply(z, v0, x0, int(heads), float(base_dt))
+    else:
+        xs, vs, vl, xl, _ = layer_scan_forward(z, v0, x0, heads, base_dt, return_state, False)
+    return (xs, vs, (vl, xl)) if return_state else (xs, vs)
+
+
+def layer_scan_forward(z, v0, x0, heads, base_dt, want_last, want_states):
+    """One launch of the stateful layer scan: (x_seq, v_seq, v_last, x_last, states)."""
+    B, L, D = z.shape[0], z.shape[1], z.shape[2] // 3
+    z = z.contiguous()
+    v0 = None if v0 is None else v0.contiguous()
+    x0 = None if x0 is None else x0.contiguous()
+    lib = _lib.load()
+    out = torch.empty(2, B, L, D, device=z.device, dtype=torch.float32)
+    last = torch.empty(2, B, D, device=z.device, dtype=torch.float32) if want_last else (None, None)
+    states = None
+    if want_states:
+        states = torch.empty(lib.gfn_gated_scan_states_floats(B, L, D), device=z.device, dtype=torch.float32)
+    n = lib.gfn_gated_scan_workspace_bytes(B, L, D)
+    ws = torch.empty(n, device=z.device, dtype=torch.uint8) if n else None
+    _lib.call_on(z, "gfn_layer_scan_forward", ptr(z), ptr(v0), ptr(x0), B, L, D, int(heads), float(base_dt),
+                 ptr(out[0]), ptr(out[1]), ptr(last[1]), ptr(last[0]), ptr(states), ptr(ws), n)
+    return out[0], out[1], last[0], last[1], states
+
+
+def layer_scan_backward(z, states, gx, gv, gvl, gxl, heads, base_dt, want_v0, want_x0):
+    """Gradients (dz, dv0, dx0) of the layer scan; any upstream gradient may be None."""
+    B, L, D = z.shape[0], z.shape[1], z.shape[2] // 3
+    z = z.contiguous()
+    gx, gv, gvl, gxl = (None if g is None else g.contiguous() for g in (gx, gv, gvl, gxl))
+    dz = torch.empty_like(z)
+    dv0 = torch.empty(B, D, device=z.device, dtype=torch.float32) if want_v0 else None
+    dx0 = torch.empty(B, D, device=z.device, dtype=torch.float32) if want_x0 else None
+    n = _lib.load().gfn_gated_scan_workspace_bytes(B, L, D)
+    ws = torch.empty(n, device=z.device, dtype=torch.uint8) if n else None
+    _lib.call_on(z, "gfn_layer_scan_backward", ptr(z), ptr(states), ptr(gx), ptr(gv), ptr(gxl), ptr(gvl), B, L, D,
+                 int(heads), float(base_dt), ptr(dz), ptr(dx0), ptr(dv0), ptr(ws), n)
+    return dz, dv0, dx0
 
 
 def functional_embedding(ids, W0, b0, W1, b1, W2, b2, Wo, bo, impulse, omega0=30.0,

@@ -14,7 +14,13 @@ from ._lib import GfnError, require_cuda
 from .cuda import ops
 from .geometry import ReactiveChristoffel, ToroidalChristoffel
 from .integrators import INTEGRATOR_CLASSES, SymplecticIntegrator
+from .norm import layer_norm
 from .packing import PackCache
+
+
+def apply_norm(norm, x, library):
+    """nn.LayerNorm `norm` of x: on the library's kernels, or by torch."""
+    return layer_norm(x, norm.weight, norm.bias, norm.eps) if library else norm(x)
 
 
 class RiemannianGating(nn.Module):
@@ -373,12 +379,27 @@ class ParallelMLayer(nn.Module):
             self.out_proj = nn.Linear(dim * 2, dim * 2)
         # True: the projections on the tensor cores (split fp16); False: torch's fp32 matmul
         self.split_gemm = True
+        # True: norm_x on the library's kernels (manifold_b200.norm); False: torch's
+        self.library_norm = False
 
     def forward(self, x, v, force, collect_christ=False):
         require_cuda(force)
         if x is not None:
             raise GfnError("ParallelMLayer with an explicit x is not used by the reference model")
-        f = self.norm_x(force)
+        z = self._projections(apply_norm(self.norm_x, force, self.library_norm))
+        x_seq, v_seq = ops.parallel_layer_scan(z, self.heads, self.base_dt)
+        return x_seq, v_seq, None, []
+
+    def stream(self, force, state=None):
+        """A segment of a longer sequence: force [B, L, dim] from state (v, x)
+        (None: zero).  Returns (x_seq, v_seq, state after the segment).  The
+        reference's scan layer always starts from zero."""
+        require_cuda(force)
+        z = self._projections(apply_norm(self.norm_x, force, True))
+        return ops.parallel_layer_scan(z, self.heads, self.base_dt, state=state, return_state=True)
+
+    def _projections(self, f):
+        """[to_A | to_dt | to_B] pre-activations of a normalised input, [B, L, 3 dim]."""
         Wcat = torch.cat([self.to_A[0].weight, self.to_dt[0].weight, self.to_B.weight], 0)
         bcat = torch.cat([self.to_A[0].bias, self.to_dt[0].bias, self.to_B.bias], 0)
         if self.split_gemm and f.is_cuda:
@@ -389,5 +410,4 @@ class ParallelMLayer(nn.Module):
             z = SplitLinear.apply(f.reshape(B * L, self.dim), Wcat, bcat).reshape(B, L, 3 * self.dim)
         else:
             z = torch.nn.functional.linear(f, Wcat, bcat)
-        x_seq, v_seq = ops.parallel_layer_scan(z, self.heads, self.base_dt)
-        return x_seq, v_seq, None, []
+        return z

@@ -14,8 +14,10 @@ import torch.nn as nn
 from ._lib import GfnError, require_cuda
 from .cuda import ops
 from .embeddings import FunctionalEmbedding, ImplicitEmbedding
-from .layers import LAYERED_MIN_ELEMS, MLayer, ParallelMLayer, use_layered_path  # noqa: F401
+from .layers import (LAYERED_MIN_ELEMS, MLayer, ParallelMLayer, apply_norm,  # noqa: F401
+                     use_layered_path)
 from .packing import PackCache
+from .sampling import process_logits
 
 
 class ImplicitReadout(nn.Module):
@@ -91,6 +93,7 @@ class Manifold(nn.Module):
         readout_type = self.physics_config.get("readout", {}).get("type", "standard")
         self.readout_norm = nn.LayerNorm(dim)
         self.readout_split = True  # False: plain fp32 torch matmul for the readout
+        self.library_norm = False  # see use_library_norm
         if readout_type in ("implicit", "binary"):
             coord_dim = emb_cfg.get("coord_dim", 16)
             self.readout = nn.Identity() if self.holographic else ImplicitReadout(dim, coord_dim)
@@ -212,7 +215,7 @@ class Manifold(nn.Module):
             cur = forces
             for layer in self.layers:
                 cur, _, _, _ = layer(None, None, force=cur)
-            x_final = cur if self.holographic else self.readout_norm(cur)
+            x_final = cur if self.holographic else apply_norm(self.readout_norm, cur, self.library_norm)
             logits = self.readout(x_final)
             return logits, (x_final[:, -1], None), []
         train = torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())
@@ -228,20 +231,83 @@ class Manifold(nn.Module):
             x_seq, v_seq, (x, v), forces = self.recurrence(input_ids, attention_mask, state, force_manual)
         if forces is None and self.return_forces:
             forces = self.embedding(input_ids)
-        out = x_seq if self.holographic else self.readout_norm(x_seq)
+        out = x_seq if self.holographic else apply_norm(self.readout_norm, x_seq, self.library_norm)
         logits = self._apply_readout(out)
         return logits, (x, v), [], list(v_seq.unbind(1)), list(x_seq.unbind(1)), forces
 
+    def use_library_norm(self, on=True):
+        """Run the model's layer norms (the readout's, and the scan layers' in
+        the scan path), forward and backward, on the library's kernels instead
+        of torch's.  Returns the model."""
+        self.library_norm = bool(on)
+        for layer in self.layers:
+            if isinstance(layer, ParallelMLayer):
+                layer.library_norm = bool(on)
+        return self
+
+    def stream(self, input_ids=None, state=None, force_manual=None):
+        """A segment of a longer sequence through the scan path (use_scan=True):
+        input_ids [B, L] (one token or many) from `state`, the list of every
+        layer's (v, x) that the previous call returned (None: the start).
+        Returns (logits [B, L, vocab], state).  The reference's scan path keeps
+        no state between calls (gfn/model.py:171-188)."""
+        if not self.use_scan:
+            raise GfnError("stream() is the scan path's; forward(state=...) carries the loop path's state")
+        cur = self._forces(input_ids, force_manual)
+        require_cuda(cur)
+        cur = cur.to(torch.float32)
+        if state is None:
+            state = [None] * len(self.layers)
+        if len(state) != len(self.layers):
+            raise GfnError(f"stream: state of {len(state)} layers for a model of {len(self.layers)}")
+        new_state = []
+        for layer, st in zip(self.layers, state):
+            cur, _, st = layer.stream(cur, st)
+            new_state.append(st)
+        if not self.holographic:
+            cur = apply_norm(self.readout_norm, cur, True)
+        return self._apply_readout(cur), new_state
+
     @torch.no_grad()
-    def generate(self, prompt_ids, max_new_tokens=50, temperature=1.0, top_k=None, top_p=None):
+    def generate(self, prompt_ids, max_new_tokens=50, temperature=1.0, top_k=None, top_p=None,
+                 repetition_penalty=1.0, frequency_penalty=0.0, presence_penalty=0.0, logit_bias=None,
+                 allowed=None, carry_state=False):
         """Autoregressive sampling with O(1) streamed state (gfn/model.py:404-469;
-        the reference unpacks 3 values from its 6-tuple there and fails)."""
+        the reference unpacks 3 values from its 6-tuple there and fails).
+
+        The penalties, logit_bias [vocab] and allowed shape the logits before
+        top_k / top_p (manifold_b200.sampling.process_logits); allowed is a mask
+        (bool [vocab], or packed words), or a function of the tokens so far (a
+        list) that returns one, or None for no limit.  A mask that leaves no
+        token raises GfnError.  carry_state: a scan model (use_scan=True)
+        continues from its state (stream()) instead of starting every call from
+        zero as the reference's does."""
         self.eval()
-        logits, state = self(prompt_ids)[:2]
+        if carry_state:
+            step = self.stream
+        else:
+            step = lambda ids, state=None: self(ids, state=state)[:2]  # noqa: E731
+        shaped = (repetition_penalty != 1.0 or frequency_penalty != 0.0 or presence_penalty != 0.0
+                  or logit_bias is not None or allowed is not None)
+        logits, state = step(prompt_ids)
         generated = prompt_ids.tolist()[0]
+        if shaped:
+            history = torch.empty(1, len(generated) + max_new_tokens, device=logits.device, dtype=torch.int64)
+            history[0, :len(generated)] = prompt_ids[0]
+            prompt = torch.tensor([len(generated)], device=logits.device)
+
+        def shape_logits(lg):
+            mask = allowed(generated) if callable(allowed) else allowed
+            n = len(generated)
+            nl = process_logits(lg, history[:, :n], None, prompt, repetition_penalty, frequency_penalty,
+                                presence_penalty, logit_bias, temperature,
+                                None if mask is None else mask.to(lg.device))
+            if not torch.isfinite(nl.max()):  # before a softmax of nothing reaches the sampler
+                raise GfnError("generate: no token is left to choose (mask, bias or logits)")
+            return nl
 
         def sample_next(lg):
-            nl = lg[:, -1, :] / temperature
+            nl = shape_logits(lg[:1, -1, :]) if shaped else lg[:, -1, :] / temperature
             if top_k is not None:
                 vals, _ = torch.topk(nl, top_k)
                 nl[nl < vals[:, [-1]]] = -float("Inf")
@@ -259,7 +325,9 @@ class Manifold(nn.Module):
         tok = sample_next(logits)
         generated.append(tok.item())
         for _ in range(max_new_tokens - 1):
-            logits, state = self(tok, state=state)[:2]
+            if shaped:
+                history[:, len(generated) - 1:len(generated)] = tok
+            logits, state = step(tok, state=state)
             tok = sample_next(logits)
             generated.append(tok.item())
         return generated

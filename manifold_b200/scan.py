@@ -1,10 +1,120 @@
 """gfn.scan mirror: y_t = a_t * y_{t-1} + x_t over dim 1 (gfn/scan.py:11-104),
-as one work-efficient pass per column on the GPU (no Hillis-Steele passes)."""
-from .cuda.ops import parallel_scan_fused
+as one work-efficient pass per column on the GPU (no Hillis-Steele passes),
+and the gated scan: the same recurrence with gradients, a carried state and
+16-bit operands."""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import GfnError, call_on, dtype_code, ptr, same_device
+from .cuda.ops import _grad_wanted, parallel_scan_fused
 
 CUDA_AVAILABLE = True
 
 
 def parallel_scan(a, x):
-    """a, x: [batch, seq_len, dim] float32 CUDA tensors -> y of the same shape."""
+    """a, x: [batch, seq_len, dim] float32 CUDA tensors -> y of the same shape.
+    Differentiable: with a gradient wanted it runs as gated_scan(a, x)."""
+    if _grad_wanted(a, x):
+        if x.dtype != torch.float32:
+            raise GfnError(f"x must be float32, got {x.dtype}")
+        return gated_scan(a, x)
     return parallel_scan_fused(a, x)
+
+
+def _operand(t):
+    """t [B, L, D] with inner stride 1 (itself where it has one: strided and
+    broadcast batches and steps are read in place)."""
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _workspace(x):
+    n = _lib.load().gfn_gated_scan_workspace_bytes(*x.shape)
+    return (torch.empty(n, device=x.device, dtype=torch.uint8) if n else None), n
+
+
+def _forward(a, x, h0, want_last, want_states):
+    B, L, D = x.shape
+    x = _operand(x)
+    a = None if a is None else _operand(a)
+    h0 = None if h0 is None else h0.contiguous()
+    h = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
+    last = torch.empty(B, D, device=x.device, dtype=torch.float32) if want_last else None
+    states = None
+    if want_states:
+        states = torch.empty(_lib.load().gfn_gated_scan_states_floats(B, L, D), device=x.device,
+                             dtype=torch.float32)
+    ws, n = _workspace(x)
+    sa = (0, 0) if a is None else a.stride()[:2]
+    call_on(x, "gfn_gated_scan_forward", ptr(a), *sa, ptr(x), *x.stride()[:2], ptr(h0), _lib.DTYPES[x.dtype],
+            B, L, D, ptr(h), ptr(last), ptr(states), ptr(ws), n)
+    return h, last, states
+
+
+class GatedScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, a, x, h0):
+        h, last, states = _forward(a, x, h0, True, True)
+        ctx.save_for_backward(a, x, states)
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dlast):
+        a, x, states = ctx.saved_tensors
+        if dh is None and dlast is None:
+            return None, None, None
+        B, L, D = x.shape
+        need_a, need_x, need_h0 = ctx.needs_input_grad
+        ao, xo = None if a is None else _operand(a), _operand(x)
+        dh = None if dh is None else _operand(dh)
+        dlast = None if dlast is None else dlast.contiguous()
+        da = torch.empty(B, L, D, device=x.device, dtype=x.dtype) if need_a else None
+        dx = torch.empty(B, L, D, device=x.device, dtype=x.dtype) if need_x else None
+        dh0 = torch.empty(B, D, device=x.device, dtype=torch.float32) if need_h0 else None
+        ws, n = _workspace(x)
+        sa = (0, 0) if a is None else ao.stride()[:2]
+        sg = (0, 0) if dh is None else dh.stride()[:2]
+        call_on(x, "gfn_gated_scan_backward", ptr(ao), *sa, ptr(xo), *xo.stride()[:2], ptr(states), ptr(dh), *sg,
+                ptr(dlast), _lib.DTYPES[x.dtype], B, L, D, ptr(da), ptr(dx), ptr(dh0), ptr(ws), n)
+        return da, dx, dh0
+
+
+def gated_scan(a, x, h0=None, return_state=False):
+    """h_t = a_t * h_{t-1} + x_t over dim 1 of x [batch, length, dim], from h0.
+
+    a: x's type, x's shape or broadcastable to it (a decay per channel, per
+    head or per step is read in place where its last dimension is whole), or
+    None (a running sum).  x: float32, bfloat16 or float16, any batch and step
+    strides.  h0: [batch, dim] float32, or None (zero).  The state is float32
+    throughout; h has x's type.  Returns h, or (h, last state [batch, dim]
+    float32) with return_state: pass that as h0 to continue the sequence, one
+    token at a time or segment by segment.  A gate of zero starts a new
+    sequence, so packed sequences need no more than that.  Differentiable
+    (once) in a, x and h0, a broadcast a included.
+
+    The length axis is split: a state passes a whole run of steps as h * P + p,
+    P the product of the run's gates, so |P| must not overflow (gates up to
+    1 in magnitude never do).
+    """
+    same_device("gated_scan", x, a, h0)
+    dtype_code(x, "x")
+    if x.dim() != 3:
+        raise GfnError(f"gated_scan: x must be [batch, length, dim], got {tuple(x.shape)}")
+    if a is not None:
+        if a.dtype != x.dtype:
+            raise GfnError(f"gated_scan: a is {a.dtype}, x {x.dtype}")
+        if a.shape != x.shape:
+            try:
+                a = a.expand(x.shape)
+            except RuntimeError:
+                raise GfnError(f"gated_scan: a {tuple(a.shape)} does not broadcast to {tuple(x.shape)}") from None
+    if h0 is not None and (h0.dtype != torch.float32 or h0.shape != (x.shape[0], x.shape[2])):
+        raise GfnError(f"gated_scan: h0 must be float32 [{x.shape[0]}, {x.shape[2]}], got {h0.dtype} "
+                       f"{tuple(h0.shape)}")
+    if _grad_wanted(a, x, h0):
+        h, last = GatedScanFn.apply(a, x, h0)
+    else:
+        h, last, _ = _forward(a, x, h0, return_state, False)
+    return (h, last) if return_state else h

@@ -54,22 +54,24 @@ def gated_scan_backward(a, x, h0, dh, dlast):
 
 
 def _sigmoid(z):
-    return 1.0 / (1.0 + np.exp(-z))
+    e = np.exp(-np.abs(z))
+    return np.where(z >= 0, 1.0, e) / (1.0 + e)
 
 
 def layer_scan_terms(z, heads, base_dt):
-    """(A, dt, sigma(zdt), head scale) of the scan layer's pre-activations [zA | zdt | zB]."""
+    """(A, 1 - A, dt, sigma(zdt), head scale) of the scan layer's pre-activations [zA | zdt | zB];
+    1 - A = sigma(-zA) keeps its digits where A rounds to 1."""
     z = np.asarray(z, np.float64)
     D = z.shape[-1] // 3
     hs = base_dt * np.repeat(1.5 ** np.arange(heads), D // heads)
-    return _sigmoid(z[..., :D]), np.logaddexp(0.0, z[..., D:2 * D]) * hs, _sigmoid(z[..., D:2 * D]), hs
+    return _sigmoid(z[..., :D]), _sigmoid(-z[..., :D]), np.logaddexp(0.0, z[..., D:2 * D]) * hs, _sigmoid(z[..., D:2 * D]), hs
 
 
 def layer_scan(z, heads, base_dt, v0=None, x0=None):
     """v_t = A_t v_{t-1} + zB_t dt_t, x_t = x_{t-1} + v_t dt_t; returns (x, v, last x, last v)."""
     z = np.asarray(z, np.float64)
     D = z.shape[-1] // 3
-    A, dt, _, _ = layer_scan_terms(z, heads, base_dt)
+    A, _, dt, _, _ = layer_scan_terms(z, heads, base_dt)
     v, vl = gated_scan(A, z[..., 2 * D:] * dt, v0)
     x, xl = gated_scan(None, v * dt, x0)
     return x, v, xl, vl
@@ -79,7 +81,7 @@ def layer_scan_backward(z, heads, base_dt, v0, gx, gv, gxl=None, gvl=None):
     """(dz, dv0, dx0) of sum(gx x) + sum(gv v) + sum(gxl x_last) + sum(gvl v_last)."""
     z = np.asarray(z, np.float64)
     D = z.shape[-1] // 3
-    A, dt, sdt, hs = layer_scan_terms(z, heads, base_dt)
+    A, nA, dt, sdt, hs = layer_scan_terms(z, heads, base_dt)
     zb = z[..., 2 * D:]
     v, _ = gated_scan(A, zb * dt, v0)
     zero = np.zeros((z.shape[0], D))
@@ -94,7 +96,7 @@ def layer_scan_backward(z, heads, base_dt, v0, gx, gv, gxl=None, gvl=None):
         if gv is not None:
             lam = lam + gv[:, t]
         vp = v[:, t - 1] if t else first
-        dz[:, t, :D] = lam * vp * A[:, t] * (1.0 - A[:, t])
+        dz[:, t, :D] = lam * vp * A[:, t] * nA[:, t]
         dz[:, t, D:2 * D] = (lam * zb[:, t] + X * v[:, t]) * hs * sdt[:, t]
         dz[:, t, 2 * D:] = lam * dt[:, t]
         m = A[:, t] * lam
