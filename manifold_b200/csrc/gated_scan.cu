@@ -18,6 +18,106 @@ int num_states(int L) { return (L + SCAN_CK - 1) / SCAN_CK; }
 
 unsigned column_blocks(int B, int D) { return (unsigned)(((long long)B * D + 127) / 128); }
 
+// Up to this length a thread walks its column alone.
+constexpr int SEQ_STEPS = 8;
+constexpr long long TICKET_BYTES = 256;  // the ticket, then the words
+
+// The runs and tiles of a launch, and its words in the workspace (all ones).
+template <class Args>
+int set_tiles(const char* what, Args* p, int run, int ct, int words, void* workspace, long long bytes,
+              cudaStream_t s, unsigned* grid) {
+  p->nchunks = (p->L + run - 1) / run;
+  p->ctiles = (p->D + ct - 1) / ct;
+  const long long tiles = (long long)p->B * p->ctiles, blocks = tiles * p->nchunks;
+  if (blocks > 0x7fffffffLL) return fail(GFN_ERR_UNSUPPORTED, "%s: %lld blocks", what, blocks);
+  *grid = (unsigned)blocks;
+  p->words = nullptr;
+  p->ticket = nullptr;
+  if (p->nchunks == 1) return GFN_OK;
+  const long long need = TICKET_BYTES + blocks * ct * words * 8;
+  if (!workspace || bytes < need)
+    return fail(GFN_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what, workspace ? bytes : 0, need);
+  if (!aligned16(workspace)) return fail(GFN_ERR_ALIGN, "%s: workspace not 16-byte aligned", what);
+  p->ticket = static_cast<unsigned*>(workspace);
+  p->words = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + TICKET_BYTES);
+  return cuda_status(cudaMemsetAsync(workspace, 0xff, (size_t)need, s), what);
+}
+
+// VEC columns per lane: every row of every operand must start on a VEC boundary.
+bool packs(const void* ptr, long long sb, long long st, int B, int L, int vec, int size) {
+  return !ptr || (reinterpret_cast<uintptr_t>(ptr) % (vec * size) == 0 && (B == 1 || sb % vec == 0) &&
+                  (L == 1 || st % vec == 0));
+}
+
+template <typename T, int VEC, int S, int NW>
+int gscan_forward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
+  unsigned grid;
+  const int st = set_tiles("gated_scan_forward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &grid);
+  if (st) return st;
+  gscan_forward_kernel<T, VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  return launch_status("gscan_forward_kernel");
+}
+
+template <typename T, int VEC, int S, int NW>
+int gscan_backward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
+  unsigned grid;
+  const int st = set_tiles("gated_scan_backward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &grid);
+  if (st) return st;
+  gscan_backward_kernel<T, VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  return launch_status("gscan_backward_kernel");
+}
+
+template <typename T, int VEC>
+int gscan_run(const GScanArgs& p, bool backward, void* ws, long long bytes, cudaStream_t s) {
+  const int z = sizeof(T);
+  const bool vec = p.D % VEC == 0 && packs(p.a, p.a_sb, p.a_st, p.B, p.L, VEC, z) &&
+                   packs(p.x, p.x_sb, p.x_st, p.B, p.L, VEC, z) && packs(p.dh, p.g_sb, p.g_st, p.B, p.L, VEC, z) &&
+                   packs(p.h, 0, 0, 1, 1, VEC, z) && packs(p.da, 0, 0, 1, 1, VEC, z) &&
+                   packs(p.dx, 0, 0, 1, 1, VEC, z);
+  if (backward) {
+    return vec ? gscan_backward<T, VEC, 8, 8>(p, ws, bytes, s) : gscan_backward<T, 1, 8, 8>(p, ws, bytes, s);
+  }
+  if (p.L <= SEQ_STEPS) {
+    gscan_forward_seq_kernel<T><<<column_blocks(p.B, p.D), 128, 0, s>>>(p);
+    return launch_status("gscan_forward_seq_kernel");
+  }
+  return vec ? gscan_forward<T, VEC, 8, 16>(p, ws, bytes, s) : gscan_forward<T, 1, 16, 16>(p, ws, bytes, s);
+}
+
+int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long long bytes, cudaStream_t s) {
+  if (dtype == GFN_F32) return gscan_run<float, 2>(p, backward, ws, bytes, s);
+  if (dtype == GFN_BF16) return gscan_run<__nv_bfloat16, 4>(p, backward, ws, bytes, s);
+  if (dtype == GFN_F16) return gscan_run<__half, 4>(p, backward, ws, bytes, s);
+  return fail(GFN_ERR_UNSUPPORTED, "gated_scan: element type %d", dtype);
+}
+
+template <int VEC>
+int lscan_forward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
+  constexpr int S = 8, NW = 16;
+  unsigned grid;
+  const int st = set_tiles("layer_scan_forward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &grid);
+  if (st) return st;
+  lscan_forward_kernel<VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  return launch_status("lscan_forward_kernel");
+}
+
+int lscan_backward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
+  constexpr int VEC = 1, S = 8, NW = 8;
+  unsigned grid;
+  const int st = set_tiles("layer_scan_backward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &grid);
+  if (st) return st;
+  lscan_backward_kernel<VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  return launch_status("lscan_backward_kernel");
+}
+
+// A state or its gradient handed through a sequence of no steps.
+int pass_through(const char* what, float* dst, const float* src, int B, int D, cudaStream_t s) {
+  if (!dst) return GFN_OK;
+  const size_t n = (size_t)B * D * sizeof(float);
+  return cuda_status(src ? cudaMemcpyAsync(dst, src, n, cudaMemcpyDeviceToDevice, s) : cudaMemsetAsync(dst, 0, n, s),
+                     what);
+}
+
 }  // namespace
 
 namespace gfn_abi {
@@ -33,7 +133,9 @@ long long gfn_gated_scan_states_floats(int batch, int length, int dim) {
 
 long long gfn_gated_scan_workspace_bytes(int batch, int length, int dim) {
   if (batch < 0 || length < 0 || dim < 0) return -1;
-  return 0;
+  if (length <= SCAN_CK || batch == 0 || dim == 0) return 0;
+  // the shortest runs (SCAN_CK steps), the widest tiles (128 columns), two words
+  return TICKET_BYTES + (long long)batch * num_states(length) * ((dim + 127LL) / 128 * 128) * 16;
 }
 
 int gfn_gated_scan_forward(const void* a, long long a_batch_stride, long long a_step_stride, const void* x,
@@ -48,13 +150,7 @@ int gfn_gated_scan_forward(const void* a, long long a_batch_stride, long long a_
   p.a = a; p.x = x; p.h0 = h0; p.h = h; p.h_last = h_last; p.states = states;
   p.a_sb = a_batch_stride; p.a_st = a_step_stride; p.x_sb = x_batch_stride; p.x_st = x_step_stride;
   p.B = batch; p.L = length; p.D = dim; p.nck = num_states(length);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = column_blocks(batch, dim);
-  if (dtype == GFN_F32) gscan_forward_seq_kernel<float><<<grid, 128, 0, s>>>(p);
-  else if (dtype == GFN_BF16) gscan_forward_seq_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-  else if (dtype == GFN_F16) gscan_forward_seq_kernel<__half><<<grid, 128, 0, s>>>(p);
-  else return fail(GFN_ERR_UNSUPPORTED, "gated_scan_forward: element type %d", dtype);
-  return launch_status("gscan_forward_seq_kernel");
+  return gscan_dispatch(p, dtype, false, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int gfn_gated_scan_backward(const void* a, long long a_batch_stride, long long a_step_stride, const void* x,
@@ -73,12 +169,8 @@ int gfn_gated_scan_backward(const void* a, long long a_batch_stride, long long a
   p.g_sb = dh_batch_stride; p.g_st = dh_step_stride;
   p.B = batch; p.L = length; p.D = dim; p.nck = num_states(length);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = column_blocks(batch, dim);
-  if (dtype == GFN_F32) gscan_backward_seq_kernel<float><<<grid, 128, 0, s>>>(p);
-  else if (dtype == GFN_BF16) gscan_backward_seq_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-  else if (dtype == GFN_F16) gscan_backward_seq_kernel<__half><<<grid, 128, 0, s>>>(p);
-  else return fail(GFN_ERR_UNSUPPORTED, "gated_scan_backward: element type %d", dtype);
-  return launch_status("gscan_backward_seq_kernel");
+  if (length == 0) return pass_through("gated_scan_backward", dh0, dh_last, batch, dim, s);
+  return gscan_dispatch(p, dtype, true, workspace, workspace_bytes, s);
 }
 
 int gfn_layer_scan_forward(const float* z, const float* v0, const float* x0, int batch, int length, int dim,
@@ -93,8 +185,14 @@ int gfn_layer_scan_forward(const float* z, const float* v0, const float* x0, int
   p.z = z; p.v0 = v0; p.x0 = x0; p.xs = x_seq; p.vs = v_seq; p.x_last = x_last; p.v_last = v_last;
   p.states = states; p.B = batch; p.L = length; p.D = dim; p.H = heads; p.nck = num_states(length);
   p.base_dt = base_dt;
-  lscan_forward_seq_kernel<<<column_blocks(batch, dim), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status("lscan_forward_seq_kernel");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (length <= SEQ_STEPS) {
+    lscan_forward_seq_kernel<<<column_blocks(batch, dim), 128, 0, s>>>(p);
+    return launch_status("lscan_forward_seq_kernel");
+  }
+  const bool vec = dim % 2 == 0 && packs(z, 0, 0, 1, 1, 2, 4) && packs(x_seq, 0, 0, 1, 1, 2, 4) &&
+                   packs(v_seq, 0, 0, 1, 1, 2, 4);
+  return vec ? lscan_forward<2>(p, workspace, workspace_bytes, s) : lscan_forward<1>(p, workspace, workspace_bytes, s);
 }
 
 int gfn_layer_scan_backward(const float* z, const float* states, const float* gx, const float* gv,
@@ -110,8 +208,12 @@ int gfn_layer_scan_backward(const float* z, const float* states, const float* gx
   p.z = z; p.states = const_cast<float*>(states); p.gx = gx; p.gv = gv; p.gxl = gx_last; p.gvl = gv_last;
   p.dz = dz; p.dv0 = dv0; p.dx0 = dx0; p.B = batch; p.L = length; p.D = dim; p.H = heads;
   p.nck = num_states(length); p.base_dt = base_dt;
-  lscan_backward_seq_kernel<<<column_blocks(batch, dim), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
-  return launch_status("lscan_backward_seq_kernel");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (length == 0) {
+    st = pass_through("layer_scan_backward", dv0, gv_last, batch, dim, s);
+    return st ? st : pass_through("layer_scan_backward", dx0, gx_last, batch, dim, s);
+  }
+  return lscan_backward(p, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"
