@@ -49,21 +49,21 @@ bool packs(const void* ptr, long long sb, long long st, int B, int L, int vec, i
                   (L == 1 || st % vec == 0));
 }
 
-template <typename T, int VEC, int S, int NW>
+template <typename T, int VEC, int S, int NW, int OCC>
 int gscan_forward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   unsigned grid;
   const int st = set_tiles("gated_scan_forward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &grid);
   if (st) return st;
-  gscan_forward_kernel<T, VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  gscan_forward_kernel<T, VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
   return launch_status("gscan_forward_kernel");
 }
 
-template <typename T, int VEC, int S, int NW>
+template <typename T, int VEC, int S, int NW, int OCC>
 int gscan_backward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   unsigned grid;
   const int st = set_tiles("gated_scan_backward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &grid);
   if (st) return st;
-  gscan_backward_kernel<T, VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  gscan_backward_kernel<T, VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
   return launch_status("gscan_backward_kernel");
 }
 
@@ -75,13 +75,13 @@ int gscan_run(const GScanArgs& p, bool backward, void* ws, long long bytes, cuda
                    packs(p.h, 0, 0, 1, 1, VEC, z) && packs(p.da, 0, 0, 1, 1, VEC, z) &&
                    packs(p.dx, 0, 0, 1, 1, VEC, z);
   if (backward) {
-    return vec ? gscan_backward<T, VEC, 8, 8>(p, ws, bytes, s) : gscan_backward<T, 1, 8, 8>(p, ws, bytes, s);
+    return vec ? gscan_backward<T, VEC, 8, 8, 2>(p, ws, bytes, s) : gscan_backward<T, 1, 8, 8, 4>(p, ws, bytes, s);
   }
   if (p.L <= SEQ_STEPS) {
     gscan_forward_seq_kernel<T><<<column_blocks(p.B, p.D), 128, 0, s>>>(p);
     return launch_status("gscan_forward_seq_kernel");
   }
-  return vec ? gscan_forward<T, VEC, 8, 16>(p, ws, bytes, s) : gscan_forward<T, 1, 16, 16>(p, ws, bytes, s);
+  return vec ? gscan_forward<T, VEC, 16, 8, 2>(p, ws, bytes, s) : gscan_forward<T, 1, 16, 8, 4>(p, ws, bytes, s);
 }
 
 int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long long bytes, cudaStream_t s) {
@@ -93,20 +93,20 @@ int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long 
 
 template <int VEC>
 int lscan_forward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
-  constexpr int S = 8, NW = 16;
+  constexpr int S = 8, NW = 8, OCC = 2;
   unsigned grid;
   const int st = set_tiles("layer_scan_forward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &grid);
   if (st) return st;
-  lscan_forward_kernel<VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  lscan_forward_kernel<VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
   return launch_status("lscan_forward_kernel");
 }
 
 int lscan_backward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
-  constexpr int VEC = 1, S = 8, NW = 8;
+  constexpr int VEC = 1, S = 8, NW = 8, OCC = 2;
   unsigned grid;
   const int st = set_tiles("layer_scan_backward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &grid);
   if (st) return st;
-  lscan_backward_kernel<VEC, S, NW><<<grid, NW * 32, 0, s>>>(p);
+  lscan_backward_kernel<VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
   return launch_status("lscan_backward_kernel");
 }
 

@@ -101,22 +101,25 @@ struct GatedState {
 
 constexpr int SCAN_GROUP = 32;  // runs whose maps are composed; the states pass from group to group
 
-// M (a map or a state) of `chunk` as its block published it; `words` is the
-// column tile's [nchunks][WORDS of a map][32 VEC] words.
-template <class M, int W, int VEC>
-GFN_DEV void await(const unsigned long long* words, int chunk, M (&out)[VEC]) {
-  constexpr int CT = 32 * VEC;
-  const unsigned long long* src = words + (long long)chunk * W * CT + (threadIdx.x & 31) * VEC;
-  unsigned long long got[VEC][M::WORDS];
+// N maps (or states) that other blocks publish for one column, from `src` on,
+// `stride` words apart.
+template <class M, int N>
+GFN_DEV void await(const unsigned long long* src, long long stride, int ct, int n, M (&out)[N]) {
+  unsigned long long got[N][M::WORDS];
   for (int spin = 0;; ++spin) {
     bool ready = true;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
+    for (int k = 0; k < N; ++k) {
 #pragma unroll
       for (int i = 0; i < M::WORDS; ++i) {
-        got[v][i] = word_load(src + i * CT + v);
-        ready = ready && (unsigned)got[v][i] != SCAN_EMPTY;
+        got[k][i] = 0;
+        if (k < n) got[k][i] = word_load(src + k * stride + i * ct);
       }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+#pragma unroll
+      for (int i = 0; i < M::WORDS; ++i) ready = ready && (unsigned)got[k][i] != SCAN_EMPTY;
     }
     if (ready) break;
     if (spin == (1 << 22)) {  // seconds: flag it and carry on with what is there
@@ -126,83 +129,98 @@ GFN_DEV void await(const unsigned long long* words, int chunk, M (&out)[VEC]) {
     __nanosleep(20);
   }
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) out[v] = M::unpack(got[v]);
+  for (int k = 0; k < N; ++k) out[k] = M::unpack(got[k]);
 }
 
-template <class M, int W, int VEC>
-GFN_DEV void publish(const M (&m)[VEC], unsigned long long* words, int chunk) {
-  constexpr int CT = 32 * VEC;
-  unsigned long long* dst = words + (long long)chunk * W * CT + (threadIdx.x & 31) * VEC;
+template <class M>
+GFN_DEV void publish(M m, unsigned long long* dst, int ct) {
+  unsigned long long w[M::WORDS];
+  m.pack(w);
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    unsigned long long w[M::WORDS];
-    m[v].pack(w);
-#pragma unroll
-    for (int i = 0; i < M::WORDS; ++i) word_store(dst + i * CT + v, w[i]);
-  }
+  for (int i = 0; i < M::WORDS; ++i) word_store(dst + i * ct, w[i]);
 }
+
+template <class Map, class State, int CT, int NW>
+struct ScanShared {
+  static constexpr int R = NW * 32 / CT;  // threads per column
+  unsigned long long maps[NW][Map::WORDS][CT];  // the warps' maps; then those of all warps before each
+  unsigned long long part[R][Map::WORDS][CT];   // maps of parts of the group
+  State in[CT];                                 // the state before this run
+  unsigned slot;
+};
 
 // The state that `chunk` (counted in the direction of the scan) of a column
-// tile receives, from its own map `own` (of the whole run; used in the last
-// run of a group) and `first`, the state before chunk 0.  The whole block
-// takes part; `teller` is true in the one warp that publishes.  `found` is
-// shared memory for one map per warp and column.
-template <class Map, class State, int VEC, int NW>
-GFN_DEV void receive(unsigned long long* words, int chunk, int nchunks, bool active, bool teller,
-                     const Map (&own)[VEC], const State (&first)[VEC],
-                     unsigned long long (*found)[Map::WORDS][32 * VEC], State (&in)[VEC]) {
-  constexpr int W = Map::WORDS, K = SCAN_GROUP / NW;
-  static_assert(SCAN_GROUP % NW == 0, "each warp fetches the same number of maps");
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// tile receives.  Call with the warps' maps in sh.maps; on return (after a
+// barrier) sh.maps[w] holds the map of the warps before w, counted in the
+// direction of the scan (REV: from the last warp), and sh.in the states.
+// R threads serve a column: the last of them chains the warps' maps and
+// publishes, all of them fetch their share of the group's earlier maps.
+// `words` is the tile's [nchunks][WORDS][CT]; first(c) the state before chunk 0.
+template <class Map, class State, int CT, int NW, bool REV, class First>
+GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* words, int chunk, int nchunks,
+                     int live, First first) {
+  constexpr int W = Map::WORDS, R = NW * 32 / CT, GS = SCAN_GROUP / R;
+  constexpr int BATCH = GS < 8 ? GS : 8;
+  const int c = threadIdx.x % CT, r = threadIdx.x / CT;
+  const bool active = c < live, teller = r == R - 1 && active;
   const int pos = chunk % SCAN_GROUP, start = chunk - pos;
-  const bool tells = teller && active && chunk + 1 < nchunks;
-  if (tells && pos < SCAN_GROUP - 1) publish<Map, W, VEC>(own, words, chunk);
-  Map acc[VEC];  // of the group's runs before this one
+  const bool tells = teller && chunk + 1 < nchunks;
+  unsigned long long* mine = words + (long long)chunk * W * CT + c;
+  Map own = Map::identity();
+  __syncthreads();
+  if (teller) {
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) acc[v] = Map::identity();
+    for (int j = 0; j < NW; ++j) {
+      const int w = REV ? NW - 1 - j : j;
+      unsigned long long x[W], y[W];
+      own.pack(y);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        x[i] = sh.maps[w][i][c];
+        sh.maps[w][i][c] = y[i];
+      }
+      own = Map::compose(Map::unpack(x), own);
+    }
+    if (tells && pos < SCAN_GROUP - 1) publish(own, mine, CT);
+  }
+  Map acc = Map::identity();  // of the group's runs before this one
   if (pos > 0) {
-    const int k0 = w * K;
-    if (active && k0 < pos) {
-      await<Map, W, VEC>(words, start + k0, acc);
-      for (int k = k0 + 1; k < min(k0 + K, pos); ++k) {
-        Map next[VEC];
-        await<Map, W, VEC>(words, start + k, next);
+    if (active && r * GS < pos) {
+      for (int k = r * GS; k < min((r + 1) * GS, pos); k += BATCH) {
+        const int n = min(BATCH, min((r + 1) * GS, pos) - k);
+        Map next[BATCH];
+        await<Map, BATCH>(words + (long long)(start + k) * W * CT + c, W * CT, CT, n, next);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) acc[v] = Map::compose(next[v], acc[v]);
+        for (int i = 0; i < BATCH; ++i)
+          if (i < n) acc = Map::compose(next[i], acc);
       }
+      unsigned long long x[W];
+      acc.pack(x);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        unsigned long long x[W];
-        acc[v].pack(x);
-#pragma unroll
-        for (int i = 0; i < W; ++i) found[w][i][lane * VEC + v] = x[i];
-      }
+      for (int i = 0; i < W; ++i) sh.part[r][i][c] = x[i];
     }
     __syncthreads();
-    const int n = (pos + K - 1) / K;
+    if (teller) {
+      acc = Map::identity();
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      acc[v] = Map::identity();
-      for (int j = 0; j < n && active; ++j) {
-        unsigned long long x[W];
+      for (int j = 0; j < R; ++j) {
+        if (j * GS < pos) {
+          unsigned long long x[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) x[i] = found[j][i][lane * VEC + v];
-        acc[v] = Map::compose(Map::unpack(x), acc[v]);
+          for (int i = 0; i < W; ++i) x[i] = sh.part[j][i][c];
+          acc = Map::compose(Map::unpack(x), acc);
+        }
       }
     }
   }
-  State at[VEC];  // at the group's start
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) at[v] = first[v];
-  if (start > 0 && active) await<State, W, VEC>(words, start - 1, at);
-  if (tells && pos == SCAN_GROUP - 1) {
-    State end[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) end[v] = at[v].through(Map::compose(own[v], acc[v]));
-    publish<State, W, VEC>(end, words, chunk);
+  if (teller) {
+    State at[1];  // at the group's start
+    if (start > 0) await<State, 1>(words + (long long)(start - 1) * W * CT + c, 0, CT, 1, at);
+    else at[0] = first(c);
+    if (tells && pos == SCAN_GROUP - 1) publish(at[0].through(Map::compose(own, acc)), mine, CT);
+    sh.in[c] = at[0].through(acc);
   }
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) in[v] = at[v].through(acc[v]);
+  __syncthreads();
 }
 
 // ------------------------------------------------------------ vector accesses
@@ -234,7 +252,7 @@ GFN_DEV void store_pack(T* p, const Pack<T, VEC>& r) {
 // by a ticket in the direction of the scan, all column tiles of one run before
 // the next: the blocks that a block waits for have started, so its wait ends.
 struct ScanTile {
-  int chunk, b, col;
+  int chunk, b, c0, col;  // c0: the tile's first column; col: this lane's first
   bool active;
   long long tile;
 };
@@ -252,82 +270,74 @@ GFN_DEV ScanTile scan_tile(const Args& p, unsigned* slot) {
   r.chunk = t / tiles;
   r.tile = t - (unsigned)r.chunk * tiles;
   r.b = (int)(r.tile / p.ctiles);
-  r.col = (int)(r.tile - (long long)r.b * p.ctiles) * (32 * VEC) + (threadIdx.x & 31) * VEC;
+  r.c0 = (int)(r.tile - (long long)r.b * p.ctiles) * (32 * VEC);
+  r.col = r.c0 + (threadIdx.x & 31) * VEC;
   r.active = r.col < p.D;
   return r;
 }
 
 // ------------------------------------------------------------------ gated scan
-template <typename T, int VEC, int S, int NW>
-__global__ void __launch_bounds__(NW * 32) gscan_forward_kernel(const GScanArgs p) {
+template <typename T, int VEC>
+GFN_DEV Pack<T, VEC> fill_pack(float v) {
+  Pack<T, VEC> r;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r.v[i] = from_f<T>(v);
+  return r;
+}
+
+// Map of S steps from a zero state; steps beyond the end hold a = 1, x = 0.
+template <typename T, int VEC, int S>
+GFN_DEV GatedMap run_map(const Pack<T, VEC> (&a)[S], const Pack<T, VEC> (&x)[S], int v) {
+  GatedMap m = GatedMap::identity();
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const float g = to_f(a[s].v[v]);
+    m.P *= g;
+    m.p = fmaf(g, m.p, to_f(x[s].v[v]));
+  }
+  if (m.P == 0.f) {  // a zero gate, or an underflow?
+    bool zero = false;
+#pragma unroll
+    for (int s = 0; s < S; ++s) zero = zero || to_f(a[s].v[v]) == 0.f;
+    if (!zero) m.P = copysignf(1.4e-45f, m.P);
+  }
+  return m;
+}
+
+template <typename T, int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) gscan_forward_kernel(const GScanArgs p) {
   constexpr int CT = 32 * VEC;
-  __shared__ unsigned long long maps[NW][1][CT], found[NW][1][CT];
-  __shared__ unsigned slot;
-  const ScanTile q = scan_tile<VEC>(p, &slot);
+  __shared__ ScanShared<GatedMap, GatedState, CT, NW> sh;
+  const ScanTile q = scan_tile<VEC>(p, &sh.slot);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = (q.chunk * NW + w) * S;
   const int n = q.active ? max(0, min(S, p.L - t0)) : 0;
   Pack<T, VEC> a[S], x[S];
-  {
-    const T* xp = static_cast<const T*>(p.x) + q.b * p.x_sb + t0 * p.x_st + q.col;
-    const T* ap = static_cast<const T*>(p.a) + q.b * p.a_sb + t0 * p.a_st + q.col;
+  const T* xp = static_cast<const T*>(p.x) + q.b * p.x_sb + t0 * p.x_st + q.col;
+  const T* ap = static_cast<const T*>(p.a) + q.b * p.a_sb + t0 * p.a_st + q.col;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        x[s] = load_pack<T, VEC>(xp + s * p.x_st);
-        if (p.a) a[s] = load_pack<T, VEC>(ap + s * p.a_st);
-      }
-    }
-    if (!p.a) {
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) a[s].v[v] = from_f<T>(1.f);
-      }
+  for (int s = 0; s < S; ++s) {
+    x[s] = fill_pack<T, VEC>(0.f);
+    a[s] = fill_pack<T, VEC>(1.f);
+    if (s < n) {
+      x[s] = load_pack<T, VEC>(xp + s * p.x_st);
+      if (p.a) a[s] = load_pack<T, VEC>(ap + s * p.a_st);
     }
   }
-  GatedMap m[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    m[v] = GatedMap::identity();
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        const float g = to_f(a[s].v[v]);
-        m[v].P *= g;
-        m[v].p = fmaf(g, m[v].p, to_f(x[s].v[v]));
-      }
-    }
-    if (m[v].P == 0.f) {  // a zero gate, or an underflow?
-      bool zero = false;
-#pragma unroll
-      for (int s = 0; s < S; ++s) zero = zero || (s < n && to_f(a[s].v[v]) == 0.f);
-      if (!zero) m[v].P = copysignf(1.4e-45f, m[v].P);
-    }
     unsigned long long wd[1];
-    m[v].pack(wd);
-    maps[w][0][lane * VEC + v] = wd[0];
+    run_map<T, VEC, S>(a, x, v).pack(wd);
+    sh.maps[w][0][lane * VEC + v] = wd[0];
   }
-  __syncthreads();
-  GatedMap before[VEC];  // of the warps before this one
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    before[v] = GatedMap::identity();
-    for (int j = 0; j < w; ++j) before[v] = GatedMap::compose(GatedMap::unpack({maps[j][0][lane * VEC + v]}), before[v]);
-  }
-  unsigned long long* words = p.words + q.tile * p.nchunks * (long long)CT;
-  GatedState first[VEC], in[VEC];
-  GatedMap own[VEC];  // of the whole run, in the last warp
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    first[v].h = (p.h0 && q.active) ? p.h0[(long long)q.b * p.D + q.col + v] : 0.f;
-    own[v] = GatedMap::compose(m[v], before[v]);
-  }
-  receive<GatedMap, GatedState, VEC, NW>(words, q.chunk, p.nchunks, q.active, w == NW - 1, own, first, found, in);
+  receive<GatedMap, GatedState, CT, NW, false>(
+      sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
+      [&](int c) { return GatedState{p.h0 ? p.h0[(long long)q.b * p.D + q.c0 + c] : 0.f}; });
+  if (n <= 0) return;
   float h[VEC];
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) h[v] = in[v].through(before[v]).h;
-  if (n <= 0) return;
+  for (int v = 0; v < VEC; ++v)
+    h[v] = sh.in[lane * VEC + v].through(GatedMap::unpack({sh.maps[w][0][lane * VEC + v]})).h;
   if (p.states && t0 % SCAN_CK == 0) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) p.states[((long long)q.b * p.nck + t0 / SCAN_CK) * p.D + q.col + v] = h[v];
@@ -335,15 +345,13 @@ __global__ void __launch_bounds__(NW * 32) gscan_forward_kernel(const GScanArgs 
   T* hp = static_cast<T*>(p.h) + ((long long)q.b * p.L + t0) * p.D + q.col;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    if (s < n) {
-      Pack<T, VEC> o;
+    Pack<T, VEC> o;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        h[v] = fmaf(to_f(a[s].v[v]), h[v], to_f(x[s].v[v]));
-        o.v[v] = from_f<T>(h[v]);
-      }
-      store_pack<T, VEC>(hp + (long long)s * p.D, o);
+    for (int v = 0; v < VEC; ++v) {
+      h[v] = fmaf(to_f(a[s].v[v]), h[v], to_f(x[s].v[v]));
+      o.v[v] = from_f<T>(h[v]);
     }
+    if (s < n) store_pack<T, VEC>(hp + (long long)s * p.D, o);
   }
   if (p.h_last && t0 + n == p.L) {
 #pragma unroll
@@ -354,121 +362,82 @@ __global__ void __launch_bounds__(NW * 32) gscan_forward_kernel(const GScanArgs 
 // Runs of NW * S = SCAN_CK steps from the last to the first: the state kept
 // before the run gives h, the messages pass from run to run as the states do
 // in the forward.
-template <typename T, int VEC, int S, int NW>
-__global__ void __launch_bounds__(NW * 32) gscan_backward_kernel(const GScanArgs p) {
+template <typename T, int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GScanArgs p) {
   static_assert(NW * S == SCAN_CK, "one kept state per run");
   constexpr int CT = 32 * VEC;
-  __shared__ unsigned long long fmaps[NW][CT], maps[NW][CT], found[NW][1][CT];
-  __shared__ unsigned slot;
-  const ScanTile q = scan_tile<VEC>(p, &slot);
+  __shared__ ScanShared<GatedMap, GatedState, CT, NW> sh;
+  __shared__ unsigned long long fmaps[NW][CT];
+  const ScanTile q = scan_tile<VEC>(p, &sh.slot);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int run = p.nchunks - 1 - q.chunk;
   const int t0 = run * SCAN_CK + w * S;
   const int n = q.active ? max(0, min(S, p.L - t0)) : 0;
   Pack<T, VEC> a[S], x[S], g[S];
-  {
-    const T* xp = static_cast<const T*>(p.x) + q.b * p.x_sb + t0 * p.x_st + q.col;
-    const T* ap = static_cast<const T*>(p.a) + q.b * p.a_sb + t0 * p.a_st + q.col;
-    const T* gp = static_cast<const T*>(p.dh) + q.b * p.g_sb + t0 * p.g_st + q.col;
+  const T* xp = static_cast<const T*>(p.x) + q.b * p.x_sb + t0 * p.x_st + q.col;
+  const T* ap = static_cast<const T*>(p.a) + q.b * p.a_sb + t0 * p.a_st + q.col;
+  const T* gp = static_cast<const T*>(p.dh) + q.b * p.g_sb + t0 * p.g_st + q.col;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        x[s] = load_pack<T, VEC>(xp + s * p.x_st);
-        if (p.a) a[s] = load_pack<T, VEC>(ap + s * p.a_st);
-        if (p.dh) g[s] = load_pack<T, VEC>(gp + s * p.g_st);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        if (!p.a) a[s].v[v] = from_f<T>(1.f);
-        if (!p.dh) g[s].v[v] = from_f<T>(0.f);
-      }
+  for (int s = 0; s < S; ++s) {
+    x[s] = g[s] = fill_pack<T, VEC>(0.f);
+    a[s] = fill_pack<T, VEC>(1.f);
+    if (s < n) {
+      x[s] = load_pack<T, VEC>(xp + s * p.x_st);
+      if (p.a) a[s] = load_pack<T, VEC>(ap + s * p.a_st);
+      if (p.dh) g[s] = load_pack<T, VEC>(gp + s * p.g_st);
     }
   }
-  GatedMap mb[VEC];  // of the message, last step first
+  float h[VEC];  // before the run
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+    h[v] = q.active ? p.states[((long long)q.b * p.nck + run) * p.D + q.col + v] : 0.f;
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    GatedMap mf = GatedMap::identity();
-    mb[v] = GatedMap::identity();
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        const float c = to_f(a[s].v[v]);
-        mf.P *= c;
-        mf.p = fmaf(c, mf.p, to_f(x[s].v[v]));
-      }
-    }
-#pragma unroll
-    for (int s = S - 1; s >= 0; --s)
-      if (s < n) mb[v].p = to_f(a[s].v[v]) * (to_f(g[s].v[v]) + mb[v].p);
-    if (mf.P == 0.f) {
-      bool zero = false;
-#pragma unroll
-      for (int s = 0; s < S; ++s) zero = zero || (s < n && to_f(a[s].v[v]) == 0.f);
-      if (!zero) mf.P = copysignf(1.4e-45f, mf.P);
-    }
-    mb[v].P = mf.P;
     unsigned long long wd[1];
+    const GatedMap mf = run_map<T, VEC, S>(a, x, v);
     mf.pack(wd);
     fmaps[w][lane * VEC + v] = wd[0];
-    mb[v].pack(wd);
-    maps[w][lane * VEC + v] = wd[0];
+    GatedMap mb = {mf.P, 0.f};  // of the message, last step first
+#pragma unroll
+    for (int s = S - 1; s >= 0; --s) mb.p = to_f(a[s].v[v]) * (to_f(g[s].v[v]) + mb.p);
+    mb.pack(wd);
+    sh.maps[w][0][lane * VEC + v] = wd[0];
   }
-  __syncthreads();
-  GatedMap after[VEC];  // of the warps behind this one, whose messages arrive first
+  receive<GatedMap, GatedState, CT, NW, true>(
+      sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
+      [&](int c) { return GatedState{p.dlast ? p.dlast[(long long)q.b * p.D + q.c0 + c] : 0.f}; });
+  if (!q.active) return;
+  float m[VEC], hp[S][VEC];  // hp: h_{t-1}
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    after[v] = GatedMap::identity();
-    for (int j = NW - 1; j > w; --j)
-      after[v] = GatedMap::compose(GatedMap::unpack({maps[j][lane * VEC + v]}), after[v]);
-  }
-  unsigned long long* words = p.words + q.tile * p.nchunks * (long long)CT;
-  // h_{t-1} of this warp's steps, from the kept state
-  float hp[S][VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    float h = 0.f;
-    if (q.active) h = p.states[((long long)q.b * p.nck + run) * p.D + q.col + v];
+    m[v] = sh.in[lane * VEC + v].through(GatedMap::unpack({sh.maps[w][0][lane * VEC + v]})).h;
     for (int j = 0; j < w; ++j) {
       const GatedMap f = GatedMap::unpack({fmaps[j][lane * VEC + v]});
-      h = pass(f.P, h, f.p);
+      h[v] = pass(f.P, h[v], f.p);
     }
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      hp[s][v] = h;
-      if (s < n) h = fmaf(to_f(a[s].v[v]), h, to_f(x[s].v[v]));
+      hp[s][v] = h[v];
+      h[v] = fmaf(to_f(a[s].v[v]), h[v], to_f(x[s].v[v]));
     }
   }
-  GatedState first[VEC], in[VEC];
-  GatedMap own[VEC];  // of the whole run, in the first warp
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    first[v].h = (p.dlast && q.active) ? p.dlast[(long long)q.b * p.D + q.col + v] : 0.f;
-    own[v] = GatedMap::compose(mb[v], after[v]);
-  }
-  receive<GatedMap, GatedState, VEC, NW>(words, q.chunk, p.nchunks, q.active, w == 0, own, first, found, in);
-  float m[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) m[v] = in[v].through(after[v]).h;
   const long long o = ((long long)q.b * p.L + t0) * p.D + q.col;
 #pragma unroll
   for (int s = S - 1; s >= 0; --s) {
-    if (s < n) {
-      Pack<T, VEC> oa, ox;
+    Pack<T, VEC> oa, ox;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float gt = to_f(g[s].v[v]) + m[v];
-        ox.v[v] = from_f<T>(gt);
-        oa.v[v] = from_f<T>(gt * hp[s][v]);
-        m[v] = to_f(a[s].v[v]) * gt;
-      }
+    for (int v = 0; v < VEC; ++v) {
+      const float gt = to_f(g[s].v[v]) + m[v];
+      ox.v[v] = from_f<T>(gt);
+      oa.v[v] = from_f<T>(gt * hp[s][v]);
+      m[v] = to_f(a[s].v[v]) * gt;
+    }
+    if (s < n) {
       if (p.dx) store_pack<T, VEC>(static_cast<T*>(p.dx) + o + (long long)s * p.D, ox);
       if (p.da) store_pack<T, VEC>(static_cast<T*>(p.da) + o + (long long)s * p.D, oa);
     }
   }
-  if (p.dh0 && run == 0 && w == 0 && q.active) {
+  if (p.dh0 && run == 0 && w == 0) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) p.dh0[(long long)q.b * p.D + q.col + v] = m[v];
   }
@@ -525,17 +494,35 @@ struct LScanArgs {
   float base_dt;
 };
 
-// sigma(z) and sigma(-z) from one exponential that cannot overflow: both keep
-// their digits far out, where 1 / (1 + exp(-z)) is already 0 or 1.
-GFN_DEV float gate(float z, float* complement) {
-  const float e = expf(-fabsf(z)), r = 1.f / (1.f + e);
-  *complement = z >= 0.f ? e * r : r;
-  return z >= 0.f ? r : e * r;
+// 1 / v to one unit in the last place, for v in [1, 6].
+GFN_DEV float quick_rcp(float v) { return __fdividef(1.f, v); }
+
+// sigma(z) and its slope sigma(z) sigma(-z) from one exponential that cannot
+// overflow: both keep their digits far out, where 1 / (1 + exp(-z)) is
+// already 0 or 1.
+GFN_DEV float gate(float z, float* slope) {
+  const float e = expf(-fabsf(z)), r = quick_rcp(1.f + e), c = e * r;
+  *slope = r * c;
+  return z >= 0.f ? r : c;
 }
 
-GFN_DEV float gate(float z) {
-  float c;
-  return gate(z, &c);
+// softplus(z) = max(z, 0) + log1p(e), e = exp(-|z|) in [0, 1], and its slope
+// sigma(z).  log1p(e) = 2 atanh(y) with y = e / (2 + e) <= 1/3: the odd series
+// up to y^15 leaves 1e-9 of the sum, and every term is positive.
+GFN_DEV float soft_step(float z, float* slope) {
+  const float e = expf(-fabsf(z));
+  const float r = quick_rcp((1.f + e) * (2.f + e));  // both quotients from one reciprocal
+  const float y = e * ((1.f + e) * r), y2 = y * y, s = (2.f + e) * r;
+  float q = 1.f / 15.f;
+  q = fmaf(q, y2, 1.f / 13.f);
+  q = fmaf(q, y2, 1.f / 11.f);
+  q = fmaf(q, y2, 1.f / 9.f);
+  q = fmaf(q, y2, 1.f / 7.f);
+  q = fmaf(q, y2, 1.f / 5.f);
+  q = fmaf(q, y2, 1.f / 3.f);
+  q = fmaf(q * y2, y, y);
+  *slope = z >= 0.f ? s : e * s;
+  return fmaf(2.f, q, fmaxf(z, 0.f));
 }
 
 GFN_DEV float head_scale(int col, int hd) {
@@ -567,74 +554,61 @@ struct LayerState {
   GFN_DEV LayerState through(LayerMap m) const { return {pass(m.P, v, m.p), x + pass(m.Q, v, m.q)}; }
 };
 
-template <int VEC, int S, int NW>
-__global__ void __launch_bounds__(NW * 32) lscan_forward_kernel(const LScanArgs p) {
+template <int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScanArgs p) {
   constexpr int CT = 32 * VEC;
-  __shared__ unsigned long long maps[NW][2][CT], found[NW][2][CT];
-  __shared__ unsigned slot;
-  const ScanTile c = scan_tile<VEC>(p, &slot);
+  __shared__ ScanShared<LayerMap, LayerState, CT, NW> sh;
+  const ScanTile c = scan_tile<VEC>(p, &sh.slot);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = (c.chunk * NW + w) * S;
   const int n = c.active ? max(0, min(S, p.L - t0)) : 0;
   const float* zp = p.z + ((long long)c.b * p.L + t0) * 3 * p.D + c.col;
   Pack<float, VEC> A[S], dt[S], bv[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
+  for (int s = 0; s < S; ++s) {  // beyond the end: A = 1, dt = 0, zB = 0
+    A[s] = fill_pack<float, VEC>(INFINITY);
+    dt[s] = fill_pack<float, VEC>(-INFINITY);
+    bv[s] = fill_pack<float, VEC>(0.f);
     if (s < n) {
       A[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D);
       dt[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + p.D);
       bv[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + 2LL * p.D);
     }
   }
-  LayerMap m[VEC];
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    const float hs = head_scale(c.col + v, p.D / p.H);
-    m[v] = LayerMap::identity();
+    const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
+    LayerMap m = LayerMap::identity();
     bool zero = false;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        A[s].v[v] = gate(A[s].v[v]);
-        dt[s].v[v] = (softplus_f(dt[s].v[v]) * p.base_dt) * hs;
-        bv[s].v[v] *= dt[s].v[v];
-        zero = zero || A[s].v[v] == 0.f;
-        m[v].P *= A[s].v[v];
-        m[v].p = fmaf(A[s].v[v], m[v].p, bv[s].v[v]);
-        m[v].Q = fmaf(dt[s].v[v], m[v].P, m[v].Q);
-        m[v].q = fmaf(dt[s].v[v], m[v].p, m[v].q);
-      }
+      float slope;
+      A[s].v[v] = gate(A[s].v[v], &slope);
+      dt[s].v[v] = soft_step(dt[s].v[v], &slope) * scale;
+      bv[s].v[v] *= dt[s].v[v];
+      zero = zero || A[s].v[v] == 0.f;
+      m.P *= A[s].v[v];
+      m.p = fmaf(A[s].v[v], m.p, bv[s].v[v]);
+      m.Q = fmaf(dt[s].v[v], m.P, m.Q);
+      m.q = fmaf(dt[s].v[v], m.p, m.q);
     }
-    if (m[v].P == 0.f && !zero) m[v].P = 1.4e-45f;
+    if (m.P == 0.f && !zero) m.P = 1.4e-45f;
     unsigned long long wd[2];
-    m[v].pack(wd);
-    maps[w][0][lane * VEC + v] = wd[0];
-    maps[w][1][lane * VEC + v] = wd[1];
+    m.pack(wd);
+    sh.maps[w][0][lane * VEC + v] = wd[0];
+    sh.maps[w][1][lane * VEC + v] = wd[1];
   }
-  __syncthreads();
-  LayerMap before[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    before[v] = LayerMap::identity();
-    for (int j = 0; j < w; ++j)
-      before[v] = LayerMap::compose(LayerMap::unpack({maps[j][0][lane * VEC + v], maps[j][1][lane * VEC + v]}),
-                                    before[v]);
-  }
-  unsigned long long* words = p.words + c.tile * p.nchunks * (2LL * CT);
-  LayerState first[VEC], in[VEC];
-  LayerMap own[VEC];  // of the whole run, in the last warp
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    const long long e = (long long)c.b * p.D + c.col + v;
-    first[v].v = (p.v0 && c.active) ? p.v0[e] : 0.f;
-    first[v].x = (p.x0 && c.active) ? p.x0[e] : 0.f;
-    own[v] = LayerMap::compose(m[v], before[v]);
-  }
-  receive<LayerMap, LayerState, VEC, NW>(words, c.chunk, p.nchunks, c.active, w == NW - 1, own, first, found, in);
+  receive<LayerMap, LayerState, CT, NW, false>(
+      sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0, [&](int j) {
+        const long long e = (long long)c.b * p.D + c.c0 + j;
+        return LayerState{p.v0 ? p.v0[e] : 0.f, p.x0 ? p.x0[e] : 0.f};
+      });
+  if (n <= 0) return;
   LayerState st[VEC];
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) st[v] = in[v].through(before[v]);
-  if (n <= 0) return;
+  for (int v = 0; v < VEC; ++v)
+    st[v] = sh.in[lane * VEC + v].through(
+        LayerMap::unpack({sh.maps[w][0][lane * VEC + v], sh.maps[w][1][lane * VEC + v]}));
   if (p.states && t0 % SCAN_CK == 0) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) p.states[((long long)c.b * p.nck + t0 / SCAN_CK) * p.D + c.col + v] = st[v].v;
@@ -642,15 +616,15 @@ __global__ void __launch_bounds__(NW * 32) lscan_forward_kernel(const LScanArgs 
   const long long o = ((long long)c.b * p.L + t0) * p.D + c.col;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    if (s < n) {
-      Pack<float, VEC> ov, ox;
+    Pack<float, VEC> ov, ox;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        st[v].v = fmaf(A[s].v[v], st[v].v, bv[s].v[v]);
-        st[v].x = fmaf(st[v].v, dt[s].v[v], st[v].x);
-        ov.v[v] = st[v].v;
-        ox.v[v] = st[v].x;
-      }
+    for (int v = 0; v < VEC; ++v) {
+      st[v].v = fmaf(A[s].v[v], st[v].v, bv[s].v[v]);
+      st[v].x = fmaf(st[v].v, dt[s].v[v], st[v].x);
+      ov.v[v] = st[v].v;
+      ox.v[v] = st[v].x;
+    }
+    if (s < n) {
       store_pack<float, VEC>(p.vs + o + (long long)s * p.D, ov);
       store_pack<float, VEC>(p.xs + o + (long long)s * p.D, ox);
     }
@@ -688,133 +662,107 @@ struct LayerBackState {
   GFN_DEV LayerBackState through(LayerBackMap f) const { return {pass(f.P, m, pass(f.R, X, f.q)), X + f.G}; }
 };
 
-template <int VEC, int S, int NW>
-__global__ void __launch_bounds__(NW * 32) lscan_backward_kernel(const LScanArgs p) {
+template <int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LScanArgs p) {
   static_assert(NW * S == SCAN_CK, "one kept state per run");
   constexpr int CT = 32 * VEC;
-  __shared__ unsigned long long fmaps[NW][CT], maps[NW][2][CT], found[NW][2][CT];
-  __shared__ unsigned slot;
-  const ScanTile c = scan_tile<VEC>(p, &slot);
+  __shared__ ScanShared<LayerBackMap, LayerBackState, CT, NW> sh;
+  __shared__ unsigned long long fmaps[NW][CT];
+  const ScanTile c = scan_tile<VEC>(p, &sh.slot);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int run = p.nchunks - 1 - c.chunk;
   const int t0 = run * SCAN_CK + w * S;
   const int n = c.active ? max(0, min(S, p.L - t0)) : 0;
   const long long o = ((long long)c.b * p.L + t0) * p.D + c.col;
   const float* zp = p.z + 3 * (o - c.col) + c.col;
-  Pack<float, VEC> za[S], zd[S], zb[S], gx[S], gv[S];
+  Pack<float, VEC> A[S], dt[S], zb[S], gx[S], gv[S], sa[S], sd[S];  // sa, sd: slopes of A and dt
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
+  for (int s = 0; s < S; ++s) {  // beyond the end: A = 1, dt = 0, zB = 0, no gradients
+    A[s] = fill_pack<float, VEC>(INFINITY);
+    dt[s] = fill_pack<float, VEC>(-INFINITY);
+    zb[s] = gx[s] = gv[s] = fill_pack<float, VEC>(0.f);
     if (s < n) {
-      za[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D);
-      zd[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + p.D);
+      A[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D);
+      dt[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + p.D);
       zb[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + 2LL * p.D);
       if (p.gx) gx[s] = load_pack<float, VEC>(p.gx + o + (long long)s * p.D);
       if (p.gv) gv[s] = load_pack<float, VEC>(p.gv + o + (long long)s * p.D);
     }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      if (!p.gx) gx[s].v[v] = 0.f;
-      if (!p.gv) gv[s].v[v] = 0.f;
-    }
   }
-  float scale[VEC];
-  LayerBackMap mb[VEC];
+  float h[VEC];  // v before the run
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+    h[v] = c.active ? p.states[((long long)c.b * p.nck + run) * p.D + c.col + v] : 0.f;
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    scale[v] = head_scale(c.col + v, p.D / p.H);
+    const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
     GatedMap mf = GatedMap::identity();
     bool zero = false;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      if (s < n) {
-        const float A = gate(za[s].v[v]), dt = (softplus_f(zd[s].v[v]) * p.base_dt) * scale[v];
-        zero = zero || A == 0.f;
-        mf.P *= A;
-        mf.p = fmaf(A, mf.p, zb[s].v[v] * dt);
-      }
+      A[s].v[v] = gate(A[s].v[v], &sa[s].v[v]);
+      dt[s].v[v] = soft_step(dt[s].v[v], &sd[s].v[v]) * scale;
+      sd[s].v[v] *= scale;
+      zero = zero || A[s].v[v] == 0.f;
+      mf.P *= A[s].v[v];
+      mf.p = fmaf(A[s].v[v], mf.p, zb[s].v[v] * dt[s].v[v]);
     }
     if (mf.P == 0.f && !zero) mf.P = 1.4e-45f;
-    mb[v] = LayerBackMap::identity();
+    LayerBackMap mb = LayerBackMap::identity();
+    mb.P = mf.P;
 #pragma unroll
     for (int s = S - 1; s >= 0; --s) {
-      if (s < n) {
-        const float A = gate(za[s].v[v]), dt = (softplus_f(zd[s].v[v]) * p.base_dt) * scale[v];
-        mb[v].G += gx[s].v[v];
-        mb[v].q = A * (fmaf(dt, mb[v].G, gv[s].v[v]) + mb[v].q);
-        mb[v].R = A * (mb[v].R + dt);
-      }
+      mb.G += gx[s].v[v];
+      mb.q = A[s].v[v] * (fmaf(dt[s].v[v], mb.G, gv[s].v[v]) + mb.q);
+      mb.R = A[s].v[v] * (mb.R + dt[s].v[v]);
     }
-    mb[v].P = mf.P;
     unsigned long long wd[2], wf[1];
     mf.pack(wf);
     fmaps[w][lane * VEC + v] = wf[0];
-    mb[v].pack(wd);
-    maps[w][0][lane * VEC + v] = wd[0];
-    maps[w][1][lane * VEC + v] = wd[1];
+    mb.pack(wd);
+    sh.maps[w][0][lane * VEC + v] = wd[0];
+    sh.maps[w][1][lane * VEC + v] = wd[1];
   }
-  __syncthreads();
-  LayerBackMap after[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    after[v] = LayerBackMap::identity();
-    for (int j = NW - 1; j > w; --j)
-      after[v] = LayerBackMap::compose(
-          LayerBackMap::unpack({maps[j][0][lane * VEC + v], maps[j][1][lane * VEC + v]}), after[v]);
-  }
-  unsigned long long* words = p.words + c.tile * p.nchunks * (2LL * CT);
+  receive<LayerBackMap, LayerBackState, CT, NW, true>(
+      sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0, [&](int j) {
+        const long long e = (long long)c.b * p.D + c.c0 + j;
+        return LayerBackState{p.gvl ? p.gvl[e] : 0.f, p.gxl ? p.gxl[e] : 0.f};
+      });
+  if (!c.active) return;
+  LayerBackState st[VEC];
   float vs[S + 1][VEC];  // v_{t-1} of this warp's steps, and the last step's v
 #pragma unroll
   for (int v = 0; v < VEC; ++v) {
-    float h = 0.f;
-    if (c.active) h = p.states[((long long)c.b * p.nck + run) * p.D + c.col + v];
+    st[v] = sh.in[lane * VEC + v].through(
+        LayerBackMap::unpack({sh.maps[w][0][lane * VEC + v], sh.maps[w][1][lane * VEC + v]}));
     for (int j = 0; j < w; ++j) {
       const GatedMap f = GatedMap::unpack({fmaps[j][lane * VEC + v]});
-      h = pass(f.P, h, f.p);
+      h[v] = pass(f.P, h[v], f.p);
     }
-    vs[0][v] = h;
+    vs[0][v] = h[v];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n)
-        h = fmaf(gate(za[s].v[v]), h, zb[s].v[v] * ((softplus_f(zd[s].v[v]) * p.base_dt) * scale[v]));
-      vs[s + 1][v] = h;
-    }
+    for (int s = 0; s < S; ++s) vs[s + 1][v] = fmaf(A[s].v[v], vs[s][v], zb[s].v[v] * dt[s].v[v]);
   }
-  LayerBackState first[VEC], in[VEC];
-  LayerBackMap own[VEC];  // of the whole run, in the first warp
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    const long long e = (long long)c.b * p.D + c.col + v;
-    first[v].m = (p.gvl && c.active) ? p.gvl[e] : 0.f;
-    first[v].X = (p.gxl && c.active) ? p.gxl[e] : 0.f;
-    own[v] = LayerBackMap::compose(mb[v], after[v]);
-  }
-  receive<LayerBackMap, LayerBackState, VEC, NW>(words, c.chunk, p.nchunks, c.active, w == 0, own, first, found, in);
-  LayerBackState st[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) st[v] = in[v].through(after[v]);
   float* dz = p.dz + 3 * (o - c.col) + c.col;
 #pragma unroll
   for (int s = S - 1; s >= 0; --s) {
-    if (s < n) {
-      Pack<float, VEC> oa, od, ob;
+    Pack<float, VEC> oa, od, ob;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float nA;
-        const float A = gate(za[s].v[v], &nA);
-        const float dt = (softplus_f(zd[s].v[v]) * p.base_dt) * scale[v];
-        st[v].X += gx[s].v[v];
-        const float l = fmaf(dt, st[v].X, gv[s].v[v]) + st[v].m;
-        oa.v[v] = l * vs[s][v] * (A * nA);
-        od.v[v] = (l * zb[s].v[v] + st[v].X * vs[s + 1][v]) * (p.base_dt * scale[v]) * gate(zd[s].v[v]);
-        ob.v[v] = l * dt;
-        st[v].m = A * l;
-      }
+    for (int v = 0; v < VEC; ++v) {
+      st[v].X += gx[s].v[v];
+      const float l = fmaf(dt[s].v[v], st[v].X, gv[s].v[v]) + st[v].m;
+      oa.v[v] = l * vs[s][v] * sa[s].v[v];
+      od.v[v] = (l * zb[s].v[v] + st[v].X * vs[s + 1][v]) * sd[s].v[v];
+      ob.v[v] = l * dt[s].v[v];
+      st[v].m = A[s].v[v] * l;
+    }
+    if (s < n) {
       store_pack<float, VEC>(dz + (long long)s * 3 * p.D, oa);
       store_pack<float, VEC>(dz + (long long)s * 3 * p.D + p.D, od);
       store_pack<float, VEC>(dz + (long long)s * 3 * p.D + 2LL * p.D, ob);
     }
   }
-  if (run == 0 && w == 0 && c.active) {
+  if (run == 0 && w == 0) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       const long long e = (long long)c.b * p.D + c.col + v;
@@ -829,14 +777,15 @@ __global__ void __launch_bounds__(128) lscan_forward_seq_kernel(const LScanArgs 
   const long long c = blockIdx.x * 128LL + threadIdx.x;
   if (c >= (long long)p.B * p.D) return;
   const long long b = c / p.D, j = c - b * p.D;
-  const float hs = head_scale((int)j, p.D / p.H);
+  const float scale = p.base_dt * head_scale((int)j, p.D / p.H);
   float v = p.v0 ? p.v0[c] : 0.f, x = p.x0 ? p.x0[c] : 0.f;
   if (p.states && p.L) p.states[c] = v;
 #pragma unroll 4
   for (int t = 0; t < p.L; ++t) {
     const float* z = p.z + (b * p.L + t) * 3 * p.D + j;
-    const float dt = (softplus_f(z[p.D]) * p.base_dt) * hs;
-    v = fmaf(gate(z[0]), v, z[2LL * p.D] * dt);
+    float slope;
+    const float dt = soft_step(z[p.D], &slope) * scale;
+    v = fmaf(gate(z[0], &slope), v, z[2LL * p.D] * dt);
     x = fmaf(v, dt, x);
     const long long e = (b * p.L + t) * p.D + j;
     p.vs[e] = v;
