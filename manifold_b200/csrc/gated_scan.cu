@@ -1,5 +1,10 @@
 // C ABI of the gated scan and of the scan layer's recurrence with their
 // backward passes (gated_scan.cuh).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "abi.h"
 #include "gated_scan.cuh"
 
@@ -43,45 +48,120 @@ int set_tiles(const char* what, Args* p, int run, int ct, int words, void* works
   return cuda_status(cudaMemsetAsync(workspace, 0xff, (size_t)need, s), what);
 }
 
-// VEC columns per lane: every row of every operand must start on a VEC boundary.
-bool packs(const void* ptr, long long sb, long long st, int B, int L, int vec, int size) {
-  return !ptr || (reinterpret_cast<uintptr_t>(ptr) % (vec * size) == 0 && (B == 1 || sb % vec == 0) &&
-                  (L == 1 || st % vec == 0));
+// Whether every row of an operand starts on 16 bytes, as a tensor copy needs it.
+bool rows16(const void* ptr, long long sb, long long st, int B, int L, int size) {
+  return !ptr || (aligned16(ptr) && (B == 1 || (sb * size % 16 == 0 && sb * size < (1LL << 40))) &&
+                  (L == 1 || (st * size % 16 == 0 && st * size < (1LL << 40))));
 }
 
-template <typename T, int VEC, int S, int NW, int OCC>
+// cuTensorMapEncodeTiled from the driver (no link-time libcuda dependency).
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+CUtensorMapDataType map_type(const float*) { return CU_TENSOR_MAP_DATA_TYPE_FLOAT32; }
+CUtensorMapDataType map_type(const __nv_bfloat16*) { return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+CUtensorMapDataType map_type(const __half*) { return CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+
+// One operand (NULL: none) as a [B][L][cols] tensor with `steps` x `ct` boxes;
+// strides in elements.
+template <typename T>
+int operand_map(CUtensorMap* m, const T* base, long long sb, long long st, int B, int L, int cols, int steps, int ct) {
+  if (!base) return GFN_OK;
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return fail(GFN_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t row = (cuuint64_t)(cols * (int)sizeof(T));
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)L, (cuuint64_t)B};
+  // the stride of a dimension of one element is never used, but has to be valid
+  const cuuint64_t strides[2] = {L > 1 ? (cuuint64_t)st * sizeof(T) : row, B > 1 ? (cuuint64_t)sb * sizeof(T) : row};
+  const cuuint32_t box[3] = {(cuuint32_t)ct, (cuuint32_t)steps, 1}, unit[3] = {1, 1, 1};
+  const CUresult r = enc(m, map_type(base), 3, const_cast<T*>(base), dims, strides, box, unit,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(GFN_ERR_CUDA, "scan: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return GFN_OK;
+}
+
+// A persistent launch: OCC blocks per SM, each with `stage` bytes for the next
+// run's operands.
+template <class Args>
+int launch(const char* what, void (*kernel)(Args, ScanMaps), const Args& p, const ScanMaps& maps, unsigned blocks, int occ, int threads, int stage,
+           cudaStream_t s) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, stage);
+  if (e != cudaSuccess) return cuda_status(e, what);
+  const unsigned slots = (unsigned)(sms * occ);
+  kernel<<<blocks < slots ? blocks : slots, threads, stage, s>>>(p, maps);
+  return launch_status(what);
+}
+
+template <int MODE, typename T, int VEC, int S, int NW, int OCC>
 int gscan_forward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
-  unsigned grid;
-  const int st = set_tiles("gated_scan_forward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &grid);
+  unsigned blocks;
+  const int st = set_tiles("gated_scan_forward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &blocks);
   if (st) return st;
-  gscan_forward_kernel<T, VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
-  return launch_status("gscan_forward_kernel");
+  ScanMaps maps = {};
+  if (MODE == SCAN_TMA) {
+    int e = operand_map(&maps.m[0], static_cast<const T*>(p.x), p.x_sb, p.x_st, p.B, p.L, p.D, S * NW, 32 * VEC);
+    if (!e) e = operand_map(&maps.m[1], static_cast<const T*>(p.a), p.a_sb, p.a_st, p.B, p.L, p.D, S * NW, 32 * VEC);
+    if (e) return e;
+  }
+  return launch("gscan_forward_kernel", gscan_forward_kernel<MODE, T, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
+                MODE == SCAN_TMA ? 2 * Stage<T, VEC, S, NW>::OPERAND : 0, s);
 }
 
-template <typename T, int VEC, int S, int NW, int OCC>
+template <int MODE, typename T, int VEC, int S, int NW, int OCC>
 int gscan_backward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
-  unsigned grid;
-  const int st = set_tiles("gated_scan_backward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &grid);
+  unsigned blocks;
+  const int st = set_tiles("gated_scan_backward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &blocks);
   if (st) return st;
-  gscan_backward_kernel<T, VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
-  return launch_status("gscan_backward_kernel");
+  ScanMaps maps = {};
+  if (MODE == SCAN_TMA) {
+    int e = operand_map(&maps.m[0], static_cast<const T*>(p.x), p.x_sb, p.x_st, p.B, p.L, p.D, S * NW, 32 * VEC);
+    if (!e) e = operand_map(&maps.m[1], static_cast<const T*>(p.a), p.a_sb, p.a_st, p.B, p.L, p.D, S * NW, 32 * VEC);
+    if (!e) e = operand_map(&maps.m[2], static_cast<const T*>(p.dh), p.g_sb, p.g_st, p.B, p.L, p.D, S * NW, 32 * VEC);
+    if (e) return e;
+  }
+  return launch("gscan_backward_kernel", gscan_backward_kernel<MODE, T, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
+                MODE == SCAN_TMA ? 3 * Stage<T, VEC, S, NW>::OPERAND : 0, s);
+}
+
+bool repeats(const void* ptr, long long sb, long long st, int B, int L) {
+  return ptr && ((B > 1 && sb == 0) || (L > 1 && st == 0));
 }
 
 template <typename T, int VEC>
-int gscan_run(const GScanArgs& p, bool backward, void* ws, long long bytes, cudaStream_t s) {
+int gscan_run(GScanArgs p, bool backward, void* ws, long long bytes, cudaStream_t s) {
   const int z = sizeof(T);
-  const bool vec = p.D % VEC == 0 && packs(p.a, p.a_sb, p.a_st, p.B, p.L, VEC, z) &&
-                   packs(p.x, p.x_sb, p.x_st, p.B, p.L, VEC, z) && packs(p.dh, p.g_sb, p.g_st, p.B, p.L, VEC, z) &&
-                   packs(p.h, 0, 0, 1, 1, VEC, z) && packs(p.da, 0, 0, 1, 1, VEC, z) &&
-                   packs(p.dx, 0, 0, 1, 1, VEC, z);
-  if (backward) {
-    return vec ? gscan_backward<T, VEC, 8, 8, 2>(p, ws, bytes, s) : gscan_backward<T, 1, 8, 8, 4>(p, ws, bytes, s);
-  }
-  if (p.L <= SEQ_STEPS) {
+  if (!backward && p.L <= SEQ_STEPS) {
     gscan_forward_seq_kernel<T><<<column_blocks(p.B, p.D), 128, 0, s>>>(p);
     return launch_status("gscan_forward_seq_kernel");
   }
-  return vec ? gscan_forward<T, VEC, 16, 8, 2>(p, ws, bytes, s) : gscan_forward<T, 1, 16, 8, 4>(p, ws, bytes, s);
+  p.broadcast = repeats(p.a, p.a_sb, p.a_st, p.B, p.L) || repeats(p.x, p.x_sb, p.x_st, p.B, p.L) ||
+                repeats(p.dh, p.g_sb, p.g_st, p.B, p.L);
+  const bool tma = !p.broadcast && p.D * z % 16 == 0 && rows16(p.a, p.a_sb, p.a_st, p.B, p.L, z) &&
+                    rows16(p.x, p.x_sb, p.x_st, p.B, p.L, z) && rows16(p.dh, p.g_sb, p.g_st, p.B, p.L, z) &&
+                    aligned16(p.h) && aligned16(p.da) && aligned16(p.dx);
+  if (tma)
+    return backward ? gscan_backward<SCAN_TMA, T, VEC, 8, 8, 2>(p, ws, bytes, s)
+                    : gscan_forward<SCAN_TMA, T, VEC, 16, 8, 2>(p, ws, bytes, s);
+  if constexpr (sizeof(T) == 2)
+    return backward ? gscan_backward<SCAN_SPLIT, T, 2, 8, 8, 3>(p, ws, bytes, s)
+                    : gscan_forward<SCAN_SPLIT, T, 2, 16, 8, 3>(p, ws, bytes, s);
+  else
+    return backward ? gscan_backward<SCAN_PLAIN, T, 1, 8, 8, 4>(p, ws, bytes, s)
+                    : gscan_forward<SCAN_PLAIN, T, 1, 16, 8, 4>(p, ws, bytes, s);
 }
 
 int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long long bytes, cudaStream_t s) {
@@ -91,23 +171,38 @@ int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long 
   return fail(GFN_ERR_UNSUPPORTED, "gated_scan: element type %d", dtype);
 }
 
-template <int VEC>
+template <int MODE, int VEC>
 int lscan_forward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   constexpr int S = 8, NW = 8, OCC = 2;
-  unsigned grid;
-  const int st = set_tiles("layer_scan_forward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &grid);
+  unsigned blocks;
+  const int st = set_tiles("layer_scan_forward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &blocks);
   if (st) return st;
-  lscan_forward_kernel<VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
-  return launch_status("lscan_forward_kernel");
+  ScanMaps maps = {};
+  if (MODE == SCAN_TMA) {
+    const long long D = p.D;
+    int e = operand_map(&maps.m[0], p.z, 3 * D * p.L, 3 * D, p.B, p.L, 3 * p.D, S * NW, 32 * VEC);
+    if (e) return e;
+  }
+  return launch("lscan_forward_kernel", lscan_forward_kernel<MODE, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
+                MODE == SCAN_TMA ? 3 * Stage<float, VEC, S, NW>::OPERAND : 0, s);
 }
 
+template <int MODE>
 int lscan_backward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   constexpr int VEC = 1, S = 8, NW = 8, OCC = 2;
-  unsigned grid;
-  const int st = set_tiles("layer_scan_backward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &grid);
+  unsigned blocks;
+  const int st = set_tiles("layer_scan_backward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &blocks);
   if (st) return st;
-  lscan_backward_kernel<VEC, S, NW, OCC><<<grid, NW * 32, 0, s>>>(p);
-  return launch_status("lscan_backward_kernel");
+  ScanMaps maps = {};
+  if (MODE == SCAN_TMA) {
+    const long long D = p.D;
+    int e = operand_map(&maps.m[0], p.z, 3 * D * p.L, 3 * D, p.B, p.L, 3 * p.D, S * NW, 32 * VEC);
+    if (!e) e = operand_map(&maps.m[1], p.gx, D * p.L, D, p.B, p.L, p.D, S * NW, 32 * VEC);
+    if (!e) e = operand_map(&maps.m[2], p.gv, D * p.L, D, p.B, p.L, p.D, S * NW, 32 * VEC);
+    if (e) return e;
+  }
+  return launch("lscan_backward_kernel", lscan_backward_kernel<MODE, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
+                MODE == SCAN_TMA ? 5 * Stage<float, VEC, S, NW>::OPERAND : 0, s);
 }
 
 // A state or its gradient handed through a sequence of no steps.
@@ -190,9 +285,9 @@ int gfn_layer_scan_forward(const float* z, const float* v0, const float* x0, int
     lscan_forward_seq_kernel<<<column_blocks(batch, dim), 128, 0, s>>>(p);
     return launch_status("lscan_forward_seq_kernel");
   }
-  const bool vec = dim % 2 == 0 && packs(z, 0, 0, 1, 1, 2, 4) && packs(x_seq, 0, 0, 1, 1, 2, 4) &&
-                   packs(v_seq, 0, 0, 1, 1, 2, 4);
-  return vec ? lscan_forward<2>(p, workspace, workspace_bytes, s) : lscan_forward<1>(p, workspace, workspace_bytes, s);
+  const bool tma = dim % 4 == 0 && aligned16(z) && aligned16(x_seq) && aligned16(v_seq);
+  return tma ? lscan_forward<SCAN_TMA, 2>(p, workspace, workspace_bytes, s)
+              : lscan_forward<SCAN_PLAIN, 1>(p, workspace, workspace_bytes, s);
 }
 
 int gfn_layer_scan_backward(const float* z, const float* states, const float* gx, const float* gv,
@@ -213,7 +308,9 @@ int gfn_layer_scan_backward(const float* z, const float* states, const float* gx
     st = pass_through("layer_scan_backward", dv0, gv_last, batch, dim, s);
     return st ? st : pass_through("layer_scan_backward", dx0, gx_last, batch, dim, s);
   }
-  return lscan_backward(p, workspace, workspace_bytes, s);
+  const bool tma = dim % 4 == 0 && aligned16(z) && aligned16(gx) && aligned16(gv) && aligned16(dz);
+  return tma ? lscan_backward<SCAN_TMA>(p, workspace, workspace_bytes, s)
+              : lscan_backward<SCAN_PLAIN>(p, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"

@@ -23,7 +23,10 @@
 // the group's start, which the group before publishes.  What is composed with
 // what does not depend on which block is faster, so results repeat bit for bit.
 #pragma once
+#include <type_traits>
+
 #include "lm_ops.cuh"
+#include "umma.cuh"
 
 namespace gfn {
 
@@ -46,6 +49,7 @@ struct GScanArgs {
   unsigned* ticket;
   int B, L, D, nck;
   int nchunks, ctiles;  // runs of steps per column; column tiles per batch row
+  int broadcast;        // an operand has a stride of zero
 };
 
 // ------------------------------------------------------------ published words
@@ -146,7 +150,18 @@ struct ScanShared {
   unsigned long long maps[NW][Map::WORDS][CT];  // the warps' maps; then those of all warps before each
   unsigned long long part[R][Map::WORDS][CT];   // maps of parts of the group
   State in[CT];                                 // the state before this run
-  unsigned slot;
+  unsigned slot[2];                             // tickets drawn ahead
+  uint64_t bar;                                 // the staged operands' arrival
+  // the thread that issues the copies: neither a teller nor, where there are others, a `beside`
+  static constexpr int ISSUER = R > 2 ? CT : 0;
+
+  GFN_DEV void init() {
+    if (threadIdx.x == 0) {
+      mbar_init(&bar, 1);
+      fence_mbar_init();
+    }
+    __syncthreads();
+  }
 };
 
 // The state that `chunk` (counted in the direction of the scan) of a column
@@ -155,10 +170,13 @@ struct ScanShared {
 // direction of the scan (REV: from the last warp), and sh.in the states.
 // R threads serve a column: the last of them chains the warps' maps and
 // publishes, all of them fetch their share of the group's earlier maps.
-// `words` is the tile's [nchunks][WORDS][CT]; first(c) the state before chunk 0.
-template <class Map, class State, int CT, int NW, bool REV, class First>
+// `words` is the tile's [nchunks][WORDS][CT]; first(c) the state before chunk 0;
+// beside(c) runs on another thread per column, between the barriers, and ahead()
+// on all threads once this block's map is out.
+template <class Map, class State, int CT, int NW, bool REV, class First, class Beside, class Ahead>
 GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* words, int chunk, int nchunks,
-                     int live, First first) {
+                     int live, First first, Beside beside, Ahead ahead) {
+  static_assert(ScanShared<Map, State, CT, NW>::R >= 2, "a second thread per column");
   constexpr int W = Map::WORDS, R = NW * 32 / CT, GS = SCAN_GROUP / R;
   constexpr int BATCH = GS < 8 ? GS : 8;
   const int c = threadIdx.x % CT, r = threadIdx.x / CT;
@@ -183,6 +201,8 @@ GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* wor
     }
     if (tells && pos < SCAN_GROUP - 1) publish(own, mine, CT);
   }
+  ahead();
+  if (r == 0) beside(c);
   Map acc = Map::identity();  // of the group's runs before this one
   if (pos > 0) {
     if (active && r * GS < pos) {
@@ -224,47 +244,73 @@ GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* wor
 }
 
 // ------------------------------------------------------------ vector accesses
+// VEC neighbouring elements as they lie in memory, in whole registers: 16-bit
+// pairs stay packed until a value is used.
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-  T v[VEC];
+struct Pack {
+  static constexpr int BYTES = sizeof(T) * VEC, N = (BYTES + 3) / 4;
+  unsigned u[N];
+
+  GFN_DEV float get(int v) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u[v]);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      return __uint_as_float((v & 1) ? u[v >> 1] & 0xffff0000u : u[v >> 1] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)((v & 1) ? u[v >> 1] >> 16 : u[v >> 1] & 0xffffu)));
+  }
+  GFN_DEV static Pack of(const float (&f)[VEC]) {
+    Pack r;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) r.u[v] = __float_as_uint(f[v]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const T lo = from_f<T>(f[2 * i]), hi = from_f<T>(2 * i + 1 < VEC ? f[2 * i + 1] : 0.f);
+        r.u[i] = (unsigned)bits16(lo) | ((unsigned)bits16(hi) << 16);
+      }
+    }
+    return r;
+  }
+  GFN_DEV static Pack fill(float v) {
+    float f[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = v;
+    return of(f);
+  }
+  GFN_DEV static Pack load(const T* p) {  // read once: evict first
+    Pack r;
+    if constexpr (N == 1) r.u[0] = __ldcs(reinterpret_cast<const unsigned*>(p));
+    else {
+      const uint2 x = __ldcs(reinterpret_cast<const uint2*>(p));
+      r.u[0] = x.x;
+      r.u[1] = x.y;
+    }
+    return r;
+  }
+  GFN_DEV void store(T* p) const {
+    if constexpr (N == 1) __stcs(reinterpret_cast<unsigned*>(p), u[0]);
+    else __stcs(reinterpret_cast<uint2*>(p), make_uint2(u[0], u[1]));
+  }
+  GFN_DEV static unsigned short bits16(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+  GFN_DEV static unsigned short bits16(__half x) { return __half_as_ushort(x); }
 };
 
-template <typename T, int VEC>
-GFN_DEV Pack<T, VEC> load_pack(const T* p) {  // read once: evict first
-  Pack<T, VEC> r;
-  constexpr int B = sizeof(T) * VEC;
-  if constexpr (B == 2) *reinterpret_cast<unsigned short*>(&r) = __ldcs(reinterpret_cast<const unsigned short*>(p));
-  else if constexpr (B == 4) *reinterpret_cast<unsigned*>(&r) = __ldcs(reinterpret_cast<const unsigned*>(p));
-  else if constexpr (B == 8) *reinterpret_cast<uint2*>(&r) = __ldcs(reinterpret_cast<const uint2*>(p));
-  else *reinterpret_cast<uint4*>(&r) = __ldcs(reinterpret_cast<const uint4*>(p));
-  return r;
-}
-template <typename T, int VEC>
-GFN_DEV void store_pack(T* p, const Pack<T, VEC>& r) {
-  constexpr int B = sizeof(T) * VEC;
-  if constexpr (B == 2) __stcs(reinterpret_cast<unsigned short*>(p), *reinterpret_cast<const unsigned short*>(&r));
-  else if constexpr (B == 4) __stcs(reinterpret_cast<unsigned*>(p), *reinterpret_cast<const unsigned*>(&r));
-  else if constexpr (B == 8) __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<const uint2*>(&r));
-  else __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&r));
-}
-
-// Which run of steps and which columns a block computes.  Runs are handed out
-// by a ticket in the direction of the scan, all column tiles of one run before
-// the next: the blocks that a block waits for have started, so its wait ends.
+// Which run of steps and which columns a block computes.  Runs are numbered in
+// the direction of the scan, all column tiles of one run before the next, and
+// handed out by a ticket: whatever a block waits for has a lower number, and
+// the lowest unfinished number is always being computed, so every wait ends.
+// A block draws its ticket one run ahead.
 struct ScanTile {
   int chunk, b, c0, col;  // c0: the tile's first column; col: this lane's first
+  int t0, rows, n;        // this warp's first step and how many it has; n: this lane's (0 beyond the columns)
+  int width;              // columns from this lane's first one on
+  int first, steps;       // the run's first step and how many it has
   bool active;
   long long tile;
 };
 
-template <int VEC, class Args>
-GFN_DEV ScanTile scan_tile(const Args& p, unsigned* slot) {
-  unsigned t = blockIdx.x;
-  if (p.words) {
-    if (threadIdx.x == 0) *slot = atomicAdd(p.ticket, 1u) + 1u;  // starts at all ones, like the words
-    __syncthreads();
-    t = *slot;
-  }
+template <int VEC, int S, int NW, bool REV, class Args>
+GFN_DEV ScanTile scan_tile(const Args& p, unsigned t) {
   ScanTile r;
   const unsigned tiles = (unsigned)p.B * p.ctiles;
   r.chunk = t / tiles;
@@ -272,17 +318,172 @@ GFN_DEV ScanTile scan_tile(const Args& p, unsigned* slot) {
   r.b = (int)(r.tile / p.ctiles);
   r.c0 = (int)(r.tile - (long long)r.b * p.ctiles) * (32 * VEC);
   r.col = r.c0 + (threadIdx.x & 31) * VEC;
-  r.active = r.col < p.D;
+  r.width = p.D - r.col;
+  r.active = r.width > 0;
+  r.first = (REV ? p.nchunks - 1 - r.chunk : r.chunk) * (NW * S);
+  r.steps = min(NW * S, p.L - r.first);
+  r.t0 = r.first + (threadIdx.x >> 5) * S;
+  r.rows = max(0, min(S, p.L - r.t0));
+  r.n = r.active ? r.rows : 0;
   return r;
 }
 
-// ------------------------------------------------------------------ gated scan
-template <typename T, int VEC>
-GFN_DEV Pack<T, VEC> fill_pack(float v) {
-  Pack<T, VEC> r;
+struct ScanTurn {
+  unsigned cur, next, drawn, total;
+
+  template <class Args>
+  GFN_DEV ScanTurn(const Args& p, unsigned (&slot)[2]) {
+    total = (unsigned)p.B * p.ctiles * (unsigned)p.nchunks;
+    cur = blockIdx.x;
+    if (p.words) {
+      if (threadIdx.x == 0) slot[1] = atomicAdd(p.ticket, 1u) + 1u;  // starts at all ones, like the words
+      __syncthreads();
+      cur = slot[1];
+    }
+  }
+  // Drawn once this run's operands have arrived, so that every block that
+  // runs has drawn its first before any draws its second.
+  template <class Args>
+  GFN_DEV void draw(const Args& p) {
+    if (p.words && threadIdx.x == 0) drawn = atomicAdd(p.ticket, 1u) + 1u;
+  }
+  template <class Args>
+  GFN_DEV void tell(const Args& p, unsigned (&slot)[2], int it) const {
+    if (p.words && threadIdx.x == 0) slot[it & 1] = drawn;
+  }
+  // after a barrier that follows tell()
+  template <class Args>
+  GFN_DEV void hear(const Args& p, const unsigned (&slot)[2], int it) {
+    next = p.words ? slot[it & 1] : cur + gridDim.x;
+  }
+};
+
+// -------------------------------------------------------------------- operands
+// How a run's operands reach the registers:
+//   TMA     rows that start on 16 bytes: one thread issues a tensor copy per
+//           operand for the NEXT run as soon as this run's values are in
+//           registers, so the memory stays busy through the exchange of maps;
+//   PLAIN   any other rows: loads when the run begins;
+//   SPLIT   PLAIN for 16-bit pairs of rows that need not start on a pair: a lane
+//           loads the aligned word that holds its first element, the last lane
+//           the word behind it too, and a pair that straddles two words takes
+//           its second half from the next lane's.  Tiles at the very ends of an
+//           operand, where such a word could reach past it, are read element
+//           by element.
+enum { SCAN_TMA, SCAN_PLAIN, SCAN_SPLIT };
+
+// S rows of this lane, `step` elements apart, of which n exist; `width` columns
+// from the lane's first one on (any value where there is no element).
+template <int MODE, typename T, int VEC, int S>
+GFN_DEV void load_rows(Pack<T, VEC> (&out)[S], const T* src, long long step, int n, int rows, int width, bool ends) {
+  if constexpr (MODE == SCAN_SPLIT) {
+    const int lane = threadIdx.x & 31;
+    unsigned behind[S];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) r.v[i] = from_f<T>(v);
-  return r;
+    for (int s = 0; s < S; ++s) {
+      out[s].u[0] = behind[s] = 0;
+      if (s < n) {
+        const T* row = src + s * step;
+        if (ends) {
+          out[s].u[0] = *reinterpret_cast<const unsigned short*>(row);
+          if (width > 1) out[s].u[0] |= (unsigned)*reinterpret_cast<const unsigned short*>(row + 1) << 16;
+        } else {
+          const unsigned* word = reinterpret_cast<const unsigned*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)3);
+          out[s].u[0] = __ldcs(word);
+          if ((reinterpret_cast<uintptr_t>(row) & 2) && (width == 2 || (lane == 31 && width > 1)))
+            behind[s] = __ldcs(word + 1);
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (s < rows) {
+        const unsigned next = __shfl_down_sync(0xffffffffu, out[s].u[0], 1);
+        if (!ends && (reinterpret_cast<uintptr_t>(src + s * step) & 2))
+          out[s].u[0] = (out[s].u[0] >> 16) | ((width == 2 || lane == 31 ? behind[s] : next) << 16);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      if (s < n) out[s] = Pack<T, VEC>::load(src + s * step);
+    }
+  }
+}
+
+// The operands as [batch][step][column] tensors with boxes of one run's steps
+// of one column tile.
+struct ScanMaps {
+  CUtensorMap m[3];
+};
+
+// Shared memory for one run's rows, [operand][NW * S][32 VEC], and the barrier
+// on which they arrive.
+template <typename T, int VEC, int S, int NW>
+struct Stage {
+  static constexpr int ROW = 32 * VEC * sizeof(T), OPERAND = NW * S * ROW;  // bytes
+  char* base;
+  uint64_t* bar;
+
+  GFN_DEV void expect(int operands) const { mbar_arrive_expect_tx(bar, (uint32_t)(operands * OPERAND)); }
+  GFN_DEV void fetch(int operand, const CUtensorMap* map, int col, const ScanTile& q) const {
+    umma::tma_load_3d(base + operand * OPERAND, map, bar, col, q.first, q.b);
+  }
+  GFN_DEV Pack<T, VEC> take(int operand, int s) const {
+    Pack<T, VEC> r;
+    const char* from = base + operand * OPERAND + ((threadIdx.x >> 5) * S + s) * ROW + (threadIdx.x & 31) * r.BYTES;
+    if constexpr (r.N == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(from);
+      r.u[0] = x.x;
+      r.u[1] = x.y;
+    } else {
+      r.u[0] = *reinterpret_cast<const unsigned*>(from);
+    }
+    return r;
+  }
+};
+
+// One row of results: whole packs, or (SPLIT) aligned words across lanes.  The
+// whole warp calls; `width`: columns from the lane's first one on.
+template <int MODE, typename T, int VEC>
+GFN_DEV void store_row(T* dst, const Pack<T, VEC>& v, int width) {
+  if constexpr (MODE == SCAN_SPLIT) {
+    unsigned short* e = reinterpret_cast<unsigned short*>(dst);
+    const unsigned next = __shfl_down_sync(0xffffffffu, v.u[0], 1);
+    const int lane = threadIdx.x & 31;
+    if (reinterpret_cast<uintptr_t>(dst) & 2) {
+      if (lane == 0 && width > 0) e[0] = (unsigned short)v.u[0];
+      if (width > 2 && lane < 31) __stcs(reinterpret_cast<unsigned*>(e + 1), (v.u[0] >> 16) | (next << 16));
+      else if (width > 1) e[1] = (unsigned short)(v.u[0] >> 16);
+    } else {
+      if (width > 1) __stcs(reinterpret_cast<unsigned*>(e), v.u[0]);
+      else if (width > 0) e[0] = (unsigned short)v.u[0];
+    }
+  } else {
+    if (width > 0) v.store(dst);
+  }
+}
+// Keeps packed values packed: without it the compiler carries the unpacked
+// floats of the first pass over to the second, in twice the registers.
+template <typename T, int VEC, int S>
+GFN_DEV void keep_packed(Pack<T, VEC> (&a)[S]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int i = 0; i < Pack<T, VEC>::N; ++i) asm volatile("" : "+r"(a[s].u[i]));
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gated scan
+// Whether a tile may hold an operand's first or last element in memory; with
+// broadcast rows (a stride of zero) any row may.
+template <int VEC, int S>
+GFN_DEV bool holds_ends(const GScanArgs& p, const ScanTile& q) {
+  const bool left = q.c0 == 0, right = q.c0 + 32 * VEC >= p.D;
+  if (p.broadcast) return left || right;
+  return (left && q.b == 0 && q.t0 == 0) || (right && q.b == p.B - 1 && q.t0 + S >= p.L);
 }
 
 // Map of S steps from a zero state; steps beyond the end hold a = 1, x = 0.
@@ -291,155 +492,225 @@ GFN_DEV GatedMap run_map(const Pack<T, VEC> (&a)[S], const Pack<T, VEC> (&x)[S],
   GatedMap m = GatedMap::identity();
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    const float g = to_f(a[s].v[v]);
+    const float g = a[s].get(v);
     m.P *= g;
-    m.p = fmaf(g, m.p, to_f(x[s].v[v]));
+    m.p = fmaf(g, m.p, x[s].get(v));
   }
   if (m.P == 0.f) {  // a zero gate, or an underflow?
     bool zero = false;
 #pragma unroll
-    for (int s = 0; s < S; ++s) zero = zero || to_f(a[s].v[v]) == 0.f;
+    for (int s = 0; s < S; ++s) zero = zero || a[s].get(v) == 0.f;
     if (!zero) m.P = copysignf(1.4e-45f, m.P);
   }
   return m;
 }
 
-template <typename T, int VEC, int S, int NW, int OCC>
-__global__ void __launch_bounds__(NW * 32, OCC) gscan_forward_kernel(const GScanArgs p) {
+template <int MODE, typename T, int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) gscan_forward_kernel(const GScanArgs p, const __grid_constant__ ScanMaps maps) {
   constexpr int CT = 32 * VEC;
+  extern __shared__ __align__(128) unsigned staged[];
   __shared__ ScanShared<GatedMap, GatedState, CT, NW> sh;
-  const ScanTile q = scan_tile<VEC>(p, &sh.slot);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t0 = (q.chunk * NW + w) * S;
-  const int n = q.active ? max(0, min(S, p.L - t0)) : 0;
-  Pack<T, VEC> a[S], x[S];
-  const T* xp = static_cast<const T*>(p.x) + q.b * p.x_sb + t0 * p.x_st + q.col;
-  const T* ap = static_cast<const T*>(p.a) + q.b * p.a_sb + t0 * p.a_st + q.col;
+  const Stage<T, VEC, S, NW> stage = {reinterpret_cast<char*>(staged), &sh.bar};
+  auto row = [](const void* base, const ScanTile& q, long long sb, long long st, int t, int col) {
+    return static_cast<const T*>(base) + q.b * sb + t * st + col;
+  };
+  auto fetch = [&](unsigned turn) {
+    if (MODE != SCAN_TMA || threadIdx.x != sh.ISSUER) return;
+    const ScanTile q = scan_tile<VEC, S, NW, false>(p, turn);
+    stage.expect(1 + (p.a != nullptr));
+    stage.fetch(0, &maps.m[0], q.c0, q);
+    if (p.a) stage.fetch(1, &maps.m[1], q.c0, q);
+  };
+  if constexpr (MODE == SCAN_TMA) sh.init();
+  ScanTurn turn(p, sh.slot);
+  if (turn.cur < turn.total) fetch(turn.cur);
+  for (int it = 0; turn.cur < turn.total; turn.cur = turn.next, ++it) {
+    const ScanTile q = scan_tile<VEC, S, NW, false>(p, turn.cur);
+    Pack<T, VEC> a[S], x[S];
+    if constexpr (MODE == SCAN_TMA) {
+      mbar_wait(&sh.bar, it & 1);
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    x[s] = fill_pack<T, VEC>(0.f);
-    a[s] = fill_pack<T, VEC>(1.f);
-    if (s < n) {
-      x[s] = load_pack<T, VEC>(xp + s * p.x_st);
-      if (p.a) a[s] = load_pack<T, VEC>(ap + s * p.a_st);
+      for (int s = 0; s < S; ++s) {
+        x[s] = stage.take(0, s);
+        a[s] = stage.take(1, s);
+      }
+    } else {
+      const bool ends = holds_ends<VEC, S>(p, q);
+      load_rows<MODE, T, VEC, S>(x, row(p.x, q, p.x_sb, p.x_st, q.t0, q.col), p.x_st, q.n, q.rows, q.width, ends);
+      if (p.a) load_rows<MODE, T, VEC, S>(a, row(p.a, q, p.a_sb, p.a_st, q.t0, q.col), p.a_st, q.n, q.rows, q.width, ends);
     }
-  }
+    turn.draw(p);
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    unsigned long long wd[1];
-    run_map<T, VEC, S>(a, x, v).pack(wd);
-    sh.maps[w][0][lane * VEC + v] = wd[0];
-  }
-  receive<GatedMap, GatedState, CT, NW, false>(
-      sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
-      [&](int c) { return GatedState{p.h0 ? p.h0[(long long)q.b * p.D + q.c0 + c] : 0.f}; });
-  if (n <= 0) return;
-  float h[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    h[v] = sh.in[lane * VEC + v].through(GatedMap::unpack({sh.maps[w][0][lane * VEC + v]})).h;
-  if (p.states && t0 % SCAN_CK == 0) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) p.states[((long long)q.b * p.nck + t0 / SCAN_CK) * p.D + q.col + v] = h[v];
-  }
-  T* hp = static_cast<T*>(p.h) + ((long long)q.b * p.L + t0) * p.D + q.col;
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    Pack<T, VEC> o;
+    for (int s = 0; s < S; ++s) {
+      if (s >= q.n) x[s] = Pack<T, VEC>::fill(0.f);
+      if (s >= q.n || !p.a) a[s] = Pack<T, VEC>::fill(1.f);
+    }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      h[v] = fmaf(to_f(a[s].v[v]), h[v], to_f(x[s].v[v]));
-      o.v[v] = from_f<T>(h[v]);
+      unsigned long long wd[1];
+      run_map<T, VEC, S>(a, x, v).pack(wd);
+      sh.maps[w][0][lane * VEC + v] = wd[0];
     }
-    if (s < n) store_pack<T, VEC>(hp + (long long)s * p.D, o);
-  }
-  if (p.h_last && t0 + n == p.L) {
+    turn.tell(p, sh.slot, it);
+    receive<GatedMap, GatedState, CT, NW, false>(
+        sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
+        [&](int c) { return GatedState{p.h0 ? p.h0[(long long)q.b * p.D + q.c0 + c] : 0.f}; },
+        [](int) {},
+        [&] {
+          turn.hear(p, sh.slot, it);
+          if (turn.next < turn.total) fetch(turn.next);
+        });
+    if (q.rows <= 0) continue;
+    keep_packed(a);
+    keep_packed(x);
+    float h[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) p.h_last[(long long)q.b * p.D + q.col + v] = h[v];
+    for (int v = 0; v < VEC; ++v)
+      h[v] = sh.in[lane * VEC + v].through(GatedMap::unpack({sh.maps[w][0][lane * VEC + v]})).h;
+    if (p.states && q.t0 % SCAN_CK == 0) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v)
+        if (v < q.width) p.states[((long long)q.b * p.nck + q.t0 / SCAN_CK) * p.D + q.col + v] = h[v];
+    }
+    T* hp = static_cast<T*>(p.h) + ((long long)q.b * p.L + q.t0) * p.D + q.col;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) h[v] = fmaf(a[s].get(v), h[v], x[s].get(v));
+      if (s < q.rows) store_row<MODE, T, VEC>(hp + (long long)s * p.D, Pack<T, VEC>::of(h), q.width);
+    }
+    if (p.h_last && q.t0 + q.rows == p.L) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v)
+        if (v < q.width) p.h_last[(long long)q.b * p.D + q.col + v] = h[v];
+    }
+  }
+}
+
+// h before each warp's steps, from the state kept before the run and the
+// warps' maps: column c, one thread.
+template <int CT, int NW>
+GFN_DEV void chain_states(const unsigned long long (*maps)[CT], const float* kept, int c, int live,
+                          float (*start)[CT]) {
+  if (c >= live) return;
+  float h = kept[c];
+#pragma unroll
+  for (int j = 0; j < NW; ++j) {
+    start[j][c] = h;
+    const GatedMap f = GatedMap::unpack({maps[j][c]});
+    h = pass(f.P, h, f.p);
   }
 }
 
 // Runs of NW * S = SCAN_CK steps from the last to the first: the state kept
 // before the run gives h, the messages pass from run to run as the states do
 // in the forward.
-template <typename T, int VEC, int S, int NW, int OCC>
-__global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GScanArgs p) {
+template <int MODE, typename T, int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GScanArgs p, const __grid_constant__ ScanMaps maps) {
   static_assert(NW * S == SCAN_CK, "one kept state per run");
   constexpr int CT = 32 * VEC;
+  extern __shared__ __align__(128) unsigned staged[];
   __shared__ ScanShared<GatedMap, GatedState, CT, NW> sh;
   __shared__ unsigned long long fmaps[NW][CT];
-  const ScanTile q = scan_tile<VEC>(p, &sh.slot);
+  __shared__ float hstart[NW][CT];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int run = p.nchunks - 1 - q.chunk;
-  const int t0 = run * SCAN_CK + w * S;
-  const int n = q.active ? max(0, min(S, p.L - t0)) : 0;
-  Pack<T, VEC> a[S], x[S], g[S];
-  const T* xp = static_cast<const T*>(p.x) + q.b * p.x_sb + t0 * p.x_st + q.col;
-  const T* ap = static_cast<const T*>(p.a) + q.b * p.a_sb + t0 * p.a_st + q.col;
-  const T* gp = static_cast<const T*>(p.dh) + q.b * p.g_sb + t0 * p.g_st + q.col;
+  const Stage<T, VEC, S, NW> stage = {reinterpret_cast<char*>(staged), &sh.bar};
+  auto row = [](const void* base, const ScanTile& q, long long sb, long long st, int t, int col) {
+    return static_cast<const T*>(base) + q.b * sb + t * st + col;
+  };
+  auto fetch = [&](unsigned turn) {
+    if (MODE != SCAN_TMA || threadIdx.x != sh.ISSUER) return;
+    const ScanTile q = scan_tile<VEC, S, NW, true>(p, turn);
+    stage.expect(1 + (p.a != nullptr) + (p.dh != nullptr));
+    stage.fetch(0, &maps.m[0], q.c0, q);
+    if (p.a) stage.fetch(1, &maps.m[1], q.c0, q);
+    if (p.dh) stage.fetch(2, &maps.m[2], q.c0, q);
+  };
+  if constexpr (MODE == SCAN_TMA) sh.init();
+  ScanTurn turn(p, sh.slot);
+  if (turn.cur < turn.total) fetch(turn.cur);
+  for (int it = 0; turn.cur < turn.total; turn.cur = turn.next, ++it) {
+    const ScanTile q = scan_tile<VEC, S, NW, true>(p, turn.cur);
+    Pack<T, VEC> a[S], x[S], g[S];
+    if constexpr (MODE == SCAN_TMA) {
+      mbar_wait(&sh.bar, it & 1);
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    x[s] = g[s] = fill_pack<T, VEC>(0.f);
-    a[s] = fill_pack<T, VEC>(1.f);
-    if (s < n) {
-      x[s] = load_pack<T, VEC>(xp + s * p.x_st);
-      if (p.a) a[s] = load_pack<T, VEC>(ap + s * p.a_st);
-      if (p.dh) g[s] = load_pack<T, VEC>(gp + s * p.g_st);
+      for (int s = 0; s < S; ++s) {
+        x[s] = stage.take(0, s);
+        a[s] = stage.take(1, s);
+        g[s] = stage.take(2, s);
+      }
+    } else {
+      const bool ends = holds_ends<VEC, S>(p, q);
+      load_rows<MODE, T, VEC, S>(x, row(p.x, q, p.x_sb, p.x_st, q.t0, q.col), p.x_st, q.n, q.rows, q.width, ends);
+      if (p.a) load_rows<MODE, T, VEC, S>(a, row(p.a, q, p.a_sb, p.a_st, q.t0, q.col), p.a_st, q.n, q.rows, q.width, ends);
+      if (p.dh) load_rows<MODE, T, VEC, S>(g, row(p.dh, q, p.g_sb, p.g_st, q.t0, q.col), p.g_st, q.n, q.rows, q.width, ends);
     }
-  }
-  float h[VEC];  // before the run
-#pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    h[v] = q.active ? p.states[((long long)q.b * p.nck + run) * p.D + q.col + v] : 0.f;
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    unsigned long long wd[1];
-    const GatedMap mf = run_map<T, VEC, S>(a, x, v);
-    mf.pack(wd);
-    fmaps[w][lane * VEC + v] = wd[0];
-    GatedMap mb = {mf.P, 0.f};  // of the message, last step first
-#pragma unroll
-    for (int s = S - 1; s >= 0; --s) mb.p = to_f(a[s].v[v]) * (to_f(g[s].v[v]) + mb.p);
-    mb.pack(wd);
-    sh.maps[w][0][lane * VEC + v] = wd[0];
-  }
-  receive<GatedMap, GatedState, CT, NW, true>(
-      sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
-      [&](int c) { return GatedState{p.dlast ? p.dlast[(long long)q.b * p.D + q.c0 + c] : 0.f}; });
-  if (!q.active) return;
-  float m[VEC], hp[S][VEC];  // hp: h_{t-1}
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    m[v] = sh.in[lane * VEC + v].through(GatedMap::unpack({sh.maps[w][0][lane * VEC + v]})).h;
-    for (int j = 0; j < w; ++j) {
-      const GatedMap f = GatedMap::unpack({fmaps[j][lane * VEC + v]});
-      h[v] = pass(f.P, h[v], f.p);
-    }
+    turn.draw(p);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      hp[s][v] = h[v];
-      h[v] = fmaf(to_f(a[s].v[v]), h[v], to_f(x[s].v[v]));
+      if (s >= q.n) x[s] = Pack<T, VEC>::fill(0.f);
+      if (s >= q.n || !p.a) a[s] = Pack<T, VEC>::fill(1.f);
+      if (s >= q.n || !p.dh) g[s] = Pack<T, VEC>::fill(0.f);
     }
-  }
-  const long long o = ((long long)q.b * p.L + t0) * p.D + q.col;
-#pragma unroll
-  for (int s = S - 1; s >= 0; --s) {
-    Pack<T, VEC> oa, ox;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      const float gt = to_f(g[s].v[v]) + m[v];
-      ox.v[v] = from_f<T>(gt);
-      oa.v[v] = from_f<T>(gt * hp[s][v]);
-      m[v] = to_f(a[s].v[v]) * gt;
-    }
-    if (s < n) {
-      if (p.dx) store_pack<T, VEC>(static_cast<T*>(p.dx) + o + (long long)s * p.D, ox);
-      if (p.da) store_pack<T, VEC>(static_cast<T*>(p.da) + o + (long long)s * p.D, oa);
-    }
-  }
-  if (p.dh0 && run == 0 && w == 0) {
+      unsigned long long wd[1];
+      const GatedMap mf = run_map<T, VEC, S>(a, x, v);
+      mf.pack(wd);
+      fmaps[w][lane * VEC + v] = wd[0];
+      GatedMap mb = {mf.P, 0.f};  // of the message, last step first
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) p.dh0[(long long)q.b * p.D + q.col + v] = m[v];
+      for (int s = S - 1; s >= 0; --s) mb.p = a[s].get(v) * (g[s].get(v) + mb.p);
+      mb.pack(wd);
+      sh.maps[w][0][lane * VEC + v] = wd[0];
+    }
+    turn.tell(p, sh.slot, it);
+    const int run = p.nchunks - 1 - q.chunk;
+    receive<GatedMap, GatedState, CT, NW, true>(
+        sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
+        [&](int c) { return GatedState{p.dlast ? p.dlast[(long long)q.b * p.D + q.c0 + c] : 0.f}; },
+        [&](int c) {
+          chain_states<CT, NW>(fmaps, p.states + ((long long)q.b * p.nck + run) * p.D + q.c0, c, p.D - q.c0, hstart);
+        },
+        [&] {
+          turn.hear(p, sh.slot, it);
+          if (turn.next < turn.total) fetch(turn.next);
+        });
+    if (q.rows <= 0) continue;
+    keep_packed(a);
+    keep_packed(x);
+    keep_packed(g);
+    float m[VEC], hp[S][VEC];  // hp: h_{t-1}
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      m[v] = sh.in[lane * VEC + v].through(GatedMap::unpack({sh.maps[w][0][lane * VEC + v]})).h;
+      hp[0][v] = hstart[w][lane * VEC + v];
+#pragma unroll
+      for (int s = 1; s < S; ++s) hp[s][v] = fmaf(a[s - 1].get(v), hp[s - 1][v], x[s - 1].get(v));
+    }
+    const long long o = ((long long)q.b * p.L + q.t0) * p.D + q.col;
+#pragma unroll
+    for (int s = S - 1; s >= 0; --s) {
+      float oa[VEC], ox[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        ox[v] = g[s].get(v) + m[v];
+        oa[v] = ox[v] * hp[s][v];
+        m[v] = a[s].get(v) * ox[v];
+      }
+      if (s < q.rows) {
+        const long long e = o + (long long)s * p.D;
+        if (p.dx) store_row<MODE, T, VEC>(static_cast<T*>(p.dx) + e, Pack<T, VEC>::of(ox), q.width);
+        if (p.da) store_row<MODE, T, VEC>(static_cast<T*>(p.da) + e, Pack<T, VEC>::of(oa), q.width);
+      }
+    }
+    if (p.dh0 && run == 0 && w == 0) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v)
+        if (v < q.width) p.dh0[(long long)q.b * p.D + q.col + v] = m[v];
+    }
   }
 }
 
@@ -554,87 +825,119 @@ struct LayerState {
   GFN_DEV LayerState through(LayerMap m) const { return {pass(m.P, v, m.p), x + pass(m.Q, v, m.q)}; }
 };
 
-template <int VEC, int S, int NW, int OCC>
-__global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScanArgs p) {
+template <int MODE, int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScanArgs p, const __grid_constant__ ScanMaps maps) {
   constexpr int CT = 32 * VEC;
+  extern __shared__ __align__(128) unsigned staged[];
   __shared__ ScanShared<LayerMap, LayerState, CT, NW> sh;
-  const ScanTile c = scan_tile<VEC>(p, &sh.slot);
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t0 = (c.chunk * NW + w) * S;
-  const int n = c.active ? max(0, min(S, p.L - t0)) : 0;
-  const float* zp = p.z + ((long long)c.b * p.L + t0) * 3 * p.D + c.col;
-  Pack<float, VEC> A[S], dt[S], bv[S];
+  const Stage<float, VEC, S, NW> stage = {reinterpret_cast<char*>(staged), &sh.bar};
+  auto fetch = [&](unsigned turn) {
+    if (MODE != SCAN_TMA || threadIdx.x != sh.ISSUER) return;
+    const ScanTile c = scan_tile<VEC, S, NW, false>(p, turn);
+    stage.expect(3);
 #pragma unroll
-  for (int s = 0; s < S; ++s) {  // beyond the end: A = 1, dt = 0, zB = 0
-    A[s] = fill_pack<float, VEC>(INFINITY);
-    dt[s] = fill_pack<float, VEC>(-INFINITY);
-    bv[s] = fill_pack<float, VEC>(0.f);
-    if (s < n) {
-      A[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D);
-      dt[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + p.D);
-      bv[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + 2LL * p.D);
+    for (int k = 0; k < 3; ++k) stage.fetch(k, &maps.m[0], k * p.D + c.c0, c);
+  };
+  if constexpr (MODE == SCAN_TMA) sh.init();
+  ScanTurn turn(p, sh.slot);
+  if (turn.cur < turn.total) fetch(turn.cur);
+  for (int it = 0; turn.cur < turn.total; turn.cur = turn.next, ++it) {
+    const ScanTile c = scan_tile<VEC, S, NW, false>(p, turn.cur);
+    Pack<float, VEC> pa[S], pd[S], pb[S];
+    if constexpr (MODE == SCAN_TMA) {
+      mbar_wait(&sh.bar, it & 1);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        pa[s] = stage.take(0, s);
+        pd[s] = stage.take(1, s);
+        pb[s] = stage.take(2, s);
+      }
+    } else {
+      const float* zp = p.z + ((long long)c.b * p.L + c.t0) * 3 * p.D + c.col;
+      load_rows<MODE, float, VEC, S>(pa, zp, 3LL * p.D, c.n, c.rows, c.width, false);
+      load_rows<MODE, float, VEC, S>(pd, zp + p.D, 3LL * p.D, c.n, c.rows, c.width, false);
+      load_rows<MODE, float, VEC, S>(pb, zp + 2LL * p.D, 3LL * p.D, c.n, c.rows, c.width, false);
     }
-  }
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
-    LayerMap m = LayerMap::identity();
-    bool zero = false;
+    turn.draw(p);
+    float A[S][VEC], dt[S][VEC], bv[S][VEC];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      float slope;
-      A[s].v[v] = gate(A[s].v[v], &slope);
-      dt[s].v[v] = soft_step(dt[s].v[v], &slope) * scale;
-      bv[s].v[v] *= dt[s].v[v];
-      zero = zero || A[s].v[v] == 0.f;
-      m.P *= A[s].v[v];
-      m.p = fmaf(A[s].v[v], m.p, bv[s].v[v]);
-      m.Q = fmaf(dt[s].v[v], m.P, m.Q);
-      m.q = fmaf(dt[s].v[v], m.p, m.q);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {  // beyond the end: A = 1, dt = 0
+        const bool on = s < c.n;
+        float slope;
+        A[s][v] = gate(on ? pa[s].get(v) : INFINITY, &slope);
+        dt[s][v] = soft_step(on ? pd[s].get(v) : -INFINITY, &slope);
+        bv[s][v] = on ? pb[s].get(v) : 0.f;
+      }
     }
-    if (m.P == 0.f && !zero) m.P = 1.4e-45f;
-    unsigned long long wd[2];
-    m.pack(wd);
-    sh.maps[w][0][lane * VEC + v] = wd[0];
-    sh.maps[w][1][lane * VEC + v] = wd[1];
-  }
-  receive<LayerMap, LayerState, CT, NW, false>(
-      sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0, [&](int j) {
-        const long long e = (long long)c.b * p.D + c.c0 + j;
-        return LayerState{p.v0 ? p.v0[e] : 0.f, p.x0 ? p.x0[e] : 0.f};
-      });
-  if (n <= 0) return;
-  LayerState st[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    st[v] = sh.in[lane * VEC + v].through(
-        LayerMap::unpack({sh.maps[w][0][lane * VEC + v], sh.maps[w][1][lane * VEC + v]}));
-  if (p.states && t0 % SCAN_CK == 0) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) p.states[((long long)c.b * p.nck + t0 / SCAN_CK) * p.D + c.col + v] = st[v].v;
-  }
-  const long long o = ((long long)c.b * p.L + t0) * p.D + c.col;
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    Pack<float, VEC> ov, ox;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-      st[v].v = fmaf(A[s].v[v], st[v].v, bv[s].v[v]);
-      st[v].x = fmaf(st[v].v, dt[s].v[v], st[v].x);
-      ov.v[v] = st[v].v;
-      ox.v[v] = st[v].x;
-    }
-    if (s < n) {
-      store_pack<float, VEC>(p.vs + o + (long long)s * p.D, ov);
-      store_pack<float, VEC>(p.xs + o + (long long)s * p.D, ox);
-    }
-  }
-  if (t0 + n == p.L) {
+      const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
+      LayerMap m = LayerMap::identity();
+      bool zero = false;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const long long e = (long long)c.b * p.D + c.col + v;
-      if (p.v_last) p.v_last[e] = st[v].v;
-      if (p.x_last) p.x_last[e] = st[v].x;
+      for (int s = 0; s < S; ++s) {
+        dt[s][v] *= scale;
+        bv[s][v] *= dt[s][v];
+        zero = zero || A[s][v] == 0.f;
+        m.P *= A[s][v];
+        m.p = fmaf(A[s][v], m.p, bv[s][v]);
+        m.Q = fmaf(dt[s][v], m.P, m.Q);
+        m.q = fmaf(dt[s][v], m.p, m.q);
+      }
+      if (m.P == 0.f && !zero) m.P = 1.4e-45f;
+      unsigned long long wd[2];
+      m.pack(wd);
+      sh.maps[w][0][lane * VEC + v] = wd[0];
+      sh.maps[w][1][lane * VEC + v] = wd[1];
+    }
+    turn.tell(p, sh.slot, it);
+    receive<LayerMap, LayerState, CT, NW, false>(
+        sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0,
+        [&](int j) {
+          const long long e = (long long)c.b * p.D + c.c0 + j;
+          return LayerState{p.v0 ? p.v0[e] : 0.f, p.x0 ? p.x0[e] : 0.f};
+        },
+        [](int) {},
+        [&] {
+          turn.hear(p, sh.slot, it);
+          if (turn.next < turn.total) fetch(turn.next);
+        });
+    if (c.n <= 0) continue;
+    LayerState st[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      st[v] = sh.in[lane * VEC + v].through(
+          LayerMap::unpack({sh.maps[w][0][lane * VEC + v], sh.maps[w][1][lane * VEC + v]}));
+    if (p.states && c.t0 % SCAN_CK == 0) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) p.states[((long long)c.b * p.nck + c.t0 / SCAN_CK) * p.D + c.col + v] = st[v].v;
+    }
+    const long long o = ((long long)c.b * p.L + c.t0) * p.D + c.col;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float ov[VEC], ox[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        st[v].v = fmaf(A[s][v], st[v].v, bv[s][v]);
+        st[v].x = fmaf(st[v].v, dt[s][v], st[v].x);
+        ov[v] = st[v].v;
+        ox[v] = st[v].x;
+      }
+      if (s < c.n) {
+        Pack<float, VEC>::of(ov).store(p.vs + o + (long long)s * p.D);
+        Pack<float, VEC>::of(ox).store(p.xs + o + (long long)s * p.D);
+      }
+    }
+    if (c.t0 + c.n == p.L) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const long long e = (long long)c.b * p.D + c.col + v;
+        if (p.v_last) p.v_last[e] = st[v].v;
+        if (p.x_last) p.x_last[e] = st[v].x;
+      }
     }
   }
 }
@@ -662,112 +965,146 @@ struct LayerBackState {
   GFN_DEV LayerBackState through(LayerBackMap f) const { return {pass(f.P, m, pass(f.R, X, f.q)), X + f.G}; }
 };
 
-template <int VEC, int S, int NW, int OCC>
-__global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LScanArgs p) {
+template <int MODE, int VEC, int S, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LScanArgs p, const __grid_constant__ ScanMaps maps) {
   static_assert(NW * S == SCAN_CK, "one kept state per run");
   constexpr int CT = 32 * VEC;
+  extern __shared__ __align__(128) unsigned staged[];
   __shared__ ScanShared<LayerBackMap, LayerBackState, CT, NW> sh;
   __shared__ unsigned long long fmaps[NW][CT];
-  const ScanTile c = scan_tile<VEC>(p, &sh.slot);
+  __shared__ float vstart[NW][CT];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int run = p.nchunks - 1 - c.chunk;
-  const int t0 = run * SCAN_CK + w * S;
-  const int n = c.active ? max(0, min(S, p.L - t0)) : 0;
-  const long long o = ((long long)c.b * p.L + t0) * p.D + c.col;
-  const float* zp = p.z + 3 * (o - c.col) + c.col;
-  Pack<float, VEC> A[S], dt[S], zb[S], gx[S], gv[S], sa[S], sd[S];  // sa, sd: slopes of A and dt
+  const Stage<float, VEC, S, NW> stage = {reinterpret_cast<char*>(staged), &sh.bar};
+  auto fetch = [&](unsigned turn) {
+    if (MODE != SCAN_TMA || threadIdx.x != sh.ISSUER) return;
+    const ScanTile c = scan_tile<VEC, S, NW, true>(p, turn);
+    stage.expect(3 + (p.gx != nullptr) + (p.gv != nullptr));
 #pragma unroll
-  for (int s = 0; s < S; ++s) {  // beyond the end: A = 1, dt = 0, zB = 0, no gradients
-    A[s] = fill_pack<float, VEC>(INFINITY);
-    dt[s] = fill_pack<float, VEC>(-INFINITY);
-    zb[s] = gx[s] = gv[s] = fill_pack<float, VEC>(0.f);
-    if (s < n) {
-      A[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D);
-      dt[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + p.D);
-      zb[s] = load_pack<float, VEC>(zp + (long long)s * 3 * p.D + 2LL * p.D);
-      if (p.gx) gx[s] = load_pack<float, VEC>(p.gx + o + (long long)s * p.D);
-      if (p.gv) gv[s] = load_pack<float, VEC>(p.gv + o + (long long)s * p.D);
+    for (int k = 0; k < 3; ++k) stage.fetch(k, &maps.m[0], k * p.D + c.c0, c);
+    if (p.gx) stage.fetch(3, &maps.m[1], c.c0, c);
+    if (p.gv) stage.fetch(4, &maps.m[2], c.c0, c);
+  };
+  if constexpr (MODE == SCAN_TMA) sh.init();
+  ScanTurn turn(p, sh.slot);
+  if (turn.cur < turn.total) fetch(turn.cur);
+  for (int it = 0; turn.cur < turn.total; turn.cur = turn.next, ++it) {
+    const ScanTile c = scan_tile<VEC, S, NW, true>(p, turn.cur);
+    Pack<float, VEC> pa[S], pd[S], pb[S], px[S], pv[S];
+    if constexpr (MODE == SCAN_TMA) {
+      mbar_wait(&sh.bar, it & 1);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        pa[s] = stage.take(0, s);
+        pd[s] = stage.take(1, s);
+        pb[s] = stage.take(2, s);
+        px[s] = stage.take(3, s);
+        pv[s] = stage.take(4, s);
+      }
+    } else {
+      const long long o = ((long long)c.b * p.L + c.t0) * p.D + c.col;
+      const float* zp = p.z + 3 * (o - c.col) + c.col;
+      load_rows<MODE, float, VEC, S>(pa, zp, 3LL * p.D, c.n, c.rows, c.width, false);
+      load_rows<MODE, float, VEC, S>(pd, zp + p.D, 3LL * p.D, c.n, c.rows, c.width, false);
+      load_rows<MODE, float, VEC, S>(pb, zp + 2LL * p.D, 3LL * p.D, c.n, c.rows, c.width, false);
+      if (p.gx) load_rows<MODE, float, VEC, S>(px, p.gx + o, p.D, c.n, c.rows, c.width, false);
+      if (p.gv) load_rows<MODE, float, VEC, S>(pv, p.gv + o, p.D, c.n, c.rows, c.width, false);
     }
-  }
-  float h[VEC];  // v before the run
-#pragma unroll
-  for (int v = 0; v < VEC; ++v)
-    h[v] = c.active ? p.states[((long long)c.b * p.nck + run) * p.D + c.col + v] : 0.f;
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
-    GatedMap mf = GatedMap::identity();
-    bool zero = false;
+    turn.draw(p);
+    float A[S][VEC], dt[S][VEC], zb[S][VEC], gx[S][VEC], gv[S][VEC];
+    float sa[S][VEC], sd[S][VEC];  // slopes of A and dt
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      A[s].v[v] = gate(A[s].v[v], &sa[s].v[v]);
-      dt[s].v[v] = soft_step(dt[s].v[v], &sd[s].v[v]) * scale;
-      sd[s].v[v] *= scale;
-      zero = zero || A[s].v[v] == 0.f;
-      mf.P *= A[s].v[v];
-      mf.p = fmaf(A[s].v[v], mf.p, zb[s].v[v] * dt[s].v[v]);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {  // beyond the end: A = 1, dt = 0, no gradients
+        const bool on = s < c.n;
+        A[s][v] = gate(on ? pa[s].get(v) : INFINITY, &sa[s][v]);
+        dt[s][v] = soft_step(on ? pd[s].get(v) : -INFINITY, &sd[s][v]);
+        zb[s][v] = on ? pb[s].get(v) : 0.f;
+        gx[s][v] = on && p.gx ? px[s].get(v) : 0.f;
+        gv[s][v] = on && p.gv ? pv[s].get(v) : 0.f;
+      }
     }
-    if (mf.P == 0.f && !zero) mf.P = 1.4e-45f;
-    LayerBackMap mb = LayerBackMap::identity();
-    mb.P = mf.P;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
+      GatedMap mf = GatedMap::identity();
+      bool zero = false;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        dt[s][v] *= scale;
+        sd[s][v] *= scale;
+        zero = zero || A[s][v] == 0.f;
+        mf.P *= A[s][v];
+        mf.p = fmaf(A[s][v], mf.p, zb[s][v] * dt[s][v]);
+      }
+      if (mf.P == 0.f && !zero) mf.P = 1.4e-45f;
+      LayerBackMap mb = LayerBackMap::identity();
+      mb.P = mf.P;
+#pragma unroll
+      for (int s = S - 1; s >= 0; --s) {
+        mb.G += gx[s][v];
+        mb.q = A[s][v] * (fmaf(dt[s][v], mb.G, gv[s][v]) + mb.q);
+        mb.R = A[s][v] * (mb.R + dt[s][v]);
+      }
+      unsigned long long wd[2], wf[1];
+      mf.pack(wf);
+      fmaps[w][lane * VEC + v] = wf[0];
+      mb.pack(wd);
+      sh.maps[w][0][lane * VEC + v] = wd[0];
+      sh.maps[w][1][lane * VEC + v] = wd[1];
+    }
+    turn.tell(p, sh.slot, it);
+    const int run = p.nchunks - 1 - c.chunk;
+    receive<LayerBackMap, LayerBackState, CT, NW, true>(
+        sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0,
+        [&](int j) {
+          const long long e = (long long)c.b * p.D + c.c0 + j;
+          return LayerBackState{p.gvl ? p.gvl[e] : 0.f, p.gxl ? p.gxl[e] : 0.f};
+        },
+        [&](int j) {
+          chain_states<CT, NW>(fmaps, p.states + ((long long)c.b * p.nck + run) * p.D + c.c0, j, p.D - c.c0, vstart);
+        },
+        [&] {
+          turn.hear(p, sh.slot, it);
+          if (turn.next < turn.total) fetch(turn.next);
+        });
+    if (!c.active) continue;
+    LayerBackState st[VEC];
+    float vs[S + 1][VEC];  // v_{t-1} of this warp's steps, and the last step's v
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      st[v] = sh.in[lane * VEC + v].through(
+          LayerBackMap::unpack({sh.maps[w][0][lane * VEC + v], sh.maps[w][1][lane * VEC + v]}));
+      vs[0][v] = vstart[w][lane * VEC + v];
+#pragma unroll
+      for (int s = 0; s < S; ++s) vs[s + 1][v] = fmaf(A[s][v], vs[s][v], zb[s][v] * dt[s][v]);
+    }
+    float* dz = p.dz + 3 * ((long long)c.b * p.L + c.t0) * p.D + c.col;
 #pragma unroll
     for (int s = S - 1; s >= 0; --s) {
-      mb.G += gx[s].v[v];
-      mb.q = A[s].v[v] * (fmaf(dt[s].v[v], mb.G, gv[s].v[v]) + mb.q);
-      mb.R = A[s].v[v] * (mb.R + dt[s].v[v]);
+      float oa[VEC], od[VEC], ob[VEC];
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        st[v].X += gx[s][v];
+        const float l = fmaf(dt[s][v], st[v].X, gv[s][v]) + st[v].m;
+        oa[v] = l * vs[s][v] * sa[s][v];
+        od[v] = (l * zb[s][v] + st[v].X * vs[s + 1][v]) * sd[s][v];
+        ob[v] = l * dt[s][v];
+        st[v].m = A[s][v] * l;
+      }
+      if (s < c.n) {
+        Pack<float, VEC>::of(oa).store(dz + 3LL * s * p.D);
+        Pack<float, VEC>::of(od).store(dz + (3LL * s + 1) * p.D);
+        Pack<float, VEC>::of(ob).store(dz + (3LL * s + 2) * p.D);
+      }
     }
-    unsigned long long wd[2], wf[1];
-    mf.pack(wf);
-    fmaps[w][lane * VEC + v] = wf[0];
-    mb.pack(wd);
-    sh.maps[w][0][lane * VEC + v] = wd[0];
-    sh.maps[w][1][lane * VEC + v] = wd[1];
-  }
-  receive<LayerBackMap, LayerBackState, CT, NW, true>(
-      sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0, [&](int j) {
-        const long long e = (long long)c.b * p.D + c.c0 + j;
-        return LayerBackState{p.gvl ? p.gvl[e] : 0.f, p.gxl ? p.gxl[e] : 0.f};
-      });
-  if (!c.active) return;
-  LayerBackState st[VEC];
-  float vs[S + 1][VEC];  // v_{t-1} of this warp's steps, and the last step's v
+    if (run == 0 && w == 0) {
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    st[v] = sh.in[lane * VEC + v].through(
-        LayerBackMap::unpack({sh.maps[w][0][lane * VEC + v], sh.maps[w][1][lane * VEC + v]}));
-    for (int j = 0; j < w; ++j) {
-      const GatedMap f = GatedMap::unpack({fmaps[j][lane * VEC + v]});
-      h[v] = pass(f.P, h[v], f.p);
-    }
-    vs[0][v] = h[v];
-#pragma unroll
-    for (int s = 0; s < S; ++s) vs[s + 1][v] = fmaf(A[s].v[v], vs[s][v], zb[s].v[v] * dt[s].v[v]);
-  }
-  float* dz = p.dz + 3 * (o - c.col) + c.col;
-#pragma unroll
-  for (int s = S - 1; s >= 0; --s) {
-    Pack<float, VEC> oa, od, ob;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      st[v].X += gx[s].v[v];
-      const float l = fmaf(dt[s].v[v], st[v].X, gv[s].v[v]) + st[v].m;
-      oa.v[v] = l * vs[s][v] * sa[s].v[v];
-      od.v[v] = (l * zb[s].v[v] + st[v].X * vs[s + 1][v]) * sd[s].v[v];
-      ob.v[v] = l * dt[s].v[v];
-      st[v].m = A[s].v[v] * l;
-    }
-    if (s < n) {
-      store_pack<float, VEC>(dz + (long long)s * 3 * p.D, oa);
-      store_pack<float, VEC>(dz + (long long)s * 3 * p.D + p.D, od);
-      store_pack<float, VEC>(dz + (long long)s * 3 * p.D + 2LL * p.D, ob);
-    }
-  }
-  if (run == 0 && w == 0) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const long long e = (long long)c.b * p.D + c.col + v;
-      if (p.dv0) p.dv0[e] = st[v].m;
-      if (p.dx0) p.dx0[e] = st[v].X;
+      for (int v = 0; v < VEC; ++v) {
+        const long long e = (long long)c.b * p.D + c.col + v;
+        if (p.dv0) p.dv0[e] = st[v].m;
+        if (p.dx0) p.dx0[e] = st[v].X;
+      }
     }
   }
 }
