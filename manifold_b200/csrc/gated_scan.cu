@@ -141,9 +141,9 @@ bool repeats(const void* ptr, long long sb, long long st, int B, int L) {
   return ptr && ((B > 1 && sb == 0) || (L > 1 && st == 0));
 }
 
-template <typename T, int VEC>
+template <typename T>
 int gscan_run(GScanArgs p, bool backward, void* ws, long long bytes, cudaStream_t s) {
-  const int z = sizeof(T);
+  constexpr int z = sizeof(T);
   if (!backward && p.L <= SEQ_STEPS) {
     gscan_forward_seq_kernel<T><<<column_blocks(p.B, p.D), 128, 0, s>>>(p);
     return launch_status("gscan_forward_seq_kernel");
@@ -154,26 +154,26 @@ int gscan_run(GScanArgs p, bool backward, void* ws, long long bytes, cudaStream_
                     rows16(p.x, p.x_sb, p.x_st, p.B, p.L, z) && rows16(p.dh, p.g_sb, p.g_st, p.B, p.L, z) &&
                     aligned16(p.h) && aligned16(p.da) && aligned16(p.dx);
   if (tma)
-    return backward ? gscan_backward<SCAN_TMA, T, VEC, 8, 8, 2>(p, ws, bytes, s)
-                    : gscan_forward<SCAN_TMA, T, VEC, 16, 8, 2>(p, ws, bytes, s);
-  if constexpr (sizeof(T) == 2)
-    return backward ? gscan_backward<SCAN_SPLIT, T, 2, 8, 8, 3>(p, ws, bytes, s)
-                    : gscan_forward<SCAN_SPLIT, T, 2, 16, 8, 3>(p, ws, bytes, s);
+    return backward ? gscan_backward<SCAN_TMA, T, 2, 8, 8, z == 2 ? 4 : 2>(p, ws, bytes, s)
+                    : gscan_forward<SCAN_TMA, T, 2, z == 2 ? 32 : 16, 8, 2>(p, ws, bytes, s);
+  if constexpr (z == 2)
+    return backward ? gscan_backward<SCAN_SPLIT, T, 2, 8, 8, 4>(p, ws, bytes, s)
+                    : gscan_forward<SCAN_SPLIT, T, 2, 16, 8, 4>(p, ws, bytes, s);
   else
     return backward ? gscan_backward<SCAN_PLAIN, T, 1, 8, 8, 4>(p, ws, bytes, s)
                     : gscan_forward<SCAN_PLAIN, T, 1, 16, 8, 4>(p, ws, bytes, s);
 }
 
 int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long long bytes, cudaStream_t s) {
-  if (dtype == GFN_F32) return gscan_run<float, 2>(p, backward, ws, bytes, s);
-  if (dtype == GFN_BF16) return gscan_run<__nv_bfloat16, 4>(p, backward, ws, bytes, s);
-  if (dtype == GFN_F16) return gscan_run<__half, 4>(p, backward, ws, bytes, s);
+  if (dtype == GFN_F32) return gscan_run<float>(p, backward, ws, bytes, s);
+  if (dtype == GFN_BF16) return gscan_run<__nv_bfloat16>(p, backward, ws, bytes, s);
+  if (dtype == GFN_F16) return gscan_run<__half>(p, backward, ws, bytes, s);
   return fail(GFN_ERR_UNSUPPORTED, "gated_scan: element type %d", dtype);
 }
 
-template <int MODE, int VEC>
+template <int MODE>
 int lscan_forward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
-  constexpr int S = 8, NW = 8, OCC = 2;
+  constexpr int VEC = 1, S = 16, NW = 8, OCC = 2;
   unsigned blocks;
   const int st = set_tiles("layer_scan_forward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &blocks);
   if (st) return st;
@@ -286,8 +286,8 @@ int gfn_layer_scan_forward(const float* z, const float* v0, const float* x0, int
     return launch_status("lscan_forward_seq_kernel");
   }
   const bool tma = dim % 4 == 0 && aligned16(z) && aligned16(x_seq) && aligned16(v_seq);
-  return tma ? lscan_forward<SCAN_TMA, 2>(p, workspace, workspace_bytes, s)
-              : lscan_forward<SCAN_PLAIN, 1>(p, workspace, workspace_bytes, s);
+  return tma ? lscan_forward<SCAN_TMA>(p, workspace, workspace_bytes, s)
+              : lscan_forward<SCAN_PLAIN>(p, workspace, workspace_bytes, s);
 }
 
 int gfn_layer_scan_backward(const float* z, const float* states, const float* gx, const float* gv,

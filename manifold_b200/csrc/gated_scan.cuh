@@ -365,11 +365,11 @@ struct ScanTurn {
 //           registers, so the memory stays busy through the exchange of maps;
 //   PLAIN   any other rows: loads when the run begins;
 //   SPLIT   PLAIN for 16-bit pairs of rows that need not start on a pair: a lane
-//           loads the aligned word that holds its first element, the last lane
-//           the word behind it too, and a pair that straddles two words takes
-//           its second half from the next lane's.  Tiles at the very ends of an
-//           operand, where such a word could reach past it, are read element
-//           by element.
+//           loads the aligned word that holds its first element, and a pair
+//           that straddles two words takes its second half from the next
+//           lane's (the tile's last element is loaded by itself).  Tiles at the
+//           very ends of an operand, where such a word could reach past it, are
+//           read element by element.
 enum { SCAN_TMA, SCAN_PLAIN, SCAN_SPLIT };
 
 // S rows of this lane, `step` elements apart, of which n exist; `width` columns
@@ -377,30 +377,34 @@ enum { SCAN_TMA, SCAN_PLAIN, SCAN_SPLIT };
 template <int MODE, typename T, int VEC, int S>
 GFN_DEV void load_rows(Pack<T, VEC> (&out)[S], const T* src, long long step, int n, int rows, int width, bool ends) {
   if constexpr (MODE == SCAN_SPLIT) {
+    static_assert(S <= 32, "lane s fetches row s's last element");
     const int lane = threadIdx.x & 31;
-    unsigned behind[S];
+    const int cols = min(32 * VEC, width + lane * VEC);  // of the tile
+    unsigned last = 0;
+    if (ends) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      out[s].u[0] = behind[s] = 0;
-      if (s < n) {
-        const T* row = src + s * step;
-        if (ends) {
+      for (int s = 0; s < S; ++s) {
+        if (s < n) {
+          const T* row = src + s * step;
           out[s].u[0] = *reinterpret_cast<const unsigned short*>(row);
           if (width > 1) out[s].u[0] |= (unsigned)*reinterpret_cast<const unsigned short*>(row + 1) << 16;
-        } else {
-          const unsigned* word = reinterpret_cast<const unsigned*>(reinterpret_cast<uintptr_t>(row) & ~(uintptr_t)3);
-          out[s].u[0] = __ldcs(word);
-          if ((reinterpret_cast<uintptr_t>(row) & 2) && (width == 2 || (lane == 31 && width > 1)))
-            behind[s] = __ldcs(word + 1);
         }
       }
-    }
+    } else {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < rows) {
+      for (int s = 0; s < S; ++s) {
+        if (s < n)
+          out[s].u[0] = __ldcs(reinterpret_cast<const unsigned*>(
+              reinterpret_cast<uintptr_t>(src + s * step) & ~(uintptr_t)3));
+      }
+      if (lane < rows)
+        last = __ldcs(reinterpret_cast<const unsigned short*>(src + lane * step) + (cols - 1 - lane * VEC));
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
         const unsigned next = __shfl_down_sync(0xffffffffu, out[s].u[0], 1);
-        if (!ends && (reinterpret_cast<uintptr_t>(src + s * step) & 2))
-          out[s].u[0] = (out[s].u[0] >> 16) | ((width == 2 || lane == 31 ? behind[s] : next) << 16);
+        const unsigned edge = __shfl_sync(0xffffffffu, last, s);
+        if (reinterpret_cast<uintptr_t>(src + s * step) & 2)
+          out[s].u[0] = (out[s].u[0] >> 16) | ((width == 2 || lane == 31 ? edge : next) << 16);
       }
     }
   } else {
