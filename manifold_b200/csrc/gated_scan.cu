@@ -48,10 +48,11 @@ int set_tiles(const char* what, Args* p, int run, int ct, int words, void* works
   return cuda_status(cudaMemsetAsync(workspace, 0xff, (size_t)need, s), what);
 }
 
-// Whether every row of an operand starts on 16 bytes, as a tensor copy needs it.
+// Whether every row of an operand starts on 16 bytes and no stride is zero, as
+// a tensor copy needs it.
 bool rows16(const void* ptr, long long sb, long long st, int B, int L, int size) {
-  return !ptr || (aligned16(ptr) && (B == 1 || (sb * size % 16 == 0 && sb * size < (1LL << 40))) &&
-                  (L == 1 || (st * size % 16 == 0 && st * size < (1LL << 40))));
+  return !ptr || (aligned16(ptr) && (B == 1 || (sb > 0 && sb * size % 16 == 0 && sb * size < (1LL << 40))) &&
+                  (L == 1 || (st > 0 && st * size % 16 == 0 && st * size < (1LL << 40))));
 }
 
 // cuTensorMapEncodeTiled from the driver (no link-time libcuda dependency).
@@ -137,31 +138,21 @@ int gscan_backward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
                 MODE == SCAN_TMA ? 3 * Stage<T, VEC, S, NW>::OPERAND : 0, s);
 }
 
-bool repeats(const void* ptr, long long sb, long long st, int B, int L) {
-  return ptr && ((B > 1 && sb == 0) || (L > 1 && st == 0));
-}
-
 template <typename T>
-int gscan_run(GScanArgs p, bool backward, void* ws, long long bytes, cudaStream_t s) {
+int gscan_run(const GScanArgs& p, bool backward, void* ws, long long bytes, cudaStream_t s) {
   constexpr int z = sizeof(T);
   if (!backward && p.L <= SEQ_STEPS) {
     gscan_forward_seq_kernel<T><<<column_blocks(p.B, p.D), 128, 0, s>>>(p);
     return launch_status("gscan_forward_seq_kernel");
   }
-  p.broadcast = repeats(p.a, p.a_sb, p.a_st, p.B, p.L) || repeats(p.x, p.x_sb, p.x_st, p.B, p.L) ||
-                repeats(p.dh, p.g_sb, p.g_st, p.B, p.L);
-  const bool tma = !p.broadcast && p.D * z % 16 == 0 && rows16(p.a, p.a_sb, p.a_st, p.B, p.L, z) &&
+  const bool tma = p.D * z % 16 == 0 && rows16(p.a, p.a_sb, p.a_st, p.B, p.L, z) &&
                     rows16(p.x, p.x_sb, p.x_st, p.B, p.L, z) && rows16(p.dh, p.g_sb, p.g_st, p.B, p.L, z) &&
                     aligned16(p.h) && aligned16(p.da) && aligned16(p.dx);
   if (tma)
     return backward ? gscan_backward<SCAN_TMA, T, 2, 8, 8, z == 2 ? 4 : 2>(p, ws, bytes, s)
                     : gscan_forward<SCAN_TMA, T, 2, z == 2 ? 32 : 16, 8, 2>(p, ws, bytes, s);
-  if constexpr (z == 2)
-    return backward ? gscan_backward<SCAN_SPLIT, T, 2, 8, 8, 4>(p, ws, bytes, s)
-                    : gscan_forward<SCAN_SPLIT, T, 2, 16, 8, 4>(p, ws, bytes, s);
-  else
-    return backward ? gscan_backward<SCAN_PLAIN, T, 1, 8, 8, 4>(p, ws, bytes, s)
-                    : gscan_forward<SCAN_PLAIN, T, 1, 16, 8, 4>(p, ws, bytes, s);
+  return backward ? gscan_backward<SCAN_PLAIN, T, 1, 8, 8, 4>(p, ws, bytes, s)
+                  : gscan_forward<SCAN_PLAIN, T, 1, 16, 8, 4>(p, ws, bytes, s);
 }
 
 int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long long bytes, cudaStream_t s) {

@@ -49,7 +49,6 @@ struct GScanArgs {
   unsigned* ticket;
   int B, L, D, nck;
   int nchunks, ctiles;  // runs of steps per column; column tiles per batch row
-  int broadcast;        // an operand has a stride of zero
 };
 
 // ------------------------------------------------------------ published words
@@ -279,7 +278,8 @@ struct Pack {
   }
   GFN_DEV static Pack load(const T* p) {  // read once: evict first
     Pack r;
-    if constexpr (N == 1) r.u[0] = __ldcs(reinterpret_cast<const unsigned*>(p));
+    if constexpr (BYTES == 2) r.u[0] = __ldcs(reinterpret_cast<const unsigned short*>(p));
+    else if constexpr (N == 1) r.u[0] = __ldcs(reinterpret_cast<const unsigned*>(p));
     else {
       const uint2 x = __ldcs(reinterpret_cast<const uint2*>(p));
       r.u[0] = x.x;
@@ -288,7 +288,8 @@ struct Pack {
     return r;
   }
   GFN_DEV void store(T* p) const {
-    if constexpr (N == 1) __stcs(reinterpret_cast<unsigned*>(p), u[0]);
+    if constexpr (BYTES == 2) __stcs(reinterpret_cast<unsigned short*>(p), (unsigned short)u[0]);
+    else if constexpr (N == 1) __stcs(reinterpret_cast<unsigned*>(p), u[0]);
     else __stcs(reinterpret_cast<uint2*>(p), make_uint2(u[0], u[1]));
   }
   GFN_DEV static unsigned short bits16(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
@@ -302,10 +303,8 @@ struct Pack {
 // A block draws its ticket one run ahead.
 struct ScanTile {
   int chunk, b, c0, col;  // c0: the tile's first column; col: this lane's first
-  int t0, rows, n;        // this warp's first step and how many it has; n: this lane's (0 beyond the columns)
-  int width;              // columns from this lane's first one on
-  int first, steps;       // the run's first step and how many it has
-  bool active;
+  int first, t0;          // the run's first step and this warp's
+  int n;                  // steps of this lane: 0 beyond the end or the columns
   long long tile;
 };
 
@@ -318,13 +317,9 @@ GFN_DEV ScanTile scan_tile(const Args& p, unsigned t) {
   r.b = (int)(r.tile / p.ctiles);
   r.c0 = (int)(r.tile - (long long)r.b * p.ctiles) * (32 * VEC);
   r.col = r.c0 + (threadIdx.x & 31) * VEC;
-  r.width = p.D - r.col;
-  r.active = r.width > 0;
   r.first = (REV ? p.nchunks - 1 - r.chunk : r.chunk) * (NW * S);
-  r.steps = min(NW * S, p.L - r.first);
   r.t0 = r.first + (threadIdx.x >> 5) * S;
-  r.rows = max(0, min(S, p.L - r.t0));
-  r.n = r.active ? r.rows : 0;
+  r.n = r.col < p.D ? max(0, min(S, p.L - r.t0)) : 0;
   return r;
 }
 
@@ -363,56 +358,18 @@ struct ScanTurn {
 //   TMA     rows that start on 16 bytes: one thread issues a tensor copy per
 //           operand for the NEXT run as soon as this run's values are in
 //           registers, so the memory stays busy through the exchange of maps;
-//   PLAIN   any other rows: loads when the run begins;
-//   SPLIT   PLAIN for 16-bit pairs of rows that need not start on a pair: a lane
-//           loads the aligned word that holds its first element, and a pair
-//           that straddles two words takes its second half from the next
-//           lane's (the tile's last element is loaded by itself).  Tiles at the
-//           very ends of an operand, where such a word could reach past it, are
-//           read element by element.
-enum { SCAN_TMA, SCAN_PLAIN, SCAN_SPLIT };
+//   PLAIN   any other rows: each lane loads one column's elements when the run
+//           begins.  (Pairs of 16-bit elements assembled from the aligned words
+//           around them measured slower: 63 against 49 us forward and 86
+//           against 78 backward at 3 x 5003 x 1001.)
+enum { SCAN_TMA, SCAN_PLAIN };
 
-// S rows of this lane, `step` elements apart, of which n exist; `width` columns
-// from the lane's first one on (any value where there is no element).
-template <int MODE, typename T, int VEC, int S>
-GFN_DEV void load_rows(Pack<T, VEC> (&out)[S], const T* src, long long step, int n, int rows, int width, bool ends) {
-  if constexpr (MODE == SCAN_SPLIT) {
-    static_assert(S <= 32, "lane s fetches row s's last element");
-    const int lane = threadIdx.x & 31;
-    const int cols = min(32 * VEC, width + lane * VEC);  // of the tile
-    unsigned last = 0;
-    if (ends) {
+// S rows of this lane, `step` elements apart, of which n exist.
+template <typename T, int VEC, int S>
+GFN_DEV void load_rows(Pack<T, VEC> (&out)[S], const T* src, long long step, int n) {
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if (s < n) {
-          const T* row = src + s * step;
-          out[s].u[0] = *reinterpret_cast<const unsigned short*>(row);
-          if (width > 1) out[s].u[0] |= (unsigned)*reinterpret_cast<const unsigned short*>(row + 1) << 16;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if (s < n)
-          out[s].u[0] = __ldcs(reinterpret_cast<const unsigned*>(
-              reinterpret_cast<uintptr_t>(src + s * step) & ~(uintptr_t)3));
-      }
-      if (lane < rows)
-        last = __ldcs(reinterpret_cast<const unsigned short*>(src + lane * step) + (cols - 1 - lane * VEC));
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const unsigned next = __shfl_down_sync(0xffffffffu, out[s].u[0], 1);
-        const unsigned edge = __shfl_sync(0xffffffffu, last, s);
-        if (reinterpret_cast<uintptr_t>(src + s * step) & 2)
-          out[s].u[0] = (out[s].u[0] >> 16) | ((width == 2 || lane == 31 ? edge : next) << 16);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (s < n) out[s] = Pack<T, VEC>::load(src + s * step);
-    }
-  }
+  for (int s = 0; s < S; ++s)
+    if (s < n) out[s] = Pack<T, VEC>::load(src + s * step);
 }
 
 // The operands as [batch][step][column] tensors with boxes of one run's steps
@@ -447,26 +404,6 @@ struct Stage {
   }
 };
 
-// One row of results: whole packs, or (SPLIT) aligned words across lanes.  The
-// whole warp calls; `width`: columns from the lane's first one on.
-template <int MODE, typename T, int VEC>
-GFN_DEV void store_row(T* dst, const Pack<T, VEC>& v, int width) {
-  if constexpr (MODE == SCAN_SPLIT) {
-    unsigned short* e = reinterpret_cast<unsigned short*>(dst);
-    const unsigned next = __shfl_down_sync(0xffffffffu, v.u[0], 1);
-    const int lane = threadIdx.x & 31;
-    if (reinterpret_cast<uintptr_t>(dst) & 2) {
-      if (lane == 0 && width > 0) e[0] = (unsigned short)v.u[0];
-      if (width > 2 && lane < 31) __stcs(reinterpret_cast<unsigned*>(e + 1), (v.u[0] >> 16) | (next << 16));
-      else if (width > 1) e[1] = (unsigned short)(v.u[0] >> 16);
-    } else {
-      if (width > 1) __stcs(reinterpret_cast<unsigned*>(e), v.u[0]);
-      else if (width > 0) e[0] = (unsigned short)v.u[0];
-    }
-  } else {
-    if (width > 0) v.store(dst);
-  }
-}
 // Keeps packed values packed: without it the compiler carries the unpacked
 // floats of the first pass over to the second, in twice the registers.
 template <typename T, int VEC, int S>
@@ -481,15 +418,6 @@ GFN_DEV void keep_packed(Pack<T, VEC> (&a)[S]) {
 }
 
 // ------------------------------------------------------------------ gated scan
-// Whether a tile may hold an operand's first or last element in memory; with
-// broadcast rows (a stride of zero) any row may.
-template <int VEC, int S>
-GFN_DEV bool holds_ends(const GScanArgs& p, const ScanTile& q) {
-  const bool left = q.c0 == 0, right = q.c0 + 32 * VEC >= p.D;
-  if (p.broadcast) return left || right;
-  return (left && q.b == 0 && q.t0 == 0) || (right && q.b == p.B - 1 && q.t0 + S >= p.L);
-}
-
 // Map of S steps from a zero state; steps beyond the end hold a = 1, x = 0.
 template <typename T, int VEC, int S>
 GFN_DEV GatedMap run_map(const Pack<T, VEC> (&a)[S], const Pack<T, VEC> (&x)[S], int v) {
@@ -540,9 +468,8 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_forward_kernel(const GScan
         a[s] = stage.take(1, s);
       }
     } else {
-      const bool ends = holds_ends<VEC, S>(p, q);
-      load_rows<MODE, T, VEC, S>(x, row(p.x, q, p.x_sb, p.x_st, q.t0, q.col), p.x_st, q.n, q.rows, q.width, ends);
-      if (p.a) load_rows<MODE, T, VEC, S>(a, row(p.a, q, p.a_sb, p.a_st, q.t0, q.col), p.a_st, q.n, q.rows, q.width, ends);
+      load_rows<T, VEC, S>(x, row(p.x, q, p.x_sb, p.x_st, q.t0, q.col), p.x_st, q.n);
+      if (p.a) load_rows<T, VEC, S>(a, row(p.a, q, p.a_sb, p.a_st, q.t0, q.col), p.a_st, q.n);
     }
     turn.draw(p);
 #pragma unroll
@@ -565,7 +492,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_forward_kernel(const GScan
           turn.hear(p, sh.slot, it);
           if (turn.next < turn.total) fetch(turn.next);
         });
-    if (q.rows <= 0) continue;
+    if (q.n <= 0) continue;
     keep_packed(a);
     keep_packed(x);
     float h[VEC];
@@ -574,20 +501,18 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_forward_kernel(const GScan
       h[v] = sh.in[lane * VEC + v].through(GatedMap::unpack({sh.maps[w][0][lane * VEC + v]})).h;
     if (p.states && q.t0 % SCAN_CK == 0) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        if (v < q.width) p.states[((long long)q.b * p.nck + q.t0 / SCAN_CK) * p.D + q.col + v] = h[v];
+      for (int v = 0; v < VEC; ++v) p.states[((long long)q.b * p.nck + q.t0 / SCAN_CK) * p.D + q.col + v] = h[v];
     }
     T* hp = static_cast<T*>(p.h) + ((long long)q.b * p.L + q.t0) * p.D + q.col;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) h[v] = fmaf(a[s].get(v), h[v], x[s].get(v));
-      if (s < q.rows) store_row<MODE, T, VEC>(hp + (long long)s * p.D, Pack<T, VEC>::of(h), q.width);
+      if (s < q.n) Pack<T, VEC>::of(h).store(hp + (long long)s * p.D);
     }
-    if (p.h_last && q.t0 + q.rows == p.L) {
+    if (p.h_last && q.t0 + q.n == p.L) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        if (v < q.width) p.h_last[(long long)q.b * p.D + q.col + v] = h[v];
+      for (int v = 0; v < VEC; ++v) p.h_last[(long long)q.b * p.D + q.col + v] = h[v];
     }
   }
 }
@@ -646,10 +571,9 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GSca
         g[s] = stage.take(2, s);
       }
     } else {
-      const bool ends = holds_ends<VEC, S>(p, q);
-      load_rows<MODE, T, VEC, S>(x, row(p.x, q, p.x_sb, p.x_st, q.t0, q.col), p.x_st, q.n, q.rows, q.width, ends);
-      if (p.a) load_rows<MODE, T, VEC, S>(a, row(p.a, q, p.a_sb, p.a_st, q.t0, q.col), p.a_st, q.n, q.rows, q.width, ends);
-      if (p.dh) load_rows<MODE, T, VEC, S>(g, row(p.dh, q, p.g_sb, p.g_st, q.t0, q.col), p.g_st, q.n, q.rows, q.width, ends);
+      load_rows<T, VEC, S>(x, row(p.x, q, p.x_sb, p.x_st, q.t0, q.col), p.x_st, q.n);
+      if (p.a) load_rows<T, VEC, S>(a, row(p.a, q, p.a_sb, p.a_st, q.t0, q.col), p.a_st, q.n);
+      if (p.dh) load_rows<T, VEC, S>(g, row(p.dh, q, p.g_sb, p.g_st, q.t0, q.col), p.g_st, q.n);
     }
     turn.draw(p);
 #pragma unroll
@@ -682,7 +606,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GSca
           turn.hear(p, sh.slot, it);
           if (turn.next < turn.total) fetch(turn.next);
         });
-    if (q.rows <= 0) continue;
+    if (q.n <= 0) continue;
     keep_packed(a);
     keep_packed(x);
     keep_packed(g);
@@ -704,16 +628,15 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GSca
         oa[v] = ox[v] * hp[s][v];
         m[v] = a[s].get(v) * ox[v];
       }
-      if (s < q.rows) {
+      if (s < q.n) {
         const long long e = o + (long long)s * p.D;
-        if (p.dx) store_row<MODE, T, VEC>(static_cast<T*>(p.dx) + e, Pack<T, VEC>::of(ox), q.width);
-        if (p.da) store_row<MODE, T, VEC>(static_cast<T*>(p.da) + e, Pack<T, VEC>::of(oa), q.width);
+        if (p.dx) Pack<T, VEC>::of(ox).store(static_cast<T*>(p.dx) + e);
+        if (p.da) Pack<T, VEC>::of(oa).store(static_cast<T*>(p.da) + e);
       }
     }
     if (p.dh0 && run == 0 && w == 0) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        if (v < q.width) p.dh0[(long long)q.b * p.D + q.col + v] = m[v];
+      for (int v = 0; v < VEC; ++v) p.dh0[(long long)q.b * p.D + q.col + v] = m[v];
     }
   }
 }
@@ -859,9 +782,9 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScan
       }
     } else {
       const float* zp = p.z + ((long long)c.b * p.L + c.t0) * 3 * p.D + c.col;
-      load_rows<MODE, float, VEC, S>(pa, zp, 3LL * p.D, c.n, c.rows, c.width, false);
-      load_rows<MODE, float, VEC, S>(pd, zp + p.D, 3LL * p.D, c.n, c.rows, c.width, false);
-      load_rows<MODE, float, VEC, S>(pb, zp + 2LL * p.D, 3LL * p.D, c.n, c.rows, c.width, false);
+      load_rows<float, VEC, S>(pa, zp, 3LL * p.D, c.n);
+      load_rows<float, VEC, S>(pd, zp + p.D, 3LL * p.D, c.n);
+      load_rows<float, VEC, S>(pb, zp + 2LL * p.D, 3LL * p.D, c.n);
     }
     turn.draw(p);
     float A[S][VEC], dt[S][VEC], bv[S][VEC];
@@ -1007,11 +930,11 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
     } else {
       const long long o = ((long long)c.b * p.L + c.t0) * p.D + c.col;
       const float* zp = p.z + 3 * (o - c.col) + c.col;
-      load_rows<MODE, float, VEC, S>(pa, zp, 3LL * p.D, c.n, c.rows, c.width, false);
-      load_rows<MODE, float, VEC, S>(pd, zp + p.D, 3LL * p.D, c.n, c.rows, c.width, false);
-      load_rows<MODE, float, VEC, S>(pb, zp + 2LL * p.D, 3LL * p.D, c.n, c.rows, c.width, false);
-      if (p.gx) load_rows<MODE, float, VEC, S>(px, p.gx + o, p.D, c.n, c.rows, c.width, false);
-      if (p.gv) load_rows<MODE, float, VEC, S>(pv, p.gv + o, p.D, c.n, c.rows, c.width, false);
+      load_rows<float, VEC, S>(pa, zp, 3LL * p.D, c.n);
+      load_rows<float, VEC, S>(pd, zp + p.D, 3LL * p.D, c.n);
+      load_rows<float, VEC, S>(pb, zp + 2LL * p.D, 3LL * p.D, c.n);
+      if (p.gx) load_rows<float, VEC, S>(px, p.gx + o, p.D, c.n);
+      if (p.gv) load_rows<float, VEC, S>(pv, p.gv + o, p.D, c.n);
     }
     turn.draw(p);
     float A[S][VEC], dt[S][VEC], zb[S][VEC], gx[S][VEC], gv[S][VEC];
@@ -1072,7 +995,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
           turn.hear(p, sh.slot, it);
           if (turn.next < turn.total) fetch(turn.next);
         });
-    if (!c.active) continue;
+    if (c.n <= 0) continue;
     LayerBackState st[VEC];
     float vs[S + 1][VEC];  // v_{t-1} of this warp's steps, and the last step's v
 #pragma unroll
