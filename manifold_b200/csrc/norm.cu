@@ -11,8 +11,9 @@
 // weight gradients are summed in a fixed order (per-block partial rows, then
 // one pass over the blocks): no atomics, the same bits on every run.
 //
-// Both passes are bound by HBM.  A row is held in registers by the threads
-// that share it, 16 elements each, and read once.
+// Both passes are bound by HBM.  A row is held in registers by the WPR warps
+// that share it (64 bytes a thread forward, 16 elements backward) and read
+// once.
 #include "abi.h"
 #include "lm_ops.cuh"
 #include "umma.cuh"
@@ -23,8 +24,6 @@ using namespace gfn_abi;
 namespace {
 
 constexpr int NORM_THREADS = 256;
-constexpr int NORM_EPT = 16;  // elements per thread
-
 struct NormArgs {
   const void* x;
   const void* dy;
@@ -38,7 +37,7 @@ struct NormArgs {
   long long rows, xs, ds;  // row strides of x and dy, in elements
   int D, blocks;
   float eps;
-  int wpr;          // warps that share a row
+  int w32;          // weights are float32 (else of the elements' type)
   int chunk_rows;   // backward: rows per stage
   int stages;
   long long bulk;   // chunks that arrive by bulk copies; the rest is read in place
@@ -75,48 +74,56 @@ GFN_DEV void store_vec(T* p, const float (&f)[VEC]) {
   }
 }
 
-GFN_DEV void group_barrier(int group, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+// w[e .. e + VEC) as float32, whichever type it has
+template <typename T, int VEC>
+GFN_DEV void load_weight(const void* w, int w32, int e, float (&f)[VEC]) {
+  if (sizeof(T) == 4 || w32) load_vec<float, VEC>(static_cast<const float*>(w) + e, f);
+  else load_vec<T, VEC>(static_cast<const T*>(w) + e, f);
 }
 
-// Sums over the warps that share a row.  `buf` [2][warps of the block], used in
-// turn: a warp is at most one sum ahead of its group.
-template <int N>
-GFN_DEV void row_sum(float (&v)[N], float* buf, int warps, int wpr, int& turn) {
+// Sums over the WPR warps that share a row (named barrier per group).  `buf`
+// holds two sets of sums, used in turn: a warp is at most one sum ahead.
+template <int N, int WPR>
+GFN_DEV void row_sum(float (&v)[N], float* buf, int warps, int& turn) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if (wpr == 1) return;
-  const int w = threadIdx.x >> 5, g = w / wpr;
-  float* b = buf + turn * warps * N;
-  turn ^= 1;
-  if ((threadIdx.x & 31) == 0) {
+  if constexpr (WPR > 1) {
+    const int w = threadIdx.x >> 5, g = w / WPR;
+    float* b = buf + turn * warps * N;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) b[w * N + i] = v[i];
-  }
-  group_barrier(g, wpr * 32);
+      for (int i = 0; i < N; ++i) b[w * N + i] = v[i];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "n"(WPR * 32) : "memory");
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = 0.f;
-  for (int k = 0; k < wpr; ++k) {
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += b[(g * wpr + k) * N + i];
+      for (int k = 0; k < WPR; ++k) v[i] += b[(g * WPR + k) * N + i];
+    }
   }
 }
 
-// wpr warps per row, one row per group; blocks of max(256, 32 wpr) threads.
-template <typename T, typename W, int VEC>
-__global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs p) {
-  constexpr int NV = NORM_EPT / VEC;
-  __shared__ float buf[2 * 32];
-  const int tpr = p.wpr * 32, warps = blockDim.x >> 5;
-  const long long row = (long long)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+// Elements per thread: 64 bytes of vectors, or 16 single elements.
+template <typename T, int VEC>
+constexpr int norm_forward_ept() { return VEC == 1 ? 16 : 64 / (int)sizeof(T); }
+constexpr int norm_forward_threads(int wpr) { return wpr * 32 > NORM_THREADS ? wpr * 32 : NORM_THREADS; }
+
+// WPR warps per row, one row per group of warps.
+template <typename T, int VEC, int WPR>
+__global__ void __launch_bounds__(norm_forward_threads(WPR), VEC == 1 ? 1 : 1024 / norm_forward_threads(WPR)) norm_forward_kernel(const NormArgs p) {
+  constexpr int TPR = WPR * 32, NV = norm_forward_ept<T, VEC>() / VEC, THREADS = norm_forward_threads(WPR);
+  __shared__ float buf[2 * THREADS / 32];
+  const long long row = (long long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
   if (row >= p.rows) return;  // a whole group: its barriers are its own
-  const int l = threadIdx.x % tpr, D = p.D;
+  const int l = threadIdx.x % TPR, D = p.D;
   const T* x = static_cast<const T*>(p.x) + row * p.xs;
   float v[NV][VEC];
   float s[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int e = (i * tpr + l) * VEC;
+    const int e = (i * TPR + l) * VEC;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
     if (e < D) load_vec<T, VEC>(x + e, v[i]);
@@ -127,12 +134,12 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs p) {
     for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
   }
   int turn = 0;
-  row_sum<1>(s, buf, warps, p.wpr, turn);
+  row_sum<1, WPR>(s, buf, THREADS / 32, turn);
   const float mu = s[0] / D;
   s[0] = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if ((i * tpr + l) * VEC < D) {
+    if ((i * TPR + l) * VEC < D) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         v[i][j] -= mu;
@@ -140,23 +147,25 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs p) {
       }
     }
   }
-  row_sum<1>(s, buf, warps, p.wpr, turn);
+  row_sum<1, WPR>(s, buf, THREADS / 32, turn);
   const float rstd = rsqrtf(s[0] / D + p.eps);
   T* y = static_cast<T*>(p.y) + row * D;
-  const W* w = static_cast<const W*>(p.w);
-  const W* b = static_cast<const W*>(p.b);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int e = (i * tpr + l) * VEC;
+    const int e = (i * TPR + l) * VEC;
     if (e < D) {
-      float wv[VEC], bv[VEC];
-      if (w) load_vec<W, VEC>(w + e, wv);
-      if (b) load_vec<W, VEC>(b + e, bv);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[i][j] *= rstd;
-        if (w) v[i][j] *= wv[j];
-        if (b) v[i][j] += bv[j];
+      for (int j = 0; j < VEC; ++j) v[i][j] *= rstd;
+      float c[VEC];
+      if (p.w) {
+        load_weight<T, VEC>(p.w, p.w32, e, c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] *= c[j];
+      }
+      if (p.b) {
+        load_weight<T, VEC>(p.b, p.w32, e, c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] += c[j];
       }
       store_vec<T, VEC>(y + e, v[i]);
     }
@@ -164,151 +173,258 @@ __global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs p) {
   if (p.stats && l == 0) p.stats[row] = make_float2(mu, rstd);
 }
 
-// NW warps compute, one more fetches: chunks of rows travel through a ring of
-// stages by bulk copies (a whole number of 16 bytes per chunk, whatever the
-// row length), so loads are in flight while rows are computed, at no cost in
-// registers.  dx is written from registers; dw and db of all the block's rows
-// stay there and leave once, as one partial row per block.
-template <typename T, typename W, int VEC, int NW>
-__global__ void __launch_bounds__((NW + 1) * 32, NW == 8 ? 2 : 1) norm_backward_kernel(const NormArgs p) {
-  constexpr int NV = NORM_EPT / VEC;
-  extern __shared__ __align__(128) char ring[];
-  __shared__ uint64_t full[4], empty[4];
-  __shared__ float buf[2 * NW * 2];
-  const int warp = threadIdx.x >> 5, D = p.D;
-  const long long chunks = (p.rows + p.chunk_rows - 1) / p.chunk_rows;
-  const int bytes = p.chunk_rows * D * (int)sizeof(T);  // of one operand's chunk
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], NW);
+// Chunks of rows travel through a ring of stages by bulk copies (a whole number
+// of 16 bytes per chunk, whatever the row length), so loads are in flight while
+// rows are computed, at no cost in registers; one thread refills the stage that
+// was read a chunk ago.  N operands with contiguous rows; blocks take chunks
+// in turn; work(rows of operand 0, chunk) is called by every warp.
+template <typename T, int N, int NW>
+struct RowRing {
+  uint64_t full[4], empty[4];
+
+  template <class Work>
+  GFN_DEV void run(const NormArgs& p, char* ring, const T* const (&src)[N], Work work) {
+    const int bytes = p.chunk_rows * p.D * (int)sizeof(T);  // of one operand's chunk
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < p.stages; ++i) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], NW);
+      }
+      fence_mbar_init();
     }
-    fence_mbar_init();
-  }
-  __syncthreads();
-  if (warp == NW) {
-    if ((threadIdx.x & 31) == 0) {
-      int it = 0;
-      for (long long c = blockIdx.x; c < p.bulk; c += gridDim.x, ++it) {
-        const int st = it % p.stages;
-        if (it >= p.stages) mbar_wait(&empty[st], (it / p.stages - 1) & 1);
-        char* dst = ring + (size_t)st * 2 * bytes;
-        const long long first = c * p.chunk_rows * (long long)D;
-        mbar_arrive_expect_tx(&full[st], 2 * bytes);
-        bulk_g2s(dst, static_cast<const T*>(p.x) + first, bytes, &full[st]);
-        bulk_g2s(dst + bytes, static_cast<const T*>(p.dy) + first, bytes, &full[st]);
+    __syncthreads();
+    auto refill = [&](long long c, int st) {
+      mbar_arrive_expect_tx(&full[st], N * bytes);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        bulk_g2s(ring + (size_t)(st * N + k) * bytes, src[k] + c * p.chunk_rows * (long long)p.D, bytes, &full[st]);
+    };
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < p.stages; ++i) {
+        const long long c = blockIdx.x + (long long)i * gridDim.x;
+        if (c < p.bulk) refill(c, i);
       }
     }
-    __syncwarp();
-    __syncthreads();  // the one before the partial sums
-    __syncthreads();
-    return;
+    int st = 0, phase = 0;
+    for (long long c = blockIdx.x; c < p.bulk; c += gridDim.x) {
+      if (threadIdx.x == 0 && c != blockIdx.x) {  // the stage of a chunk ago, once all warps have read it
+        const long long ahead = c + (long long)(p.stages - 1) * gridDim.x;
+        const int was = st ? st - 1 : p.stages - 1;
+        if (ahead < p.bulk) {
+          mbar_wait(&empty[was], st ? phase : phase ^ 1);
+          refill(ahead, was);
+        }
+      }
+      __syncwarp();
+      mbar_wait(&full[st], phase);
+      work(reinterpret_cast<const T*>(ring + (size_t)st * N * bytes), c);
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) umma::mbar_arrive(&empty[st]);
+      if (++st == p.stages) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
   }
-  const int tpr = p.wpr * 32, group = warp / p.wpr, groups = NW / p.wpr, l = threadIdx.x % tpr;
-  const W* w = static_cast<const W*>(p.w);
-  float wv[NV][VEC], aw[NV][VEC], ab[NV][VEC];
+};
+
+// The forward over many contiguous rows that do not start on 16 bytes: single
+// elements come from shared memory, and the weights stay in registers.  (From
+// 128-bit rows the direct kernel is as fast: 49 against 51 us at 65536 x 512
+// float32; here 39 against 70 us at 20011 x 1001 bfloat16.)
+template <typename T, int WPR>
+__global__ void __launch_bounds__(256, 3) norm_forward_ring_kernel(const NormArgs p) {
+  constexpr int VEC = 1, NW = 8, TPR = WPR * 32, GROUPS = NW / WPR, NV = 16 / VEC;
+  extern __shared__ __align__(128) char ring[];
+  __shared__ RowRing<T, 1, NW> rows;
+  __shared__ float buf[2 * NW];
+  const int D = p.D, group = (threadIdx.x >> 5) / WPR, l = threadIdx.x % TPR;
+  float wv[NV][VEC], bv[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int e = (i * tpr + l) * VEC;
+    const int e = (i * TPR + l) * VEC;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       wv[i][j] = 1.f;
-      aw[i][j] = ab[i][j] = 0.f;
+      bv[i][j] = 0.f;
     }
-    if (w && e < D) load_vec<W, VEC>(w + e, wv[i]);
+    if (p.w && e < D) load_weight<T, VEC>(p.w, p.w32, e, wv[i]);
+    if (p.b && e < D) load_weight<T, VEC>(p.b, p.w32, e, bv[i]);
   }
-  int it = 0, turn = 0;
+  int turn = 0;
+  auto one = [&](const T* x, long long row) {
+    float v[NV][VEC], s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * TPR + l) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
+      if (e < D) load_vec<T, VEC>(x + e, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
+    }
+    row_sum<1, WPR>(s, buf, NW, turn);
+    const float mu = s[0] / D;
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if ((i * TPR + l) * VEC < D) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] -= mu;
+          s[0] = fmaf(v[i][j], v[i][j], s[0]);
+        }
+      }
+    }
+    row_sum<1, WPR>(s, buf, NW, turn);
+    const float rstd = rsqrtf(s[0] / D + p.eps);
+    T* y = static_cast<T*>(p.y) + row * D;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * TPR + l) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] *= rstd;  // rounded before the weight, as in norm_forward_kernel
+        v[i][j] = p.b ? __fadd_rn(__fmul_rn(v[i][j], wv[i][j]), bv[i][j]) : v[i][j] * wv[i][j];
+      }
+      if (e < D) store_vec<T, VEC>(y + e, v[i]);
+    }
+    if (p.stats && l == 0) p.stats[row] = make_float2(mu, rstd);
+  };
+  const T* const src[1] = {static_cast<const T*>(p.x)};
+  rows.run(p, ring, src, [&](const T* x, long long c) {
+    for (int r = group; r < p.chunk_rows; r += GROUPS) one(x + r * D, c * p.chunk_rows + r);
+  });
+  for (long long row = p.bulk * p.chunk_rows + (long long)blockIdx.x * GROUPS + group; row < p.rows;
+       row += (long long)gridDim.x * GROUPS)  // what is left of a chunk
+    one(static_cast<const T*>(p.x) + row * D, row);
+}
+
+// dx is written from registers; dw and db of all the block's rows stay there
+// and leave once, as one partial row per block.
+template <typename T, int VEC, int WPR>
+struct NormBackward {
+  static constexpr int NW = WPR > 8 ? WPR : 8, TPR = WPR * 32, GROUPS = NW / WPR, EPT = 16, NV = EPT / VEC;
+  float wv[NV][VEC], aw[NV][VEC], ab[NV][VEC];
+  int l, turn = 0;
+
+  GFN_DEV void row(const NormArgs& p, const T* x, const T* dy, T* dx, float2 stat, float* buf) {
+    const int D = p.D;
+    float xh[NV][VEC], g[NV][VEC];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (i * TPR + l) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        xh[i][j] = stat.x;
+        g[i][j] = 0.f;
+      }
+      if (e < D) {
+        load_vec<T, VEC>(x + e, xh[i]);
+        load_vec<T, VEC>(dy + e, g[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        xh[i][j] = (xh[i][j] - stat.x) * stat.y;
+        aw[i][j] = fmaf(g[i][j], xh[i][j], aw[i][j]);
+        ab[i][j] += g[i][j];
+        g[i][j] *= wv[i][j];
+        s[0] += g[i][j];
+        s[1] = fmaf(g[i][j], xh[i][j], s[1]);
+      }
+    }
+    row_sum<2, WPR>(s, buf, NW, turn);
+    if (dx) {
+      const float m1 = s[0] / D, m2 = s[1] / D;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = (i * TPR + l) * VEC;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) g[i][j] = stat.y * (g[i][j] - m1 - xh[i][j] * m2);
+        if (e < D) store_vec<T, VEC>(dx + e, g[i]);
+      }
+    }
+  }
+};
+
+template <typename T, int VEC, int WPR>
+__global__ void __launch_bounds__(NormBackward<T, VEC, WPR>::NW * 32, WPR > 8 ? 1 : 2) norm_backward_kernel(const NormArgs p) {
+  using Work = NormBackward<T, VEC, WPR>;
+  constexpr int NW = Work::NW, TPR = Work::TPR, GROUPS = Work::GROUPS, NV = Work::NV, EPT = Work::EPT;
+  extern __shared__ __align__(128) char ring[];
+  __shared__ RowRing<T, 2, NW> ops;
+  __shared__ float buf[2 * NW * 2];
+  const int warp = threadIdx.x >> 5, D = p.D, group = warp / WPR;
+  Work k;
+  k.l = threadIdx.x % TPR;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int e = (i * TPR + k.l) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      k.wv[i][j] = 1.f;
+      k.aw[i][j] = k.ab[i][j] = 0.f;
+    }
+    if (p.w && e < D) load_weight<T, VEC>(p.w, p.w32, e, k.wv[i]);
+  }
+  T* dx = static_cast<T*>(p.y);
   float2 next = make_float2(0.f, 0.f);  // statistics of this group's next row, fetched ahead
+  const long long stride = (long long)gridDim.x * p.chunk_rows;
   {
     const long long row = (long long)blockIdx.x * p.chunk_rows + group;
     if (row < p.rows) next = p.stats[row];
   }
-  for (long long c = blockIdx.x; c < chunks; c += gridDim.x, ++it) {
-    const int st = it % p.stages;
-    const bool bulk = c < p.bulk;
+  const T* const src[2] = {static_cast<const T*>(p.x), static_cast<const T*>(p.dy)};
+  ops.run(p, ring, src, [&](const T* cx, long long c) {
+    const T* cd = cx + p.chunk_rows * D;
+    const long long first = c * p.chunk_rows;
+    for (int r = group; r < p.chunk_rows; r += GROUPS) {
+      const float2 stat = next;
+      const long long ahead = r + GROUPS < p.chunk_rows ? first + r + GROUPS : first + stride + group;
+      if (ahead < p.rows) next = p.stats[ahead];
+      k.row(p, cx + r * D, cd + r * D, dx ? dx + (first + r) * D : nullptr, stat, buf);
+    }
+  });
+  long long c = blockIdx.x;
+  if (c < p.bulk) c += (p.bulk - c + gridDim.x - 1) / gridDim.x * gridDim.x;
+  for (; c * p.chunk_rows < p.rows; c += gridDim.x) {  // rows read in place
     const long long first = c * p.chunk_rows;
     const int rows = (int)min((long long)p.chunk_rows, p.rows - first);
-    const T* cx = reinterpret_cast<const T*>(ring + (size_t)st * 2 * bytes);
-    const T* cd = reinterpret_cast<const T*>(ring + (size_t)st * 2 * bytes + bytes);
-    if (bulk) mbar_wait(&full[st], (it / p.stages) & 1);
-    for (int r = group; r < rows; r += groups) {
+    for (int r = group; r < rows; r += GROUPS) {
       const long long row = first + r;
-      const T* x = bulk ? cx + r * D : static_cast<const T*>(p.x) + row * p.xs;
-      const T* dy = bulk ? cd + r * D : static_cast<const T*>(p.dy) + row * p.ds;
-      const float2 stat = next;
-      {
-        const long long ahead = r + groups < rows ? row + groups : first + (long long)gridDim.x * p.chunk_rows + group;
-        if (ahead < p.rows) next = p.stats[ahead];
-      }
-      float xh[NV][VEC], g[NV][VEC];
-      float s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int e = (i * tpr + l) * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          xh[i][j] = stat.x;
-          g[i][j] = 0.f;
-        }
-        if (e < D) {
-          load_vec<T, VEC>(x + e, xh[i]);
-          load_vec<T, VEC>(dy + e, g[i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          xh[i][j] = (xh[i][j] - stat.x) * stat.y;
-          aw[i][j] = fmaf(g[i][j], xh[i][j], aw[i][j]);
-          ab[i][j] += g[i][j];
-          g[i][j] *= wv[i][j];
-          s[0] += g[i][j];
-          s[1] = fmaf(g[i][j], xh[i][j], s[1]);
-        }
-      }
-      row_sum<2>(s, buf, NW, p.wpr, turn);
-      const float m1 = s[0] / D, m2 = s[1] / D;
-      if (p.y) {
-        T* dx = static_cast<T*>(p.y) + row * D;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int e = (i * tpr + l) * VEC;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) g[i][j] = stat.y * (g[i][j] - m1 - xh[i][j] * m2);
-          if (e < D) store_vec<T, VEC>(dx + e, g[i]);
-        }
-      }
-    }
-    if (bulk) {
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) umma::mbar_arrive(&empty[st]);
+      k.row(p, static_cast<const T*>(p.x) + row * p.xs, static_cast<const T*>(p.dy) + row * p.ds,
+            dx ? dx + row * D : nullptr, p.stats[row], buf);
     }
   }
+  if (!p.part) return;
   // dw, db: the groups' sums meet in shared memory (the ring is free: every
   // copy has landed and been read), in the order of the groups
   __syncthreads();
-  if (!p.part) {
-    __syncthreads();
-    return;
-  }
-  float* sums = reinterpret_cast<float*>(ring);  // [groups][2][tpr * NORM_EPT]
-  const int width = tpr * NORM_EPT;
+  float* sums = reinterpret_cast<float*>(ring);  // [GROUPS][2][TPR * EPT]
+  constexpr int WIDTH = TPR * EPT;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const int e = (i * tpr + l) * VEC + j;
-      sums[(group * 2) * width + e] = aw[i][j];
-      sums[(group * 2 + 1) * width + e] = ab[i][j];
+      const int e = (i * TPR + k.l) * VEC + j;
+      sums[(group * 2) * WIDTH + e] = k.aw[i][j];
+      sums[(group * 2 + 1) * WIDTH + e] = k.ab[i][j];
     }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < 2 * D; e += NW * 32) {
-    const int k = e >= D, col = e - k * D;
+    const int which = e >= D, col = e - which * D;
     float t = 0.f;
-    for (int g = 0; g < groups; ++g) t += sums[(g * 2 + k) * width + col];
-    p.part[((long long)blockIdx.x * 2 + k) * D + col] = t;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) t += sums[(g * 2 + which) * WIDTH + col];
+    p.part[((long long)blockIdx.x * 2 + which) * D + col] = t;
   }
 }
 
@@ -391,90 +507,146 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_dw_long_kernel(const NormAr
   p.part[(2LL * blockIdx.y + 1) * p.D + i] = sb;
 }
 
-// The blocks' partial rows, in order: 32 columns x 8 slices of the blocks.
+// The blocks' partial rows, in order: 32 columns x 32 slices of the blocks.
 // grid (columns / 32, dw or db)
 template <typename W>
-__global__ void __launch_bounds__(NORM_THREADS) norm_dw_sum_kernel(const NormArgs p) {
-  __shared__ float buf[8][32];
+__global__ void __launch_bounds__(1024) norm_dw_sum_kernel(const NormArgs p) {
+  constexpr int PER = 10;  // partial rows per slice, all in flight; 32 PER >= NORM_MAX_BLOCKS
+  __shared__ float buf[32][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, col = blockIdx.x * 32 + lane, k = blockIdx.y;
-  const int per = (p.blocks + 7) / 8, b1 = min(p.blocks, (slice + 1) * per);
-  float s = 0.f;
-  if (col < p.D) {
-#pragma unroll 8
-    for (int b = slice * per; b < b1; ++b) s += p.part[((long long)b * 2 + k) * p.D + col];
-  }
-  buf[slice][lane] = s;
-  __syncthreads();
-  W* out = static_cast<W*>(k ? p.db : p.dw);
-  if (slice == 0 && col < p.D && out) {
-    s = 0.f;
+  float v[PER], s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += buf[i][lane];
-    out[col] = from_f<W>(s);
+  for (int i = 0; i < PER; ++i) {
+    const int b = slice * PER + i;
+    v[i] = b < p.blocks && col < p.D ? p.part[((long long)b * 2 + k) * p.D + col] : 0.f;
   }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) s += v[i];
+  buf[lane][slice] = s;
+  __syncthreads();
+  s = warp_sum(buf[slice][lane]);  // warp `slice` sums column `slice` of the tile
+  W* out = static_cast<W*>(k ? p.db : p.dw);
+  const int c = blockIdx.x * 32 + slice;
+  if (lane == 0 && c < p.D && out) out[c] = from_f<W>(s);
 }
 
 constexpr int NORM_MAX_BLOCKS = 296;
 constexpr int NORM_SMEM = 100 * 1024;  // ring per block: two blocks per SM
+constexpr int RING_SMEM = 64 * 1024;   // forward: three blocks per SM
+constexpr int RING_ROWS = 4096;        // rows from which the forward streams through the ring
 
 int norm_blocks(long long rows) { return (int)(rows < NORM_MAX_BLOCKS ? rows : NORM_MAX_BLOCKS); }
 
-// Warps per row: the smallest power of two whose registers hold the row.
-int warps_per_row(int D) {
-  int w = 1;
-  while (w * 32 * NORM_EPT < D) w *= 2;
-  return w;
+template <typename W>
+void norm_dw_sum(const NormArgs& p, cudaStream_t s) {
+  norm_dw_sum_kernel<W><<<dim3((p.D + 31) / 32, 2), 1024, 0, s>>>(p);
 }
 
-template <typename T, typename W, int VEC, int NW>
-int norm_backward_run(NormArgs p, cudaStream_t s) {
-  const int groups = NW / p.wpr, row = p.D * (int)sizeof(T);
+// How the rows of `operands` contiguous operands travel through the ring; false
+// where they do not (rows apart, odd addresses, rows too long for two stages).
+bool plan_ring(NormArgs* p, int groups, int operands, int row, int smem, bool whole) {
   int unit = 1;  // rows that make whole 16-byte pieces
   while ((long long)unit * row % 16) unit *= 2;
   int rows = groups > unit ? groups : unit;
-  while (rows * row <= 4096 && p.rows / (2 * rows) >= NORM_MAX_BLOCKS) rows *= 2;  // short rows: longer copies
-  const size_t sums = (size_t)NW * 32 * NORM_EPT * 2 * 4;
-  const bool bulk = (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.dy)) % 16 == 0 &&
-                    (p.rows == 1 || (p.xs == p.D && p.ds == p.D)) && (size_t)rows * row * 4 <= NORM_SMEM;
-  if (!bulk) rows = groups;
-  p.chunk_rows = rows;
-  p.stages = bulk ? (int)(NORM_SMEM / ((size_t)rows * row * 2)) : 1;
-  if (p.stages > 4) p.stages = 4;
-  p.bulk = bulk ? p.rows / rows : 0;
+  while (rows * row <= 4096 && p->rows / (2 * rows) >= NORM_MAX_BLOCKS) rows *= 2;  // short rows: longer copies
+  if (!whole || (size_t)rows * row * 2 * operands > (size_t)smem) return false;
+  p->chunk_rows = rows;
+  p->stages = (int)(smem / ((size_t)rows * row * operands));
+  if (p->stages > 4) p->stages = 4;
+  p->bulk = p->rows / rows;
+  return true;
+}
+
+template <typename T, int VEC, int WPR>
+int norm_backward_run(NormArgs p, cudaStream_t s) {
+  using Work = NormBackward<T, VEC, WPR>;
+  const int row = p.D * (int)sizeof(T);
+  const size_t sums = (size_t)Work::NW * 32 * Work::EPT * 2 * 4;
+  const bool whole = (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.dy)) % 16 == 0 &&
+                     (p.rows == 1 || (p.xs == p.D && p.ds == p.D));
+  const bool bulk = plan_ring(&p, Work::GROUPS, 2, row, NORM_SMEM, whole);
+  if (!bulk) {
+    p.chunk_rows = Work::GROUPS;
+    p.bulk = 0;
+  }
+  const int rows = p.chunk_rows;
   const long long chunks = (p.rows + rows - 1) / rows;
-  const int most = NW == 8 ? NORM_MAX_BLOCKS : NORM_MAX_BLOCKS / 2;
+  const int most = WPR > 8 ? NORM_MAX_BLOCKS / 2 : NORM_MAX_BLOCKS;
   p.blocks = (int)(chunks < most ? chunks : most);
   if (!p.dw && !p.db) p.part = nullptr;
   size_t smem = bulk ? (size_t)p.stages * rows * row * 2 : 0;
   if (smem < sums) smem = sums;
-  cudaError_t e = cudaFuncSetAttribute(norm_backward_kernel<T, W, VEC, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e = cudaFuncSetAttribute(norm_backward_kernel<T, VEC, WPR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)smem);
   if (e != cudaSuccess) return cuda_status(e, "norm_backward_kernel: shared memory");
-  norm_backward_kernel<T, W, VEC, NW><<<p.blocks, (NW + 1) * 32, smem, s>>>(p);
-  if (p.part) norm_dw_sum_kernel<W><<<dim3((p.D + 31) / 32, 2), NORM_THREADS, 0, s>>>(p);
+  norm_backward_kernel<T, VEC, WPR><<<p.blocks, Work::NW * 32, smem, s>>>(p);
+  if (p.part) {
+    if (p.w32) norm_dw_sum<float>(p, s);
+    else norm_dw_sum<T>(p, s);
+  }
   return launch_status("norm_backward_kernel");
 }
 
-template <typename T, typename W, int VEC>
-int norm_short_run(const NormArgs& p, bool backward, cudaStream_t s) {
-  if (backward) return p.wpr <= 8 ? norm_backward_run<T, W, VEC, 8>(p, s) : norm_backward_run<T, W, VEC, 16>(p, s);
-  const int threads = p.wpr * 32 > 256 ? p.wpr * 32 : 256, per = threads / (p.wpr * 32);
+template <typename T, int VEC, int WPR>
+int norm_forward_run(const NormArgs& p, cudaStream_t s) {
+  constexpr int threads = norm_forward_threads(WPR), per = threads / (WPR * 32);
   const long long blocks = (p.rows + per - 1) / per;
   if (blocks > 0x7fffffffLL) return fail(GFN_ERR_UNSUPPORTED, "layer_norm_forward: %lld blocks", blocks);
-  norm_forward_kernel<T, W, VEC><<<(unsigned)blocks, threads, 0, s>>>(p);
+  norm_forward_kernel<T, VEC, WPR><<<(unsigned)blocks, threads, 0, s>>>(p);
   return launch_status("norm_forward_kernel");
+}
+
+template <typename T, int WPR>
+int norm_forward_ring_run(const NormArgs& p, cudaStream_t s) {
+  const int smem = (int)((size_t)p.stages * p.chunk_rows * p.D * sizeof(T));
+  cudaError_t e = cudaFuncSetAttribute(norm_forward_ring_kernel<T, WPR>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_status(e, "norm_forward_ring_kernel: shared memory");
+  const long long most = NORM_MAX_BLOCKS * 3 / 2;
+  norm_forward_ring_kernel<T, WPR><<<(unsigned)(p.bulk < most ? p.bulk : most), 256, smem, s>>>(p);
+  return launch_status("norm_forward_ring_kernel");
+}
+
+// The fewest warps whose registers hold a row.
+template <typename T, int VEC>
+int norm_short_run(const NormArgs& p, bool backward, cudaStream_t s) {
+  if (backward) {
+    if (p.D <= 512) return norm_backward_run<T, VEC, 1>(p, s);
+    if (p.D <= 1024) return norm_backward_run<T, VEC, 2>(p, s);
+    if (p.D <= 2048) return norm_backward_run<T, VEC, 4>(p, s);
+    if (p.D <= 4096) return norm_backward_run<T, VEC, 8>(p, s);
+    return norm_backward_run<T, VEC, 16>(p, s);
+  }
+  if constexpr (VEC == 1) {
+    NormArgs q = p;
+    const bool whole = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.xs == p.D;
+    const int groups = p.D <= 512 ? 8 : p.D <= 1024 ? 4 : p.D <= 2048 ? 2 : 1;
+    if (p.D <= 4096 && p.rows >= RING_ROWS && plan_ring(&q, groups, 1, p.D * (int)sizeof(T), RING_SMEM, whole)) {
+      if (groups == 8) return norm_forward_ring_run<T, 1>(q, s);
+      if (groups == 4) return norm_forward_ring_run<T, 2>(q, s);
+      if (groups == 2) return norm_forward_ring_run<T, 4>(q, s);
+      return norm_forward_ring_run<T, 8>(q, s);
+    }
+  }
+  constexpr int warp = 32 * norm_forward_ept<T, VEC>();  // elements that one warp holds
+  if (p.D <= warp) return norm_forward_run<T, VEC, 1>(p, s);
+  if (p.D <= 2 * warp) return norm_forward_run<T, VEC, 2>(p, s);
+  if (p.D <= 4 * warp) return norm_forward_run<T, VEC, 4>(p, s);
+  if (p.D <= 8 * warp) return norm_forward_run<T, VEC, 8>(p, s);
+  return norm_forward_run<T, VEC, 16>(p, s);
 }
 
 template <typename T, typename W>
 int norm_run(NormArgs p, bool backward, cudaStream_t s) {
-  p.wpr = warps_per_row(p.D);
-  if (p.wpr <= (backward ? 16 : 32)) {
-    constexpr int VEC = 16 / sizeof(T);
+  p.w32 = sizeof(W) == 4;
+  constexpr int VEC = 16 / sizeof(T);
+  {
     const uintptr_t ends = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.dy) |
                            reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.w) |
                            reinterpret_cast<uintptr_t>(p.b);
     const bool vec = p.D % VEC == 0 && ends % 16 == 0 && (p.rows == 1 || (p.xs % VEC == 0 && p.ds % VEC == 0));
-    return vec ? norm_short_run<T, W, VEC>(p, backward, s) : norm_short_run<T, W, 1>(p, backward, s);
+    const int most = backward || !vec ? 8192 : 16 * 32 * norm_forward_ept<T, VEC>();  // 16 warps' registers
+    if (p.D <= most) return vec ? norm_short_run<T, VEC>(p, backward, s) : norm_short_run<T, 1>(p, backward, s);
   }
   const unsigned grid = (unsigned)(p.rows < (1 << 20) ? p.rows : (1 << 20));
   if (!backward) {
@@ -489,7 +661,7 @@ int norm_run(NormArgs p, bool backward, cudaStream_t s) {
   if (!p.dw && !p.db) return GFN_OK;
   p.blocks = norm_blocks(p.rows);
   norm_dw_long_kernel<T><<<dim3((p.D + NORM_THREADS - 1) / NORM_THREADS, p.blocks), NORM_THREADS, 0, s>>>(p);
-  norm_dw_sum_kernel<W><<<dim3((p.D + 31) / 32, 2), NORM_THREADS, 0, s>>>(p);
+  norm_dw_sum<W>(p, s);
   return launch_status("norm_dw kernels");
 }
 
