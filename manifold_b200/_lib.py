@@ -138,8 +138,9 @@ def check(status, what):
 
 
 def call(name, *args):
-    fn = getattr(load(), name)
-    check(fn(*args), name)
+    status = getattr(_lib or load(), name)(*args)
+    if status != 0:
+        check(status, name)
 
 
 def ptr(t):
@@ -150,7 +151,10 @@ def ptr(t):
 
 
 def stream_of(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the device's current stream (the raw handle: the Stream object
+    that torch.cuda.current_stream builds around it costs as much as a launch)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def device_error(reset=True, device=None):
@@ -174,20 +178,23 @@ def dtype_code(t, name):
 def call_on(t, name, *args):
     """`call` on tensor t's device, with that device's current stream as the
     last argument (the device is made current when it is not)."""
-    dev = t.device
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, stream_of(dev))
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            call(name, *args, stream_of(dev))
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def same_device(what, first, *others):
     """Every operand on one CUDA device."""
-    require_cuda(first, *others)
+    index = first.get_device() if first.is_cuda else -1
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
+            require_cuda(first, t)
             raise GfnError(f"{what}: operands on {first.device} and {t.device}")
+    if index < 0:
+        require_cuda(first)
 
 
 def require_cuda(*tensors):

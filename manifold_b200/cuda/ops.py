@@ -496,30 +496,34 @@ def layer_scan_forward(z, v0, x0, heads, base_dt, want_last, want_states):
     v0 = None if v0 is None else v0.contiguous()
     x0 = None if x0 is None else x0.contiguous()
     lib = _lib.load()
-    out = torch.empty(2, B, L, D, device=z.device, dtype=torch.float32)
-    last = torch.empty(2, B, D, device=z.device, dtype=torch.float32) if want_last else (None, None)
-    states = None
+    x_seq = z.new_empty((B, L, D))
+    v_seq = torch.empty_like(x_seq)
+    v_last = x_last = states = ws = None
+    if want_last:
+        v_last = z.new_empty((B, D))
+        x_last = torch.empty_like(v_last)
     if want_states:
-        states = torch.empty(lib.gfn_gated_scan_states_floats(B, L, D), device=z.device, dtype=torch.float32)
+        states = z.new_empty(lib.gfn_gated_scan_states_floats(B, L, D))
     n = lib.gfn_gated_scan_workspace_bytes(B, L, D)
-    ws = torch.empty(n, device=z.device, dtype=torch.uint8) if n else None
-    _lib.call_on(z, "gfn_layer_scan_forward", ptr(z), ptr(v0), ptr(x0), B, L, D, int(heads), float(base_dt),
-                 ptr(out[0]), ptr(out[1]), ptr(last[1]), ptr(last[0]), ptr(states), ptr(ws), n)
-    return out[0], out[1], last[0], last[1], states
+    if n:
+        ws = z.new_empty(n, dtype=torch.uint8)
+    _lib.call_on(z, "gfn_layer_scan_forward", z.data_ptr(), ptr(v0), ptr(x0), B, L, D, int(heads), float(base_dt),
+                 x_seq.data_ptr(), v_seq.data_ptr(), ptr(x_last), ptr(v_last), ptr(states), ptr(ws), n)
+    return x_seq, v_seq, v_last, x_last, states
 
 
 def layer_scan_backward(z, states, gx, gv, gvl, gxl, heads, base_dt, want_v0, want_x0):
     """Gradients (dz, dv0, dx0) of the layer scan; any upstream gradient may be None."""
     B, L, D = z.shape[0], z.shape[1], z.shape[2] // 3
     z = z.contiguous()
-    gx, gv, gvl, gxl = (None if g is None else g.contiguous() for g in (gx, gv, gvl, gxl))
+    gx, gv, gvl, gxl = [None if g is None else g.contiguous() for g in (gx, gv, gvl, gxl)]
     dz = torch.empty_like(z)
-    dv0 = torch.empty(B, D, device=z.device, dtype=torch.float32) if want_v0 else None
-    dx0 = torch.empty(B, D, device=z.device, dtype=torch.float32) if want_x0 else None
+    dv0 = z.new_empty((B, D)) if want_v0 else None
+    dx0 = z.new_empty((B, D)) if want_x0 else None
     n = _lib.load().gfn_gated_scan_workspace_bytes(B, L, D)
-    ws = torch.empty(n, device=z.device, dtype=torch.uint8) if n else None
-    _lib.call_on(z, "gfn_layer_scan_backward", ptr(z), ptr(states), ptr(gx), ptr(gv), ptr(gxl), ptr(gvl), B, L, D,
-                 int(heads), float(base_dt), ptr(dz), ptr(dx0), ptr(dv0), ptr(ws), n)
+    ws = z.new_empty(n, dtype=torch.uint8) if n else None
+    _lib.call_on(z, "gfn_layer_scan_backward", z.data_ptr(), states.data_ptr(), ptr(gx), ptr(gv), ptr(gxl), ptr(gvl),
+                 B, L, D, int(heads), float(base_dt), dz.data_ptr(), ptr(dx0), ptr(dv0), ptr(ws), n)
     return dz, dv0, dx0
 
 

@@ -16,36 +16,36 @@ from ._lib import GfnError, call_on, dtype_code, ptr, same_device
 
 
 def _rows(t, dim):
-    """t as [rows, dim] with inner stride 1 (a view where one exists)."""
-    t = t.reshape(-1, dim)
-    return t if dim == 1 or t.stride(1) == 1 else t.contiguous()
-
-
-def _row_stride(t, dim):
-    return t.stride(0) if t.shape[0] > 1 else dim
+    """(t or a copy of it, rows, row stride): rows of `dim` elements with inner
+    stride 1, in place where t has them."""
+    if t.is_contiguous():
+        return t, t.numel() // dim, dim
+    r = t.reshape(-1, dim)
+    if (dim > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < dim):  # rows that overlap are expanded ones
+        r = r.contiguous()
+    return r, r.shape[0], r.stride(0) if r.shape[0] > 1 else dim
 
 
 def _forward(x, weight, bias, eps, want_stats):
     D = x.shape[-1]
-    xr = _rows(x, D)
-    if xr.shape[0] > 1 and xr.stride(0) < D:  # rows that overlap (an expanded input)
-        xr = xr.contiguous()
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    stats = torch.empty(xr.shape[0], 2, device=x.device, dtype=torch.float32) if want_stats else None
+    xr, rows, stride = _rows(x, D)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
     w = weight if weight is not None else bias
-    code = dtype_code(x, "x")
-    call_on(x, "gfn_layer_norm_forward", ptr(xr), _row_stride(xr, D), ptr(weight), ptr(bias), code,
-            code if w is None else dtype_code(w, "weight"), xr.shape[0], D, float(eps), ptr(y), ptr(stats))
-    return y, xr, stats
+    code = _lib.DTYPES[x.dtype]
+    call_on(x, "gfn_layer_norm_forward", xr.data_ptr(), stride, ptr(weight), ptr(bias), code,
+            code if w is None else _lib.DTYPES[w.dtype], rows, D, eps, y.data_ptr(), ptr(stats))
+    return y, stats
 
 
 class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, xr, stats = _forward(x, weight, bias, eps, True)
-        # the caller's own tensor where possible, so that a later in-place change of it is noticed
+        y, stats = _forward(x, weight, bias, eps, True)
+        # the caller's own tensor, so that a later in-place change of it is noticed
         ctx.save_for_backward(x, weight, stats)
-        ctx.bias_like = None if bias is None else bias.dtype
+        w = weight if weight is not None else bias
+        ctx.wdt = x.dtype if w is None else w.dtype
         return y
 
     @staticmethod
@@ -53,24 +53,18 @@ class LayerNormFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         D = x.shape[-1]
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        xr, dr = _rows(x, D), _rows(dy, D)
-        rows = xr.shape[0]
-        if rows > 1 and xr.stride(0) < D:
-            xr = xr.contiguous()
-        if rows > 1 and dr.stride(0) < D:
-            dr = dr.contiguous()
-        wdt = weight.dtype if weight is not None else (ctx.bias_like or x.dtype)
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need_x else None
-        dw = torch.empty(D, device=x.device, dtype=wdt) if need_w else None
-        db = torch.empty(D, device=x.device, dtype=wdt) if need_b else None
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        xr, rows, xs = _rows(x, D)
+        dr, _, ds = _rows(dy, D)
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+        dw = x.new_empty(D, dtype=ctx.wdt) if need_w else None
+        db = x.new_empty(D, dtype=ctx.wdt) if need_b else None
         ws, n = None, 0
         if need_w or need_b:
             n = _lib.load().gfn_layer_norm_backward_workspace_floats(rows, D)
-            ws = torch.empty(n, device=x.device, dtype=torch.float32)
-        call_on(x, "gfn_layer_norm_backward", ptr(xr), _row_stride(xr, D), ptr(dr), _row_stride(dr, D),
-                ptr(weight), ptr(stats), dtype_code(x, "x"), _lib.DTYPES[wdt], rows, D, ptr(dx), ptr(dw),
-                ptr(db), ptr(ws), n)
+            ws = x.new_empty(n, dtype=torch.float32)
+        call_on(x, "gfn_layer_norm_backward", xr.data_ptr(), xs, dr.data_ptr(), ds, ptr(weight), stats.data_ptr(),
+                _lib.DTYPES[x.dtype], _lib.DTYPES[ctx.wdt], rows, D, ptr(dx), ptr(dw), ptr(db), ptr(ws), n)
         return dx, dw, db, None
 
 
@@ -87,21 +81,27 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise GfnError(f"layer_norm: x must have a last dimension of at least 1, got {tuple(x.shape)}")
     dtype_code(x, "x")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if t.shape != (x.shape[-1],):
-            raise GfnError(f"layer_norm: {name} must be [{x.shape[-1]}], got {tuple(t.shape)}")
-        if t.dtype not in (torch.float32, x.dtype):
-            raise GfnError(f"layer_norm: {name} must be float32 or {x.dtype}, got {t.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise GfnError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    grad = torch.is_grad_enabled()
+    wants = grad and x.requires_grad
+    if weight is not None:
+        weight = _weight("weight", weight, x)
+        wants = wants or (grad and weight.requires_grad)
+    if bias is not None:
+        bias = _weight("bias", bias, x)
+        wants = wants or (grad and bias.requires_grad)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise GfnError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
+    if wants:
         return LayerNormFn.apply(x, weight, bias, eps)
     return _forward(x, weight, bias, eps, False)[0]
+
+
+def _weight(name, t, x):
+    if t.dim() != 1 or t.shape[0] != x.shape[-1]:
+        raise GfnError(f"layer_norm: {name} must be [{x.shape[-1]}], got {tuple(t.shape)}")
+    if t.dtype != torch.float32 and t.dtype != x.dtype:
+        raise GfnError(f"layer_norm: {name} must be float32 or {x.dtype}, got {t.dtype}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class LayerNorm(nn.LayerNorm):

@@ -19,15 +19,16 @@ def pack_token_mask(mask):
     return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
 
 
-def _per_row(v, name, B, positive):
-    """(number, per-row tensor or None) of a parameter given as either."""
-    if not torch.is_tensor(v):
+def _per_row(v, name, x, positive):
+    """(number, pointer or None) of a parameter given as a number or per row of x."""
+    if not isinstance(v, torch.Tensor):
         if positive and not v > 0:
             raise GfnError(f"process_logits: {name} must be positive, got {v}")
-        return float(v), None
-    if v.dtype != torch.float32 or v.shape != (B,):
-        raise GfnError(f"process_logits: {name} must be a number or float32 [{B}], got {v.dtype} {tuple(v.shape)}")
-    return 1.0, v.contiguous()
+        return v, None
+    if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != x.shape[0] or v.get_device() != x.get_device():
+        raise GfnError(f"process_logits: {name} must be a number or float32 [{x.shape[0]}] on {x.device}, got "
+                       f"{v.dtype} {tuple(v.shape)} on {v.device}")
+    return 1.0, v if v.is_contiguous() else v.contiguous()
 
 
 def _rows_or_shared(t, name, B, n):
@@ -39,10 +40,11 @@ def _rows_or_shared(t, name, B, n):
     return t, (t.stride(0) if t.dim() == 2 else 0)
 
 
-def _index(t, name, shape):
-    if t.dtype not in (torch.int64, torch.int32) or t.shape != shape:
-        raise GfnError(f"process_logits: {name} must be int64 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
-    return t.to(torch.int64)
+def _lengths(t, name, B):
+    if t.dim() != 1 or t.shape[0] != B or (t.dtype != torch.int64 and t.dtype != torch.int32):
+        raise GfnError(f"process_logits: {name} must be int64 [{B}], got {t.dtype} {tuple(t.shape)}")
+    t = t if t.dtype == torch.int64 else t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repetition_penalty=1.0,
@@ -66,27 +68,30 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
     same_device("process_logits", logits, tokens, lengths, prompt_lengths, bias, allowed)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise GfnError(f"process_logits: logits must be [batch, vocab], got {tuple(logits.shape)}")
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         raise GfnError("process_logits is not differentiable: call it under torch.no_grad() or on logits.detach()")
     code = dtype_code(logits, "logits")
     B, V = logits.shape
-    x = logits if V == 1 or logits.stride(1) == 1 else logits.contiguous()
-    T = 0
+    x = logits if logits.is_contiguous() or V == 1 or logits.stride(1) == 1 else logits.contiguous()
+    T = ts = 0
     if tokens is not None:
-        tokens = _index(tokens, "tokens", (B, tokens.shape[-1]))
+        if tokens.dim() != 2 or tokens.shape[0] != B or (tokens.dtype != torch.int64 and tokens.dtype != torch.int32):
+            raise GfnError(f"process_logits: tokens must be int64 [{B}, T], got {tokens.dtype} {tuple(tokens.shape)}")
         T = tokens.shape[1]
-        if T > 1 and tokens.stride(1) != 1:
+        if tokens.dtype != torch.int64:
+            tokens = tokens.to(torch.int64)
+        ts, step = tokens.stride()
+        if T > 1 and step != 1:
             tokens = tokens.contiguous()
-        lengths = None if lengths is None else _index(lengths, "lengths", (B,)).contiguous()
-        if prompt_lengths is not None:
-            prompt_lengths = _index(prompt_lengths, "prompt_lengths", (B,)).contiguous()
+            ts = T
+        lengths = None if lengths is None else _lengths(lengths, "lengths", B)
+        prompt_lengths = None if prompt_lengths is None else _lengths(prompt_lengths, "prompt_lengths", B)
     elif lengths is not None or prompt_lengths is not None:
         raise GfnError("process_logits: lengths need tokens")
-    rep, rep_rows = _per_row(repetition_penalty, "repetition_penalty", B, True)
-    freq, freq_rows = _per_row(frequency_penalty, "frequency_penalty", B, False)
-    pres, pres_rows = _per_row(presence_penalty, "presence_penalty", B, False)
-    temp, temp_rows = _per_row(temperature, "temperature", B, True)
-    same_device("process_logits", logits, rep_rows, freq_rows, pres_rows, temp_rows)
+    rep, rep_rows = _per_row(repetition_penalty, "repetition_penalty", logits, True)
+    freq, freq_rows = _per_row(frequency_penalty, "frequency_penalty", logits, False)
+    pres, pres_rows = _per_row(presence_penalty, "presence_penalty", logits, False)
+    temp, temp_rows = _per_row(temperature, "temperature", logits, True)
     bs = ms = 0
     if bias is not None:
         bias, bs = _rows_or_shared(bias.to(torch.float32), "bias", B, V)
@@ -98,8 +103,8 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
         if allowed.dtype != torch.int32:
             raise GfnError(f"process_logits: allowed must be bool or int32 words, got {allowed.dtype}")
         allowed, ms = _rows_or_shared(allowed, "allowed", B, (V + 31) // 32)
-    out = torch.empty(B, V, device=logits.device, dtype=logits.dtype)
-    call_on(logits, "gfn_process_logits", ptr(x), x.stride(0) if B > 1 else V, code, B, V, ptr(tokens),
-            tokens.stride(0) if T else 0, T, ptr(lengths), ptr(prompt_lengths), rep, ptr(rep_rows), freq,
-            ptr(freq_rows), pres, ptr(pres_rows), temp, ptr(temp_rows), ptr(bias), bs, ptr(allowed), ms, ptr(out))
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    call_on(logits, "gfn_process_logits", x.data_ptr(), x.stride(0) if B > 1 else V, code, B, V, ptr(tokens), ts, T,
+            ptr(lengths), ptr(prompt_lengths), rep, ptr(rep_rows), freq, ptr(freq_rows), pres, ptr(pres_rows), temp,
+            ptr(temp_rows), ptr(bias), bs, ptr(allowed), ms, out.data_ptr())
     return out

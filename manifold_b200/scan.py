@@ -25,29 +25,31 @@ def parallel_scan(a, x):
 def _operand(t):
     """t [B, L, D] with inner stride 1 (itself where it has one: strided and
     broadcast batches and steps are read in place)."""
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def _workspace(x):
-    n = _lib.load().gfn_gated_scan_workspace_bytes(*x.shape)
-    return (torch.empty(n, device=x.device, dtype=torch.uint8) if n else None), n
+def _workspace(x, B, L, D):
+    n = _lib.load().gfn_gated_scan_workspace_bytes(B, L, D)
+    return (x.new_empty(n, dtype=torch.uint8) if n else None), n
 
 
 def _forward(a, x, h0, want_last, want_states):
     B, L, D = x.shape
     x = _operand(x)
-    a = None if a is None else _operand(a)
     h0 = None if h0 is None else h0.contiguous()
-    h = torch.empty(B, L, D, device=x.device, dtype=x.dtype)
-    last = torch.empty(B, D, device=x.device, dtype=torch.float32) if want_last else None
+    h = torch.empty_like(x, memory_format=torch.contiguous_format)
+    last = x.new_empty((B, D), dtype=torch.float32) if want_last else None
     states = None
     if want_states:
-        states = torch.empty(_lib.load().gfn_gated_scan_states_floats(B, L, D), device=x.device,
-                             dtype=torch.float32)
-    ws, n = _workspace(x)
-    sa = (0, 0) if a is None else a.stride()[:2]
-    call_on(x, "gfn_gated_scan_forward", ptr(a), *sa, ptr(x), *x.stride()[:2], ptr(h0), _lib.DTYPES[x.dtype],
-            B, L, D, ptr(h), ptr(last), ptr(states), ptr(ws), n)
+        states = x.new_empty(_lib.load().gfn_gated_scan_states_floats(B, L, D), dtype=torch.float32)
+    ws, n = _workspace(x, B, L, D)
+    pa = sa = ta = 0
+    if a is not None:
+        a = _operand(a)
+        pa, (sa, ta, _) = a.data_ptr(), a.stride()
+    sx, tx, _ = x.stride()
+    call_on(x, "gfn_gated_scan_forward", pa, sa, ta, x.data_ptr(), sx, tx, ptr(h0), _lib.DTYPES[x.dtype], B, L, D,
+            h.data_ptr(), ptr(last), ptr(states), ptr(ws), n)
     return h, last, states
 
 
@@ -67,16 +69,21 @@ class GatedScanFn(torch.autograd.Function):
             return None, None, None
         B, L, D = x.shape
         need_a, need_x, need_h0 = ctx.needs_input_grad
-        ao, xo = None if a is None else _operand(a), _operand(x)
-        dh = None if dh is None else _operand(dh)
+        x = _operand(x)
         dlast = None if dlast is None else dlast.contiguous()
-        da = torch.empty(B, L, D, device=x.device, dtype=x.dtype) if need_a else None
-        dx = torch.empty(B, L, D, device=x.device, dtype=x.dtype) if need_x else None
-        dh0 = torch.empty(B, D, device=x.device, dtype=torch.float32) if need_h0 else None
-        ws, n = _workspace(x)
-        sa = (0, 0) if a is None else ao.stride()[:2]
-        sg = (0, 0) if dh is None else dh.stride()[:2]
-        call_on(x, "gfn_gated_scan_backward", ptr(ao), *sa, ptr(xo), *xo.stride()[:2], ptr(states), ptr(dh), *sg,
+        da = torch.empty_like(x, memory_format=torch.contiguous_format) if need_a else None
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+        dh0 = x.new_empty((B, D), dtype=torch.float32) if need_h0 else None
+        ws, n = _workspace(x, B, L, D)
+        pa = sa = ta = pg = sg = tg = 0
+        if a is not None:
+            a = _operand(a)
+            pa, (sa, ta, _) = a.data_ptr(), a.stride()
+        if dh is not None:
+            dh = _operand(dh)
+            pg, (sg, tg, _) = dh.data_ptr(), dh.stride()
+        sx, tx, _ = x.stride()
+        call_on(x, "gfn_gated_scan_backward", pa, sa, ta, x.data_ptr(), sx, tx, states.data_ptr(), pg, sg, tg,
                 ptr(dlast), _lib.DTYPES[x.dtype], B, L, D, ptr(da), ptr(dx), ptr(dh0), ptr(ws), n)
         return da, dx, dh0
 
