@@ -5,9 +5,11 @@ The library is built in-tree (``manifold_b200/libgfn_b200.so``) by
 missing or a call fails, a ``GfnError`` is raised.
 """
 import ctypes
+import functools
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GFN_B200_LIB") or os.path.join(_HERE, "libgfn_b200.so")
@@ -195,6 +197,19 @@ def same_device(what, first, *others):
             raise GfnError(f"{what}: operands on {first.device} and {t.device}")
     if index < 0:
         require_cuda(first)
+
+
+def first_order(backward):
+    """Decorator of an autograd Function's backward whose result is not
+    differentiable: once_differentiable, entered only when a graph of the
+    gradients is being recorded (its bookkeeping costs as much as a launch)."""
+    checked = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def require_cuda(*tensors):

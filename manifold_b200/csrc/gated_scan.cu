@@ -29,13 +29,21 @@ constexpr long long TICKET_BYTES = 256;  // the ticket, then the words
 
 // The runs and tiles of a launch, and its words in the workspace (all ones).
 template <class Args>
-int set_tiles(const char* what, Args* p, int run, int ct, int words, void* workspace, long long bytes,
+int set_tiles(const char* what, Args* p, int run, int ct, int words, int occ, void* workspace, long long bytes,
               cudaStream_t s, unsigned* grid) {
   p->nchunks = (p->L + run - 1) / run;
   p->ctiles = (p->D + ct - 1) / ct;
   const long long tiles = (long long)p->B * p->ctiles, blocks = tiles * p->nchunks;
   if (blocks > 0x7fffffffLL) return fail(GFN_ERR_UNSUPPORTED, "%s: %lld blocks", what, blocks);
   *grid = (unsigned)blocks;
+  // The runs of one column tile that are under way at once wait for one another
+  // once per group.  With at most one of them a chain of states is enough
+  // (composing maps nobody waits for cost 12 of 154 instructions per element in
+  // the layer's backward); with more a group covers them twice over.
+  const long long slots = 148LL * occ;
+  p->group = 1;
+  if (tiles < slots)
+    while (p->group < SCAN_GROUP && tiles * p->group < 2 * slots) p->group *= 2;
   p->words = nullptr;
   p->ticket = nullptr;
   if (p->nchunks == 1) return GFN_OK;
@@ -110,7 +118,7 @@ int launch(const char* what, void (*kernel)(Args, ScanMaps), const Args& p, cons
 template <int MODE, typename T, int VEC, int S, int NW, int OCC>
 int gscan_forward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   unsigned blocks;
-  const int st = set_tiles("gated_scan_forward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &blocks);
+  const int st = set_tiles("gated_scan_forward", &p, S * NW, 32 * VEC, 1, OCC, ws, bytes, s, &blocks);
   if (st) return st;
   ScanMaps maps = {};
   if (MODE == SCAN_TMA) {
@@ -125,7 +133,7 @@ int gscan_forward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
 template <int MODE, typename T, int VEC, int S, int NW, int OCC>
 int gscan_backward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   unsigned blocks;
-  const int st = set_tiles("gated_scan_backward", &p, S * NW, 32 * VEC, 1, ws, bytes, s, &blocks);
+  const int st = set_tiles("gated_scan_backward", &p, S * NW, 32 * VEC, 1, OCC, ws, bytes, s, &blocks);
   if (st) return st;
   ScanMaps maps = {};
   if (MODE == SCAN_TMA) {
@@ -149,10 +157,10 @@ int gscan_run(const GScanArgs& p, bool backward, void* ws, long long bytes, cuda
                     rows16(p.x, p.x_sb, p.x_st, p.B, p.L, z) && rows16(p.dh, p.g_sb, p.g_st, p.B, p.L, z) &&
                     aligned16(p.h) && aligned16(p.da) && aligned16(p.dx);
   if (tma)
-    return backward ? gscan_backward<SCAN_TMA, T, 2, 8, 8, z == 2 ? 4 : 2>(p, ws, bytes, s)
+    return backward ? gscan_backward<SCAN_TMA, T, 2, 8, 8, z == 2 ? 3 : 2>(p, ws, bytes, s)
                     : gscan_forward<SCAN_TMA, T, 2, z == 2 ? 32 : 16, 8, 2>(p, ws, bytes, s);
   return backward ? gscan_backward<SCAN_PLAIN, T, 1, 8, 8, 4>(p, ws, bytes, s)
-                  : gscan_forward<SCAN_PLAIN, T, 1, 16, 8, 4>(p, ws, bytes, s);
+                  : gscan_forward<SCAN_PLAIN, T, 1, 16, 8, 3>(p, ws, bytes, s);
 }
 
 int gscan_dispatch(const GScanArgs& p, int dtype, bool backward, void* ws, long long bytes, cudaStream_t s) {
@@ -166,7 +174,7 @@ template <int MODE>
 int lscan_forward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   constexpr int VEC = 1, S = 16, NW = 8, OCC = 2;
   unsigned blocks;
-  const int st = set_tiles("layer_scan_forward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &blocks);
+  const int st = set_tiles("layer_scan_forward", &p, S * NW, 32 * VEC, 2, OCC, ws, bytes, s, &blocks);
   if (st) return st;
   ScanMaps maps = {};
   if (MODE == SCAN_TMA) {
@@ -182,7 +190,7 @@ template <int MODE>
 int lscan_backward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
   constexpr int VEC = 1, S = 8, NW = 8, OCC = 2;
   unsigned blocks;
-  const int st = set_tiles("layer_scan_backward", &p, S * NW, 32 * VEC, 2, ws, bytes, s, &blocks);
+  const int st = set_tiles("layer_scan_backward", &p, S * NW, 32 * VEC, 2, OCC, ws, bytes, s, &blocks);
   if (st) return st;
   ScanMaps maps = {};
   if (MODE == SCAN_TMA) {

@@ -18,7 +18,7 @@
 // h -> P h + p; the warps' maps meet in shared memory, the blocks' maps in
 // global memory, and then the block walks its registers once more to write the
 // results.  Many blocks per column tile keep the memory busy when batch * dim
-// is far too small to fill the GPU.  Runs form groups of SCAN_GROUP: a run
+// is far too small to fill the GPU.  Runs form groups: a run
 // composes the maps of its group before it and applies them to the state at
 // the group's start, which the group before publishes.  What is composed with
 // what does not depend on which block is faster, so results repeat bit for bit.
@@ -49,6 +49,7 @@ struct GScanArgs {
   unsigned* ticket;
   int B, L, D, nck;
   int nchunks, ctiles;  // runs of steps per column; column tiles per batch row
+  int group;            // runs whose maps are composed; the states pass from group to group
 };
 
 // ------------------------------------------------------------ published words
@@ -102,7 +103,7 @@ struct GatedState {
   GFN_DEV GatedState through(GatedMap m) const { return {pass(m.P, h, m.p)}; }
 };
 
-constexpr int SCAN_GROUP = 32;  // runs whose maps are composed; the states pass from group to group
+constexpr int SCAN_GROUP = 32;  // the most runs in a group
 
 // N maps (or states) that other blocks publish for one column, from `src` on,
 // `stride` words apart.
@@ -174,13 +175,13 @@ struct ScanShared {
 // on all threads once this block's map is out.
 template <class Map, class State, int CT, int NW, bool REV, class First, class Beside, class Ahead>
 GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* words, int chunk, int nchunks,
-                     int live, First first, Beside beside, Ahead ahead) {
+                     int group, int live, First first, Beside beside, Ahead ahead) {
   static_assert(ScanShared<Map, State, CT, NW>::R >= 2, "a second thread per column");
   constexpr int W = Map::WORDS, R = NW * 32 / CT, GS = SCAN_GROUP / R;
   constexpr int BATCH = GS < 8 ? GS : 8;
   const int c = threadIdx.x % CT, r = threadIdx.x / CT;
   const bool active = c < live, teller = r == R - 1 && active;
-  const int pos = chunk % SCAN_GROUP, start = chunk - pos;
+  const int pos = chunk % group, start = chunk - pos;
   const bool tells = teller && chunk + 1 < nchunks;
   unsigned long long* mine = words + (long long)chunk * W * CT + c;
   Map own = Map::identity();
@@ -198,7 +199,7 @@ GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* wor
       }
       own = Map::compose(Map::unpack(x), own);
     }
-    if (tells && pos < SCAN_GROUP - 1) publish(own, mine, CT);
+    if (tells && pos < group - 1) publish(own, mine, CT);
   }
   ahead();
   if (r == 0) beside(c);
@@ -236,7 +237,7 @@ GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* wor
     State at[1];  // at the group's start
     if (start > 0) await<State, 1>(words + (long long)(start - 1) * W * CT + c, 0, CT, 1, at);
     else at[0] = first(c);
-    if (tells && pos == SCAN_GROUP - 1) publish(at[0].through(Map::compose(own, acc)), mine, CT);
+    if (tells && pos == group - 1) publish(at[0].through(Map::compose(own, acc)), mine, CT);
     sh.in[c] = at[0].through(acc);
   }
   __syncthreads();
@@ -485,7 +486,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_forward_kernel(const GScan
     }
     turn.tell(p, sh.slot, it);
     receive<GatedMap, GatedState, CT, NW, false>(
-        sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
+        sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.group, p.D - q.c0,
         [&](int c) { return GatedState{p.h0 ? p.h0[(long long)q.b * p.D + q.c0 + c] : 0.f}; },
         [](int) {},
         [&] {
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GSca
     turn.tell(p, sh.slot, it);
     const int run = p.nchunks - 1 - q.chunk;
     receive<GatedMap, GatedState, CT, NW, true>(
-        sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.D - q.c0,
+        sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.group, p.D - q.c0,
         [&](int c) { return GatedState{p.dlast ? p.dlast[(long long)q.b * p.D + q.c0 + c] : 0.f}; },
         [&](int c) {
           chain_states<CT, NW>(fmaps, p.states + ((long long)q.b * p.nck + run) * p.D + q.c0, c, p.D - q.c0, hstart);
@@ -688,7 +689,7 @@ struct LScanArgs {
   float* dx0;
   unsigned long long* words;  // as in GScanArgs
   unsigned* ticket;
-  int B, L, D, H, nck, nchunks, ctiles;
+  int B, L, D, H, nck, nchunks, ctiles, group;
   float base_dt;
 };
 
@@ -705,19 +706,18 @@ GFN_DEV float gate(float z, float* slope) {
 }
 
 // softplus(z) = max(z, 0) + log1p(e), e = exp(-|z|) in [0, 1], and its slope
-// sigma(z).  log1p(e) = 2 atanh(y) with y = e / (2 + e) <= 1/3: the odd series
-// up to y^15 leaves 1e-9 of the sum, and every term is positive.
+// sigma(z).  log1p(e) = 2 atanh(y) with y = e / (2 + e) <= 1/3, and
+// atanh(y) / y as a polynomial in y^2 (interpolated at the Chebyshev nodes of
+// [0, 1/9]: within 8e-9 of it, an eighth of a float32 rounding), so that a
+// small step keeps its digits, which log(1 + e) would lose.
 GFN_DEV float soft_step(float z, float* slope) {
   const float e = expf(-fabsf(z));
   const float r = quick_rcp((1.f + e) * (2.f + e));  // both quotients from one reciprocal
   const float y = e * ((1.f + e) * r), y2 = y * y, s = (2.f + e) * r;
-  float q = 1.f / 15.f;
-  q = fmaf(q, y2, 1.f / 13.f);
-  q = fmaf(q, y2, 1.f / 11.f);
-  q = fmaf(q, y2, 1.f / 9.f);
-  q = fmaf(q, y2, 1.f / 7.f);
-  q = fmaf(q, y2, 1.f / 5.f);
-  q = fmaf(q, y2, 1.f / 3.f);
+  float q = 0.14078889f;
+  q = fmaf(q, y2, 0.13982579f);
+  q = fmaf(q, y2, 0.20012298f);
+  q = fmaf(q, y2, 0.33333161f);
   q = fmaf(q * y2, y, y);
   *slope = z >= 0.f ? s : e * s;
   return fmaf(2.f, q, fmaxf(z, 0.f));
@@ -727,6 +727,16 @@ GFN_DEV float head_scale(int col, int hd) {
   float hs = 1.f;
   for (int i = 0; i < col / hd; ++i) hs *= 1.5f;
   return hs;
+}
+
+// A run's product of gates P, held above zero where no gate is zero (see gate_product).
+template <int S, int VEC>
+GFN_DEV float keep_positive(float P, const float (&A)[S][VEC], int v) {
+  if (P != 0.f) return P;
+  bool zero = false;
+#pragma unroll
+  for (int s = 0; s < S; ++s) zero = zero || A[s][v] == 0.f;
+  return zero ? 0.f : 1.4e-45f;
 }
 
 struct LayerMap {  // v -> P v + p, x -> x + Q v + q
@@ -787,34 +797,41 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScan
       load_rows<float, VEC, S>(pb, zp + 2LL * p.D, 3LL * p.D, c.n);
     }
     turn.draw(p);
+    if (c.n < S) {  // beyond the end: A = 1, dt = 0
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s >= c.n) {
+          pa[s] = Pack<float, VEC>::fill(INFINITY);
+          pd[s] = Pack<float, VEC>::fill(-INFINITY);
+          pb[s] = Pack<float, VEC>::fill(0.f);
+        }
+      }
+    }
     float A[S][VEC], dt[S][VEC], bv[S][VEC];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {  // beyond the end: A = 1, dt = 0
-        const bool on = s < c.n;
+      for (int v = 0; v < VEC; ++v) {
         float slope;
-        A[s][v] = gate(on ? pa[s].get(v) : INFINITY, &slope);
-        dt[s][v] = soft_step(on ? pd[s].get(v) : -INFINITY, &slope);
-        bv[s][v] = on ? pb[s].get(v) : 0.f;
+        A[s][v] = gate(pa[s].get(v), &slope);
+        dt[s][v] = soft_step(pd[s].get(v), &slope);
+        bv[s][v] = pb[s].get(v);
       }
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
       LayerMap m = LayerMap::identity();
-      bool zero = false;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         dt[s][v] *= scale;
         bv[s][v] *= dt[s][v];
-        zero = zero || A[s][v] == 0.f;
         m.P *= A[s][v];
         m.p = fmaf(A[s][v], m.p, bv[s][v]);
         m.Q = fmaf(dt[s][v], m.P, m.Q);
         m.q = fmaf(dt[s][v], m.p, m.q);
       }
-      if (m.P == 0.f && !zero) m.P = 1.4e-45f;
+      m.P = keep_positive<S, VEC>(m.P, A, v);
       unsigned long long wd[2];
       m.pack(wd);
       sh.maps[w][0][lane * VEC + v] = wd[0];
@@ -822,7 +839,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScan
     }
     turn.tell(p, sh.slot, it);
     receive<LayerMap, LayerState, CT, NW, false>(
-        sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0,
+        sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.group, p.D - c.c0,
         [&](int j) {
           const long long e = (long long)c.b * p.D + c.c0 + j;
           return LayerState{p.v0 ? p.v0[e] : 0.f, p.x0 ? p.x0[e] : 0.f};
@@ -937,34 +954,43 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
       if (p.gv) load_rows<float, VEC, S>(pv, p.gv + o, p.D, c.n);
     }
     turn.draw(p);
+    if (c.n < S || !p.gx || !p.gv) {  // beyond the end: A = 1, dt = 0, no gradients
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s >= c.n) {
+          pa[s] = Pack<float, VEC>::fill(INFINITY);
+          pd[s] = Pack<float, VEC>::fill(-INFINITY);
+          pb[s] = Pack<float, VEC>::fill(0.f);
+        }
+        if (s >= c.n || !p.gx) px[s] = Pack<float, VEC>::fill(0.f);
+        if (s >= c.n || !p.gv) pv[s] = Pack<float, VEC>::fill(0.f);
+      }
+    }
     float A[S][VEC], dt[S][VEC], zb[S][VEC], gx[S][VEC], gv[S][VEC];
     float sa[S][VEC], sd[S][VEC];  // slopes of A and dt
 #pragma unroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {  // beyond the end: A = 1, dt = 0, no gradients
-        const bool on = s < c.n;
-        A[s][v] = gate(on ? pa[s].get(v) : INFINITY, &sa[s][v]);
-        dt[s][v] = soft_step(on ? pd[s].get(v) : -INFINITY, &sd[s][v]);
-        zb[s][v] = on ? pb[s].get(v) : 0.f;
-        gx[s][v] = on && p.gx ? px[s].get(v) : 0.f;
-        gv[s][v] = on && p.gv ? pv[s].get(v) : 0.f;
+      for (int v = 0; v < VEC; ++v) {
+        A[s][v] = gate(pa[s].get(v), &sa[s][v]);
+        dt[s][v] = soft_step(pd[s].get(v), &sd[s][v]);
+        zb[s][v] = pb[s].get(v);
+        gx[s][v] = px[s].get(v);
+        gv[s][v] = pv[s].get(v);
       }
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
       GatedMap mf = GatedMap::identity();
-      bool zero = false;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         dt[s][v] *= scale;
         sd[s][v] *= scale;
-        zero = zero || A[s][v] == 0.f;
         mf.P *= A[s][v];
         mf.p = fmaf(A[s][v], mf.p, zb[s][v] * dt[s][v]);
       }
-      if (mf.P == 0.f && !zero) mf.P = 1.4e-45f;
+      mf.P = keep_positive<S, VEC>(mf.P, A, v);
       LayerBackMap mb = LayerBackMap::identity();
       mb.P = mf.P;
 #pragma unroll
@@ -983,7 +1009,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
     turn.tell(p, sh.slot, it);
     const int run = p.nchunks - 1 - c.chunk;
     receive<LayerBackMap, LayerBackState, CT, NW, true>(
-        sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.D - c.c0,
+        sh, p.words + c.tile * p.nchunks * (2LL * CT), c.chunk, p.nchunks, p.group, p.D - c.c0,
         [&](int j) {
           const long long e = (long long)c.b * p.D + c.c0 + j;
           return LayerBackState{p.gvl ? p.gvl[e] : 0.f, p.gxl ? p.gxl[e] : 0.f};

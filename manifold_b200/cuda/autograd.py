@@ -5,8 +5,8 @@ reverse replay that returns the gradients of every operand, the friction
 gate's weights included."""
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
+from .._lib import first_order
 from . import ops
 
 
@@ -87,7 +87,7 @@ class LayerScanFn(Function):
         return xs, vs, vl, xl
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, gx, gv, gvl, gxl):
         if gx is None and gv is None and gvl is None and gxl is None:
             return None, None, None, None, None

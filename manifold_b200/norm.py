@@ -9,10 +9,9 @@ return the gradients of x, weight and bias.  CUDA tensors only.
 """
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import GfnError, call_on, dtype_code, ptr, same_device
+from ._lib import GfnError, call_on, dtype_code, first_order, ptr, same_device
 
 
 def _rows(t, dim):
@@ -49,7 +48,7 @@ class LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         D = x.shape[-1]

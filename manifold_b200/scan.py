@@ -3,10 +3,9 @@ as one work-efficient pass per column on the GPU (no Hillis-Steele passes),
 and the gated scan: the same recurrence with gradients, a carried state and
 16-bit operands."""
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import GfnError, call_on, dtype_code, ptr, same_device
+from ._lib import GfnError, call_on, dtype_code, first_order, ptr, same_device
 from .cuda.ops import _grad_wanted, parallel_scan_fused
 
 CUDA_AVAILABLE = True
@@ -62,7 +61,7 @@ class GatedScanFn(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @once_differentiable
+    @first_order
     def backward(ctx, dh, dlast):
         a, x, states = ctx.saved_tensors
         if dh is None and dlast is None:
