@@ -44,7 +44,7 @@ enum { GFN_F32 = 0, GFN_BF16 = 1, GFN_F16 = 2 };
 
 /* Device error bits recorded by kernels. */
 enum {
-  GFN_DEVERR_MBAR_TIMEOUT = 1, /* a bounded wait for a bulk copy gave up */
+  GFN_DEVERR_MBAR_TIMEOUT = 1, /* a bounded wait (bulk copy, another block's scan state) gave up */
   GFN_DEVERR_BAD_TOKEN = 2,    /* a token id outside [0, vocab) (force 0 used) */
   GFN_DEVERR_F16_RANGE = 4,    /* layered GFN_MIX_SPLIT_F16: an activation |x| >= 2^15 */
 };
@@ -509,7 +509,8 @@ int gfn_layer_norm_backward(const void* x, long long x_row_stride, const void* d
  * (contiguous) and dh0 may be NULL.  Length 0 passes the state through.
  * States are float32.  `workspace` of gfn_gated_scan_workspace_bytes(),
  * 16-byte aligned, serves both passes of both scans; calls that run at the
- * same time need one each. */
+ * same time need one each.  Rows that start on 16 bytes (no stride of zero)
+ * travel by tensor copies.  Results repeat bit for bit. */
 long long gfn_gated_scan_states_floats(int batch, int length, int dim);
 long long gfn_gated_scan_workspace_bytes(int batch, int length, int dim);
 int gfn_gated_scan_forward(const void* a, long long a_batch_stride, long long a_step_stride, const void* x,

@@ -28,7 +28,7 @@ def _operand(t):
 
 
 def _workspace(x, B, L, D):
-    n = _lib.load().gfn_gated_scan_workspace_bytes(B, L, D)
+    n = _lib.load().gfn_gated_scan_workspace_bytes(B, L, D) if L > 1 else 0
     return (x.new_empty(n, dtype=torch.uint8) if n else None), n
 
 
@@ -108,6 +108,7 @@ def gated_scan(a, x, h0=None, return_state=False):
     dtype_code(x, "x")
     if x.dim() != 3:
         raise GfnError(f"gated_scan: x must be [batch, length, dim], got {tuple(x.shape)}")
+    wants = x.requires_grad
     if a is not None:
         if a.dtype != x.dtype:
             raise GfnError(f"gated_scan: a is {a.dtype}, x {x.dtype}")
@@ -116,10 +117,13 @@ def gated_scan(a, x, h0=None, return_state=False):
                 a = a.expand(x.shape)
             except RuntimeError:
                 raise GfnError(f"gated_scan: a {tuple(a.shape)} does not broadcast to {tuple(x.shape)}") from None
-    if h0 is not None and (h0.dtype != torch.float32 or h0.shape != (x.shape[0], x.shape[2])):
-        raise GfnError(f"gated_scan: h0 must be float32 [{x.shape[0]}, {x.shape[2]}], got {h0.dtype} "
-                       f"{tuple(h0.shape)}")
-    if _grad_wanted(a, x, h0):
+        wants = wants or a.requires_grad
+    if h0 is not None:
+        if h0.dtype != torch.float32 or h0.shape != (x.shape[0], x.shape[2]):
+            raise GfnError(f"gated_scan: h0 must be float32 [{x.shape[0]}, {x.shape[2]}], got {h0.dtype} "
+                           f"{tuple(h0.shape)}")
+        wants = wants or h0.requires_grad
+    if wants and torch.is_grad_enabled():
         h, last = GatedScanFn.apply(a, x, h0)
     else:
         h, last, _ = _forward(a, x, h0, return_state, False)

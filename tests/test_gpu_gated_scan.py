@@ -172,6 +172,31 @@ def test_gated_scan_zero_gates_start_new_sequences(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gated_scan_growing_gates(dtype):
+    a, x, h0, dh, dl = _inputs(2, 400, 48, dtype, 17, 0.95)
+    _run((a * 1.06).to(dtype), x, h0, dh, dl)
+
+
+@pytest.mark.gpu
+def test_gated_scan_calls_on_two_streams_at_once():
+    # blocks of one call wait for one another, never for another call's
+    args = [_inputs(1, 20000, 96, torch.bfloat16, 30 + i, 0.9)[:3] for i in range(2)]
+    want = [gfn.gated_scan(*t) for t in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(gfn.gated_scan(*args[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
+    assert gfn.cuda.ops.device_error() == 0
+
+
+@pytest.mark.gpu
 def test_gated_scan_underflowing_products():
     # the product of a run's gates is below float32; the state is not lost to NaN
     a = torch.full((1, 900, 64), 1e-3, device=DEV)
