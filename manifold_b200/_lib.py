@@ -181,7 +181,7 @@ def call_on(t, name, *args):
     """`call` on tensor t's device, with that device's current stream as the
     last argument (the device is made current when it is not)."""
     index = t.get_device()
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():  # a CUDA tensor exists, so CUDA is initialised
         call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):

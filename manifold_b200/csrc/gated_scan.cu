@@ -5,8 +5,8 @@
 
 #include <mutex>
 
-#include "abi.h"
 #include "gated_scan.cuh"
+#include "lm_host.h"
 
 using namespace gfn;
 using namespace gfn_abi;
@@ -40,7 +40,10 @@ int set_tiles(const char* what, Args* p, int run, int ct, int words, int occ, vo
   // once per group.  With at most one of them a chain of states is enough
   // (composing maps nobody waits for cost 12 of 154 instructions per element in
   // the layer's backward); with more a group covers them twice over.
-  const long long slots = 148LL * occ;
+  int sms = 0;
+  const int st = sm_count(&sms);
+  if (st) return st;
+  const long long slots = (long long)sms * occ;
   p->group = 1;
   if (tiles < slots)
     while (p->group < SCAN_GROUP && tiles * p->group < 2 * slots) p->group *= 2;
@@ -103,13 +106,11 @@ int operand_map(CUtensorMap* m, const T* base, long long sb, long long st, int B
 // A persistent launch: OCC blocks per SM, each with `stage` bytes for the next
 // run's operands.
 template <class Args>
-int launch(const char* what, void (*kernel)(Args, ScanMaps), const Args& p, const ScanMaps& maps, unsigned blocks, int occ, int threads, int stage,
-           cudaStream_t s) {
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, stage);
-  if (e != cudaSuccess) return cuda_status(e, what);
+int launch(const char* what, void (*kernel)(Args, ScanMaps), const Args& p, const ScanMaps& maps, unsigned blocks,
+           int occ, int threads, int stage, std::atomic<unsigned long long>* done, cudaStream_t s) {
+  int sms = 0, st = sm_count(&sms);
+  if (!st && stage) st = shared_limit(kernel, stage, done, what);
+  if (st) return st;
   const unsigned slots = (unsigned)(sms * occ);
   kernel<<<blocks < slots ? blocks : slots, threads, stage, s>>>(p, maps);
   return launch_status(what);
@@ -126,8 +127,9 @@ int gscan_forward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
     if (!e) e = operand_map(&maps.m[1], static_cast<const T*>(p.a), p.a_sb, p.a_st, p.B, p.L, p.D, S * NW, 32 * VEC);
     if (e) return e;
   }
+  static std::atomic<unsigned long long> done{0};
   return launch("gscan_forward_kernel", gscan_forward_kernel<MODE, T, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
-                MODE == SCAN_TMA ? 2 * Stage<T, VEC, S, NW>::OPERAND : 0, s);
+                MODE == SCAN_TMA ? 2 * Stage<T, VEC, S, NW>::OPERAND : 0, &done, s);
 }
 
 template <int MODE, typename T, int VEC, int S, int NW, int OCC>
@@ -142,8 +144,9 @@ int gscan_backward(GScanArgs p, void* ws, long long bytes, cudaStream_t s) {
     if (!e) e = operand_map(&maps.m[2], static_cast<const T*>(p.dh), p.g_sb, p.g_st, p.B, p.L, p.D, S * NW, 32 * VEC);
     if (e) return e;
   }
+  static std::atomic<unsigned long long> done{0};
   return launch("gscan_backward_kernel", gscan_backward_kernel<MODE, T, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
-                MODE == SCAN_TMA ? 3 * Stage<T, VEC, S, NW>::OPERAND : 0, s);
+                MODE == SCAN_TMA ? 3 * Stage<T, VEC, S, NW>::OPERAND : 0, &done, s);
 }
 
 template <typename T>
@@ -182,8 +185,9 @@ int lscan_forward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
     int e = operand_map(&maps.m[0], p.z, 3 * D * p.L, 3 * D, p.B, p.L, 3 * p.D, S * NW, 32 * VEC);
     if (e) return e;
   }
+  static std::atomic<unsigned long long> done{0};
   return launch("lscan_forward_kernel", lscan_forward_kernel<MODE, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
-                MODE == SCAN_TMA ? 3 * Stage<float, VEC, S, NW>::OPERAND : 0, s);
+                MODE == SCAN_TMA ? 3 * Stage<float, VEC, S, NW>::OPERAND : 0, &done, s);
 }
 
 template <int MODE>
@@ -200,8 +204,9 @@ int lscan_backward(LScanArgs p, void* ws, long long bytes, cudaStream_t s) {
     if (!e) e = operand_map(&maps.m[2], p.gv, D * p.L, D, p.B, p.L, p.D, S * NW, 32 * VEC);
     if (e) return e;
   }
+  static std::atomic<unsigned long long> done{0};
   return launch("lscan_backward_kernel", lscan_backward_kernel<MODE, VEC, S, NW, OCC>, p, maps, blocks, OCC, NW * 32,
-                MODE == SCAN_TMA ? 5 * Stage<float, VEC, S, NW>::OPERAND : 0, s);
+                MODE == SCAN_TMA ? 5 * Stage<float, VEC, S, NW>::OPERAND : 0, &done, s);
 }
 
 // A state or its gradient handed through a sequence of no steps.

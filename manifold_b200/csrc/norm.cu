@@ -14,7 +14,7 @@
 // Both passes are bound by HBM.  A row is held in registers by the WPR warps
 // that share it (64 bytes a thread forward, 16 elements backward) and read
 // once.
-#include "abi.h"
+#include "lm_host.h"
 #include "lm_ops.cuh"
 #include "umma.cuh"
 
@@ -582,9 +582,9 @@ int norm_backward_run(NormArgs p, cudaStream_t s) {
   if (!p.dw && !p.db) p.part = nullptr;
   size_t smem = bulk ? (size_t)p.stages * rows * row * 2 : 0;
   if (smem < sums) smem = sums;
-  cudaError_t e = cudaFuncSetAttribute(norm_backward_kernel<T, VEC, WPR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)smem);
-  if (e != cudaSuccess) return cuda_status(e, "norm_backward_kernel: shared memory");
+  static std::atomic<unsigned long long> done{0};
+  const int st = shared_limit(norm_backward_kernel<T, VEC, WPR>, NORM_SMEM, &done, "norm_backward_kernel: shared memory");
+  if (st) return st;
   norm_backward_kernel<T, VEC, WPR><<<p.blocks, Work::NW * 32, smem, s>>>(p);
   if (p.part) {
     if (p.w32) norm_dw_sum<float>(p, s);
@@ -605,9 +605,10 @@ int norm_forward_run(const NormArgs& p, cudaStream_t s) {
 template <typename T, int WPR>
 int norm_forward_ring_run(const NormArgs& p, cudaStream_t s) {
   const int smem = (int)((size_t)p.stages * p.chunk_rows * p.D * sizeof(T));
-  cudaError_t e = cudaFuncSetAttribute(norm_forward_ring_kernel<T, WPR>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return cuda_status(e, "norm_forward_ring_kernel: shared memory");
+  static std::atomic<unsigned long long> done{0};
+  const int st = shared_limit(norm_forward_ring_kernel<T, WPR>, RING_SMEM, &done,
+                              "norm_forward_ring_kernel: shared memory");
+  if (st) return st;
   const long long most = NORM_MAX_BLOCKS * 3 / 2;
   norm_forward_ring_kernel<T, WPR><<<(unsigned)(p.bulk < most ? p.bulk : most), 256, smem, s>>>(p);
   return launch_status("norm_forward_ring_kernel");

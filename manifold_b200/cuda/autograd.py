@@ -79,19 +79,19 @@ class LayerScanFn(Function):
     gradients of its pre-activations and of the carried state (v0, x0)."""
 
     @staticmethod
-    def forward(ctx, z, v0, x0, heads, base_dt):
-        xs, vs, vl, xl, states = ops.layer_scan_forward(z, v0, x0, heads, base_dt, True, True)
+    def forward(ctx, z, v0, x0, heads, base_dt, return_state):
+        xs, vs, vl, xl, states = ops.layer_scan_forward(z, v0, x0, heads, base_dt, return_state, True)
         ctx.save_for_backward(z, states)
         ctx.args = (heads, base_dt)
         ctx.set_materialize_grads(False)
-        return xs, vs, vl, xl
+        return (xs, vs, vl, xl) if return_state else (xs, vs)
 
     @staticmethod
     @first_order
-    def backward(ctx, gx, gv, gvl, gxl):
+    def backward(ctx, gx, gv, gvl=None, gxl=None):
         if gx is None and gv is None and gvl is None and gxl is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         z, states = ctx.saved_tensors
         dz, dv0, dx0 = ops.layer_scan_backward(z, states, gx, gv, gvl, gxl, *ctx.args, ctx.needs_input_grad[1],
                                                ctx.needs_input_grad[2])
-        return dz, dv0, dx0, None, None
+        return dz, dv0, dx0, None, None, None

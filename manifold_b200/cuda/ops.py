@@ -483,10 +483,10 @@ def _layer_scan(z, heads, base_dt, state, return_state):
                            f"got {t.dtype} {tuple(t.shape)}")
     if _grad_wanted(z, v0, x0):
         from .autograd import LayerScanFn
-        xs, vs, vl, xl = LayerScanFn.apply(z, v0, x0, int(heads), float(base_dt))
+        out = LayerScanFn.apply(z, v0, x0, int(heads), float(base_dt), return_state)
     else:
-        xs, vs, vl, xl, _ = layer_scan_forward(z, v0, x0, heads, base_dt, return_state, False)
-    return (xs, vs, (vl, xl)) if return_state else (xs, vs)
+        out = layer_scan_forward(z, v0, x0, heads, base_dt, return_state, False)
+    return (out[0], out[1], (out[2], out[3])) if return_state else (out[0], out[1])
 
 
 def layer_scan_forward(z, v0, x0, heads, base_dt, want_last, want_states):

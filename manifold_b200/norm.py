@@ -51,19 +51,23 @@ class LayerNormFn(torch.autograd.Function):
     @first_order
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
-        D = x.shape[-1]
+        D, wdt = x.shape[-1], ctx.wdt
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         xr, rows, xs = _rows(x, D)
         dr, _, ds = _rows(dy, D)
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-        dw = x.new_empty(D, dtype=ctx.wdt) if need_w else None
-        db = x.new_empty(D, dtype=ctx.wdt) if need_b else None
-        ws, n = None, 0
+        dx = dw = db = ws = None
+        n = 0
+        if need_x:
+            dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        if need_w:
+            dw = x.new_empty(D, dtype=wdt)
+        if need_b:
+            db = x.new_empty(D, dtype=wdt)
         if need_w or need_b:
             n = _lib.load().gfn_layer_norm_backward_workspace_floats(rows, D)
             ws = x.new_empty(n, dtype=torch.float32)
         call_on(x, "gfn_layer_norm_backward", xr.data_ptr(), xs, dr.data_ptr(), ds, ptr(weight), stats.data_ptr(),
-                _lib.DTYPES[x.dtype], _lib.DTYPES[ctx.wdt], rows, D, ptr(dx), ptr(dw), ptr(db), ptr(ws), n)
+                _lib.DTYPES[x.dtype], _lib.DTYPES[wdt], rows, D, ptr(dx), ptr(dw), ptr(db), ptr(ws), n)
         return dx, dw, db, None
 
 

@@ -54,20 +54,20 @@ def _forward(a, x, h0, want_last, want_states):
 
 class GatedScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, a, x, h0):
-        h, last, states = _forward(a, x, h0, True, True)
+    def forward(ctx, a, x, h0, return_state):
+        h, last, states = _forward(a, x, h0, return_state, True)
         ctx.save_for_backward(a, x, states)
         ctx.set_materialize_grads(False)
-        return h, last
+        return (h, last) if return_state else h
 
     @staticmethod
     @first_order
-    def backward(ctx, dh, dlast):
+    def backward(ctx, dh, dlast=None):
         a, x, states = ctx.saved_tensors
         if dh is None and dlast is None:
-            return None, None, None
+            return None, None, None, None
         B, L, D = x.shape
-        need_a, need_x, need_h0 = ctx.needs_input_grad
+        need_a, need_x, need_h0, _ = ctx.needs_input_grad
         x = _operand(x)
         dlast = None if dlast is None else dlast.contiguous()
         da = torch.empty_like(x, memory_format=torch.contiguous_format) if need_a else None
@@ -84,7 +84,7 @@ class GatedScanFn(torch.autograd.Function):
         sx, tx, _ = x.stride()
         call_on(x, "gfn_gated_scan_backward", pa, sa, ta, x.data_ptr(), sx, tx, states.data_ptr(), pg, sg, tg,
                 ptr(dlast), _lib.DTYPES[x.dtype], B, L, D, ptr(da), ptr(dx), ptr(dh0), ptr(ws), n)
-        return da, dx, dh0
+        return da, dx, dh0, None
 
 
 def gated_scan(a, x, h0=None, return_state=False):
@@ -124,7 +124,6 @@ def gated_scan(a, x, h0=None, return_state=False):
                            f"{tuple(h0.shape)}")
         wants = wants or h0.requires_grad
     if wants and torch.is_grad_enabled():
-        h, last = GatedScanFn.apply(a, x, h0)
-    else:
-        h, last, _ = _forward(a, x, h0, return_state, False)
+        return GatedScanFn.apply(a, x, h0, return_state)
+    h, last, _ = _forward(a, x, h0, return_state, False)
     return (h, last) if return_state else h
