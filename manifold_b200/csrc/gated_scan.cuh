@@ -708,33 +708,52 @@ struct LScanArgs {
 };
 
 // 1 / v to one unit in the last place, for v in [1, 6].
-GFN_DEV float quick_rcp(float v) { return __fdividef(1.f, v); }
-
-// sigma(z) and its slope sigma(z) sigma(-z) from one exponential that cannot
-// overflow: both keep their digits far out, where 1 / (1 + exp(-z)) is
-// already 0 or 1.
-GFN_DEV float gate(float z, float* slope) {
-  const float e = expf(-fabsf(z)), r = quick_rcp(1.f + e), c = e * r;
-  *slope = r * c;
-  return z >= 0.f ? r : c;
+GFN_DEV float quick_rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+GFN_DEV F2 quick_rcp(F2 v) {
+  float lo, hi;
+  split(v, lo, hi);
+  return f2(quick_rcp(lo), quick_rcp(hi));
 }
 
-// softplus(z) = max(z, 0) + log1p(e), e = exp(-|z|) in [0, 1], and its slope
-// sigma(z).  log1p(e) = 2 atanh(y) with y = e / (2 + e) <= 1/3, and
-// atanh(y) / y as a polynomial in y^2 (interpolated at the Chebyshev nodes of
-// [0, 1/9]: within 8e-9 of it, an eighth of a float32 rounding), so that a
-// small step keeps its digits, which log(1 + e) would lose.
-GFN_DEV float soft_step(float z, float* slope) {
-  const float e = expf(-fabsf(z));
-  const float r = quick_rcp((1.f + e) * (2.f + e));  // both quotients from one reciprocal
-  const float y = e * ((1.f + e) * r), y2 = y * y, s = (2.f + e) * r;
-  float q = 0.14078889f;
-  q = fmaf(q, y2, 0.13982579f);
-  q = fmaf(q, y2, 0.20012298f);
-  q = fmaf(q, y2, 0.33333161f);
-  q = fmaf(q * y2, y, y);
-  *slope = z >= 0.f ? s : e * s;
-  return fmaf(2.f, q, fmaxf(z, 0.f));
+// Two gates at a time, sigma(z) and its slope sigma(z) sigma(-z), from one
+// exponential each that cannot overflow: both keep their digits far out, where
+// 1 / (1 + exp(-z)) is already 0 or 1.
+GFN_DEV void gates(float z0, float z1, float& a0, float& a1, F2& slope) {
+  const F2 e = f2(expf(-fabsf(z0)), expf(-fabsf(z1)));
+  const F2 r = quick_rcp(e + f2(1.f)), c = e * r;
+  slope = r * c;
+  float r0, r1, c0, c1;
+  split(r, r0, r1);
+  split(c, c0, c1);
+  a0 = z0 >= 0.f ? r0 : c0;
+  a1 = z1 >= 0.f ? r1 : c1;
+}
+
+// Two steps at a time: softplus(z) = max(z, 0) + log1p(e), e = exp(-|z|) in
+// [0, 1], and its slope sigma(z).  log1p(e) = 2 atanh(y) with
+// y = e / (2 + e) <= 1/3, and atanh(y) / y as a polynomial in y^2 (interpolated
+// at the Chebyshev nodes of [0, 1/9]: within 8e-9 of it, an eighth of a
+// float32 rounding), so that a small step keeps its digits, which log(1 + e)
+// would lose.
+GFN_DEV F2 soft_steps(float z0, float z1, F2& slope) {
+  const F2 e = f2(expf(-fabsf(z0)), expf(-fabsf(z1)));
+  const F2 e1 = e + f2(1.f), e2 = e + f2(2.f);
+  const F2 r = quick_rcp(e1 * e2);  // both quotients from one reciprocal
+  const F2 y = e * (e1 * r), y2 = y * y, s = e2 * r, c = e * s;
+  F2 q = f2(0.14078889f);
+  q = fma2(q, y2, f2(0.13982579f));
+  q = fma2(q, y2, f2(0.20012298f));
+  q = fma2(q, y2, f2(0.33333161f));
+  q = fma2(q * y2, y, y);
+  float s0, s1, c0, c1;
+  split(s, s0, s1);
+  split(c, c0, c1);
+  slope = f2(z0 >= 0.f ? s0 : c0, z1 >= 0.f ? s1 : c1);
+  return fma2(f2(2.f), q, f2(fmaxf(z0, 0.f), fmaxf(z1, 0.f)));
 }
 
 GFN_DEV float head_scale(int col, int hd) {
@@ -827,23 +846,19 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScan
     }
     float A[S][VEC], dt[S][VEC], bv[S][VEC];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        float slope;
-        A[s][v] = gate(pa[s].get(v), &slope);
-        dt[s][v] = soft_step(pd[s].get(v), &slope);
-        bv[s][v] = pb[s].get(v);
-      }
-    }
-#pragma unroll
     for (int v = 0; v < VEC; ++v) {
       const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
       LayerMap m = LayerMap::identity();
 #pragma unroll
+      for (int s = 0; s < S; s += 2) {
+        F2 slope;
+        gates(pa[s].get(v), pa[s + 1].get(v), A[s][v], A[s + 1][v], slope);
+        const F2 d = soft_steps(pd[s].get(v), pd[s + 1].get(v), slope) * f2(scale);
+        split(d, dt[s][v], dt[s + 1][v]);
+        split(d * f2(pb[s].get(v), pb[s + 1].get(v)), bv[s][v], bv[s + 1][v]);
+      }
+#pragma unroll
       for (int s = 0; s < S; ++s) {
-        dt[s][v] *= scale;
-        bv[s][v] *= dt[s][v];
         m.P *= A[s][v];
         m.p = fmaf(A[s][v], m.p, bv[s][v]);
         m.Q = fmaf(dt[s][v], m.P, m.Q);
@@ -992,24 +1007,23 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
     float A[S][VEC], dt[S][VEC], zb[S][VEC], gx[S][VEC], gv[S][VEC];
     float sa[S][VEC], sd[S][VEC];  // slopes of A and dt
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
+    for (int v = 0; v < VEC; ++v) {
+      const F2 scale = f2(p.base_dt * head_scale(c.col + v, p.D / p.H));
+      GatedMap mf = GatedMap::identity();
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        A[s][v] = gate(pa[s].get(v), &sa[s][v]);
-        dt[s][v] = soft_step(pd[s].get(v), &sd[s][v]);
+      for (int s = 0; s < S; s += 2) {
+        F2 slope;
+        gates(pa[s].get(v), pa[s + 1].get(v), A[s][v], A[s + 1][v], slope);
+        split(slope, sa[s][v], sa[s + 1][v]);
+        const F2 d = soft_steps(pd[s].get(v), pd[s + 1].get(v), slope) * scale;
+        split(d, dt[s][v], dt[s + 1][v]);
+        split(slope * scale, sd[s][v], sd[s + 1][v]);
+      }
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
         zb[s][v] = pb[s].get(v);
         gx[s][v] = px[s].get(v);
         gv[s][v] = pv[s].get(v);
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
-      GatedMap mf = GatedMap::identity();
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        dt[s][v] *= scale;
-        sd[s][v] *= scale;
         mf.P *= A[s][v];
         mf.p = fmaf(A[s][v], mf.p, zb[s][v] * dt[s][v]);
       }
@@ -1093,16 +1107,25 @@ __global__ void __launch_bounds__(128) lscan_forward_seq_kernel(const LScanArgs 
   const float scale = p.base_dt * head_scale((int)j, p.D / p.H);
   float v = p.v0 ? p.v0[c] : 0.f, x = p.x0 ? p.x0[c] : 0.f;
   if (p.states && p.L) p.states[c] = v;
-#pragma unroll 4
-  for (int t = 0; t < p.L; ++t) {
+  for (int t = 0; t < p.L; t += 2) {
     const float* z = p.z + (b * p.L + t) * 3 * p.D + j;
-    float slope;
-    const float dt = soft_step(z[p.D], &slope) * scale;
-    v = fmaf(gate(z[0], &slope), v, z[2LL * p.D] * dt);
-    x = fmaf(v, dt, x);
     const long long e = (b * p.L + t) * p.D + j;
+    const bool two = t + 1 < p.L;
+    const float *z1 = two ? z + 3LL * p.D : z;
+    F2 slope;
+    float A0, A1, dt0, dt1;
+    gates(z[0], z1[0], A0, A1, slope);
+    split(soft_steps(z[p.D], z1[p.D], slope) * f2(scale), dt0, dt1);
+    v = fmaf(A0, v, z[2LL * p.D] * dt0);
+    x = fmaf(v, dt0, x);
     p.vs[e] = v;
     p.xs[e] = x;
+    if (two) {
+      v = fmaf(A1, v, z1[2LL * p.D] * dt1);
+      x = fmaf(v, dt1, x);
+      p.vs[e + p.D] = v;
+      p.xs[e + p.D] = x;
+    }
   }
   if (p.v_last) p.v_last[c] = v;
   if (p.x_last) p.x_last[c] = x;

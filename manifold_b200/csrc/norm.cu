@@ -105,18 +105,106 @@ GFN_DEV void row_sum(float (&v)[N], float* buf, int warps, int& turn) {
   }
 }
 
-// Elements per thread: 64 bytes of vectors, or 16 single elements.
-template <typename T, int VEC>
-constexpr int norm_forward_ept() { return VEC == 1 ? 16 : 64 / (int)sizeof(T); }
+// A thread's elements of a row, in pairs where there are pairs.
+template <int NV, int VEC>
+struct Row {
+  static_assert(VEC % 2 == 0, "");
+  F2 q[NV][VEC / 2];
+
+  GFN_DEV void take(const float (&v)[NV][VEC]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) q[i][j] = f2(v[i][2 * j], v[i][2 * j + 1]);
+    }
+  }
+  GFN_DEV float sum() const {
+    F2 t = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) t = t + q[i][j];
+    }
+    float lo, hi;
+    split(t, lo, hi);
+    return lo + hi;
+  }
+  // subtracts mu; the sum of squares of what is in the row
+  GFN_DEV float centre(float mu, int D, int tpr, int l) {
+    const F2 m = f2(-mu);
+    F2 t = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if ((i * tpr + l) * VEC < D) {
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          q[i][j] = q[i][j] + m;
+          t = fma2(q[i][j], q[i][j], t);
+        }
+      }
+    }
+    float lo, hi;
+    split(t, lo, hi);
+    return lo + hi;
+  }
+  GFN_DEV void scale(int i, float c) {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) q[i][j] = q[i][j] * f2(c);
+  }
+  GFN_DEV void multiply(int i, const float (&c)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) q[i][j] = q[i][j] * f2(c[2 * j], c[2 * j + 1]);
+  }
+  GFN_DEV void add(int i, const float (&c)[VEC]) {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) q[i][j] = q[i][j] + f2(c[2 * j], c[2 * j + 1]);
+  }
+  GFN_DEV void give(int i, float (&v)[VEC]) const {
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) split(q[i][j], v[2 * j], v[2 * j + 1]);
+  }
+};
+
+template <int NV>
+struct Row<NV, 1> {
+  float q[NV];
+
+  GFN_DEV void take(const float (&v)[NV][1]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) q[i] = v[i][0];
+  }
+  GFN_DEV float sum() const {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) t += q[i];
+    return t;
+  }
+  GFN_DEV float centre(float mu, int D, int tpr, int l) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (i * tpr + l < D) {
+        q[i] -= mu;
+        t = fmaf(q[i], q[i], t);
+      }
+    }
+    return t;
+  }
+  GFN_DEV void scale(int i, float c) { q[i] *= c; }
+  GFN_DEV void multiply(int i, const float (&c)[1]) { q[i] *= c[0]; }
+  GFN_DEV void add(int i, const float (&c)[1]) { q[i] = __fadd_rn(q[i], c[0]); }
+  GFN_DEV void give(int i, float (&v)[1]) const { v[0] = q[i]; }
+};
+
 constexpr int norm_forward_threads(int wpr) { return wpr * 32 > NORM_THREADS ? wpr * 32 : NORM_THREADS; }
 
 // WPR warps per row, one row per group of warps.  One pass over x: 49 us at
 // 65536 x 512 float32 (5.5 TB/s with the launch), 22 us at 20480 x 1024
 // bfloat16, where converting and reducing 16-bit values takes about as long as
 // the memory.
-template <typename T, int VEC, int WPR>
+template <typename T, int VEC, int WPR, int EPT>
 __global__ void __launch_bounds__(norm_forward_threads(WPR), VEC == 1 ? 1 : 1024 / norm_forward_threads(WPR)) norm_forward_kernel(const NormArgs p) {
-  constexpr int TPR = WPR * 32, NV = norm_forward_ept<T, VEC>() / VEC, THREADS = norm_forward_threads(WPR);
+  constexpr int TPR = WPR * 32, NV = EPT / VEC, THREADS = norm_forward_threads(WPR);
   __shared__ float buf[2 * THREADS / 32];
   const long long row = (long long)blockIdx.x * (THREADS / TPR) + threadIdx.x / TPR;
   if (row >= p.rows) return;  // a whole group: its barriers are its own
@@ -131,25 +219,13 @@ __global__ void __launch_bounds__(norm_forward_threads(WPR), VEC == 1 ? 1 : 1024
     for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
     if (e < D) load_vec<T, VEC>(x + e, v[i]);
   }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
-  }
+  Row<NV, VEC> q;
+  q.take(v);
+  s[0] = q.sum();
   int turn = 0;
   row_sum<1, WPR>(s, buf, THREADS / 32, turn);
   const float mu = s[0] / D;
-  s[0] = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if ((i * TPR + l) * VEC < D) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[i][j] -= mu;
-        s[0] = fmaf(v[i][j], v[i][j], s[0]);
-      }
-    }
-  }
+  s[0] = q.centre(mu, D, TPR, l);
   row_sum<1, WPR>(s, buf, THREADS / 32, turn);
   const float rstd = rsqrtf(s[0] / D + p.eps);
   T* y = static_cast<T*>(p.y) + row * D;
@@ -157,19 +233,17 @@ __global__ void __launch_bounds__(norm_forward_threads(WPR), VEC == 1 ? 1 : 1024
   for (int i = 0; i < NV; ++i) {
     const int e = (i * TPR + l) * VEC;
     if (e < D) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] *= rstd;
       float c[VEC];
+      q.scale(i, rstd);
       if (p.w) {
         load_weight<T, VEC>(p.w, p.w32, e, c);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] *= c[j];
+        q.multiply(i, c);
       }
       if (p.b) {
         load_weight<T, VEC>(p.b, p.w32, e, c);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] += c[j];
+        q.add(i, c);
       }
+      q.give(i, v[i]);
       store_vec<T, VEC>(y + e, v[i]);
     }
   }
@@ -311,9 +385,9 @@ __global__ void __launch_bounds__(256, 3) norm_forward_ring_kernel(const NormArg
 // at 65536 x 512 float32, the sums of the partial rows included (5.3 TB/s);
 // 39 us at 20011 x 1001 bfloat16, bound there by single-element accesses.  A
 // pass of its own for dw and db took 2.6 times as long.
-template <typename T, int VEC, int WPR>
+template <typename T, int VEC, int WPR, int EPT_>
 struct NormBackward {
-  static constexpr int NW = WPR > 8 ? WPR : 8, TPR = WPR * 32, GROUPS = NW / WPR, EPT = 16, NV = EPT / VEC;
+  static constexpr int NW = WPR > 8 ? WPR : 8, TPR = WPR * 32, GROUPS = NW / WPR, EPT = EPT_, NV = EPT / VEC;
   float wv[NV][VEC], aw[NV][VEC], ab[NV][VEC];
   int l, turn = 0;
 
@@ -360,9 +434,10 @@ struct NormBackward {
   }
 };
 
-template <typename T, int VEC, int WPR>
-__global__ void __launch_bounds__(NormBackward<T, VEC, WPR>::NW * 32, WPR > 8 ? 1 : 2) norm_backward_kernel(const NormArgs p) {
-  using Work = NormBackward<T, VEC, WPR>;
+template <typename T, int VEC, int WPR, int EPT_>
+__global__ void __launch_bounds__(NormBackward<T, VEC, WPR, EPT_>::NW * 32, WPR > 8 ? 1 : 2)
+    norm_backward_kernel(const NormArgs p) {
+  using Work = NormBackward<T, VEC, WPR, EPT_>;
   constexpr int NW = Work::NW, TPR = Work::TPR, GROUPS = Work::GROUPS, NV = Work::NV, EPT = Work::EPT;
   extern __shared__ __align__(128) char ring[];
   __shared__ RowRing<T, 2, NW> ops;
@@ -563,9 +638,9 @@ bool plan_ring(NormArgs* p, int groups, int operands, int row, int smem, bool wh
   return true;
 }
 
-template <typename T, int VEC, int WPR>
+template <typename T, int VEC, int WPR, int EPT>
 int norm_backward_run(NormArgs p, cudaStream_t s) {
-  using Work = NormBackward<T, VEC, WPR>;
+  using Work = NormBackward<T, VEC, WPR, EPT>;
   const int row = p.D * (int)sizeof(T);
   const size_t sums = (size_t)Work::NW * 32 * Work::EPT * 2 * 4;
   const bool whole = (reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.dy)) % 16 == 0 &&
@@ -583,9 +658,9 @@ int norm_backward_run(NormArgs p, cudaStream_t s) {
   size_t smem = bulk ? (size_t)p.stages * rows * row * 2 : 0;
   if (smem < sums) smem = sums;
   static std::atomic<unsigned long long> done{0};
-  const int st = shared_limit(norm_backward_kernel<T, VEC, WPR>, NORM_SMEM, &done, "norm_backward_kernel: shared memory");
+  const int st = shared_limit(norm_backward_kernel<T, VEC, WPR, EPT>, NORM_SMEM, &done, "norm_backward_kernel: shared memory");
   if (st) return st;
-  norm_backward_kernel<T, VEC, WPR><<<p.blocks, Work::NW * 32, smem, s>>>(p);
+  norm_backward_kernel<T, VEC, WPR, EPT><<<p.blocks, Work::NW * 32, smem, s>>>(p);
   if (p.part) {
     if (p.w32) norm_dw_sum<float>(p, s);
     else norm_dw_sum<T>(p, s);
@@ -593,12 +668,12 @@ int norm_backward_run(NormArgs p, cudaStream_t s) {
   return launch_status("norm_backward_kernel");
 }
 
-template <typename T, int VEC, int WPR>
+template <typename T, int VEC, int WPR, int EPT>
 int norm_forward_run(const NormArgs& p, cudaStream_t s) {
   constexpr int threads = norm_forward_threads(WPR), per = threads / (WPR * 32);
   const long long blocks = (p.rows + per - 1) / per;
   if (blocks > 0x7fffffffLL) return fail(GFN_ERR_UNSUPPORTED, "layer_norm_forward: %lld blocks", blocks);
-  norm_forward_kernel<T, VEC, WPR><<<(unsigned)blocks, threads, 0, s>>>(p);
+  norm_forward_kernel<T, VEC, WPR, EPT><<<(unsigned)blocks, threads, 0, s>>>(p);
   return launch_status("norm_forward_kernel");
 }
 
@@ -614,15 +689,24 @@ int norm_forward_ring_run(const NormArgs& p, cudaStream_t s) {
   return launch_status("norm_forward_ring_kernel");
 }
 
+// Elements per thread in the forward: 64 bytes of vectors, or 16 single
+// elements; half of that where it holds the row in one warp (bfloat16 65536 x
+// 512: 35 against 41 us).
+template <typename T, int VEC>
+constexpr int norm_forward_ept() {
+  return VEC == 1 ? 16 : 64 / (int)sizeof(T);
+}
+
 // The fewest warps whose registers hold a row.
 template <typename T, int VEC>
 int norm_short_run(const NormArgs& p, bool backward, cudaStream_t s) {
   if (backward) {
-    if (p.D <= 512) return norm_backward_run<T, VEC, 1>(p, s);
-    if (p.D <= 1024) return norm_backward_run<T, VEC, 2>(p, s);
-    if (p.D <= 2048) return norm_backward_run<T, VEC, 4>(p, s);
-    if (p.D <= 4096) return norm_backward_run<T, VEC, 8>(p, s);
-    return norm_backward_run<T, VEC, 16>(p, s);
+    if (p.D <= 256) return norm_backward_run<T, VEC, 1, 8>(p, s);
+    if (p.D <= 512) return norm_backward_run<T, VEC, 1, 16>(p, s);
+    if (p.D <= 1024) return norm_backward_run<T, VEC, 2, 16>(p, s);
+    if (p.D <= 2048) return norm_backward_run<T, VEC, 4, 16>(p, s);
+    if (p.D <= 4096) return norm_backward_run<T, VEC, 8, 16>(p, s);
+    return norm_backward_run<T, VEC, 16, 16>(p, s);
   }
   if constexpr (VEC == 1) {
     NormArgs q = p;
@@ -635,12 +719,13 @@ int norm_short_run(const NormArgs& p, bool backward, cudaStream_t s) {
       return norm_forward_ring_run<T, 8>(q, s);
     }
   }
-  constexpr int warp = 32 * norm_forward_ept<T, VEC>();  // elements that one warp holds
-  if (p.D <= warp) return norm_forward_run<T, VEC, 1>(p, s);
-  if (p.D <= 2 * warp) return norm_forward_run<T, VEC, 2>(p, s);
-  if (p.D <= 4 * warp) return norm_forward_run<T, VEC, 4>(p, s);
-  if (p.D <= 8 * warp) return norm_forward_run<T, VEC, 8>(p, s);
-  return norm_forward_run<T, VEC, 16>(p, s);
+  constexpr int EPT = norm_forward_ept<T, VEC>(), warp = 32 * EPT;  // elements that one warp holds
+  if (p.D <= warp / 2) return norm_forward_run<T, VEC, 1, EPT / 2>(p, s);
+  if (p.D <= warp) return norm_forward_run<T, VEC, 1, EPT>(p, s);
+  if (p.D <= 2 * warp) return norm_forward_run<T, VEC, 2, EPT>(p, s);
+  if (p.D <= 4 * warp) return norm_forward_run<T, VEC, 4, EPT>(p, s);
+  if (p.D <= 8 * warp) return norm_forward_run<T, VEC, 8, EPT>(p, s);
+  return norm_forward_run<T, VEC, 16, EPT>(p, s);
 }
 
 template <typename T, typename W>
