@@ -309,9 +309,9 @@ struct RowRing {
 // elements come from shared memory, and the weights stay in registers.  (From
 // 128-bit rows the direct kernel is as fast: 49 against 51 us at 65536 x 512
 // float32; here 39 against 70 us at 20011 x 1001 bfloat16.)
-template <typename T, int WPR>
+template <typename T, int WPR, int EPT>
 __global__ void __launch_bounds__(256, 3) norm_forward_ring_kernel(const NormArgs p) {
-  constexpr int VEC = 1, NW = 8, TPR = WPR * 32, GROUPS = NW / WPR, NV = 16 / VEC;
+  constexpr int VEC = 1, NW = 8, TPR = WPR * 32, GROUPS = NW / WPR, NV = EPT / VEC;
   extern __shared__ __align__(128) char ring[];
   __shared__ RowRing<T, 1, NW> rows;
   __shared__ float buf[2 * NW];
@@ -677,15 +677,15 @@ int norm_forward_run(const NormArgs& p, cudaStream_t s) {
   return launch_status("norm_forward_kernel");
 }
 
-template <typename T, int WPR>
+template <typename T, int WPR, int EPT>
 int norm_forward_ring_run(const NormArgs& p, cudaStream_t s) {
   const int smem = (int)((size_t)p.stages * p.chunk_rows * p.D * sizeof(T));
   static std::atomic<unsigned long long> done{0};
-  const int st = shared_limit(norm_forward_ring_kernel<T, WPR>, RING_SMEM, &done,
+  const int st = shared_limit(norm_forward_ring_kernel<T, WPR, EPT>, RING_SMEM, &done,
                               "norm_forward_ring_kernel: shared memory");
   if (st) return st;
   const long long most = NORM_MAX_BLOCKS * 3 / 2;
-  norm_forward_ring_kernel<T, WPR><<<(unsigned)(p.bulk < most ? p.bulk : most), 256, smem, s>>>(p);
+  norm_forward_ring_kernel<T, WPR, EPT><<<(unsigned)(p.bulk < most ? p.bulk : most), 256, smem, s>>>(p);
   return launch_status("norm_forward_ring_kernel");
 }
 
@@ -701,6 +701,9 @@ constexpr int norm_forward_ept() {
 template <typename T, int VEC>
 int norm_short_run(const NormArgs& p, bool backward, cudaStream_t s) {
   if (backward) {
+    if constexpr (VEC <= 4) {
+      if (p.D <= 128) return norm_backward_run<T, VEC, 1, 4>(p, s);
+    }
     if (p.D <= 256) return norm_backward_run<T, VEC, 1, 8>(p, s);
     if (p.D <= 512) return norm_backward_run<T, VEC, 1, 16>(p, s);
     if (p.D <= 1024) return norm_backward_run<T, VEC, 2, 16>(p, s);
@@ -713,10 +716,11 @@ int norm_short_run(const NormArgs& p, bool backward, cudaStream_t s) {
     const bool whole = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.xs == p.D;
     const int groups = p.D <= 512 ? 8 : p.D <= 1024 ? 4 : p.D <= 2048 ? 2 : 1;
     if (p.D <= 4096 && p.rows >= RING_ROWS && plan_ring(&q, groups, 1, p.D * (int)sizeof(T), RING_SMEM, whole)) {
-      if (groups == 8) return norm_forward_ring_run<T, 1>(q, s);
-      if (groups == 4) return norm_forward_ring_run<T, 2>(q, s);
-      if (groups == 2) return norm_forward_ring_run<T, 4>(q, s);
-      return norm_forward_ring_run<T, 8>(q, s);
+      if (p.D <= 128) return norm_forward_ring_run<T, 1, 4>(q, s);
+      if (groups == 8) return norm_forward_ring_run<T, 1, 16>(q, s);
+      if (groups == 4) return norm_forward_ring_run<T, 2, 16>(q, s);
+      if (groups == 2) return norm_forward_ring_run<T, 4, 16>(q, s);
+      return norm_forward_ring_run<T, 8, 16>(q, s);
     }
   }
   constexpr int EPT = norm_forward_ept<T, VEC>(), warp = 32 * EPT;  // elements that one warp holds
