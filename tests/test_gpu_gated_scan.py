@@ -265,6 +265,30 @@ def test_gated_scan_strides_and_broadcast_gates(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 61])
+def test_gated_scan_other_orders_of_batch_and_time(dtype, D):
+    g = torch.Generator().manual_seed(D)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).to(DEV)  # noqa: E731
+    gate = lambda *s: torch.rand(*s, generator=g).to(dtype).to(DEV)  # noqa: E731
+    h0 = torch.randn(5, D, generator=g).to(DEV)
+    # time-major storage: the batch stride is the smaller one
+    a, x, dh = gate(270, 5, D).transpose(0, 1), r(270, 5, D).transpose(0, 1), r(270, 5, D).transpose(0, 1)
+    _run(a, x, h0, dh, None)
+    # windows that overlap: a step stride below the width, a batch stride below the sequence
+    base = r(5 * 8 + 270 * 8 + D)
+    x = base.as_strided((5, 270, D), (8, 8, 1))
+    with torch.no_grad():
+        h, last = gfn.gated_scan(a, x, h0, return_state=True)
+    _check_scan(a, x, h0, h, last)
+    # every second step, every second row
+    a, x, dh = gate(10, 540, D)[::2, ::2], r(10, 540, D)[::2, 1::2], r(10, 540, D)[1::2, ::2]
+    _run(a, x, h0, dh, None)
+    # each operand in an order of its own
+    _run(gate(270, 5, D).transpose(0, 1), r(5, 270, D), h0, r(5, 270, 2 * D)[..., D:], None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_gated_scan_segments_and_single_tokens_continue_the_state(dtype):
     a, x, h0, _, _ = _inputs(2, 333, 70, dtype, 21, 0.8)
     h, last = gfn.gated_scan(a, x, h0, return_state=True)
