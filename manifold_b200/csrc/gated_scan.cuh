@@ -795,10 +795,12 @@ struct LayerState {
   GFN_DEV LayerState through(LayerMap m) const { return {pass(m.P, v, m.p), x + pass(m.Q, v, m.q)}; }
 };
 
-// 20 bytes per element, and 86 instructions: two exponentials, two reciprocals
-// and a polynomial.  Runs of 128 steps of 32 columns, two blocks per SM: at
-// 32 x 2048 x 512 134 us, 5.0 TB/s (runs of 64 steps of 64 columns 155 us); at
-// 1 x 20000 x 256, where 8 column tiles leave 5 rounds of blocks, 42 us.
+// 20 bytes per element, and 70 instructions: two exponentials, two reciprocals
+// and a polynomial, two steps at a time where packed arithmetic does both (one
+// at a time 86 instructions and 134 us).  Runs of 128 steps of 32 columns, two
+// blocks per SM: at 32 x 2048 x 512 128 us, 5.2 TB/s (runs of 64 steps of 64
+// columns 155 us); at 1 x 20000 x 256, where 8 column tiles leave 5 rounds of
+// blocks, 40 us.
 template <int MODE, int VEC, int S, int NW, int OCC>
 __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScanArgs p, const __grid_constant__ ScanMaps maps) {
   constexpr int CT = 32 * VEC;
@@ -942,11 +944,11 @@ struct LayerBackState {
   GFN_DEV LayerBackState through(LayerBackMap f) const { return {pass(f.P, m, pass(f.R, X, f.q)), X + f.G}; }
 };
 
-// 28 bytes per element (32 with a gradient of v) and 142 instructions, issued
-// at 63% of the rate: instructions and memory bind about equally.  The gates,
-// steps and slopes stay in registers between the two walks (recomputing them
-// took 298 us); v is recomputed from its kept state instead of read.  At
-// 32 x 2048 x 512 222 us, 4.2 TB/s.
+// 28 bytes per element (32 with a gradient of v) and 128 instructions, issued
+// at 55% of the rate: instructions, the exchange's waits and memory share the
+// time.  The gates, steps and slopes stay in registers between the two walks
+// (recomputing them took 298 us); v is recomputed from its kept state instead
+// of read.  At 32 x 2048 x 512 220 us, 4.3 TB/s.
 template <int MODE, int VEC, int S, int NW, int OCC>
 __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LScanArgs p, const __grid_constant__ ScanMaps maps) {
   static_assert(NW * S == SCAN_CK, "one kept state per run");

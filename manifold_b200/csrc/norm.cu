@@ -105,97 +105,6 @@ GFN_DEV void row_sum(float (&v)[N], float* buf, int warps, int& turn) {
   }
 }
 
-// A thread's elements of a row, in pairs where there are pairs.
-template <int NV, int VEC>
-struct Row {
-  static_assert(VEC % 2 == 0, "");
-  F2 q[NV][VEC / 2];
-
-  GFN_DEV void take(const float (&v)[NV][VEC]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int j = 0; j < VEC / 2; ++j) q[i][j] = f2(v[i][2 * j], v[i][2 * j + 1]);
-    }
-  }
-  GFN_DEV float sum() const {
-    F2 t = f2(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int j = 0; j < VEC / 2; ++j) t = t + q[i][j];
-    }
-    float lo, hi;
-    split(t, lo, hi);
-    return lo + hi;
-  }
-  // subtracts mu; the sum of squares of what is in the row
-  GFN_DEV float centre(float mu, int D, int tpr, int l) {
-    const F2 m = f2(-mu);
-    F2 t = f2(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if ((i * tpr + l) * VEC < D) {
-#pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
-          q[i][j] = q[i][j] + m;
-          t = fma2(q[i][j], q[i][j], t);
-        }
-      }
-    }
-    float lo, hi;
-    split(t, lo, hi);
-    return lo + hi;
-  }
-  GFN_DEV void scale(int i, float c) {
-#pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) q[i][j] = q[i][j] * f2(c);
-  }
-  GFN_DEV void multiply(int i, const float (&c)[VEC]) {
-#pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) q[i][j] = q[i][j] * f2(c[2 * j], c[2 * j + 1]);
-  }
-  GFN_DEV void add(int i, const float (&c)[VEC]) {
-#pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) q[i][j] = q[i][j] + f2(c[2 * j], c[2 * j + 1]);
-  }
-  GFN_DEV void give(int i, float (&v)[VEC]) const {
-#pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) split(q[i][j], v[2 * j], v[2 * j + 1]);
-  }
-};
-
-template <int NV>
-struct Row<NV, 1> {
-  float q[NV];
-
-  GFN_DEV void take(const float (&v)[NV][1]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) q[i] = v[i][0];
-  }
-  GFN_DEV float sum() const {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) t += q[i];
-    return t;
-  }
-  GFN_DEV float centre(float mu, int D, int tpr, int l) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (i * tpr + l < D) {
-        q[i] -= mu;
-        t = fmaf(q[i], q[i], t);
-      }
-    }
-    return t;
-  }
-  GFN_DEV void scale(int i, float c) { q[i] *= c; }
-  GFN_DEV void multiply(int i, const float (&c)[1]) { q[i] *= c[0]; }
-  GFN_DEV void add(int i, const float (&c)[1]) { q[i] = __fadd_rn(q[i], c[0]); }
-  GFN_DEV void give(int i, float (&v)[1]) const { v[0] = q[i]; }
-};
-
 constexpr int norm_forward_threads(int wpr) { return wpr * 32 > NORM_THREADS ? wpr * 32 : NORM_THREADS; }
 
 // WPR warps per row, one row per group of warps.  One pass over x: 49 us at
@@ -219,13 +128,25 @@ __global__ void __launch_bounds__(norm_forward_threads(WPR), VEC == 1 ? 1 : 1024
     for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
     if (e < D) load_vec<T, VEC>(x + e, v[i]);
   }
-  Row<NV, VEC> q;
-  q.take(v);
-  s[0] = q.sum();
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s[0] += v[i][j];
+  }
   int turn = 0;
   row_sum<1, WPR>(s, buf, THREADS / 32, turn);
   const float mu = s[0] / D;
-  s[0] = q.centre(mu, D, TPR, l);
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if ((i * TPR + l) * VEC < D) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[i][j] -= mu;
+        s[0] = fmaf(v[i][j], v[i][j], s[0]);
+      }
+    }
+  }
   row_sum<1, WPR>(s, buf, THREADS / 32, turn);
   const float rstd = rsqrtf(s[0] / D + p.eps);
   T* y = static_cast<T*>(p.y) + row * D;
@@ -233,17 +154,19 @@ __global__ void __launch_bounds__(norm_forward_threads(WPR), VEC == 1 ? 1 : 1024
   for (int i = 0; i < NV; ++i) {
     const int e = (i * TPR + l) * VEC;
     if (e < D) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] *= rstd;
       float c[VEC];
-      q.scale(i, rstd);
       if (p.w) {
         load_weight<T, VEC>(p.w, p.w32, e, c);
-        q.multiply(i, c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] *= c[j];
       }
       if (p.b) {
         load_weight<T, VEC>(p.b, p.w32, e, c);
-        q.add(i, c);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] += c[j];
       }
-      q.give(i, v[i]);
       store_vec<T, VEC>(y + e, v[i]);
     }
   }
