@@ -157,7 +157,7 @@ int gscan_run(const GScanArgs& p, bool backward, void* ws, long long bytes, cuda
                     rows16(p.x, p.x_sb, p.x_st, p.B, p.L, z) && rows16(p.dh, p.g_sb, p.g_st, p.B, p.L, z) &&
                     aligned16(p.h) && aligned16(p.da) && aligned16(p.dx);
   if (tma)
-    return backward ? gscan_backward<SCAN_TMA, T, 2, 8, 8, z == 2 ? 3 : 2>(p, ws, bytes, s)
+    return backward ? gscan_backward<SCAN_TMA, T, 2, z == 2 ? 16 : 8, 8, 2>(p, ws, bytes, s)
                     : gscan_forward<SCAN_TMA, T, 2, z == 2 ? 32 : 16, 8, 2>(p, ws, bytes, s);
   return backward ? gscan_backward<SCAN_PLAIN, T, 1, 8, 8, 4>(p, ws, bytes, s)
                   : gscan_forward<SCAN_PLAIN, T, 1, 16, 8, 3>(p, ws, bytes, s);

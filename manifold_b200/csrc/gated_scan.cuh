@@ -31,7 +31,7 @@
 //             16 x 2048 x 512 float32    44 us, 4.6 TB/s
 //             1 x 65536 x 512 bfloat16   58 us, 3.4 TB/s
 //             3 x 5003 x 1001 bfloat16   50 us, 1.8 TB/s (rows off 16 bytes)
-//   backward  118, 71, 110 and 79 us: 5.7, 4.7, 3.1 and 1.9 TB/s
+//   backward  118, 72, 99 and 79 us: 5.7, 4.6, 3.4 and 1.9 TB/s
 // With many columns they run at the memory's rate.  With few, what is left is
 // the way of a map through global memory and the wait for the group's state,
 // about 5,000 of a block's 13,000 cycles per run; off 16 bytes, the loads'
@@ -547,12 +547,12 @@ GFN_DEV void chain_states(const unsigned long long (*maps)[CT], const float* kep
   }
 }
 
-// Runs of NW * S = SCAN_CK steps from the last to the first: the state kept
-// before the run gives h, the messages pass from run to run as the states do
-// in the forward.
+// Runs of NW * S steps from the last to the first: the state kept before the
+// run gives h, the messages pass from run to run as the states do in the
+// forward.
 template <int MODE, typename T, int VEC, int S, int NW, int OCC>
 __global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GScanArgs p, const __grid_constant__ ScanMaps maps) {
-  static_assert(NW * S == SCAN_CK, "one kept state per run");
+  static_assert(NW * S % SCAN_CK == 0, "a kept state at every run's start");
   constexpr int CT = 32 * VEC;
   extern __shared__ __align__(128) unsigned staged[];
   __shared__ ScanShared<GatedMap, GatedState, CT, NW> sh;
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) gscan_backward_kernel(const GSca
         sh, p.words + q.tile * p.nchunks * (long long)CT, q.chunk, p.nchunks, p.group, p.D - q.c0,
         [&](int c) { return GatedState{p.dlast ? p.dlast[(long long)q.b * p.D + q.c0 + c] : 0.f}; },
         [&](int c) {
-          chain_states<CT, NW>(fmaps, p.states + ((long long)q.b * p.nck + run) * p.D + q.c0, c, p.D - q.c0, hstart);
+          chain_states<CT, NW>(fmaps, p.states + ((long long)q.b * p.nck + q.first / SCAN_CK) * p.D + q.c0, c, p.D - q.c0, hstart);
         },
         [&] {
           turn.hear(p, sh.slot, it);
@@ -951,7 +951,7 @@ struct LayerBackState {
 // of read.  At 32 x 2048 x 512 220 us, 4.3 TB/s.
 template <int MODE, int VEC, int S, int NW, int OCC>
 __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LScanArgs p, const __grid_constant__ ScanMaps maps) {
-  static_assert(NW * S == SCAN_CK, "one kept state per run");
+  static_assert(NW * S % SCAN_CK == 0, "a kept state at every run's start");
   constexpr int CT = 32 * VEC;
   extern __shared__ __align__(128) unsigned staged[];
   __shared__ ScanShared<LayerBackMap, LayerBackState, CT, NW> sh;
@@ -1054,7 +1054,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
           return LayerBackState{p.gvl ? p.gvl[e] : 0.f, p.gxl ? p.gxl[e] : 0.f};
         },
         [&](int j) {
-          chain_states<CT, NW>(fmaps, p.states + ((long long)c.b * p.nck + run) * p.D + c.c0, j, p.D - c.c0, vstart);
+          chain_states<CT, NW>(fmaps, p.states + ((long long)c.b * p.nck + c.first / SCAN_CK) * p.D + c.c0, j, p.D - c.c0, vstart);
         },
         [&] {
           turn.hear(p, sh.slot, it);
