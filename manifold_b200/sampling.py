@@ -68,8 +68,11 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
     same_device("process_logits", logits, tokens, lengths, prompt_lengths, bias, allowed)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise GfnError(f"process_logits: logits must be [batch, vocab], got {tuple(logits.shape)}")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise GfnError("process_logits is not differentiable: call it under torch.no_grad() or on logits.detach()")
+    if torch.is_grad_enabled():
+        for t in (logits, bias, repetition_penalty, frequency_penalty, presence_penalty, temperature):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise GfnError("process_logits is not differentiable: call it under torch.no_grad() or on detached "
+                               "tensors")
     code = dtype_code(logits, "logits")
     B, V = logits.shape
     x = logits if logits.is_contiguous() or V == 1 or logits.stride(1) == 1 else logits.contiguous()

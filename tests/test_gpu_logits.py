@@ -188,6 +188,19 @@ def test_process_logits_refusals_on_the_gpu():
             gfn.process_logits(bad)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,shape", [("bias", (64,)), ("repetition_penalty", (2,)), ("frequency_penalty", (2,)),
+                                        ("presence_penalty", (2,)), ("temperature", (2,))])
+def test_process_logits_refuses_to_cut_a_gradient(name, shape):
+    """No operand that wants a gradient is silently detached."""
+    lg, t = torch.zeros(2, 64, device=DEV), torch.ones(shape, device=DEV, requires_grad=True)
+    with pytest.raises(gfn.GfnError):
+        gfn.process_logits(lg, **{name: t})
+    with torch.no_grad():
+        gfn.process_logits(lg, **{name: t})
+    gfn.process_logits(lg, **{name: t.detach()})
+
+
 def test_process_logits_refusals():
     with pytest.raises(gfn.GfnError):  # no CPU path
         gfn.process_logits(torch.zeros(1, 8))
