@@ -77,10 +77,12 @@ GFN_DEV float finish_logit(float v, float bias, bool allowed, const RowTerms& r)
 // groups of VEC, and only a row's first and last places go one by one.  A
 // block owns THREADS * VEC * UNROLL places of one row.  Its logits, biases and
 // mask words are on their way to registers while it counts the history.
+// Without history four blocks per SM are asked for (with a bias and a mask 34
+// registers would leave three: 27 us against 29 at 256 x 50257 bfloat16).
 // BIAS: 0 none, 1 in aligned groups too, 2 one by one.
 template <typename T, int VEC, int UNROLL, bool HIST, int BIAS, bool MASK>
-__global__ void __launch_bounds__(LOGITS_THREADS) logits_kernel(const LogitsArgs p) {
-  constexpr int STEP = LOGITS_THREADS * VEC, RUN = STEP * UNROLL, HEAD = 2;
+__global__ void __launch_bounds__(LOGITS_THREADS, HIST ? 0 : 4) logits_kernel(const LogitsArgs p) {
+  constexpr int STEP = LOGITS_THREADS * VEC, RUN = STEP * UNROLL, HEAD = 2, CHUNK = 4;
   __shared__ __align__(16) unsigned counts[HIST ? RUN : 1];
   const long long row = blockIdx.y;
   const int phase = VEC > 1 ? (int)((row * p.V) % VEC) : 0;
@@ -130,19 +132,26 @@ __global__ void __launch_bounds__(LOGITS_THREADS) logits_kernel(const LogitsArgs
       *reinterpret_cast<uint4*>(counts + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     auto count = [&](int i, long long t) {
+      const unsigned place = (unsigned)((int)t + phase - start);
+      if (i >= len) return;
       if ((unsigned long long)t >= (unsigned)p.V) gfn_flag_error(kDevErrBadToken);
-      else if ((unsigned)((int)t + phase - start) < (unsigned)RUN) {
-        if (i < pl) atomicOr(&counts[(int)t + phase - start], LOGITS_SEEN);
-        else atomicAdd(&counts[(int)t + phase - start], 1u);
+      else if (place < (unsigned)RUN) {
+        if (i < pl) atomicOr(&counts[place], LOGITS_SEEN);
+        else atomicAdd(&counts[place], 1u);
       }
     };
 #pragma unroll
-    for (int k = 0; k < HEAD; ++k) {
-      const int i = threadIdx.x + k * LOGITS_THREADS;
-      if (i < len) count(i, ahead[k]);
+    for (int k = 0; k < HEAD; ++k) count((int)threadIdx.x + k * LOGITS_THREADS, ahead[k]);
+    // the rest of a long history, CHUNK loads under way at once (a plain loop of
+    // one token: 38 us against 20 at 8 x 50257 float32 with 30000 tokens)
+    for (int from = HEAD * LOGITS_THREADS; from < len; from += CHUNK * LOGITS_THREADS) {
+      const int i = from + (int)threadIdx.x;
+      long long t[CHUNK];
+#pragma unroll
+      for (int k = 0; k < CHUNK; ++k) t[k] = i + k * LOGITS_THREADS < len ? tok[i + k * LOGITS_THREADS] : 0;
+#pragma unroll
+      for (int k = 0; k < CHUNK; ++k) count(i + k * LOGITS_THREADS, t[k]);
     }
-#pragma unroll 4
-    for (int i = threadIdx.x + HEAD * LOGITS_THREADS; i < len; i += LOGITS_THREADS) count(i, tok[i]);
     __syncthreads();
   }
 #pragma unroll
@@ -236,6 +245,7 @@ int gfn_process_logits(const void* logits, long long logits_row_stride, int dtyp
                 history);
   if (history > 0 && !tokens) return fail(GFN_ERR_INVALID, "process_logits: a history without tokens");
   if (batch > 65535) return fail(GFN_ERR_UNSUPPORTED, "process_logits: batch %d above 65535", batch);
+  if (history > 1 << 30) return fail(GFN_ERR_UNSUPPORTED, "process_logits: history %d above 2^30", history);
   if ((!repetition_rows && !(repetition > 0.f)) || (!temperature_rows && !(temperature > 0.f)))
     return fail(GFN_ERR_INVALID, "process_logits: repetition penalty and temperature must be positive");
   if (batch == 0) return GFN_OK;
