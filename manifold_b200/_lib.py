@@ -5,11 +5,9 @@ The library is built in-tree (``manifold_b200/libgfn_b200.so``) by
 missing or a call fails, a ``GfnError`` is raised.
 """
 import ctypes
-import functools
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GFN_B200_LIB") or os.path.join(_HERE, "libgfn_b200.so")
@@ -131,6 +129,30 @@ def load():
     return lib
 
 
+# what _torch_ops calls, in the order of its GFN_ENTRIES
+TORCH_ENTRIES = ("gfn_status_string", "gfn_last_error_message", "gfn_layer_norm_forward",
+                 "gfn_layer_norm_backward_workspace_floats", "gfn_layer_norm_backward",
+                 "gfn_gated_scan_states_floats", "gfn_gated_scan_workspace_bytes", "gfn_gated_scan_forward",
+                 "gfn_gated_scan_backward", "gfn_layer_scan_forward", "gfn_layer_scan_backward",
+                 "gfn_process_logits")
+_torch_ops = None
+
+
+def torch_ops():
+    """The C++ binding of the language-model operators (csrc/torch_ops.cpp),
+    loaded and bound to the library once.  Raises GfnError if it is absent."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = load()
+        try:
+            from . import _torch_ops as module
+        except ImportError as e:
+            raise GfnError(f"manifold_b200/_torch_ops.so: {e}; build it with manifold_b200.build.build()") from e
+        module.bind(tuple(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in TORCH_ENTRIES), GfnError)
+        _torch_ops = module
+    return _torch_ops
+
+
 def check(status, what):
     if status != 0:
         lib = load()
@@ -177,17 +199,6 @@ def dtype_code(t, name):
     return code
 
 
-def call_on(t, name, *args):
-    """`call` on tensor t's device, with that device's current stream as the
-    last argument (the device is made current when it is not)."""
-    index = t.get_device()
-    if index == torch._C._cuda_getDevice():  # a CUDA tensor exists, so CUDA is initialised
-        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-
-
 def same_device(what, first, *others):
     """Every operand on one CUDA device."""
     index = first.get_device() if first.is_cuda else -1
@@ -197,19 +208,6 @@ def same_device(what, first, *others):
             raise GfnError(f"{what}: operands on {first.device} and {t.device}")
     if index < 0:
         require_cuda(first)
-
-
-def first_order(backward):
-    """Decorator of an autograd Function's backward whose result is not
-    differentiable: once_differentiable, entered only when a graph of the
-    gradients is being recorded (its bookkeeping costs as much as a launch)."""
-    checked = once_differentiable(backward)
-
-    @functools.wraps(backward)
-    def run(ctx, *grads):
-        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-    return run
 
 
 def require_cuda(*tensors):

@@ -1,4 +1,4 @@
-"""Builds libgfn_b200.so in-tree for sm_100a (nvcc; no GPU needed)."""
+"""Builds libgfn_b200.so and _torch_ops.so in-tree for sm_100a (nvcc; no GPU needed)."""
 import os
 import subprocess
 

@@ -6,7 +6,6 @@ gate's weights included."""
 import torch
 from torch.autograd import Function
 
-from .._lib import first_order
 from . import ops
 
 
@@ -72,26 +71,3 @@ def leapfrog_fused_autograd(x, v, f, U, W, dt, dt_scale, steps, topology=0, Wf=N
                             plasticity=0.0, R=2.0, r=1.0, Wi=None):
     return LeapfrogFusedFn.apply(x, v, f, U, W, dt, dt_scale, steps, topology, Wf, bf, plasticity, R,
                                  r, Wi)
-
-
-class LayerScanFn(Function):
-    """The scan layer's recurrence (gfn/layers/parallel.py:101-121) with the
-    gradients of its pre-activations and of the carried state (v0, x0)."""
-
-    @staticmethod
-    def forward(ctx, z, v0, x0, heads, base_dt, return_state):
-        xs, vs, vl, xl, states = ops.layer_scan_forward(z, v0, x0, heads, base_dt, return_state, True)
-        ctx.save_for_backward(z, states)
-        ctx.args = (heads, base_dt)
-        ctx.set_materialize_grads(False)
-        return (xs, vs, vl, xl) if return_state else (xs, vs)
-
-    @staticmethod
-    @first_order
-    def backward(ctx, gx, gv, gvl=None, gxl=None):
-        if gx is None and gv is None and gvl is None and gxl is None:
-            return None, None, None, None, None, None
-        z, states = ctx.saved_tensors
-        dz, dv0, dx0 = ops.layer_scan_backward(z, states, gx, gv, gvl, gxl, *ctx.args, ctx.needs_input_grad[1],
-                                               ctx.needs_input_grad[2])
-        return dz, dv0, dx0, None, None, None

@@ -481,50 +481,8 @@ def _layer_scan(z, heads, base_dt, state, return_state):
         if t is not None and (t.dtype != torch.float32 or t.shape != (z.shape[0], z.shape[2] // 3)):
             raise GfnError(f"parallel_layer_scan: state {name} must be float32 [{z.shape[0]}, {z.shape[2] // 3}], "
                            f"got {t.dtype} {tuple(t.shape)}")
-    if _grad_wanted(z, v0, x0):
-        from .autograd import LayerScanFn
-        out = LayerScanFn.apply(z, v0, x0, int(heads), float(base_dt), return_state)
-    else:
-        out = layer_scan_forward(z, v0, x0, heads, base_dt, return_state, False)
-    return (out[0], out[1], (out[2], out[3])) if return_state else (out[0], out[1])
-
-
-def layer_scan_forward(z, v0, x0, heads, base_dt, want_last, want_states):
-    """One launch of the stateful layer scan: (x_seq, v_seq, v_last, x_last, states)."""
-    B, L, D = z.shape[0], z.shape[1], z.shape[2] // 3
-    z = z.contiguous()
-    v0 = None if v0 is None else v0.contiguous()
-    x0 = None if x0 is None else x0.contiguous()
-    lib = _lib.load()
-    x_seq = z.new_empty((B, L, D))
-    v_seq = torch.empty_like(x_seq)
-    v_last = x_last = states = ws = None
-    if want_last:
-        v_last = z.new_empty((B, D))
-        x_last = torch.empty_like(v_last)
-    if want_states:
-        states = z.new_empty(lib.gfn_gated_scan_states_floats(B, L, D))
-    n = lib.gfn_gated_scan_workspace_bytes(B, L, D)
-    if n:
-        ws = z.new_empty(n, dtype=torch.uint8)
-    _lib.call_on(z, "gfn_layer_scan_forward", z.data_ptr(), ptr(v0), ptr(x0), B, L, D, int(heads), float(base_dt),
-                 x_seq.data_ptr(), v_seq.data_ptr(), ptr(x_last), ptr(v_last), ptr(states), ptr(ws), n)
-    return x_seq, v_seq, v_last, x_last, states
-
-
-def layer_scan_backward(z, states, gx, gv, gvl, gxl, heads, base_dt, want_v0, want_x0):
-    """Gradients (dz, dv0, dx0) of the layer scan; any upstream gradient may be None."""
-    B, L, D = z.shape[0], z.shape[1], z.shape[2] // 3
-    z = z.contiguous()
-    gx, gv, gvl, gxl = [None if g is None else g.contiguous() for g in (gx, gv, gvl, gxl)]
-    dz = torch.empty_like(z)
-    dv0 = z.new_empty((B, D)) if want_v0 else None
-    dx0 = z.new_empty((B, D)) if want_x0 else None
-    n = _lib.load().gfn_gated_scan_workspace_bytes(B, L, D)
-    ws = z.new_empty(n, dtype=torch.uint8) if n else None
-    _lib.call_on(z, "gfn_layer_scan_backward", z.data_ptr(), states.data_ptr(), ptr(gx), ptr(gv), ptr(gxl), ptr(gvl),
-                 B, L, D, int(heads), float(base_dt), dz.data_ptr(), ptr(dx0), ptr(dv0), ptr(ws), n)
-    return dz, dv0, dx0
+    out = _lib.torch_ops().layer_scan(z, v0, x0, int(heads), float(base_dt), return_state, _grad_wanted(z, v0, x0))
+    return (out[0], out[1], (out[2], out[3])) if return_state else out
 
 
 def functional_embedding(ids, W0, b0, W1, b1, W2, b2, Wo, bo, impulse, omega0=30.0,

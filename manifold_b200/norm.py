@@ -10,65 +10,7 @@ return the gradients of x, weight and bias.  CUDA tensors only.
 import torch
 import torch.nn as nn
 
-from . import _lib
-from ._lib import GfnError, call_on, dtype_code, first_order, ptr, same_device
-
-
-def _rows(t, dim):
-    """(t or a copy of it, rows, row stride): rows of `dim` elements with inner
-    stride 1, in place where t has them."""
-    if t.is_contiguous():
-        return t, t.numel() // dim, dim
-    r = t.reshape(-1, dim)
-    if (dim > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < dim):  # rows that overlap are expanded ones
-        r = r.contiguous()
-    return r, r.shape[0], r.stride(0) if r.shape[0] > 1 else dim
-
-
-def _forward(x, weight, bias, eps, want_stats):
-    D = x.shape[-1]
-    xr, rows, stride = _rows(x, D)
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    stats = x.new_empty((rows, 2), dtype=torch.float32) if want_stats else None
-    w = weight if weight is not None else bias
-    code = _lib.DTYPES[x.dtype]
-    call_on(x, "gfn_layer_norm_forward", xr.data_ptr(), stride, ptr(weight), ptr(bias), code,
-            code if w is None else _lib.DTYPES[w.dtype], rows, D, eps, y.data_ptr(), ptr(stats))
-    return y, stats
-
-
-class LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = _forward(x, weight, bias, eps, True)
-        # the caller's own tensor, so that a later in-place change of it is noticed
-        ctx.save_for_backward(x, weight, stats)
-        w = weight if weight is not None else bias
-        ctx.wdt = x.dtype if w is None else w.dtype
-        return y
-
-    @staticmethod
-    @first_order
-    def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        D, wdt = x.shape[-1], ctx.wdt
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        xr, rows, xs = _rows(x, D)
-        dr, _, ds = _rows(dy, D)
-        dx = dw = db = ws = None
-        n = 0
-        if need_x:
-            dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-        if need_w:
-            dw = x.new_empty(D, dtype=wdt)
-        if need_b:
-            db = x.new_empty(D, dtype=wdt)
-        if need_w or need_b:
-            n = _lib.load().gfn_layer_norm_backward_workspace_floats(rows, D)
-            ws = x.new_empty(n, dtype=torch.float32)
-        call_on(x, "gfn_layer_norm_backward", xr.data_ptr(), xs, dr.data_ptr(), ds, ptr(weight), stats.data_ptr(),
-                _lib.DTYPES[x.dtype], _lib.DTYPES[wdt], rows, D, ptr(dx), ptr(dw), ptr(db), ptr(ws), n)
-        return dx, dw, db, None
+from ._lib import GfnError, dtype_code, same_device, torch_ops
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -94,9 +36,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         wants = wants or (grad and bias.requires_grad)
         if weight is not None and weight.dtype != bias.dtype:
             raise GfnError(f"layer_norm: weight is {weight.dtype}, bias {bias.dtype}")
-    if wants:
-        return LayerNormFn.apply(x, weight, bias, eps)
-    return _forward(x, weight, bias, eps, False)[0]
+    return torch_ops().layer_norm(x, weight, bias, eps, wants)
 
 
 def _weight(name, t, x):

@@ -3,8 +3,7 @@ bias, the temperature and a grammar mask, in one kernel (the reference samples
 from bare logits, gfn/model.py:404-469).  CUDA tensors only."""
 import torch
 
-from . import _lib
-from ._lib import GfnError, call_on, dtype_code, ptr, same_device
+from ._lib import GfnError, dtype_code, same_device, torch_ops
 
 
 def pack_token_mask(mask):
@@ -76,7 +75,7 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
     code = dtype_code(logits, "logits")
     B, V = logits.shape
     x = logits if logits.is_contiguous() or V == 1 or logits.stride(1) == 1 else logits.contiguous()
-    T = ts = 0
+    ts = 0
     if tokens is not None:
         if tokens.dim() != 2 or tokens.shape[0] != B or (tokens.dtype != torch.int64 and tokens.dtype != torch.int32):
             raise GfnError(f"process_logits: tokens must be int64 [{B}, T], got {tokens.dtype} {tuple(tokens.shape)}")
@@ -106,8 +105,5 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
         if allowed.dtype != torch.int32:
             raise GfnError(f"process_logits: allowed must be bool or int32 words, got {allowed.dtype}")
         allowed, ms = _rows_or_shared(allowed, "allowed", B, (V + 31) // 32)
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    call_on(logits, "gfn_process_logits", x.data_ptr(), x.stride(0) if B > 1 else V, code, B, V, ptr(tokens), ts, T,
-            ptr(lengths), ptr(prompt_lengths), rep, ptr(rep_rows), freq, ptr(freq_rows), pres, ptr(pres_rows), temp,
-            ptr(temp_rows), ptr(bias), bs, ptr(allowed), ms, out.data_ptr())
-    return out
+    return torch_ops().process_logits(x, tokens, ts, lengths, prompt_lengths, rep, freq, pres, temp, rep_rows, freq_rows,
+                                      pres_rows, temp_rows, bias, bs, allowed, ms)

@@ -4,8 +4,7 @@ and the gated scan: the same recurrence with gradients, a carried state and
 16-bit operands."""
 import torch
 
-from . import _lib
-from ._lib import GfnError, call_on, dtype_code, first_order, ptr, same_device
+from ._lib import GfnError, dtype_code, same_device, torch_ops
 from .cuda.ops import _grad_wanted, parallel_scan_fused
 
 CUDA_AVAILABLE = True
@@ -19,72 +18,6 @@ def parallel_scan(a, x):
             raise GfnError(f"x must be float32, got {x.dtype}")
         return gated_scan(a, x)
     return parallel_scan_fused(a, x)
-
-
-def _operand(t):
-    """t [B, L, D] with inner stride 1 (itself where it has one: strided and
-    broadcast batches and steps are read in place)."""
-    return t if t.is_contiguous() or t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
-
-
-def _workspace(x, B, L, D):
-    n = _lib.load().gfn_gated_scan_workspace_bytes(B, L, D) if L > 1 else 0
-    return (x.new_empty(n, dtype=torch.uint8) if n else None), n
-
-
-def _forward(a, x, h0, want_last, want_states):
-    B, L, D = x.shape
-    x = _operand(x)
-    h0 = None if h0 is None else h0.contiguous()
-    h = torch.empty_like(x, memory_format=torch.contiguous_format)
-    last = x.new_empty((B, D), dtype=torch.float32) if want_last else None
-    states = None
-    if want_states:
-        states = x.new_empty(_lib.load().gfn_gated_scan_states_floats(B, L, D), dtype=torch.float32)
-    ws, n = _workspace(x, B, L, D)
-    pa = sa = ta = 0
-    if a is not None:
-        a = _operand(a)
-        pa, (sa, ta, _) = a.data_ptr(), a.stride()
-    sx, tx, _ = x.stride()
-    call_on(x, "gfn_gated_scan_forward", pa, sa, ta, x.data_ptr(), sx, tx, ptr(h0), _lib.DTYPES[x.dtype], B, L, D,
-            h.data_ptr(), ptr(last), ptr(states), ptr(ws), n)
-    return h, last, states
-
-
-class GatedScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, a, x, h0, return_state):
-        h, last, states = _forward(a, x, h0, return_state, True)
-        ctx.save_for_backward(a, x, states)
-        ctx.set_materialize_grads(False)
-        return (h, last) if return_state else h
-
-    @staticmethod
-    @first_order
-    def backward(ctx, dh, dlast=None):
-        a, x, states = ctx.saved_tensors
-        if dh is None and dlast is None:
-            return None, None, None, None
-        B, L, D = x.shape
-        need_a, need_x, need_h0, _ = ctx.needs_input_grad
-        x = _operand(x)
-        dlast = None if dlast is None else dlast.contiguous()
-        da = torch.empty_like(x, memory_format=torch.contiguous_format) if need_a else None
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-        dh0 = x.new_empty((B, D), dtype=torch.float32) if need_h0 else None
-        ws, n = _workspace(x, B, L, D)
-        pa = sa = ta = pg = sg = tg = 0
-        if a is not None:
-            a = _operand(a)
-            pa, (sa, ta, _) = a.data_ptr(), a.stride()
-        if dh is not None:
-            dh = _operand(dh)
-            pg, (sg, tg, _) = dh.data_ptr(), dh.stride()
-        sx, tx, _ = x.stride()
-        call_on(x, "gfn_gated_scan_backward", pa, sa, ta, x.data_ptr(), sx, tx, states.data_ptr(), pg, sg, tg,
-                ptr(dlast), _lib.DTYPES[x.dtype], B, L, D, ptr(da), ptr(dx), ptr(dh0), ptr(ws), n)
-        return da, dx, dh0, None
 
 
 def gated_scan(a, x, h0=None, return_state=False):
@@ -123,7 +56,5 @@ def gated_scan(a, x, h0=None, return_state=False):
             raise GfnError(f"gated_scan: h0 must be float32 [{x.shape[0]}, {x.shape[2]}], got {h0.dtype} "
                            f"{tuple(h0.shape)}")
         wants = wants or h0.requires_grad
-    if wants and torch.is_grad_enabled():
-        return GatedScanFn.apply(a, x, h0, return_state)
-    h, last, _ = _forward(a, x, h0, return_state, False)
-    return (h, last) if return_state else h
+    out = torch_ops().gated_scan(a, x, h0, return_state, wants and torch.is_grad_enabled())
+    return out if return_state else out[0]
