@@ -2,7 +2,8 @@
 // layer's scan, logit shaping): allocation, streams and autograd nodes around
 // the C ABI, in C++ because a small call is bound by the host.  A call through
 // ctypes and a Python autograd Function took 10.8 us forward and, trained,
-// 104 us where the engine's own hand-over between threads is 45.
+// 104 us, of which the hand-over to the engine's thread and back is 45; here a
+// call takes 7 and a small training step 65 to 80.
 // Arguments arrive checked (norm.py, scan.py, cuda/ops.py, sampling.py); the
 // entry points of the C ABI are handed over by bind(), so that one library is
 // loaded whoever calls.
