@@ -18,15 +18,20 @@ def pack_token_mask(mask):
     return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
 
 
-def _per_row(v, name, x, positive):
-    """(number, pointer or None) of a parameter given as a number or per row of x."""
+_CUT = "process_logits is not differentiable: call it under torch.no_grad() or on detached tensors"
+
+
+def _per_row(v, name, B, x, grad, positive):
+    """(number, tensor or None) of a parameter given as a number or per row of x."""
     if not isinstance(v, torch.Tensor):
         if positive and not v > 0:
             raise GfnError(f"process_logits: {name} must be positive, got {v}")
         return v, None
-    if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != x.shape[0] or v.get_device() != x.get_device():
-        raise GfnError(f"process_logits: {name} must be a number or float32 [{x.shape[0]}] on {x.device}, got "
+    if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != B or v.get_device() != x.get_device():
+        raise GfnError(f"process_logits: {name} must be a number or float32 [{B}] on {x.device}, got "
                        f"{v.dtype} {tuple(v.shape)} on {v.device}")
+    if grad and v.requires_grad:
+        raise GfnError(_CUT)
     return 1.0, v if v.is_contiguous() else v.contiguous()
 
 
@@ -67,12 +72,10 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
     same_device("process_logits", logits, tokens, lengths, prompt_lengths, bias, allowed)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise GfnError(f"process_logits: logits must be [batch, vocab], got {tuple(logits.shape)}")
-    if torch.is_grad_enabled():
-        for t in (logits, bias, repetition_penalty, frequency_penalty, presence_penalty, temperature):
-            if isinstance(t, torch.Tensor) and t.requires_grad:
-                raise GfnError("process_logits is not differentiable: call it under torch.no_grad() or on detached "
-                               "tensors")
-    code = dtype_code(logits, "logits")
+    grad = torch.is_grad_enabled()
+    if grad and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        raise GfnError(_CUT)
+    dtype_code(logits, "logits")
     B, V = logits.shape
     x = logits if logits.is_contiguous() or V == 1 or logits.stride(1) == 1 else logits.contiguous()
     ts = 0
@@ -90,10 +93,10 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
         prompt_lengths = None if prompt_lengths is None else _lengths(prompt_lengths, "prompt_lengths", B)
     elif lengths is not None or prompt_lengths is not None:
         raise GfnError("process_logits: lengths need tokens")
-    rep, rep_rows = _per_row(repetition_penalty, "repetition_penalty", logits, True)
-    freq, freq_rows = _per_row(frequency_penalty, "frequency_penalty", logits, False)
-    pres, pres_rows = _per_row(presence_penalty, "presence_penalty", logits, False)
-    temp, temp_rows = _per_row(temperature, "temperature", logits, True)
+    rep, rep_rows = _per_row(repetition_penalty, "repetition_penalty", B, logits, grad, True)
+    freq, freq_rows = _per_row(frequency_penalty, "frequency_penalty", B, logits, grad, False)
+    pres, pres_rows = _per_row(presence_penalty, "presence_penalty", B, logits, grad, False)
+    temp, temp_rows = _per_row(temperature, "temperature", B, logits, grad, True)
     bs = ms = 0
     if bias is not None:
         bias, bs = _rows_or_shared(bias.to(torch.float32), "bias", B, V)
