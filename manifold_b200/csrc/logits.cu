@@ -13,10 +13,9 @@
 // and then streams its logits once.
 //
 // 35 us at 256 x 50257 bfloat16 with biases, masks and up to 2048 tokens of
-// history (3.1 TB/s); 13 us a call, launch and checks included, for one row of
-// 32000.  The bytes would take 17 us: the rest is instructions (70 per element
-// there, 30 without history, bias and mask), half of them what a thread does
-// once for its 8 elements.
+// history (3.1 TB/s); 9 us a call, launch and checks included, for one row of
+// 32000.  The bytes would take 17 us: the rest is instructions, 58 per element
+// there, 25 without history (27 us) and 14 without bias and mask too.
 #include "abi.h"
 #include "lm_ops.cuh"
 
