@@ -1,6 +1,7 @@
 """Builds libgfn_b200.so and _torch_ops.so in-tree for sm_100a (nvcc; no GPU needed)."""
 import os
 import subprocess
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -8,7 +9,7 @@ CSRC = os.path.join(HERE, "csrc")
 
 def build(verbose=False):
     """Run the csrc Makefile (incremental).  Raises on a compiler error."""
-    res = subprocess.run(["make", "-j4", "-C", CSRC], capture_output=True, text=True)
+    res = subprocess.run(["make", "-j4", "-C", CSRC, f"PYTHON={sys.executable}"], capture_output=True, text=True)
     if verbose or res.returncode != 0:
         print(res.stdout)
         print(res.stderr)
