@@ -37,6 +37,7 @@
 // about 5,000 of a block's 13,000 cycles per run; off 16 bytes, the loads'
 // latency and 70 (forward) to 113 (backward) instructions per element.
 #pragma once
+#include <cfloat>
 #include <type_traits>
 
 #include "lm_ops.cuh"
@@ -90,31 +91,181 @@ GFN_DEV void word_store(unsigned long long* p, unsigned long long v) {
   asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
 
-// Product of two runs' gates.  A product of non-zero gates that underflows is
-// held at the smallest float, so that an infinite state stays infinite as it
-// does step by step (0 * inf would be NaN); its weight is 1e-45.
-GFN_DEV float gate_product(float a, float b) {
-  const float r = a * b;
-  return (r == 0.f && a != 0.f && b != 0.f) ? copysignf(1.4e-45f, r) : r;
+// ------------------------------------------------------------ products of gates
+// A product P of the gates of many steps leaves float32's range long before
+// P h does, and may come back (256 gates of 0.5, then 256 of 1.9).  It is held in
+// 32 bits of wider range: a product from 2^-99 to 2^100, 0 or NaN is that float,
+// and codes that are other floats stand for 2^-278 to 2^-99 and 2^100 to 2^278
+// with 20 bits after the point, as the high word of a float64 has them (one such
+// rounding is eight of float32's, on a product that has decayed or grown by 2^99).
+// Above that it is infinite: any state would be.  Below it is GAIN_TINY: every
+// finite state has underflowed to zero, an infinite one stays infinite.  Both
+// remain, whatever gates follow, as such a state does step by step.
+constexpr unsigned GAIN_TINY = 1u, GAIN_INF = 0x7f800000u;
+constexpr unsigned GAIN_LOW_CODES = 0x00800000u, GAIN_HIGH_CODES = 0x72000000u;  // of 2^-278 and of 2^100
+constexpr unsigned GAIN_PLAIN = 0x0e000000u;  // 2^-99: floats from here to GAIN_HIGH_CODES are themselves
+constexpr float GAIN_LEAST = 0x1p-99f;
+constexpr int GAIN_STUCK = 1 << 20;  // |e| of a product beyond the codes
+
+GFN_DEV unsigned gain_magnitude(float g) { return __float_as_uint(g) & 0x7fffffffu; }
+GFN_DEV bool gain_plain(float g) { return gain_magnitude(g) - GAIN_PLAIN < GAIN_HIGH_CODES - GAIN_PLAIN; }
+
+struct Gain {  // m 2^e
+  float m;     // of either sign, from 1 on; 0 or NaN
+  int e;
+
+  GFN_DEV static Gain of_plain(float g) {
+    return {__uint_as_float((__float_as_uint(g) & 0x807fffffu) | 0x3f800000u), (int)(gain_magnitude(g) >> 23) - 127};
+  }
+  GFN_DEV static Gain of(float g) {
+    const unsigned u = gain_magnitude(g), sign = __float_as_uint(g) & 0x80000000u;
+    if (gain_plain(g)) return of_plain(g);
+    if (u == 0 || u > GAIN_INF) return {g, 0};
+    if (u == GAIN_TINY || u == GAIN_INF)
+      return {__uint_as_float(sign | 0x3f800000u), u == GAIN_TINY ? -GAIN_STUCK : GAIN_STUCK};
+    const unsigned w = u < GAIN_PLAIN ? u - GAIN_LOW_CODES : u - GAIN_HIGH_CODES;
+    return {__uint_as_float(sign | ((w & 0x000fffffu) << 3) | 0x3f800000u),
+            (int)(w >> 20) + (u < GAIN_PLAIN ? -278 : 100)};
+  }
+  // this, then l (fewer than 64 products are multiplied before they are packed)
+  GFN_DEV void append(Gain l) {
+    m *= l.m;
+    if (e > -GAIN_STUCK / 2 && e < GAIN_STUCK / 2) e += l.e;
+  }
+  GFN_DEV float pack() const {
+    const unsigned u = gain_magnitude(m), sign = __float_as_uint(m) & 0x80000000u;
+    const int x = (int)(u >> 23) - 127 + e;
+    if (u == 0) return e < GAIN_STUCK / 2 ? m : __uint_as_float(0x7fffffffu);  // 0 after an infinity: NaN
+    if (u > GAIN_INF) return m;
+    if (x >= -99 && x < 100) return __uint_as_float(sign | (u + ((unsigned)e << 23)));
+    if (x < -278) return __uint_as_float(sign | GAIN_TINY);
+    if (x >= 278) return __uint_as_float(sign | GAIN_INF);
+    const unsigned w = ((u & 0x007fffffu) + 4u) >> 3;  // to 20 bits; 2^20 moves into the exponent
+    return __uint_as_float(sign | ((x < 0 ? ((unsigned)(x + 278) << 20) + GAIN_LOW_CODES
+                                          : ((unsigned)(x - 100) << 20) + GAIN_HIGH_CODES) + w));
+  }
+  GFN_DEV float carry(float h, float p) const {  // P h + p
+    const double P = (double)m * __hiloint2double((max(-1000, min(1000, e)) + 1023) << 20, 0);
+    return (float)fma(P, (double)h, (double)p);
+  }
+};
+
+// A P below 2^-99 drops a state below 2^73 times what is added to it: at most
+// 2^-26 of that, half of a rounding.
+GFN_DEV bool gain_small(float P) { return fabsf(P) < GAIN_LEAST; }
+GFN_DEV bool gain_drops(float h, float p) { return fabsf(h) <= fminf(0x1p73f * fabsf(p), FLT_MAX); }
+// P h + p for a packed P.
+GFN_DEV float carry(float P, float h, float p) {
+  if (gain_plain(P)) return fmaf(P, h, p);
+  return h == 0.f || (gain_small(P) && gain_drops(h, p)) ? p : Gain::of(P).carry(h, p);
 }
-// P h + p; a zero state passes as p alone (an overflowed P must not make NaN of it).
+// The same for other factors.  In both a zero state passes as p alone (an infinite P must not make NaN of it).
 GFN_DEV float pass(float P, float h, float p) { return h == 0.f ? p : fmaf(P, h, p); }
 
-// Maps of a run of steps and how they compose: `compose(l, e)` applies e first.
+// The rare ways through a run or a group are calls: in line their registers
+// would be taken from the walk over the operands.
+//
+// The packed product of n gates, mantissas and exponents multiplied apart.
+__device__ __noinline__ float gain_of_gates(const float* gates, int n) {
+  Gain r = {1.f, 0};
+  float special = 1.f;
+  for (int s = 0; s < n; ++s) {
+    float g = gates[s];
+    if (g == 0.f || !(fabsf(g) < INFINITY)) {
+      special *= g;
+    } else {
+      if (fabsf(g) < 0x1p-126f) {  // subnormal
+        g *= 0x1p32f;
+        r.e -= 32;
+      }
+      const unsigned u = __float_as_uint(g);
+      r.m *= __uint_as_float((u & 0x807fffffu) | 0x3f800000u);
+      r.e += (int)((u >> 23) & 255u) - 127;
+    }
+  }
+  return special != 1.f ? special : r.pack();  // 0, an infinity or NaN among the gates decides
+}
+
+// The same of S gates, given as float32's products of every 8 of them and the
+// largest magnitude among them.  Such a product is right if it is in the plain
+// range and no part of it can have left float32's normal range on the way: with
+// magnitudes up to 2^(26 / 8) what follows a part grows by 2^26 at most, so the
+// part was at least 2^-126.
+template <int S, class Gate>
+GFN_DEV float gain_run(const float (&eights)[S / 8], float largest, Gate gate) {
+  static_assert(S <= 32, "");
+  float all = eights[0];
+  bool right = largest <= 9.5f && gain_plain(eights[0]);
+#pragma unroll
+  for (int k = 1; k < S / 8; ++k) {
+    all *= eights[k];
+    right = right && gain_plain(eights[k]);
+  }
+  if (right && gain_plain(all) && (S <= 16 || largest <= 1.f)) return all;
+  if (right) {
+    Gain r = Gain::of_plain(eights[0]);
+#pragma unroll
+    for (int k = 1; k < S / 8; ++k) {
+      const Gain l = Gain::of_plain(eights[k]);
+      r = {r.m * l.m, r.e + l.e};
+    }
+    return r.pack();
+  }
+  float gates[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) gates[s] = gate(s);
+  return gain_of_gates(gates, S);
+}
+
+// Maps of a run of steps, and chains of them: append(l) puts l behind what is
+// there.  Chain is right for every P.  Quick serves the usual case in float32,
+// products of at most 1 that drop what they are handed where they are below 2^-99;
+// where that does not hold, ok turns false and the maps have to be gone through
+// again as a Chain.  append_plain(l) is for a P from 2^-99 to 1.
 struct GatedMap {  // h -> P h + p
   static constexpr int WORDS = 1;
   float P, p;
-  GFN_DEV static GatedMap identity() { return {1.f, 0.f}; }
-  GFN_DEV static GatedMap compose(GatedMap l, GatedMap e) { return {gate_product(l.P, e.P), pass(l.P, e.p, l.p)}; }
   GFN_DEV void pack(unsigned long long (&w)[WORDS]) const { w[0] = scan_word(P, p); }
   GFN_DEV static GatedMap unpack(const unsigned long long (&w)[WORDS]) { return {word_lo(w[0]), word_hi(w[0])}; }
+  struct Chain {
+    Gain P = {1.f, 0};
+    float p = 0.f;
+    GFN_DEV void append(GatedMap l) {
+      p = carry(l.P, p, l.p);
+      P.append(Gain::of(l.P));
+    }
+    GFN_DEV GatedMap map() const { return {P.pack(), p}; }
+  };
+  struct Quick {
+    float P = 1.f, p = 0.f;
+    bool ok = true;
+    GFN_DEV void append_plain(GatedMap l) {
+      p = fmaf(l.P, p, l.p);
+      P *= l.P;
+    }
+    GFN_DEV void append(GatedMap l) {
+      if (gain_small(l.P)) {
+        ok = ok && (gain_drops(p, l.p) || (l.P == 0.f && fabsf(p) < INFINITY));
+        l.P = 0.f;
+      }
+      ok = ok && fabsf(l.P) <= 1.f;
+      append_plain(l);
+    }
+    GFN_DEV bool right() const { return ok; }
+    GFN_DEV GatedMap map() const { return {ok ? P : INFINITY, p}; }
+  };
 };
 struct GatedState {
   static constexpr int WORDS = 1;
   float h;
   GFN_DEV void pack(unsigned long long (&w)[1]) const { w[0] = scan_word(h, 0.f); }
   GFN_DEV static GatedState unpack(const unsigned long long (&w)[1]) { return {word_lo(w[0])}; }
-  GFN_DEV GatedState through(GatedMap m) const { return {pass(m.P, h, m.p)}; }
+  GFN_DEV GatedState through(GatedMap m) const { return {carry(m.P, h, m.p)}; }
+  GFN_DEV bool through(const GatedMap::Quick& m, GatedState& out) const {  // whether it can
+    const bool small = gain_small(m.P);
+    out.h = fmaf(small ? 0.f : m.P, h, m.p);
+    return m.right() && (!small || gain_drops(h, m.p));
+  }
 };
 
 constexpr int SCAN_GROUP = 32;  // the most runs in a group
@@ -178,6 +329,39 @@ struct ScanShared {
   }
 };
 
+// The map of warp j of a run (counted in the direction of the scan) for column c,
+// and in its place what is before it.
+template <class Map, bool REV, int CT, int NW, class Chain>
+GFN_DEV Map before_warp(const Chain& before, unsigned long long (*maps)[Map::WORDS][CT], int j, int c) {
+  unsigned long long x[Map::WORDS], y[Map::WORDS];
+  unsigned long long(&at)[Map::WORDS][CT] = maps[REV ? NW - 1 - j : j];
+  before.map().pack(y);
+#pragma unroll
+  for (int i = 0; i < Map::WORDS; ++i) {
+    x[i] = at[i][c];
+    at[i][c] = y[i];
+  }
+  return Map::unpack(x);
+}
+template <class Map, bool REV, int CT, int NW>
+__device__ __noinline__ Map chain_warps(unsigned long long (*maps)[Map::WORDS][CT], int c) {
+  typename Map::Chain all;
+  for (int j = 0; j < NW; ++j) all.append(before_warp<Map, REV, CT, NW>(all, maps, j, c));
+  return all.map();
+}
+// `at` through the n maps of the group before a run, which are all published.
+template <class Map, class State>
+__device__ __noinline__ State chain_group(State at, const unsigned long long* words, long long stride, int ct, int n) {
+  typename Map::Chain all;
+  for (int k = 0; k < n; ++k) {
+    Map next[1];
+    await<Map, 1>(words + k * stride, 0, ct, 1, next);
+    all.append(next[0]);
+    all.P = Gain::of(all.P.pack());
+  }
+  return at.through(all.map());
+}
+
 // The state that `chunk` (counted in the direction of the scan) of a column
 // tile receives.  Call with the warps' maps in sh.maps; on return (after a
 // barrier) sh.maps[w] holds the map of the warps before w, counted in the
@@ -198,61 +382,80 @@ GFN_DEV void receive(ScanShared<Map, State, CT, NW>& sh, unsigned long long* wor
   const int pos = chunk % group, start = chunk - pos;
   const bool tells = teller && chunk + 1 < nchunks;
   unsigned long long* mine = words + (long long)chunk * W * CT + c;
-  Map own = Map::identity();
+  Map own;  // of this run
   __syncthreads();
   if (teller) {
+    float P = 1.f;
+    bool plain = true;  // a product of at most 1, and no part of it below the plain range
 #pragma unroll
     for (int j = 0; j < NW; ++j) {
-      const int w = REV ? NW - 1 - j : j;
-      unsigned long long x[W], y[W];
-      own.pack(y);
+      const float f = word_lo(sh.maps[j][0][c]);
+      plain = plain && fabsf(f) <= 1.f;
+      P *= f;
+    }
+    if (plain && fabsf(P) >= GAIN_LEAST) {
+      typename Map::Quick all;
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        x[i] = sh.maps[w][i][c];
-        sh.maps[w][i][c] = y[i];
-      }
-      own = Map::compose(Map::unpack(x), own);
+      for (int j = 0; j < NW; ++j) all.append_plain(before_warp<Map, REV, CT, NW>(all, sh.maps, j, c));
+      own = all.map();
+    } else {
+      own = chain_warps<Map, REV, CT, NW>(sh.maps, c);
     }
     if (tells && pos < group - 1) publish(own, mine, CT);
   }
   ahead();
   if (r == 0) beside(c);
-  Map acc = Map::identity();  // of the group's runs before this one
+  typename Map::Quick acc;  // of the group's runs before this one
   if (pos > 0) {
     if (active && r * GS < pos) {
       for (int k = r * GS; k < min((r + 1) * GS, pos); k += BATCH) {
         const int n = min(BATCH, min((r + 1) * GS, pos) - k);
         Map next[BATCH];
         await<Map, BATCH>(words + (long long)(start + k) * W * CT + c, W * CT, CT, n, next);
+        float least = 1.f, most = 0.f;
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-          if (i < n) acc = Map::compose(next[i], acc);
+        for (int i = 0; i < BATCH; ++i) {
+          if (i < n) {
+            least = fminf(least, fabsf(next[i].P));
+            most = fmaxf(most, fabsf(next[i].P));
+          }
+        }
+        if (least >= GAIN_LEAST && most <= 1.f) {  // a NaN goes through as one
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i)
+            if (i < n) acc.append_plain(next[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i)
+            if (i < n) acc.append(next[i]);
+        }
       }
       unsigned long long x[W];
-      acc.pack(x);
+      acc.map().pack(x);
 #pragma unroll
       for (int i = 0; i < W; ++i) sh.part[r][i][c] = x[i];
     }
     __syncthreads();
     if (teller) {
-      acc = Map::identity();
+      acc = typename Map::Quick();
 #pragma unroll
       for (int j = 0; j < R; ++j) {
         if (j * GS < pos) {
           unsigned long long x[W];
 #pragma unroll
           for (int i = 0; i < W; ++i) x[i] = sh.part[j][i][c];
-          acc = Map::compose(Map::unpack(x), acc);
+          acc.append(Map::unpack(x));
         }
       }
     }
   }
   if (teller) {
-    State at[1];  // at the group's start
+    State at[1], in;  // at the group's start; before this run
     if (start > 0) await<State, 1>(words + (long long)(start - 1) * W * CT + c, 0, CT, 1, at);
     else at[0] = first(c);
-    if (tells && pos == group - 1) publish(at[0].through(Map::compose(own, acc)), mine, CT);
-    sh.in[c] = at[0].through(acc);
+    if (!at[0].through(acc, in)) in = chain_group<Map, State>(at[0], words + (long long)start * W * CT + c, W * CT, CT, pos);
+    if (tells && pos == group - 1) publish(in.through(own), mine, CT);
+    sh.in[c] = in;
   }
   __syncthreads();
 }
@@ -436,20 +639,15 @@ GFN_DEV void keep_packed(Pack<T, VEC> (&a)[S]) {
 // Map of S steps from a zero state; steps beyond the end hold a = 1, x = 0.
 template <typename T, int VEC, int S>
 GFN_DEV GatedMap run_map(const Pack<T, VEC> (&a)[S], const Pack<T, VEC> (&x)[S], int v) {
-  GatedMap m = GatedMap::identity();
+  float eights[S / 8], p = 0.f, largest = 0.f;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const float g = a[s].get(v);
-    m.P *= g;
-    m.p = fmaf(g, m.p, x[s].get(v));
+    eights[s / 8] = s % 8 ? eights[s / 8] * g : g;
+    largest = fmaxf(largest, fabsf(g));
+    p = fmaf(g, p, x[s].get(v));
   }
-  if (m.P == 0.f) {  // a zero gate, or an underflow?
-    bool zero = false;
-#pragma unroll
-    for (int s = 0; s < S; ++s) zero = zero || a[s].get(v) == 0.f;
-    if (!zero) m.P = copysignf(1.4e-45f, m.P);
-  }
-  return m;
+  return {gain_run<S>(eights, largest, [&](int s) { return a[s].get(v); }), p};
 }
 
 template <int MODE, typename T, int VEC, int S, int NW, int OCC>
@@ -543,7 +741,7 @@ GFN_DEV void chain_states(const unsigned long long (*maps)[CT], const float* kep
   for (int j = 0; j < NW; ++j) {
     start[j][c] = h;
     const GatedMap f = GatedMap::unpack({maps[j][c]});
-    h = pass(f.P, h, f.p);
+    h = carry(f.P, h, f.p);
   }
 }
 
@@ -762,23 +960,9 @@ GFN_DEV float head_scale(int col, int hd) {
   return hs;
 }
 
-// A run's product of gates P, held above zero where no gate is zero (see gate_product).
-template <int S, int VEC>
-GFN_DEV float keep_positive(float P, const float (&A)[S][VEC], int v) {
-  if (P != 0.f) return P;
-  bool zero = false;
-#pragma unroll
-  for (int s = 0; s < S; ++s) zero = zero || A[s][v] == 0.f;
-  return zero ? 0.f : 1.4e-45f;
-}
-
 struct LayerMap {  // v -> P v + p, x -> x + Q v + q
   static constexpr int WORDS = 2;
   float P, p, Q, q;
-  GFN_DEV static LayerMap identity() { return {1.f, 0.f, 0.f, 0.f}; }
-  GFN_DEV static LayerMap compose(LayerMap l, LayerMap e) {
-    return {gate_product(l.P, e.P), pass(l.P, e.p, l.p), fmaf(l.Q, e.P, e.Q), e.q + pass(l.Q, e.p, l.q)};
-  }
   GFN_DEV void pack(unsigned long long (&w)[2]) const {
     w[0] = scan_word(P, p);
     w[1] = scan_word(Q, q);
@@ -786,13 +970,51 @@ struct LayerMap {  // v -> P v + p, x -> x + Q v + q
   GFN_DEV static LayerMap unpack(const unsigned long long (&w)[2]) {
     return {word_lo(w[0]), word_hi(w[0]), word_lo(w[1]), word_hi(w[1])};
   }
+  struct Chain {
+    Gain P = {1.f, 0};
+    float p = 0.f, Q = 0.f, q = 0.f;
+    GFN_DEV void append(LayerMap l) {
+      Q = P.carry(l.Q, Q);
+      q += pass(l.Q, p, l.q);
+      p = carry(l.P, p, l.p);
+      P.append(Gain::of(l.P));
+    }
+    GFN_DEV LayerMap map() const { return {P.pack(), p, Q, q}; }
+  };
+  struct Quick {
+    float P = 1.f, p = 0.f, Q = 0.f, q = 0.f, most = 0.f;  // most: the largest Q appended
+    bool ok = true;
+    GFN_DEV void append_plain(LayerMap l) {
+      most = fmaxf(most, l.Q);
+      Q = fmaf(l.Q, P, Q);
+      q += pass(l.Q, p, l.q);
+      p = fmaf(l.P, p, l.p);
+      P *= l.P;
+    }
+    GFN_DEV void append(LayerMap l) {
+      if (gain_small(l.P)) {
+        ok = ok && (gain_drops(p, l.p) || (l.P == 0.f && fabsf(p) < INFINITY));
+        l.P = 0.f;
+      }
+      ok = ok && fabsf(l.P) <= 1.f;
+      append_plain(l);
+    }
+    // Q adds up to 32 terms of Q P with a P below 2^-99 that may have been 0
+    GFN_DEV bool right() const { return ok && most <= fminf(0x1p68f * Q, FLT_MAX); }
+    GFN_DEV LayerMap map() const { return {right() ? P : INFINITY, p, Q, q}; }
+  };
 };
 struct LayerState {
   static constexpr int WORDS = 1;
   float v, x;
   GFN_DEV void pack(unsigned long long (&w)[1]) const { w[0] = scan_word(v, x); }
   GFN_DEV static LayerState unpack(const unsigned long long (&w)[1]) { return {word_lo(w[0]), word_hi(w[0])}; }
-  GFN_DEV LayerState through(LayerMap m) const { return {pass(m.P, v, m.p), x + pass(m.Q, v, m.q)}; }
+  GFN_DEV LayerState through(LayerMap m) const { return {carry(m.P, v, m.p), x + pass(m.Q, v, m.q)}; }
+  GFN_DEV bool through(const LayerMap::Quick& m, LayerState& out) const {
+    const bool small = gain_small(m.P);
+    out = {fmaf(small ? 0.f : m.P, v, m.p), x + pass(m.Q, v, m.q)};
+    return m.right() && (!small || gain_drops(v, m.p));
+  }
 };
 
 // 20 bytes per element, and 70 instructions: two exponentials, two reciprocals
@@ -850,7 +1072,8 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScan
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       const float scale = p.base_dt * head_scale(c.col + v, p.D / p.H);
-      LayerMap m = LayerMap::identity();
+      LayerMap m = {1.f, 0.f, 0.f, 0.f};
+      float eights[S / 8];
 #pragma unroll
       for (int s = 0; s < S; s += 2) {
         F2 slope;
@@ -862,11 +1085,12 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScan
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         m.P *= A[s][v];
+        eights[s / 8] = s % 8 ? eights[s / 8] * A[s][v] : A[s][v];
         m.p = fmaf(A[s][v], m.p, bv[s][v]);
         m.Q = fmaf(dt[s][v], m.P, m.Q);
         m.q = fmaf(dt[s][v], m.p, m.q);
       }
-      m.P = keep_positive<S, VEC>(m.P, A, v);
+      m.P = gain_run<S>(eights, 1.f, [&](int s) { return A[s][v]; });
       unsigned long long wd[2];
       m.pack(wd);
       sh.maps[w][0][lane * VEC + v] = wd[0];
@@ -924,10 +1148,6 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScan
 struct LayerBackMap {  // m -> P m + R X + q, X -> X + G
   static constexpr int WORDS = 2;
   float P, q, R, G;
-  GFN_DEV static LayerBackMap identity() { return {1.f, 0.f, 0.f, 0.f}; }
-  GFN_DEV static LayerBackMap compose(LayerBackMap l, LayerBackMap e) {
-    return {gate_product(l.P, e.P), pass(l.P, e.q, pass(l.R, e.G, l.q)), fmaf(l.P, e.R, l.R), l.G + e.G};
-  }
   GFN_DEV void pack(unsigned long long (&w)[2]) const {
     w[0] = scan_word(P, q);
     w[1] = scan_word(R, G);
@@ -935,13 +1155,50 @@ struct LayerBackMap {  // m -> P m + R X + q, X -> X + G
   GFN_DEV static LayerBackMap unpack(const unsigned long long (&w)[2]) {
     return {word_lo(w[0]), word_hi(w[0]), word_lo(w[1]), word_hi(w[1])};
   }
+  struct Chain {
+    Gain P = {1.f, 0};
+    float q = 0.f, R = 0.f, G = 0.f;
+    GFN_DEV void append(LayerBackMap l) {
+      q = carry(l.P, q, pass(l.R, G, l.q));
+      R = carry(l.P, R, l.R);
+      G += l.G;
+      P.append(Gain::of(l.P));
+    }
+    GFN_DEV LayerBackMap map() const { return {P.pack(), q, R, G}; }
+  };
+  struct Quick {
+    float P = 1.f, q = 0.f, R = 0.f, G = 0.f;
+    bool ok = true;
+    GFN_DEV void append_plain(LayerBackMap l) {
+      q = fmaf(l.P, q, pass(l.R, G, l.q));
+      R = fmaf(l.P, R, l.R);
+      G += l.G;
+      P *= l.P;
+    }
+    GFN_DEV void append(LayerBackMap l) {
+      if (gain_small(l.P)) {
+        ok = ok && gain_drops(q, pass(l.R, G, l.q)) && gain_drops(R, l.R);
+        l.P = 0.f;
+      }
+      ok = ok && fabsf(l.P) <= 1.f;
+      append_plain(l);
+    }
+    GFN_DEV bool right() const { return ok; }
+    GFN_DEV LayerBackMap map() const { return {ok ? P : INFINITY, q, R, G}; }
+  };
 };
 struct LayerBackState {
   static constexpr int WORDS = 1;
   float m, X;
   GFN_DEV void pack(unsigned long long (&w)[1]) const { w[0] = scan_word(m, X); }
   GFN_DEV static LayerBackState unpack(const unsigned long long (&w)[1]) { return {word_lo(w[0]), word_hi(w[0])}; }
-  GFN_DEV LayerBackState through(LayerBackMap f) const { return {pass(f.P, m, pass(f.R, X, f.q)), X + f.G}; }
+  GFN_DEV LayerBackState through(LayerBackMap f) const { return {carry(f.P, m, pass(f.R, X, f.q)), X + f.G}; }
+  GFN_DEV bool through(const LayerBackMap::Quick& f, LayerBackState& out) const {
+    const bool small = gain_small(f.P);
+    const float in = pass(f.R, X, f.q);
+    out = {fmaf(small ? 0.f : f.P, m, in), X + f.G};
+    return f.right() && (!small || gain_drops(m, in));
+  }
 };
 
 // 28 bytes per element (32 with a gradient of v) and 128 instructions, issued
@@ -1011,7 +1268,7 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       const F2 scale = f2(p.base_dt * head_scale(c.col + v, p.D / p.H));
-      GatedMap mf = GatedMap::identity();
+      float eights[S / 8], mp = 0.f;
 #pragma unroll
       for (int s = 0; s < S; s += 2) {
         F2 slope;
@@ -1026,12 +1283,11 @@ __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LSca
         zb[s][v] = pb[s].get(v);
         gx[s][v] = px[s].get(v);
         gv[s][v] = pv[s].get(v);
-        mf.P *= A[s][v];
-        mf.p = fmaf(A[s][v], mf.p, zb[s][v] * dt[s][v]);
+        eights[s / 8] = s % 8 ? eights[s / 8] * A[s][v] : A[s][v];
+        mp = fmaf(A[s][v], mp, zb[s][v] * dt[s][v]);
       }
-      mf.P = keep_positive<S, VEC>(mf.P, A, v);
-      LayerBackMap mb = LayerBackMap::identity();
-      mb.P = mf.P;
+      const GatedMap mf = {gain_run<S>(eights, 1.f, [&](int s) { return A[s][v]; }), mp};
+      LayerBackMap mb = {mf.P, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = S - 1; s >= 0; --s) {
         mb.G += gx[s][v];

@@ -33,9 +33,9 @@ def gated_scan(a, x, h0=None, return_state=False):
     sequence, so packed sequences need no more than that.  Differentiable
     (once) in a, x and h0, a broadcast a included.
 
-    The length axis is split: a state passes a whole run of steps as h * P + p,
-    P the product of the run's gates, so |P| must not overflow (gates up to
-    1 in magnitude never do).
+    The length axis is split: a state passes a whole run of steps as h * P + p.
+    P, the product of the run's gates, has an exponent range of its own, so gates
+    may decay and grow by any amounts for which h itself stays in float32's range.
     """
     same_device("gated_scan", x, a, h0)
     dtype_code(x, "x")
