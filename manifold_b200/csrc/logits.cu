@@ -51,24 +51,50 @@ struct alignas(sizeof(T) * VEC) Group {
   T v[VEC];
 };
 
+// Quotients by a row's penalty and temperature are products with 1 / d, since a
+// long history puts a penalised token before almost every warp and a division at
+// each then costs a third of the time (256 x 50257 bfloat16 with 2048 tokens: 53 us
+// against 40).  Rows whose 1 / d could leave float32's range divide.
 struct RowTerms {
-  float rep, inv_rep, freq, pres, scale;  // scale: 1 / temperature
+  float rep, inv_rep, freq, pres, temp, inv_temp;
+  bool divides;
 };
+GFN_DEV bool reciprocal_serves(float d) { return d >= 0x1p-100f && d <= 0x1p100f; }
 
-// The penalties of one token with history word c.  Divisions by the row's
-// penalty and temperature are multiplications by their reciprocals (one
-// rounding more each): a long history puts a penalised token before almost
-// every warp, and the divisions then cost more than the memory.
-GFN_DEV float penalise(float v, unsigned c, const RowTerms& r) {
+// v / d given 1 / d.  For 16-bit results the product's two roundings do; for
+// float32 ones (EXACT) it is corrected by its residual, which makes it the rounded
+// quotient (Markstein, 1990) unless the residual loses digits: `odd` then, and for
+// 0, infinities and NaN.
+template <bool EXACT>
+GFN_DEV float quotient(float v, float d, float inv, bool& odd) {
+  const float q = v * inv;
+  if (!EXACT) return q;
+  odd = odd || !(fminf(fabsf(v), fabsf(q)) >= 0x1p-100f && fabsf(q) <= 0x1p126f);
+  return fmaf(fmaf(-q, d, v), inv, q);
+}
+
+// The penalties of one token with history word c.
+template <bool EXACT>
+GFN_DEV float penalise(float v, unsigned c, const RowTerms& r, bool& odd) {
   const float n = (float)(c & ~LOGITS_SEEN);
-  const float w = v * (v > 0.f ? r.inv_rep : r.rep);
+  bool strange = false;
+  const float q = quotient<EXACT>(v, r.rep, r.inv_rep, strange), w = v > 0.f ? q : v * r.rep;
+  odd = odd || (strange && c && v > 0.f);
   v = c ? w : v;
   return n > 0.f ? v - fmaf(r.freq, n, r.pres) : v;
 }
 
-GFN_DEV float finish_logit(float v, float bias, bool allowed, const RowTerms& r) {
-  v = (v + bias) * r.scale;
-  return allowed ? v : -INFINITY;
+template <bool EXACT>
+GFN_DEV float finish_logit(float v, float bias, const RowTerms& r, bool& odd) {
+  return quotient<EXACT>(v + bias, r.temp, r.inv_temp, odd);
+}
+
+// The whole of it by divisions.
+GFN_DEV float shaped_logit(float v, unsigned c, float bias, const RowTerms& r) {
+  const float n = (float)(c & ~LOGITS_SEEN);
+  if (c) v = v > 0.f ? v / r.rep : v * r.rep;
+  if (n > 0.f) v -= fmaf(r.freq, n, r.pres);
+  return (v + bias) / r.temp;
 }
 
 // Token j of a row stands at place j + phase, where places that are multiples
@@ -81,6 +107,7 @@ GFN_DEV float finish_logit(float v, float bias, bool allowed, const RowTerms& r)
 // BIAS: 0 none, 1 in aligned groups too, 2 one by one.
 template <typename T, int VEC, int UNROLL, bool HIST, int BIAS, bool MASK>
 __global__ void __launch_bounds__(LOGITS_THREADS, HIST ? 0 : 4) logits_kernel(const LogitsArgs p) {
+  constexpr bool EXACT = sizeof(T) == 4;
   constexpr int STEP = LOGITS_THREADS * VEC, RUN = STEP * UNROLL, HEAD = 2, CHUNK = 4;
   __shared__ __align__(16) unsigned counts[HIST ? RUN : 1];
   const long long row = blockIdx.y;
@@ -116,7 +143,9 @@ __global__ void __launch_bounds__(LOGITS_THREADS, HIST ? 0 : 4) logits_kernel(co
   r.inv_rep = 1.f / r.rep;
   r.freq = p.freq_rows ? p.freq_rows[row] : p.freq;
   r.pres = p.pres_rows ? p.pres_rows[row] : p.pres;
-  r.scale = 1.f / (p.temp_rows ? p.temp_rows[row] : p.temp);
+  r.temp = p.temp_rows ? p.temp_rows[row] : p.temp;
+  r.inv_temp = 1.f / r.temp;
+  r.divides = !reciprocal_serves(r.temp) || (HIST && !reciprocal_serves(r.rep));
   if (HIST) {
     const long long* tok = p.tokens + row * p.ts;
     long long ahead[HEAD];  // the first tokens, fetched beside the row's length
@@ -156,8 +185,8 @@ __global__ void __launch_bounds__(LOGITS_THREADS, HIST ? 0 : 4) logits_kernel(co
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const int i = start + u * STEP + (int)threadIdx.x * VEC;
-    if (i >= phase && i + VEC <= last) {
-      Group<T, VEC> o;
+    if (i >= phase && i + VEC <= last && !r.divides) {
+      bool odd = false;
       float v[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[e] = to_f(xv[u].v[e]);
@@ -168,20 +197,25 @@ __global__ void __launch_bounds__(LOGITS_THREADS, HIST ? 0 : 4) logits_kernel(co
         for (int e = 0; e < VEC; ++e) any |= c.v[e];
         if (any) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[e] = penalise(v[e], c.v[e], r);
+          for (int e = 0; e < VEC; ++e) v[e] = penalise<EXACT>(v[e], c.v[e], r, odd);
         }
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        o.v[e] = from_f<T>(finish_logit(v[e], BIAS ? bv[u].v[e] : 0.f, !MASK || ((av[u] >> e) & 1u), r));
-      *reinterpret_cast<Group<T, VEC>*>(y + i) = o;
-    } else if (VEC > 1) {  // a group that the row's end cuts
-      for (int k = max(i, phase); k < min(i + VEC, last); ++k) {
-        const int j = k - phase;
-        float v = to_f(x[k]);
-        if (HIST) v = penalise(v, counts[k - start], r);
-        y[k] = from_f<T>(finish_logit(v, BIAS ? bias[k] : 0.f, !MASK || ((allowed[j >> 5] >> (j & 31)) & 1u), r));
+      for (int e = 0; e < VEC; ++e) v[e] = finish_logit<EXACT>(v[e], BIAS ? bv[u].v[e] : 0.f, r, odd);
+      if (!EXACT || !odd) {
+        Group<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(!MASK || ((av[u] >> e) & 1u) ? v[e] : -INFINITY);
+        *reinterpret_cast<Group<T, VEC>*>(y + i) = o;
+        continue;
       }
+    }
+    // one by one: a group that the row's end cuts, or that needs divisions
+#pragma unroll 1
+    for (int k = max(i, phase); k < min(i + VEC, last); ++k) {
+      const int j = k - phase;
+      const float v = shaped_logit(to_f(x[k]), HIST ? counts[k - start] : 0u, BIAS ? bias[k] : 0.f, r);
+      y[k] = from_f<T>(!MASK || ((allowed[j >> 5] >> (j & 31)) & 1u) ? v : -INFINITY);
     }
   }
 }
