@@ -698,6 +698,10 @@ size_t type_size(int dtype) { return dtype == GFN_F32 ? 4 : 2; }
 
 }  // namespace
 
+namespace gfn_abi {
+cudaError_t error_word_norm(int* v, int reset, cudaStream_t s) { return gfn_unit_error_word(v, reset, s); }
+}  // namespace gfn_abi
+
 extern "C" {
 
 int gfn_layer_norm_forward(const void* x, long long x_row_stride, const void* weight, const void* bias,
