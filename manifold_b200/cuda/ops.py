@@ -438,6 +438,9 @@ def parallel_scan_fused(a, x, workspace=True):
     require_cuda(a, x)
     x = _f32c(x, "x")
     a = _f32c(a, "a")
+    if x.dim() != 3 or (a is not None and a.numel() != x.numel()):
+        raise GfnError(f"parallel_scan_fused: a {None if a is None else tuple(a.shape)} and x {tuple(x.shape)} must "
+                       "be [batch, length, dim]")
     B, L, D = x.shape
     y = torch.empty_like(x)
     ws = None
@@ -457,11 +460,14 @@ def parallel_layer_scan(z, heads, base_dt=0.1, state=None, return_state=False):
     (None: zero); with return_state the result is (x_seq, v_seq, (v, x)), the
     state after the last step.  Differentiable in z and the state.  Calls with
     a state, return_state or a gradient split the length axis when the columns
-    alone do not fill the GPU, and take any dim."""
+    alone do not fill the GPU; so do those whose rows do not start on 16 bytes,
+    as the one-pass kernel of the others needs it."""
     require_cuda(z)
-    if state is not None or return_state or _grad_wanted(z):
+    if state is not None or return_state or _grad_wanted(z) or z.dim() != 3 or z.shape[2] % 12:
         return _layer_scan(z, heads, base_dt, state, return_state)
     z = _f32c(z, "z")
+    if z.data_ptr() % 16:
+        return _layer_scan(z, heads, base_dt, state, return_state)
     B, L, D3 = z.shape
     D = D3 // 3
     x_seq = torch.empty(B, L, D, device=z.device, dtype=torch.float32)

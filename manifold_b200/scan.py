@@ -12,12 +12,20 @@ CUDA_AVAILABLE = True
 
 def parallel_scan(a, x):
     """a, x: [batch, seq_len, dim] float32 CUDA tensors -> y of the same shape.
-    Differentiable: with a gradient wanted it runs as gated_scan(a, x)."""
-    if _grad_wanted(a, x):
+    Differentiable.  With a gradient wanted it runs as gated_scan(a, x), and so
+    it does where a has another shape than x (it is broadcast) or rows do not
+    start on 16 bytes."""
+    if _grad_wanted(a, x) or not _one_pass(a, x):
         if x.dtype != torch.float32:
             raise GfnError(f"x must be float32, got {x.dtype}")
         return gated_scan(a, x)
     return parallel_scan_fused(a, x)
+
+
+def _one_pass(a, x):
+    """Whether parallel_scan_fused takes the operands: one shape, whole and aligned rows of 4."""
+    return (x.dim() == 3 and x.shape[2] % 4 == 0 and (a is None or a.shape == x.shape)
+            and all(t is None or not t.is_contiguous() or t.data_ptr() % 16 == 0 for t in (a, x)))
 
 
 def gated_scan(a, x, h0=None, return_state=False):
