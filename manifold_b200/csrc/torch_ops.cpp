@@ -332,10 +332,14 @@ struct Unlocked {  // other Python threads run meanwhile
   ~Unlocked() { PyEval_RestoreThread(state); }
 };
 
+// An operand.  There is no forward mode: a tensor that carries a tangent is
+// refused, since the result would come back without one.
 Tensor tensor_arg(PyObject* o) {
   if (o == Py_None) return Tensor();
   if (!THPVariable_Check(o)) throw Failure("a tensor or None expected");
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  if (t._fw_grad(0).defined()) throw Failure("forward-mode differentiation is not implemented for this operator");
+  return t;
 }
 double number_arg(PyObject* o) {
   const double v = PyFloat_AsDouble(o);

@@ -28,6 +28,11 @@ def _grad_wanted(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _has_tangent(*ts):
+    """Whether one carries a forward-mode tangent (torch.autograd.forward_ad), which the kernels would drop."""
+    return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
 def christoffel_fused(v, U, W, x=None, V_w=None, plasticity=0.0, sing_thresh=1.0,
                       sing_strength=1.0, topology=0, R=2.0, r=1.0):
     """Gamma(v) for one head (gfn/cuda/ops.py:88-118).  topology 0: the low-rank
@@ -463,7 +468,7 @@ def parallel_layer_scan(z, heads, base_dt=0.1, state=None, return_state=False):
     alone do not fill the GPU; so do those whose rows do not start on 16 bytes,
     as the one-pass kernel of the others needs it."""
     require_cuda(z)
-    if state is not None or return_state or _grad_wanted(z) or z.dim() != 3 or z.shape[2] % 12:
+    if state is not None or return_state or _grad_wanted(z) or _has_tangent(z) or z.dim() != 3 or z.shape[2] % 12:
         return _layer_scan(z, heads, base_dt, state, return_state)
     z = _f32c(z, "z")
     if z.data_ptr() % 16:

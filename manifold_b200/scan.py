@@ -5,7 +5,7 @@ and the gated scan: the same recurrence with gradients, a carried state and
 import torch
 
 from ._lib import GfnError, dtype_code, same_device, torch_ops
-from .cuda.ops import _grad_wanted, parallel_scan_fused
+from .cuda.ops import _grad_wanted, _has_tangent, parallel_scan_fused
 
 CUDA_AVAILABLE = True
 
@@ -15,7 +15,7 @@ def parallel_scan(a, x):
     Differentiable.  With a gradient wanted it runs as gated_scan(a, x), and so
     it does where a has another shape than x (it is broadcast) or rows do not
     start on 16 bytes."""
-    if _grad_wanted(a, x) or not _one_pass(a, x):
+    if _grad_wanted(a, x) or _has_tangent(a, x) or not _one_pass(a, x):
         if x.dtype != torch.float32:
             raise GfnError(f"x must be float32, got {x.dtype}")
         return gated_scan(a, x)
