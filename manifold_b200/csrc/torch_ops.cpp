@@ -55,6 +55,23 @@ void check(int status, const char* what) {
                   "): " + api.gfn_last_error_message());
 }
 
+// Runs `f`, the body of a node's backward.  It runs on a thread of the engine,
+// which hands the caller's thread a Python error as it is and makes a RuntimeError
+// of any other.
+template <class F>
+variable_list backward_body(F f) {
+  try {
+    return f();
+  } catch (const Failure& e) {
+    const PyGILState_STATE held = PyGILState_Ensure();
+    PyErr_SetString(gfn_error, e.what());
+    python_error error;
+    error.persist();
+    PyGILState_Release(held);
+    throw error;
+  }
+}
+
 int extent(int64_t n, const char* what) {
   if (n > INT_MAX) throw Failure(std::string(what) + ": extent " + std::to_string(n) + " above 2^31 - 1");
   return (int)n;
@@ -142,6 +159,10 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return backward_body([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const bool recording = at::GradMode::is_enabled();
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
@@ -231,6 +252,10 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return backward_body([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const bool recording = at::GradMode::is_enabled();
     const Tensor dlast = grads.size() > 1 ? grads[1] : Tensor();
     if (!grads[0].defined() && !dlast.defined()) return variable_list(4);
@@ -296,6 +321,10 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return backward_body([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const bool recording = at::GradMode::is_enabled();
     Tensor g[4];  // of x_seq, v_seq, v_last, x_last
     bool any = false;
