@@ -6,6 +6,10 @@ generation reads the prompt in one call, then one token at a time from the
 carried state, with a repetition penalty and a grammar mask that allows only
 brackets which keep the string balanced.
 
+It shows the calls, not a model worth having: 200 steps take the loss from 1.61
+to 1.46, the entropy of the bare token frequencies (1.47), and 2000 steps to 1.37,
+where the strings' own is 1.04.  That the answer is balanced is the mask's doing.
+
     python examples/scan_lm.py [--steps 200]
 """
 import argparse

@@ -23,19 +23,21 @@
 // which the group before publishes.  What is composed with what does not
 // depend on which block is faster, so results repeat bit for bit.
 // (Looking back for the nearest state instead did not, and one block per
-// column with no split took 33.7 ms where this takes 55 us, at 1 x 65536 x 512.)
+// column with no split took 33.7 ms where this takes 62 us, at 1 x 65536 x 512.)
 //
 // Measured on B200 (CUDA events around workspace clearing and kernel; copy
 // bandwidth 6.46 TB/s):
 //   forward   128 x 512 x 512 float32    75 us, 5.4 TB/s
-//             16 x 2048 x 512 float32    44 us, 4.6 TB/s
-//             1 x 65536 x 512 bfloat16   58 us, 3.4 TB/s
-//             3 x 5003 x 1001 bfloat16   50 us, 1.8 TB/s (rows off 16 bytes)
-//   backward  118, 72, 99 and 79 us: 5.7, 4.6, 3.4 and 1.9 TB/s
+//             16 x 2048 x 512 float32    46 us, 4.4 TB/s
+//             1 x 65536 x 512 bfloat16   62 us, 3.2 TB/s
+//             3 x 5003 x 1001 bfloat16   54 us, 1.7 TB/s (rows off 16 bytes)
+//   backward  118, 74, 100 and 84 us: 5.7, 4.5, 3.3 and 1.8 TB/s
+// (With products of gates in plain float32, wrong where they leave its range, 44,
+// 59 and 52 us forward and 71, 96 and 80 backward for the last three.)
 // With many columns they run at the memory's rate.  With few, what is left is
 // the way of a map through global memory and the wait for the group's state,
-// about 5,000 of a block's 13,000 cycles per run; off 16 bytes, the loads'
-// latency and 70 (forward) to 113 (backward) instructions per element.
+// about 6,000 of a block's 14,000 cycles per run; off 16 bytes, the loads'
+// latency and 67 (forward) to 114 (backward) instructions per element.
 #pragma once
 #include <cfloat>
 #include <type_traits>
@@ -1017,12 +1019,12 @@ struct LayerState {
   }
 };
 
-// 20 bytes per element, and 70 instructions: two exponentials, two reciprocals
+// 20 bytes per element, and 72 instructions: two exponentials, two reciprocals
 // and a polynomial, two steps at a time where packed arithmetic does both (one
 // at a time 86 instructions and 134 us).  Runs of 128 steps of 32 columns, two
-// blocks per SM: at 32 x 2048 x 512 128 us, 5.2 TB/s (runs of 64 steps of 64
+// blocks per SM: at 32 x 2048 x 512 132 us, 5.1 TB/s (runs of 64 steps of 64
 // columns 155 us); at 1 x 20000 x 256, where 8 column tiles leave 5 rounds of
-// blocks, 40 us.
+// blocks, 43 us.
 template <int MODE, int VEC, int S, int NW, int OCC>
 __global__ void __launch_bounds__(NW * 32, OCC) lscan_forward_kernel(const LScanArgs p, const __grid_constant__ ScanMaps maps) {
   constexpr int CT = 32 * VEC;
@@ -1205,7 +1207,7 @@ struct LayerBackState {
 // at 55% of the rate: instructions, the exchange's waits and memory share the
 // time.  The gates, steps and slopes stay in registers between the two walks
 // (recomputing them took 298 us); v is recomputed from its kept state instead
-// of read.  At 32 x 2048 x 512 220 us, 4.3 TB/s.
+// of read.  At 32 x 2048 x 512 226 us, 4.2 TB/s.
 template <int MODE, int VEC, int S, int NW, int OCC>
 __global__ void __launch_bounds__(NW * 32, OCC) lscan_backward_kernel(const LScanArgs p, const __grid_constant__ ScanMaps maps) {
   static_assert(NW * S % SCAN_CK == 0, "a kept state at every run's start");

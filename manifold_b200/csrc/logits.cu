@@ -12,9 +12,11 @@
 // that run in shared memory (integer atomics, so the order does not matter)
 // and then streams its logits once.
 //
-// 35 us at 256 x 50257 bfloat16 with biases, masks and up to 2048 tokens of
-// history (3.1 TB/s); 9 us a call, launch and checks included, for one row of
-// 32000.  The bytes would take 17 us: the rest is instructions, 58 per element
+// 256 x 50257 bfloat16 with biases, masks and up to 2048 tokens of history takes
+// 35 us as one call among others with lengths spread over the history (3.1 TB/s),
+// and 41 us by CUDA events around a single call behind a cleared L2, as the other
+// figures here are taken; 9 us a call, launch and checks included, for one row of
+// 32000.  The bytes would take 17 us: the rest is instructions, 59 per element
 // there, 25 without history (27 us) and 14 without bias and mask too.
 #include "abi.h"
 #include "lm_ops.cuh"
@@ -54,7 +56,7 @@ struct alignas(sizeof(T) * VEC) Group {
 // Quotients by a row's penalty and temperature are products with 1 / d, since a
 // long history puts a penalised token before almost every warp and a division at
 // each then costs a third of the time (256 x 50257 bfloat16 with 2048 tokens: 53 us
-// against 40).  Rows whose 1 / d could leave float32's range divide.
+// against 41).  Rows whose 1 / d could leave float32's range divide.
 struct RowTerms {
   float rep, inv_rep, freq, pres, temp, inv_temp;
   bool divides;
@@ -251,8 +253,8 @@ int logits_dispatch(LogitsArgs p, cudaStream_t s) {
   const bool vec = xy % (VEC * sizeof(T)) == 0 && (p.B == 1 || (p.xs - p.V) % VEC == 0);
   p.bias_groups = p.bias && aligned16(p.bias) && (p.B == 1 || (p.bs - p.V) % VEC == 0);
   // Few tokens: small blocks, to use more SMs.  Many: larger ones, since every
-  // block of a row reads its whole history (two groups a thread: 39 us at
-  // 256 x 50257 bfloat16 with 2048 tokens; four groups 43, one 49).
+  // block of a row reads its whole history (at 256 x 50257 bfloat16 with 2048
+  // tokens, when this was chosen: two groups a thread 39 us, four 43, one 49).
   const bool many = (long long)p.B * p.V > 592LL * LOGITS_THREADS * VEC;
   if (vec) return many ? logits_history<T, VEC, 2>(p, s) : logits_history<T, VEC, 1>(p, s);
   return many ? logits_history<T, 1, 8>(p, s) : logits_history<T, 1, 2>(p, s);

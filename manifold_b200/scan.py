@@ -31,9 +31,10 @@ def _one_pass(a, x):
 def gated_scan(a, x, h0=None, return_state=False):
     """h_t = a_t * h_{t-1} + x_t over dim 1 of x [batch, length, dim], from h0.
 
-    a: x's type, x's shape or broadcastable to it (a decay per channel, per
-    head or per step is read in place where its last dimension is whole), or
-    None (a running sum).  x: float32, bfloat16 or float16, any batch and step
+    a: x's type, x's shape or broadcastable to it (a decay per channel is read
+    in place, by the path of rows that do not start on 16 bytes; one whose last
+    dimension is broadcast, per head or per step, is first copied to x's shape),
+    or None (a running sum).  x: float32, bfloat16 or float16, any batch and step
     strides.  h0: [batch, dim] float32, or None (zero).  The state is float32
     throughout; h has x's type.  Returns h, or (h, last state [batch, dim]
     float32) with return_state: pass that as h0 to continue the sequence, one
