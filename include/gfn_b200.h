@@ -562,6 +562,81 @@ int gfn_process_logits(const void* logits, long long logits_row_stride, int dtyp
                        gfn_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Token embedding y_n = scale W[id_n] and its table's gradient
+ * dW_v = scale (sum of dy_n over the n with id_n = v) (the nn.Embedding of
+ * gfn/model.py:52-66).  ids [tokens] int64 (ids_are_64) or int32; weight
+ * [vocab][dim] of `dtype` with a row stride, inner stride 1; y [tokens][dim]
+ * contiguous.  A token outside [0, vocab) gives a row of zeros, takes no part
+ * in the gradient and sets GFN_DEVERR_BAD_TOKEN.  The backward writes every
+ * row of dweight [vocab][dim] (contiguous, of `dtype`); tokens equal to
+ * padding_id (-1: none) take no part.  Sums are float32 in the order of the
+ * tokens, rounded once; results repeat bit for bit.  Its workspace of
+ * gfn_token_embed_backward_workspace_bytes() (negative: too large) is 16-byte
+ * aligned.  16-byte aligned rows take 128-bit accesses. */
+int gfn_token_embed_forward(const void* ids, int ids_are_64, long long tokens, const void* weight,
+                            long long weight_row_stride, int dtype, int vocab, int dim, float scale, void* y,
+                            gfn_stream_t stream);
+long long gfn_token_embed_backward_workspace_bytes(long long tokens, int vocab, int dim);
+int gfn_token_embed_backward(const void* ids, int ids_are_64, long long tokens, const void* dy,
+                             long long dy_row_stride, int dtype, int vocab, int dim, float scale,
+                             long long padding_id, void* dweight, void* workspace, long long workspace_bytes,
+                             gfn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Log probabilities of given tokens, the entropy and the `top` (0 .. 32) most
+ * probable tokens of every row of logits [rows][vocab] (row stride in
+ * elements, inner stride 1), and the gradient of all three.  tokens [rows]
+ * int64 or NULL; logprobs [rows], entropy [rows] or NULL, top_logprobs and
+ * top_tokens [rows][top] (largest first, ties: lowest token first, NaN above
+ * all).  A token equal to ignore_index has log probability 0 and no gradient;
+ * another one outside [0, vocab) gives NaN and sets GFN_DEVERR_BAD_TOKEN.  A
+ * logit of -inf has probability 0 and adds nothing to the entropy.  A row
+ * without a logit above -inf has log probabilities of -inf, entropy 0 and a
+ * gradient of zeros; one with NaN or +inf has NaN throughout.  stats
+ * [rows][2] float (NULL for inference) keeps what the backward needs.
+ * Backward: d_logprobs, d_entropy [rows], d_top [rows][top], each NULL where
+ * there is none; entropy and top_tokens as the forward wrote them; dlogits
+ * [rows][vocab] contiguous of `dtype`, another buffer than the logits. */
+int gfn_token_logprobs_forward(const void* logits, long long logits_row_stride, int dtype, long long rows, int vocab,
+                               const long long* tokens, long long ignore_index, int top, float* logprobs,
+                               float* entropy, float* top_logprobs, long long* top_tokens, float* stats,
+                               gfn_stream_t stream);
+int gfn_token_logprobs_backward(const void* logits, long long logits_row_stride, int dtype, long long rows, int vocab,
+                                const long long* tokens, long long ignore_index, int top, const long long* top_tokens,
+                                const float* stats, const float* entropy, const float* d_logprobs,
+                                const float* d_entropy, const float* d_top, void* dlogits, gfn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Linear attention with a decay for each head,
+ *   S_t = decay_h S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
+ * and its gradients: the gated scan above with a matrix for a state.
+ * q, k [batch][length][heads][kdim], v, o [batch][length][heads][vdim] of
+ * `dtype`; q, k, v, d_o with inner stride 1 and element strides {batch,
+ * length, heads} in host memory (0 allowed: broadcast); o, dq, dk, dv
+ * contiguous, 16-byte aligned.  decay [heads] float in [0, 1] (the nearer end
+ * is taken outside).  state, state_out, d_state_out, d_state
+ * [batch][heads][kdim][vdim] float or NULL (zero / not wanted).  lengths
+ * [batch] int64 (lengths_are_64) or int32, or NULL (all `length`; clamped to
+ * [0, length]): tokens behind a sequence's length are not read, do not reach
+ * the state, and get zeros.  kdim, vdim up to 128.  A block of 64 tokens is
+ * one step: NaN or infinity in k or v reaches that block's earlier outputs
+ * too.  `workspace` of gfn_decay_attention_workspace_bytes() (on the current
+ * device), 16-byte aligned, serves either pass.  Results repeat bit for bit. */
+long long gfn_decay_attention_workspace_bytes(int batch, int length, int heads, int kdim, int vdim);
+int gfn_decay_attention_forward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                                const void* v, const long long* v_strides, const float* decay, const float* state,
+                                const void* lengths, int lengths_are_64, int dtype, int batch, int length, int heads,
+                                int kdim, int vdim, float scale, void* o, float* state_out, void* workspace,
+                                long long workspace_bytes, gfn_stream_t stream);
+int gfn_decay_attention_backward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
+                                 const void* v, const long long* v_strides, const void* d_o,
+                                 const long long* do_strides, const float* decay, const float* state,
+                                 const float* d_state_out, const void* lengths, int lengths_are_64, int dtype,
+                                 int batch, int length, int heads, int kdim, int vdim, float scale, void* dq, void* dk,
+                                 void* dv, float* d_state, void* workspace, long long workspace_bytes,
+                                 gfn_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * FunctionalEmbedding, mode 'binary', coord_dim 16, hidden 64, 2 hidden
  * SIREN layers (gfn/embeddings.py:121-206): ids [n] -> forces [n, dim],
  * float32 (out_f32) or bfloat16 (out_bf16, raw uint16 storage).

@@ -16,11 +16,12 @@ from .integrators import (DormandPrinceIntegrator, EulerIntegrator, ForestRuthIn
                           HeunIntegrator, LeapfrogIntegrator, OmelyanIntegrator, RK4Integrator,
                           SymplecticIntegrator, VerletIntegrator, YoshidaIntegrator)
 from .integrators import INTEGRATOR_CLASSES as INTEGRATORS
-from .embeddings import FunctionalEmbedding, ImplicitEmbedding, SineLayer
+from .embeddings import Embedding, FunctionalEmbedding, ImplicitEmbedding, SineLayer, embed_tokens
+from .attention import decay_attention
 from .scan import gated_scan, parallel_scan
 from .losses import CrossEntropyLoss, cross_entropy
 from .norm import LayerNorm, layer_norm
-from .sampling import pack_token_mask, process_logits
+from .sampling import TokenLogprobs, pack_token_mask, process_logits, token_logprobs
 from . import cuda
 
 __all__ = ["CrossEntropyLoss", "cross_entropy", "GFN", "Manifold", "GLayer", "MLayer", "ParallelMLayer", "RiemannianGating",
@@ -30,4 +31,5 @@ __all__ = ["CrossEntropyLoss", "cross_entropy", "GFN", "Manifold", "GLayer", "ML
            "OmelyanIntegrator",
            "FunctionalEmbedding", "ImplicitEmbedding", "SineLayer", "ImplicitReadout",
            "parallel_scan", "gated_scan", "LayerNorm", "layer_norm", "process_logits",
-           "pack_token_mask", "GfnError", "INTEGRATORS"]
+           "pack_token_mask", "token_logprobs", "TokenLogprobs", "embed_tokens", "Embedding", "decay_attention",
+           "GfnError", "INTEGRATORS"]

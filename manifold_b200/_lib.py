@@ -85,6 +85,16 @@ _SIGS = {
     "gfn_layer_scan_backward": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _p, _p, _p, _p, _ll, _p],
     "gfn_process_logits": [_p, _ll, _i, _i, _i, _p, _ll, _i, _p, _p, _f, _p, _f, _p, _f, _p, _f, _p, _p, _ll, _p,
                            _ll, _p, _p],
+    "gfn_token_embed_forward": [_p, _i, _ll, _p, _ll, _i, _i, _i, _f, _p, _p],
+    "gfn_token_embed_backward_workspace_bytes": [_ll, _i, _i],
+    "gfn_token_embed_backward": [_p, _i, _ll, _p, _ll, _i, _i, _i, _f, _ll, _p, _p, _ll, _p],
+    "gfn_token_logprobs_forward": [_p, _ll, _i, _ll, _i, _p, _ll, _i, _p, _p, _p, _p, _p, _p],
+    "gfn_token_logprobs_backward": [_p, _ll, _i, _ll, _i, _p, _ll, _i, _p, _p, _p, _p, _p, _p, _p, _p],
+    "gfn_decay_attention_workspace_bytes": [_i, _i, _i, _i, _i],
+    "gfn_decay_attention_forward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _p, _p, _p,
+                                    _ll, _p],
+    "gfn_decay_attention_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f,
+                                     _p, _p, _p, _p, _p, _ll, _p],
 }
 _RESTYPES = {
     "gfn_status_string": ctypes.c_char_p,
@@ -101,6 +111,8 @@ _RESTYPES = {
     "gfn_layer_norm_backward_workspace_floats": ctypes.c_longlong,
     "gfn_gated_scan_states_floats": ctypes.c_longlong,
     "gfn_gated_scan_workspace_bytes": ctypes.c_longlong,
+    "gfn_token_embed_backward_workspace_bytes": ctypes.c_longlong,
+    "gfn_decay_attention_workspace_bytes": ctypes.c_longlong,
 }
 
 EXPORTED = tuple(_SIGS)
@@ -134,7 +146,9 @@ TORCH_ENTRIES = ("gfn_status_string", "gfn_last_error_message", "gfn_layer_norm_
                  "gfn_layer_norm_backward_workspace_floats", "gfn_layer_norm_backward",
                  "gfn_gated_scan_states_floats", "gfn_gated_scan_workspace_bytes", "gfn_gated_scan_forward",
                  "gfn_gated_scan_backward", "gfn_layer_scan_forward", "gfn_layer_scan_backward",
-                 "gfn_process_logits")
+                 "gfn_process_logits", "gfn_token_embed_forward", "gfn_token_embed_backward_workspace_bytes",
+                 "gfn_token_embed_backward", "gfn_token_logprobs_forward", "gfn_token_logprobs_backward",
+                 "gfn_decay_attention_workspace_bytes", "gfn_decay_attention_forward", "gfn_decay_attention_backward")
 _torch_ops = None
 
 

@@ -34,5 +34,7 @@ cudaError_t error_word_readout(int* v, int reset, cudaStream_t s);
 cudaError_t error_word_logits(int* v, int reset, cudaStream_t s);
 cudaError_t error_word_gated_scan(int* v, int reset, cudaStream_t s);
 cudaError_t error_word_norm(int* v, int reset, cudaStream_t s);
+cudaError_t error_word_token_embed(int* v, int reset, cudaStream_t s);
+cudaError_t error_word_logprobs(int* v, int reset, cudaStream_t s);
 
 }  // namespace gfn_abi

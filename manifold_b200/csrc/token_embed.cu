@@ -1,0 +1,614 @@
+// Embedding of token ids and the gradient of its table:
+//
+//   y_n  = scale W[id_n]
+//   dW_v = scale (sum of dy_n over the n with id_n = v)
+//
+// (the reference's nn.Embedding, gfn/model.py:52-66, whose gradient it leaves
+// to torch).  Both are bound by HBM.  The gradient sorts the tokens by id, a
+// stable radix sort, so that every row of the table has one owner that sums
+// its tokens in the order of the sequence: no float atomics, the same bits on
+// every run.  Sums are float32 and are rounded once.
+#include "lm_host.h"
+#include "lm_ops.cuh"
+
+using namespace gfn;
+using namespace gfn_abi;
+
+namespace {
+
+constexpr int EMBED_THREADS = 256;
+constexpr int EMBED_GROUPS = 4;  // groups of 16 bytes a thread has on their way at once
+
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, 1994).
+struct Divisor {
+  unsigned d, shift;
+  unsigned long long m;
+};
+Divisor divisor(unsigned d) {
+  unsigned l = 0;
+  while (l < 31 && (1u << l) < d) ++l;
+  return {d, 31 + l, (1ull << (31 + l)) / d + 1};
+}
+GFN_DEV unsigned quotient(unsigned n, const Divisor& v) { return (unsigned)((n * v.m) >> v.shift); }
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+GFN_DEV long long id_at(const void* ids, bool wide, long long n) {
+  return wide ? static_cast<const long long*>(ids)[n] : (long long)static_cast<const int*>(ids)[n];
+}
+
+// ------------------------------------------------------------------ forward
+struct EmbedArgs {
+  const void* ids;
+  const void* w;
+  void* y;
+  long long N, ws, total;  // tokens, row stride of the table, groups of y
+  int V, D, wide;
+  float scale;
+  Divisor per_row;  // groups per row (VECLOAD), else elements per row
+};
+
+// y in groups of VEC elements, 16 bytes where y starts on 16 bytes.  With
+// VECLOAD the rows of table and y are whole groups; otherwise a group may lie
+// across two rows and its elements are fetched one by one.
+template <typename T, int VEC, bool VECLOAD>
+__global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(const EmbedArgs p) {
+  constexpr int TILE = EMBED_THREADS * EMBED_GROUPS;
+  const long long first = (long long)blockIdx.x * TILE;
+  const T* w = static_cast<const T*>(p.w);
+  if constexpr (VECLOAD) {
+    const long long row0 = first / p.per_row.d;
+    const unsigned rem = (unsigned)(first - row0 * p.per_row.d);
+    const T* src[EMBED_GROUPS];
+    Pack<T, VEC> v[EMBED_GROUPS];
+#pragma unroll
+    for (int u = 0; u < EMBED_GROUPS; ++u) {
+      const unsigned at = threadIdx.x + u * EMBED_THREADS, off = rem + at, r = quotient(off, p.per_row);
+      src[u] = nullptr;
+      if (first + at < p.total) {
+        const long long id = id_at(p.ids, p.wide, row0 + r);
+        if ((unsigned long long)id < (unsigned)p.V) src[u] = w + id * p.ws + (long long)(off - r * p.per_row.d) * VEC;
+        else gfn_flag_error(kDevErrBadToken);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < EMBED_GROUPS; ++u)
+      if (src[u]) v[u] = *reinterpret_cast<const Pack<T, VEC>*>(src[u]);
+#pragma unroll
+    for (int u = 0; u < EMBED_GROUPS; ++u) {
+      const long long g = first + threadIdx.x + u * EMBED_THREADS;
+      if (g >= p.total) continue;
+      Pack<T, VEC> o;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(src[u] ? to_f(v[u].v[e]) * p.scale : 0.f);
+      reinterpret_cast<Pack<T, VEC>*>(p.y)[g] = o;
+    }
+  } else {
+    const long long all = p.N * p.D;
+    const long long row0 = first * VEC / p.D;
+    const unsigned rem = (unsigned)(first * VEC - row0 * p.D);
+#pragma unroll
+    for (int u = 0; u < EMBED_GROUPS; ++u) {
+      const unsigned at = threadIdx.x + u * EMBED_THREADS;
+      const long long e0 = (first + at) * VEC;
+      if (e0 >= all) continue;
+      unsigned r = quotient(rem + at * VEC, p.per_row), c = rem + at * VEC - r * (unsigned)p.D;
+      const T* src = nullptr;
+      Pack<T, VEC> o;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (c == (unsigned)p.D) {
+          c = 0;
+          ++r;
+        }
+        if ((e == 0 || c == 0) && e0 + e < all) {
+          const long long id = id_at(p.ids, p.wide, row0 + r);
+          src = (unsigned long long)id < (unsigned)p.V ? w + id * p.ws : nullptr;
+          if (!src) gfn_flag_error(kDevErrBadToken);
+        }
+        o.v[e] = from_f<T>(src && e0 + e < all ? to_f(src[c]) * p.scale : 0.f);
+        ++c;
+      }
+      T* y = static_cast<T*>(p.y) + e0;
+      if (VEC > 1 && e0 + VEC <= all) *reinterpret_cast<Pack<T, VEC>*>(y) = o;
+      else
+        for (int e = 0; e < VEC && e0 + e < all; ++e) y[e] = o.v[e];
+    }
+  }
+}
+
+template <typename T>
+int embed_forward(EmbedArgs p, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  const bool rows = aligned16(p.w) && aligned16(p.y) && p.D % VEC == 0 && p.ws % VEC == 0;
+  const int vec = aligned16(p.y) ? VEC : 1;
+  p.total = (p.N * p.D + vec - 1) / vec;
+  p.per_row = divisor((unsigned)(rows ? p.D / VEC : p.D));
+  const long long blocks = (p.total + EMBED_THREADS * EMBED_GROUPS - 1) / (EMBED_THREADS * EMBED_GROUPS);
+  if (blocks > 0x7fffffffLL) return fail(GFN_ERR_UNSUPPORTED, "embed: %lld x %d elements", p.N, p.D);
+  if (rows) embed_kernel<T, VEC, true><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
+  else if (vec > 1) embed_kernel<T, VEC, false><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
+  else embed_kernel<T, 1, false><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
+  return launch_status("embed_kernel");
+}
+
+// ----------------------------------------------------------------- gradient
+// The sort: digits of up to 9 bits, least significant first.  A tile of
+// tokens is ranked by a block; where it writes a digit follows from the counts
+// of every digit in every tile, which the kernel before left in global memory.
+constexpr int SORT_THREADS = 256, SORT_WARPS = 8, SORT_ITEMS = 8, SORT_SUB = SORT_THREADS * SORT_ITEMS;
+constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILES = 256;
+// Tokens (in sorted order) that one group of threads sums.
+constexpr int SUM_RUN = 32, SUM_THREADS = 128, SUM_AHEAD = 8;
+
+struct SortArgs {
+  const void* ids;
+  unsigned* keys[2];
+  unsigned* pos[2];
+  unsigned* counts;  // [passes][tiles][SORT_BINS]
+  void* dw;
+  long long dw_bytes;
+  long long padding;
+  int N, V, wide, tiles, subs, bits, passes;  // subs: parts of SORT_SUB tokens in a tile; bits of a digit
+};
+
+// The token's row, or V where it takes no part (padding, or outside the table).
+GFN_DEV unsigned sort_key(const SortArgs& p, long long n, bool flag) {
+  const long long id = id_at(p.ids, p.wide, n);
+  if ((unsigned long long)id >= (unsigned)p.V) {
+    if (flag) gfn_flag_error(kDevErrBadToken);
+    return p.V;
+  }
+  return id == p.padding ? (unsigned)p.V : (unsigned)id;
+}
+
+// Part `part` of `parts` of the table's gradient becomes zero: the blocks
+// beyond the sort's own fill it meanwhile.
+GFN_DEV void zero_part(void* dw, long long bytes, long long part, long long parts) {
+  char* b = static_cast<char*>(dw);
+  const long long head = min((16 - (long long)(reinterpret_cast<uintptr_t>(b) & 15)) & 15, bytes);
+  const long long groups = (bytes - head) / 16, tail = head + groups * 16;
+  const long long per = (groups + parts - 1) / parts;
+  const long long end = min((part + 1) * per, groups);
+  uint4* g = reinterpret_cast<uint4*>(b + head);
+  for (long long i = part * per + threadIdx.x; i < end; i += blockDim.x) g[i] = make_uint4(0, 0, 0, 0);
+  if (part == 0) {
+    for (long long i = threadIdx.x; i < head; i += blockDim.x) b[i] = 0;
+    for (long long i = tail + threadIdx.x; i < bytes; i += blockDim.x) b[i] = 0;
+  }
+}
+
+// Stage `stage` of `stages` of that filling, by the blocks from `first` on.
+GFN_DEV void zero_stage(const SortArgs& p, int first, int stage, int stages) {
+  const long long n = gridDim.x - first;
+  zero_part(p.dw, p.dw_bytes, stage * n + (blockIdx.x - first), n * stages);
+}
+
+// The counts of the first digit, and zeros for those of the later ones.
+__global__ void __launch_bounds__(SORT_THREADS) embed_count_kernel(const SortArgs p) {
+  if ((int)blockIdx.x >= p.tiles) return zero_stage(p, p.tiles, 0, p.passes + 1);
+  __shared__ unsigned bins[SORT_BINS];
+  for (int i = threadIdx.x; i < SORT_BINS; i += SORT_THREADS) bins[i] = 0;
+  __syncthreads();
+  const long long from = (long long)blockIdx.x * p.subs * SORT_SUB, to = min(from + (long long)p.subs * SORT_SUB, (long long)p.N);
+  const unsigned mask = (1u << p.bits) - 1;
+  for (long long n = from + threadIdx.x; n < to; n += SORT_THREADS) atomicAdd(&bins[sort_key(p, n, true) & mask], 1u);
+  __syncthreads();
+  for (int i = threadIdx.x; i < SORT_BINS; i += SORT_THREADS) {
+    p.counts[(long long)blockIdx.x * SORT_BINS + i] = bins[i];
+    for (int q = 1; q < p.passes; ++q) p.counts[((long long)q * p.tiles + blockIdx.x) * SORT_BINS + i] = 0;
+  }
+}
+
+struct SortShared {
+  unsigned warp[SORT_WARPS][SORT_BINS];  // a warp's count of each digit, then where its first one goes
+  unsigned next[SORT_BINS];              // where the block's next one goes
+  unsigned sums[SORT_WARPS];
+};
+
+// Exclusive sums over the bins of `v[2]` (this thread's bins 2 t and 2 t + 1).
+GFN_DEV void scan_bins(SortShared& sh, const unsigned (&v)[2], unsigned (&out)[2]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned s = v[0] + v[1], inc = s;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned t = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += t;
+  }
+  if (lane == 31) sh.sums[warp] = inc;
+  __syncthreads();
+  unsigned before = 0;
+  for (int w = 0; w < warp; ++w) before += sh.sums[w];
+  out[0] = before + inc - s;
+  out[1] = out[0] + v[0];
+  __syncthreads();
+}
+
+// Ranks SORT_SUB tokens from `from` on (below `to`) by the digit of their key
+// at `shift` and hands (key, position, place) of each to `put`; sh.next moves on.
+template <class Key, class Put>
+GFN_DEV void rank_part(SortShared& sh, long long from, long long to, unsigned shift, unsigned mask, Key key, Put put) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < SORT_WARPS * SORT_BINS; i += SORT_THREADS) (&sh.warp[0][0])[i] = 0;
+  __syncthreads();
+  unsigned k[SORT_ITEMS], ps[SORT_ITEMS], rank[SORT_ITEMS];
+#pragma unroll
+  for (int r = 0; r < SORT_ITEMS; ++r) {
+    const long long n = from + (warp * SORT_ITEMS + r) * 32 + lane;
+    k[r] = ps[r] = 0;
+    if (n < to) key(n, k[r], ps[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < SORT_ITEMS; ++r) {
+    const long long n = from + (warp * SORT_ITEMS + r) * 32 + lane;
+    const unsigned d = n < to ? (k[r] >> shift) & mask : ~0u;
+    const unsigned same = __match_any_sync(0xffffffffu, d), before = __popc(same & ((1u << lane) - 1));
+    if (n < to) rank[r] = sh.warp[warp][d] + before;
+    __syncwarp();
+    if (n < to && before == 0) sh.warp[warp][d] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < SORT_BINS; b += SORT_THREADS) {
+    unsigned at = sh.next[b];
+#pragma unroll
+    for (int w = 0; w < SORT_WARPS; ++w) {
+      const unsigned c = sh.warp[w][b];
+      sh.warp[w][b] = at;
+      at += c;
+    }
+    sh.next[b] = at;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < SORT_ITEMS; ++r) {
+    const long long n = from + (warp * SORT_ITEMS + r) * 32 + lane;
+    if (n < to) put(k[r], ps[r], sh.warp[warp][(k[r] >> shift) & mask] + rank[r]);
+  }
+  __syncthreads();
+}
+
+// One digit of the sort.  The counts of the next digit are collected on the way.
+__global__ void __launch_bounds__(SORT_THREADS) embed_rank_kernel(const SortArgs p, int pass) {
+  if ((int)blockIdx.x >= p.tiles) return zero_stage(p, p.tiles, pass + 1, p.passes + 1);
+  __shared__ SortShared sh;
+  const unsigned mask = (1u << p.bits) - 1, shift = pass * p.bits;
+  const unsigned* counts = p.counts + (long long)pass * p.tiles * SORT_BINS;
+  unsigned total[2] = {0, 0}, before[2] = {0, 0}, start[2];
+#pragma unroll 8
+  for (int t = 0; t < p.tiles; ++t) {
+    const uint2 c = reinterpret_cast<const uint2*>(counts + (long long)t * SORT_BINS)[threadIdx.x];
+    total[0] += c.x;
+    total[1] += c.y;
+    if (t < (int)blockIdx.x) {
+      before[0] += c.x;
+      before[1] += c.y;
+    }
+  }
+  scan_bins(sh, total, start);
+  sh.next[2 * threadIdx.x] = start[0] + before[0];
+  sh.next[2 * threadIdx.x + 1] = start[1] + before[1];
+  __syncthreads();
+  const long long from = (long long)blockIdx.x * p.subs * SORT_SUB, to = min(from + (long long)p.subs * SORT_SUB, (long long)p.N);
+  const unsigned *ki = p.keys[(pass + 1) & 1], *pi = p.pos[(pass + 1) & 1];
+  unsigned *ko = p.keys[pass & 1], *po = p.pos[pass & 1];
+  unsigned* following = pass + 1 < p.passes ? p.counts + (long long)(pass + 1) * p.tiles * SORT_BINS : nullptr;
+  for (long long at = from; at < to; at += SORT_SUB)
+    rank_part(sh, at, to, shift, mask,
+              [&](long long n, unsigned& k, unsigned& ps) {
+                if (pass == 0) {
+                  k = sort_key(p, n, false);
+                  ps = (unsigned)n;
+                } else {
+                  k = ki[n];
+                  ps = pi[n];
+                }
+              },
+              [&](unsigned k, unsigned ps, unsigned place) {
+                ko[place] = k;
+                po[place] = ps;
+                if (following) atomicAdd(&following[(place / (p.subs * SORT_SUB)) * SORT_BINS + ((k >> (shift + p.bits)) & mask)], 1u);
+              });
+}
+
+// The whole sort of up to SORT_SUB tokens by one block; the others fill zeros.
+__global__ void __launch_bounds__(SORT_THREADS) embed_sort_kernel(const SortArgs p) {
+  if (blockIdx.x >= 1) return zero_stage(p, 1, 0, 1);
+  __shared__ SortShared sh;
+  __shared__ unsigned keys[SORT_SUB], pos[SORT_SUB];
+  const unsigned mask = (1u << p.bits) - 1;
+  for (int n = threadIdx.x; n < p.N; n += SORT_THREADS) {
+    keys[n] = sort_key(p, n, true);
+    pos[n] = n;
+  }
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const unsigned shift = pass * p.bits;
+    for (int i = threadIdx.x; i < SORT_BINS; i += SORT_THREADS) sh.next[i] = 0;
+    __syncthreads();
+    for (int n = threadIdx.x; n < p.N; n += SORT_THREADS) atomicAdd(&sh.next[(keys[n] >> shift) & mask], 1u);
+    __syncthreads();
+    const unsigned v[2] = {sh.next[2 * threadIdx.x], sh.next[2 * threadIdx.x + 1]};
+    unsigned start[2];
+    scan_bins(sh, v, start);
+    sh.next[2 * threadIdx.x] = start[0];
+    sh.next[2 * threadIdx.x + 1] = start[1];
+    __syncthreads();
+    const bool last = pass == p.passes - 1;
+    rank_part(sh, 0, p.N, shift, mask,
+              [&](long long n, unsigned& k, unsigned& ps) {
+                k = keys[n];
+                ps = pos[n];
+              },
+              [&](unsigned k, unsigned ps, unsigned place) {  // every thread has read its own by now
+                (last ? p.keys[(p.passes - 1) & 1] : keys)[place] = k;
+                (last ? p.pos[(p.passes - 1) & 1] : pos)[place] = ps;
+              });
+  }
+}
+
+struct SumArgs {
+  const unsigned* keys;
+  const unsigned* pos;
+  const void* dy;
+  void* dw;
+  float* part;  // [runs][2][D]: what a run's first and last row have of a row that goes on in the neighbour
+  long long ds;
+  int N, V, D;
+  float scale;
+};
+
+// A group of blockDim.x threads sums SUM_RUN sorted tokens over the columns
+// of its threads, VEC each.  Rows of the table whose tokens lie within are
+// written; the first and the last may be shared with the neighbouring groups
+// and go to `part`.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const SumArgs p) {
+  extern __shared__ unsigned sum_shared[];
+  unsigned* key = sum_shared + threadIdx.y * (2 * SUM_RUN + 2) + 1;  // key[-1] .. key[SUM_RUN]
+  unsigned* pos = key + SUM_RUN + 1;
+  const long long run = (long long)blockIdx.x * blockDim.y + threadIdx.y, from = run * SUM_RUN;
+  const unsigned none = (unsigned)p.V;
+  for (int i = (int)threadIdx.x - 1; i <= SUM_RUN; i += blockDim.x) {
+    const long long n = from + i;
+    key[i] = n >= 0 && n < p.N ? p.keys[n] : n < 0 ? ~0u : none;
+    if (i >= 0 && i < SUM_RUN) pos[i] = n < p.N ? p.pos[n] : 0u;
+  }
+  __syncthreads();
+  const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+  if (col >= p.D || key[0] >= none) return;
+  const T* dy = static_cast<const T*>(p.dy) + col;
+  float acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  bool open = key[0] == key[-1];
+  auto store = [&](float* dst) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dst[e] = acc[e];
+  };
+  for (int i0 = 0; i0 < SUM_RUN; i0 += SUM_AHEAD) {
+    Pack<T, VEC> v[SUM_AHEAD];
+#pragma unroll
+    for (int i = 0; i < SUM_AHEAD; ++i)
+      if (key[i0 + i] < none) v[i] = *reinterpret_cast<const Pack<T, VEC>*>(dy + (long long)pos[i0 + i] * p.ds);
+#pragma unroll
+    for (int i = 0; i < SUM_AHEAD; ++i) {
+      const unsigned k = key[i0 + i];
+      if (k >= none) return;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += to_f(v[i].v[e]);
+      if (key[i0 + i + 1] == k) continue;
+      if (open) store(p.part + run * 2 * p.D + col);
+      else {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(acc[e] * p.scale);
+        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(p.dw) + (long long)k * p.D + col) = o;
+      }
+      open = false;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    }
+  }
+  if (key[SUM_RUN] == key[SUM_RUN - 1]) store(p.part + (run * 2 + (open ? 0 : 1)) * p.D + col);
+}
+
+// Rows shared by several groups of SUM_RUN tokens: the group in which such a
+// row begins adds the parts, eight interleaved sums joined in a fixed order.  A
+// block looks at JOIN_RUNS groups and adds what begins there over JOIN_COLS
+// columns.
+constexpr int JOIN_RUNS = 8, JOIN_COLS = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * JOIN_RUNS) embed_join_kernel(const SumArgs p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long runs = ((long long)p.N + SUM_RUN - 1) / SUM_RUN, base = (long long)blockIdx.x * JOIN_RUNS;
+  __shared__ unsigned row[JOIN_RUNS];
+  __shared__ long long stop[JOIN_RUNS];  // behind the last run whose first token is the row's
+  __shared__ float sums[JOIN_RUNS][JOIN_COLS];
+  {
+    const long long run = base + warp, from = run * SUM_RUN, end = from + SUM_RUN;
+    unsigned k = p.V;
+    if (end < p.N) {
+      k = p.keys[end - 1];
+      if (p.keys[end] != k || (p.keys[from] == k && from > 0 && p.keys[from - 1] == k)) k = p.V;
+    }
+    if (k < (unsigned)p.V) {
+      long long last = run + 1;
+      for (;;) {
+        const long long r = last + lane;
+        const int n = __popc(__ballot_sync(0xffffffffu, r < runs && p.keys[r * SUM_RUN] == k));  // sorted: they come first
+        last += n;
+        if (n < 32) break;
+      }
+      if (lane == 0) stop[warp] = last;
+    }
+    if (lane == 0) row[warp] = k;
+  }
+  __syncthreads();
+  for (int w = 0; w < JOIN_RUNS; ++w) {
+    const unsigned k = row[w];
+    if (k >= (unsigned)p.V) continue;
+    const long long run = base + w, last = stop[w];
+    for (int from = blockIdx.y * JOIN_COLS; from < p.D; from += gridDim.y * JOIN_COLS) {
+      float acc[JOIN_COLS / 32];
+#pragma unroll
+      for (int j = 0; j < JOIN_COLS / 32; ++j) {
+        const int col = from + lane + 32 * j;
+        acc[j] = warp == 0 && col < p.D ? p.part[(run * 2 + 1) * p.D + col] : 0.f;
+      }
+#pragma unroll 4
+      for (long long r = run + 1 + warp; r < last; r += JOIN_RUNS) {
+#pragma unroll
+        for (int j = 0; j < JOIN_COLS / 32; ++j) {
+          const int col = from + lane + 32 * j;
+          if (col < p.D) acc[j] += p.part[r * 2 * p.D + col];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < JOIN_COLS / 32; ++j) sums[warp][lane + 32 * j] = acc[j];
+      __syncthreads();
+      if (threadIdx.x < JOIN_COLS && from + (int)threadIdx.x < p.D) {
+        float t = sums[0][threadIdx.x];
+#pragma unroll
+        for (int g = 1; g < JOIN_RUNS; ++g) t += sums[g][threadIdx.x];
+        static_cast<T*>(p.dw)[(long long)k * p.D + from + threadIdx.x] = from_f<T>(t * p.scale);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// How the tokens are divided and where the workspace holds what.
+struct Plan {
+  int bits, passes, tiles, subs;
+  long long runs, keys, counts, part, bytes;
+};
+Plan embed_plan(long long N, int V, int D) {
+  Plan q = {};
+  int need = 1;
+  while (need < 32 && ((unsigned)V >> need)) ++need;  // V itself is a key
+  q.passes = (need + SORT_BITS - 1) / SORT_BITS;
+  q.bits = (need + q.passes - 1) / q.passes;
+  const long long parts = (N + SORT_SUB - 1) / SORT_SUB;
+  q.subs = (int)((parts + SORT_TILES - 1) / SORT_TILES);
+  if (q.subs < 1) q.subs = 1;
+  q.tiles = (int)((parts + q.subs - 1) / q.subs);
+  q.runs = (N + SUM_RUN - 1) / SUM_RUN;
+  auto up = [](long long b) { return (b + 255) / 256 * 256; };
+  q.keys = up(4 * N);
+  q.counts = 4 * q.keys;
+  q.part = q.counts + (parts > 1 ? up(4LL * q.passes * q.tiles * SORT_BINS) : 0);
+  q.bytes = q.part + up(8 * q.runs * D);
+  return q;
+}
+
+template <typename T>
+int embed_sum(const SumArgs& p, long long runs, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  const bool vec = aligned16(p.dy) && aligned16(p.dw) && p.D % VEC == 0 && (p.N == 1 || p.ds % VEC == 0);
+  const int per = vec ? VEC : 1, need = (p.D + per - 1) / per;
+  int lanes = 8;
+  while (lanes < SUM_THREADS && lanes < need) lanes *= 2;
+  const dim3 block((unsigned)lanes, (unsigned)(SUM_THREADS / lanes));
+  const dim3 grid((unsigned)((runs + block.y - 1) / block.y), (unsigned)((need + lanes - 1) / lanes));
+  if (grid.y > 65535) return fail(GFN_ERR_UNSUPPORTED, "token_embed backward: dim %d", p.D);
+  const int shared = (int)block.y * (2 * SUM_RUN + 2) * 4;
+  if (vec) embed_sum_kernel<T, VEC><<<grid, block, shared, s>>>(p);
+  else embed_sum_kernel<T, 1><<<grid, block, shared, s>>>(p);
+  const int st = launch_status("embed_sum_kernel");
+  if (st != GFN_OK || runs < 2) return st;
+  const int cols = (p.D + JOIN_COLS - 1) / JOIN_COLS;
+  const dim3 joins((unsigned)((runs + JOIN_RUNS - 1) / JOIN_RUNS), (unsigned)(cols < 65535 ? cols : 65535));
+  embed_join_kernel<T><<<joins, 32 * JOIN_RUNS, 0, s>>>(p);
+  return launch_status("embed_join_kernel");
+}
+
+}  // namespace
+
+namespace gfn_abi {
+cudaError_t error_word_token_embed(int* v, int reset, cudaStream_t s) { return gfn_unit_error_word(v, reset, s); }
+}  // namespace gfn_abi
+
+extern "C" {
+
+int gfn_token_embed_forward(const void* ids, int ids_are_64, long long tokens, const void* weight,
+                            long long weight_row_stride, int dtype, int vocab, int dim, float scale, void* y,
+                            gfn_stream_t stream) {
+  if (tokens < 0 || vocab <= 0 || dim <= 0 || (tokens > 0 && (!ids || !weight || !y)))
+    return fail(GFN_ERR_INVALID, "token_embed: tokens=%lld vocab=%d dim=%d or a NULL operand", tokens, vocab, dim);
+  if (dim > 1 << 30) return fail(GFN_ERR_UNSUPPORTED, "token_embed: dim %d above 2^30", dim);
+  if (tokens == 0) return GFN_OK;
+  EmbedArgs p = {};
+  p.ids = ids; p.w = weight; p.y = y; p.N = tokens; p.ws = weight_row_stride; p.V = vocab; p.D = dim;
+  p.wide = ids_are_64 != 0; p.scale = scale;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == GFN_F32) return embed_forward<float>(p, s);
+  if (dtype == GFN_BF16) return embed_forward<__nv_bfloat16>(p, s);
+  if (dtype == GFN_F16) return embed_forward<__half>(p, s);
+  return fail(GFN_ERR_UNSUPPORTED, "token_embed: element type %d", dtype);
+}
+
+long long gfn_token_embed_backward_workspace_bytes(long long tokens, int vocab, int dim) {
+  if (tokens < 0 || tokens > 0x7fffffffLL || vocab <= 0 || dim <= 0) return -1;
+  return embed_plan(tokens, vocab, dim).bytes;
+}
+
+int gfn_token_embed_backward(const void* ids, int ids_are_64, long long tokens, const void* dy,
+                             long long dy_row_stride, int dtype, int vocab, int dim, float scale,
+                             long long padding_id, void* dweight, void* workspace, long long workspace_bytes,
+                             gfn_stream_t stream) {
+  if (tokens < 0 || vocab <= 0 || dim <= 0 || !dweight || (tokens > 0 && (!ids || !dy || !workspace)))
+    return fail(GFN_ERR_INVALID, "token_embed backward: tokens=%lld vocab=%d dim=%d or a NULL operand", tokens, vocab,
+                dim);
+  if (tokens > 0x7fffffffLL || vocab == 0x7fffffff)
+    return fail(GFN_ERR_UNSUPPORTED, "token_embed backward: %lld tokens, vocabulary of %d", tokens, vocab);
+  if (dtype != GFN_F32 && dtype != GFN_BF16 && dtype != GFN_F16)
+    return fail(GFN_ERR_UNSUPPORTED, "token_embed backward: element type %d", dtype);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const long long dw_bytes = (long long)vocab * dim * (dtype == GFN_F32 ? 4 : 2);
+  if (tokens == 0) {
+    const cudaError_t e = cudaMemsetAsync(dweight, 0, (size_t)dw_bytes, s);
+    return e == cudaSuccess ? GFN_OK : cuda_status(e, "token_embed backward");
+  }
+  const Plan q = embed_plan(tokens, vocab, dim);
+  if (workspace_bytes < q.bytes || !aligned16(workspace))
+    return fail(GFN_ERR_INVALID, "token_embed backward: a workspace of %lld bytes, 16-byte aligned, is needed", q.bytes);
+  int sms = 0;
+  int st = sm_count(&sms);
+  if (st != GFN_OK) return st;
+  char* ws = static_cast<char*>(workspace);
+  SortArgs a = {};
+  a.ids = ids;
+  a.keys[0] = reinterpret_cast<unsigned*>(ws);
+  a.keys[1] = reinterpret_cast<unsigned*>(ws + q.keys);
+  a.pos[0] = reinterpret_cast<unsigned*>(ws + 2 * q.keys);
+  a.pos[1] = reinterpret_cast<unsigned*>(ws + 3 * q.keys);
+  a.counts = reinterpret_cast<unsigned*>(ws + q.counts);
+  a.dw = dweight; a.dw_bytes = dw_bytes; a.padding = padding_id;
+  a.N = (int)tokens; a.V = vocab; a.wide = ids_are_64 != 0;
+  a.tiles = q.tiles; a.subs = q.subs; a.bits = q.bits; a.passes = q.passes;
+  const unsigned fill = (unsigned)(4 * sms);
+  if (tokens <= SORT_SUB) {
+    embed_sort_kernel<<<1 + fill, SORT_THREADS, 0, s>>>(a);
+    if ((st = launch_status("embed_sort_kernel")) != GFN_OK) return st;
+  } else {
+    embed_count_kernel<<<(unsigned)q.tiles + fill, SORT_THREADS, 0, s>>>(a);
+    if ((st = launch_status("embed_count_kernel")) != GFN_OK) return st;
+    for (int pass = 0; pass < q.passes; ++pass) {
+      embed_rank_kernel<<<(unsigned)q.tiles + fill, SORT_THREADS, 0, s>>>(a, pass);
+      if ((st = launch_status("embed_rank_kernel")) != GFN_OK) return st;
+    }
+  }
+  SumArgs b = {};
+  b.keys = a.keys[(q.passes - 1) & 1]; b.pos = a.pos[(q.passes - 1) & 1];
+  b.dy = dy; b.dw = dweight; b.part = reinterpret_cast<float*>(ws + q.part);
+  b.ds = dy_row_stride; b.N = a.N; b.V = vocab; b.D = dim; b.scale = scale;
+  if (dtype == GFN_F32) return embed_sum<float>(b, q.runs, s);
+  if (dtype == GFN_BF16) return embed_sum<__nv_bfloat16>(b, q.runs, s);
+  return embed_sum<__half>(b, q.runs, s);
+}
+
+}  // extern "C"

@@ -1,10 +1,12 @@
 // PyTorch side of the language-model operators (layer norm, gated scan, the
-// layer's scan, logit shaping): allocation, streams and autograd nodes around
+// layer's scan, logit shaping, token embedding, log probabilities, attention
+// with decay): allocation, streams and autograd nodes around
 // the C ABI, in C++ because a small call is bound by the host.  A call through
 // ctypes and a Python autograd Function took 10.8 us forward and, trained,
 // 104 us, of which the hand-over to the engine's thread and back is 45; here a
 // call takes 7 and a small training step 65 to 80.
-// Arguments arrive checked (norm.py, scan.py, cuda/ops.py, sampling.py); the
+// Arguments arrive checked (norm.py, scan.py, cuda/ops.py, sampling.py,
+// embeddings.py, attention.py); the
 // entry points of the C ABI are handed over by bind(), so that one library is
 // loaded whoever calls.
 #include <Python.h>
@@ -22,6 +24,7 @@
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "../../include/gfn_b200.h"
 
@@ -36,7 +39,10 @@ using torch::autograd::variable_list;
   X(gfn_status_string) X(gfn_last_error_message) X(gfn_layer_norm_forward)                        \
   X(gfn_layer_norm_backward_workspace_floats) X(gfn_layer_norm_backward)                          \
   X(gfn_gated_scan_states_floats) X(gfn_gated_scan_workspace_bytes) X(gfn_gated_scan_forward)     \
-  X(gfn_gated_scan_backward) X(gfn_layer_scan_forward) X(gfn_layer_scan_backward) X(gfn_process_logits)
+  X(gfn_gated_scan_backward) X(gfn_layer_scan_forward) X(gfn_layer_scan_backward) X(gfn_process_logits)     \
+  X(gfn_token_embed_forward) X(gfn_token_embed_backward_workspace_bytes) X(gfn_token_embed_backward)  \
+  X(gfn_token_logprobs_forward) X(gfn_token_logprobs_backward)                                    \
+  X(gfn_decay_attention_workspace_bytes) X(gfn_decay_attention_forward) X(gfn_decay_attention_backward)
 struct Api {
 #define X(name) decltype(&::name) name;
   GFN_ENTRIES(X)
@@ -355,6 +361,229 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
   }
 };
 
+// ----------------------------------------------------------------- embedding
+Tensor embed_run(const Tensor& ids, const Tensor& w, double scale) {
+  at::AutoDispatchBelowADInplaceOrView plain;
+  const Launch on(w);
+  const int V = extent(w.size(0), "embed_tokens"), D = extent(w.size(1), "embed_tokens");
+  const Tensor i = whole(ids), t = w.is_contiguous() || D == 1 || w.stride(1) == 1 ? w : w.contiguous();
+  std::vector<int64_t> shape = ids.sizes().vec();
+  shape.push_back(D);
+  Tensor y = fresh(w, shape, w.scalar_type());
+  check(api.gfn_token_embed_forward(ptr(i), i.scalar_type() == at::kLong, i.numel(), t.data_ptr(), t.stride(0),
+                                    code_of(w), V, D, (float)scale, ptr(y), on.stream),
+        "gfn_token_embed_forward");
+  return y;
+}
+
+struct EmbedNode : torch::autograd::Function<EmbedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& w, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["vocab"] = w.size(0);
+    return embed_run(ids, w, scale);
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return backward_body([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    const bool recording = at::GradMode::is_enabled();
+    const Tensor ids = ctx->get_saved_variables()[0];
+    Tensor dw;
+    {
+      at::AutoDispatchBelowADInplaceOrView plain;
+      const Tensor& dy = grads[0];
+      const Launch on(dy);
+      const int V = extent(ctx->saved_data["vocab"].toInt(), "embed_tokens");
+      const int D = extent(dy.size(-1), "embed_tokens");
+      const Tensor i = whole(ids);
+      const Rows g = rows_of(dy, D);
+      dw = fresh(dy, {V, D}, dy.scalar_type());
+      const long long n = api.gfn_token_embed_backward_workspace_bytes(g.n, V, D);
+      if (n < 0) throw Failure("embed_tokens: too many tokens");
+      const Tensor ws = fresh(dy, {n}, at::kByte);
+      check(api.gfn_token_embed_backward(ptr(i), i.scalar_type() == at::kLong, g.n, ptr(g.t), g.stride, code_of(dy), V,
+                                         D, (float)ctx->saved_data["scale"].toDouble(),
+                                         ctx->saved_data["padding"].toInt(), dw.data_ptr(), ptr(ws), n, on.stream),
+            "gfn_token_embed_backward");
+    }
+    return first_order({Tensor(), dw, Tensor(), Tensor()}, grads, recording);
+  }
+};
+
+// --------------------------------------------------------- log probabilities
+struct Probs {
+  Tensor lp, ent, top_lp, top_id, stats;
+  variable_list outputs() const {
+    variable_list r;
+    for (const Tensor& t : {lp, ent, top_lp, top_id})
+      if (t.defined()) r.push_back(t);
+    return r;
+  }
+};
+
+// tokens: whole int64 of the logits' leading shape, or undefined
+Probs logprob_run(const Tensor& x, const Tensor& tokens, int64_t top, bool entropy, int64_t ignore, bool keep) {
+  at::AutoDispatchBelowADInplaceOrView plain;
+  const Launch on(x);
+  const int V = extent(x.size(-1), "token_logprobs");
+  const Rows r = rows_of(x, V);
+  const std::vector<int64_t> lead(x.sizes().begin(), x.sizes().end() - 1);
+  std::vector<int64_t> wide = lead;
+  wide.push_back(top);
+  Probs o;
+  if (tokens.defined()) o.lp = fresh(x, lead, at::kFloat);
+  if (entropy) o.ent = fresh(x, lead, at::kFloat);
+  if (top) {
+    o.top_lp = fresh(x, wide, at::kFloat);
+    o.top_id = fresh(x, wide, at::kLong);
+  }
+  if (keep) o.stats = fresh(x, {r.n, 2}, at::kFloat);
+  check(api.gfn_token_logprobs_forward(ptr(r.t), r.stride, code_of(x), r.n, V, static_cast<long long*>(ptr(tokens)),
+                                       ignore, (int)top, fptr(o.lp), fptr(o.ent), fptr(o.top_lp),
+                                       static_cast<long long*>(ptr(o.top_id)), fptr(o.stats), on.stream),
+        "gfn_token_logprobs_forward");
+  return o;
+}
+
+struct LogprobNode : torch::autograd::Function<LogprobNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& given, int64_t top, bool entropy,
+                               int64_t ignore) {
+    const Tensor tokens = given.value_or(Tensor());
+    const Probs o = logprob_run(x, tokens, top, entropy, ignore, true);
+    ctx->save_for_backward({x, tokens, o.stats, o.ent, o.top_id});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["top"] = top;
+    ctx->set_materialize_grads(false);
+    if (o.top_id.defined()) ctx->mark_non_differentiable({o.top_id});
+    return o.outputs();
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return backward_body([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    const bool recording = at::GradMode::is_enabled();
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &tokens = saved[1], &stats = saved[2], &ent = saved[3], &top_id = saved[4];
+    size_t at = 0;
+    const Tensor none, glp = tokens.defined() ? grads[at++] : none, ge = ent.defined() ? grads[at++] : none,
+                       gt = top_id.defined() ? grads[at++] : none;
+    if (!glp.defined() && !ge.defined() && !gt.defined()) return variable_list(5);
+    Tensor dx;
+    {
+      at::AutoDispatchBelowADInplaceOrView plain;
+      const Launch on(x);
+      const int V = extent(x.size(-1), "token_logprobs");
+      const Rows r = rows_of(x, V);
+      const Tensor a = whole(glp), b = whole(ge), c = whole(gt);
+      dx = fresh(x);
+      check(api.gfn_token_logprobs_backward(ptr(r.t), r.stride, code_of(x), r.n, V,
+                                            static_cast<long long*>(ptr(tokens)), ctx->saved_data["ignore"].toInt(),
+                                            (int)ctx->saved_data["top"].toInt(), static_cast<long long*>(ptr(top_id)),
+                                            fptr(stats), fptr(ent), fptr(a), fptr(b), fptr(c), ptr(dx), on.stream),
+            "gfn_token_logprobs_backward");
+    }
+    return first_order({dx, Tensor(), Tensor(), Tensor(), Tensor()}, grads, recording);
+  }
+};
+
+// ------------------------------------------------------ attention with decay
+// [batch, length, heads, dim] with inner stride 1, in place where it has that.
+struct Heads {
+  Tensor t;
+  long long strides[3];
+  explicit Heads(const Tensor& u) : t(u.is_contiguous() || u.stride(3) == 1 || u.size(3) == 1 ? u : u.contiguous()) {
+    for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
+  }
+  const void* p() const { return ptr(t); }
+};
+
+struct AttnShape {
+  int B, L, H, K, V;
+  AttnShape(const Tensor& q, const Tensor& v)
+      : B(extent(q.size(0), "decay_attention")), L(extent(q.size(1), "decay_attention")),
+        H(extent(q.size(2), "decay_attention")), K(extent(q.size(3), "decay_attention")),
+        V(extent(v.size(3), "decay_attention")) {}
+  Tensor state(const Tensor& q) const { return fresh(q, {B, H, K, V}, at::kFloat); }
+  Tensor workspace(const Tensor& q, long long* n) const {
+    *n = api.gfn_decay_attention_workspace_bytes(B, L, H, K, V);
+    if (*n < 0) throw Failure(std::string("decay_attention: ") + api.gfn_last_error_message());
+    return *n ? fresh(q, {*n}, at::kByte) : Tensor();
+  }
+};
+
+Tensor attn_run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& state,
+                const Tensor& lengths, double scale, Tensor* last) {
+  at::AutoDispatchBelowADInplaceOrView plain;
+  const Launch on(q);
+  const AttnShape s(q, v);
+  const Heads hq(q), hk(k), hv(v);
+  const Tensor start = whole(state);
+  Tensor o = fresh(v, {s.B, s.L, s.H, s.V}, v.scalar_type());
+  if (last) *last = s.state(q);
+  long long n = 0;
+  const Tensor ws = s.workspace(q, &n);
+  check(api.gfn_decay_attention_forward(hq.p(), hq.strides, hk.p(), hk.strides, hv.p(), hv.strides, fptr(decay),
+                                        fptr(start), ptr(lengths), lengths.defined() && lengths.scalar_type() == at::kLong,
+                                        code_of(q), s.B, s.L, s.H, s.K, s.V, (float)scale, ptr(o),
+                                        last ? fptr(*last) : nullptr, ptr(ws), n, on.stream),
+        "gfn_decay_attention_forward");
+  return o;
+}
+
+struct AttnNode : torch::autograd::Function<AttnNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                               const Tensor& decay, const Maybe& start, const Maybe& lens, double scale,
+                               bool want_last) {
+    const Tensor state = start.value_or(Tensor()), lengths = lens.value_or(Tensor());
+    Tensor last;
+    Tensor o = attn_run(q, k, v, decay, state, lengths, scale, want_last ? &last : nullptr);
+    ctx->save_for_backward({q, k, v, decay, state, lengths});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return want_last ? variable_list{o, last} : variable_list{o};
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return backward_body([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    const bool recording = at::GradMode::is_enabled();
+    const Tensor dlast = grads.size() > 1 ? grads[1] : Tensor();
+    if (!grads[0].defined() && !dlast.defined()) return variable_list(8);
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &decay = saved[3], &state = saved[4], &lengths = saved[5];
+    Tensor dq, dk, dv, ds;
+    {
+      at::AutoDispatchBelowADInplaceOrView plain;
+      const Launch on(q);
+      const AttnShape s(q, v);
+      const Heads hq(q), hk(k), hv(v), ho(grads[0].defined() ? grads[0] : at::zeros({1}, v.options()).expand(v.sizes()));
+      const Tensor start = whole(state), gl = whole(dlast);
+      dq = fresh(q, q.sizes(), q.scalar_type());
+      dk = fresh(k, k.sizes(), k.scalar_type());
+      dv = fresh(v, v.sizes(), v.scalar_type());
+      // inputs are numbered without the absent ones
+      if (state.defined() && ctx->needs_input_grad(4)) ds = s.state(q);
+      long long n = 0;
+      const Tensor ws = s.workspace(q, &n);
+      check(api.gfn_decay_attention_backward(hq.p(), hq.strides, hk.p(), hk.strides, hv.p(), hv.strides, ho.p(),
+                                             ho.strides, fptr(decay), fptr(start), fptr(gl), ptr(lengths),
+                                             lengths.defined() && lengths.scalar_type() == at::kLong, code_of(q), s.B,
+                                             s.L, s.H, s.K, s.V, (float)ctx->saved_data["scale"].toDouble(), ptr(dq),
+                                             ptr(dk), ptr(dv), fptr(ds), ptr(ws), n, on.stream),
+            "gfn_decay_attention_backward");
+    }
+    return first_order({dq, dk, dv, Tensor(), ds, Tensor(), Tensor(), Tensor()}, grads, recording);
+  }
+};
+
 // ------------------------------------------------------------------- Python
 struct Unlocked {  // other Python threads run meanwhile
   PyThreadState* state = PyEval_SaveThread();
@@ -489,6 +718,60 @@ PyObject* py_process_logits(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// embed_tokens(ids, weight, scale, padding, train) -> y
+PyObject* py_embed_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 5, [&] {
+    const Tensor ids = tensor_arg(v[0]), w = tensor_arg(v[1]);
+    const double scale = number_arg(v[2]);
+    const int64_t padding = integer_arg(v[3]);
+    const bool train = flag_arg(v[4]);
+    Tensor y;
+    {
+      Unlocked u;
+      y = train ? EmbedNode::apply(ids, w, scale, padding) : embed_run(ids, w, scale);
+    }
+    return THPVariable_Wrap(y);
+  });
+}
+
+// token_logprobs(x, tokens, top, entropy, ignore_index, train) -> those of (logprobs, entropy, top_logprobs, top_tokens)
+// that are asked for
+PyObject* py_token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 6, [&] {
+    const Tensor x = tensor_arg(v[0]), tokens = tensor_arg(v[1]);
+    const int64_t top = integer_arg(v[2]), ignore = integer_arg(v[4]);
+    const bool entropy = flag_arg(v[3]), train = flag_arg(v[5]);
+    variable_list out;
+    {
+      Unlocked u;
+      const Tensor t = whole(tokens);
+      out = train ? LogprobNode::apply(x, maybe(t), top, entropy, ignore)
+                  : logprob_run(x, t, top, entropy, ignore, false).outputs();
+    }
+    return tuple_of(out);
+  });
+}
+
+// decay_attention(q, k, v, decay, state, lengths, scale, want_last, train) -> (o,) or (o, last)
+PyObject* py_decay_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 9, [&] {
+    const Tensor q = tensor_arg(v[0]), k = tensor_arg(v[1]), val = tensor_arg(v[2]), decay = tensor_arg(v[3]),
+                 state = tensor_arg(v[4]), lengths = tensor_arg(v[5]);
+    const double scale = number_arg(v[6]);
+    const bool want_last = flag_arg(v[7]), train = flag_arg(v[8]);
+    variable_list out;
+    {
+      Unlocked u;
+      if (train) out = AttnNode::apply(q, k, val, decay, maybe(state), maybe(lengths), scale, want_last);
+      else {
+        Tensor last, o = attn_run(q, k, val, decay, state, lengths, scale, want_last ? &last : nullptr);
+        out = want_last ? variable_list{o, last} : variable_list{o};
+      }
+    }
+    return tuple_of(out);
+  });
+}
+
 // bind(addresses, error): the entry points of GFN_ENTRIES and the class of the library's errors
 PyObject* py_bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   constexpr Py_ssize_t COUNT = sizeof(Api) / sizeof(void*);
@@ -513,8 +796,9 @@ PyObject* py_bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
 }
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind),       METHOD(layer_norm),     METHOD(gated_scan),
-                         METHOD(layer_scan), METHOD(process_logits), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(bind),           METHOD(layer_norm),      METHOD(gated_scan),
+                         METHOD(layer_scan),     METHOD(process_logits),  METHOD(embed_tokens),
+                         METHOD(token_logprobs), METHOD(decay_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods};
 
 }  // namespace

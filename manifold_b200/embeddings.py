@@ -3,14 +3,53 @@
 FunctionalEmbedding (the one the LM-shaped configuration uses) runs as one
 fused SIREN kernel over all [B, L] tokens; ImplicitEmbedding keeps the
 reference's module and evaluates with torch GPU ops (it is not on any
-benchmarked path).
+benchmarked path).  embed_tokens and Embedding look a table up on the
+library's kernels and sum its gradient by sorted tokens.
 """
 import numpy as np
 import torch
 import torch.nn as nn
 
-from ._lib import GfnError, require_cuda
+from ._lib import GfnError, dtype_code, require_cuda, same_device, torch_ops
 from .cuda import ops
+
+
+def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
+    """scale * weight[ids], of shape [*ids.shape, dim] and the weight's type.
+
+    ids: int64 or int32 of any shape.  weight [vocab, dim]: float32, bfloat16 or
+    float16; rows of a wider table are read in place.  scale: a number.
+    Differentiable (once) in weight: the rows of every token are summed in
+    float32, in the order of the tokens (the tokens are sorted; no atomics), so
+    results repeat bit for bit; tokens equal to padding_idx take no part.  A
+    token outside the vocabulary gives a row of zeros, takes no part in the
+    gradient and sets a device error bit (gfn.cuda.ops.device_error).
+    """
+    same_device("embed_tokens", weight, ids)
+    dtype_code(weight, "weight")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise GfnError(f"embed_tokens: weight must be [vocab, dim], got {tuple(weight.shape)}")
+    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
+        raise GfnError(f"embed_tokens: ids must be int64 or int32, got {ids.dtype}")
+    if isinstance(scale, torch.Tensor):
+        raise GfnError("embed_tokens: scale must be a number (multiply by a tensor afterwards)")
+    pad = -1
+    if padding_idx is not None:
+        pad = padding_idx if padding_idx >= 0 else padding_idx + weight.shape[0]
+        if not 0 <= pad < weight.shape[0]:
+            raise GfnError(f"embed_tokens: padding_idx {padding_idx} outside a vocabulary of {weight.shape[0]}")
+    return torch_ops().embed_tokens(ids, weight, scale, pad, weight.requires_grad and torch.is_grad_enabled())
+
+
+class Embedding(nn.Embedding):
+    """nn.Embedding (the same parameters and state_dict) on the kernels, with a factor."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, device=None, dtype=None):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
+        self.scale = scale
+
+    def forward(self, input_ids):
+        return embed_tokens(input_ids, self.weight, self.scale, self.padding_idx)
 
 
 class SineLayer(nn.Module):

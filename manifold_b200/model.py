@@ -13,11 +13,11 @@ import torch.nn as nn
 
 from ._lib import GfnError, require_cuda
 from .cuda import ops
-from .embeddings import FunctionalEmbedding, ImplicitEmbedding
+from .embeddings import FunctionalEmbedding, ImplicitEmbedding, embed_tokens
 from .layers import (LAYERED_MIN_ELEMS, MLayer, ParallelMLayer, apply_norm,  # noqa: F401
                      use_layered_path)
 from .packing import PackCache
-from .sampling import process_logits
+from .sampling import process_logits, token_logprobs
 
 
 class ImplicitReadout(nn.Module):
@@ -94,6 +94,7 @@ class Manifold(nn.Module):
         self.readout_norm = nn.LayerNorm(dim)
         self.readout_split = True  # False: plain fp32 torch matmul for the readout
         self.library_norm = False  # see use_library_norm
+        self.library_embedding = False  # see use_library_embedding
         if readout_type in ("implicit", "binary"):
             coord_dim = emb_cfg.get("coord_dim", 16)
             self.readout = nn.Identity() if self.holographic else ImplicitReadout(dim, coord_dim)
@@ -132,6 +133,8 @@ class Manifold(nn.Module):
             return force_manual
         if isinstance(self.embedding, FunctionalEmbedding):
             return self.embedding(input_ids, out_dtype=self.force_dtype)
+        if self.library_embedding and isinstance(self.embedding, nn.Embedding):
+            return embed_tokens(input_ids, self.embedding.weight, padding_idx=self.embedding.padding_idx)
         return self.embedding(input_ids)
 
     def _apply_readout(self, out):
@@ -245,6 +248,14 @@ class Manifold(nn.Module):
                 layer.library_norm = bool(on)
         return self
 
+    def use_library_embedding(self, on=True):
+        """Look the tokens up, and sum their rows' gradient, on the library's
+        kernels instead of torch's nn.Embedding (embed_tokens: the same values;
+        the gradient's sums run in the order of the tokens and repeat bit for
+        bit).  Returns the model."""
+        self.library_embedding = bool(on)
+        return self
+
     def stream(self, input_ids=None, state=None, force_manual=None):
         """A segment of a longer sequence through the scan path (use_scan=True):
         input_ids [B, L] (one token or many) from `state`, the list of every
@@ -271,7 +282,7 @@ class Manifold(nn.Module):
     @torch.no_grad()
     def generate(self, prompt_ids, max_new_tokens=50, temperature=1.0, top_k=None, top_p=None,
                  repetition_penalty=1.0, frequency_penalty=0.0, presence_penalty=0.0, logit_bias=None,
-                 allowed=None, carry_state=False):
+                 allowed=None, carry_state=False, logprobs=None):
         """Autoregressive sampling with O(1) streamed state (gfn/model.py:404-469;
         the reference unpacks 3 values from its 6-tuple there and fails).
 
@@ -281,7 +292,12 @@ class Manifold(nn.Module):
         list) that returns one, or None for no limit.  A mask that leaves no
         token raises GfnError.  carry_state: a scan model (use_scan=True)
         continues from its state (stream()) instead of starting every call from
-        zero as the reference's does."""
+        zero as the reference's does.
+
+        logprobs (0 to 32): returns (tokens, steps) with, for each new token, a
+        dict of the token, its log probability, the entropy and that many top
+        alternatives (top_tokens, top_logprobs), all of the model's own logits,
+        before temperature, penalties and masks (token_logprobs)."""
         self.eval()
         if carry_state:
             step = self.stream
@@ -322,12 +338,24 @@ class Manifold(nn.Module):
                 return torch.argmax(nl, dim=-1, keepdim=True)
             return torch.multinomial(torch.softmax(nl, dim=-1), num_samples=1)
 
+        steps = []
+
+        def note(lg, tok):
+            if logprobs is not None:
+                steps.append((tok, token_logprobs(lg[:1, -1], tok.view(1), top=logprobs, entropy=True)))
+
         tok = sample_next(logits)
+        note(logits, tok)
         generated.append(tok.item())
         for _ in range(max_new_tokens - 1):
             if shaped:
                 history[:, len(generated) - 1:len(generated)] = tok
             logits, state = step(tok, state=state)
             tok = sample_next(logits)
+            note(logits, tok)
             generated.append(tok.item())
-        return generated
+        if logprobs is None:
+            return generated
+        return generated, [dict(token=t.item(), logprob=r.logprobs.item(), entropy=r.entropy.item(),
+                                top_tokens=r.top_tokens[0].tolist() if logprobs else [],
+                                top_logprobs=r.top_logprobs[0].tolist() if logprobs else []) for t, r in steps]

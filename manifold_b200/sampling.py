@@ -1,6 +1,10 @@
 """Logits before sampling: penalties for the tokens of a row's history, a
 bias, the temperature and a grammar mask, in one kernel (the reference samples
-from bare logits, gfn/model.py:404-469).  CUDA tensors only."""
+from bare logits, gfn/model.py:404-469); and what the logits say of given
+tokens: log probabilities, the entropy and the top alternatives, with their
+gradient.  CUDA tensors only."""
+from typing import NamedTuple, Optional
+
 import torch
 
 from ._lib import GfnError, dtype_code, same_device, torch_ops
@@ -110,3 +114,45 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repet
         allowed, ms = _rows_or_shared(allowed, "allowed", B, (V + 31) // 32)
     return torch_ops().process_logits(x, tokens, ts, lengths, prompt_lengths, rep, freq, pres, temp, rep_rows, freq_rows,
                                       pres_rows, temp_rows, bias, bs, allowed, ms)
+
+
+class TokenLogprobs(NamedTuple):
+    """Float32 of the logits' leading shape (the last two: [..., top], int64 tokens); None where not asked for."""
+    logprobs: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    top_logprobs: Optional[torch.Tensor]
+    top_tokens: Optional[torch.Tensor]
+
+
+def token_logprobs(logits, tokens=None, top=0, entropy=False, ignore_index=-100):
+    """TokenLogprobs of logits [..., vocab]: the log probability of each row's
+    token, the row's entropy, and its `top` most probable tokens (at most 32,
+    largest first, the lowest token first where logits are equal).
+
+    logits: float32, bfloat16 or float16; rows of a wider tensor are read in
+    place.  tokens: int64 or int32 of the logits' leading shape, or None.  A token
+    equal to ignore_index has log probability 0 and no gradient; another one
+    outside the vocabulary gives NaN and sets a device error bit
+    (gfn.cuda.ops.device_error).  Logits of -inf (masked tokens) have probability
+    0.  A row that has none above -inf gives -inf, entropy 0 and a gradient of
+    zeros; one with NaN or +inf gives NaN.  Differentiable (once) in the logits,
+    through every float result.
+    """
+    same_device("token_logprobs", logits, tokens)
+    dtype_code(logits, "logits")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise GfnError(f"token_logprobs: logits must be [..., vocab], got {tuple(logits.shape)}")
+    if not isinstance(top, int) or not 0 <= top <= min(32, logits.shape[-1]):
+        raise GfnError(f"token_logprobs: top must be 0 to {min(32, logits.shape[-1])}, got {top}")
+    if tokens is not None:
+        if tokens.shape != logits.shape[:-1] or (tokens.dtype != torch.int64 and tokens.dtype != torch.int32):
+            raise GfnError(f"token_logprobs: tokens must be int64 {tuple(logits.shape[:-1])}, got {tokens.dtype} "
+                           f"{tuple(tokens.shape)}")
+        if tokens.dtype != torch.int64:
+            tokens = tokens.to(torch.int64)
+    elif not top and not entropy:
+        raise GfnError("token_logprobs: nothing asked for (tokens, top or entropy)")
+    out = iter(torch_ops().token_logprobs(logits, tokens, top, entropy, ignore_index,
+                                          logits.requires_grad and torch.is_grad_enabled()))
+    return TokenLogprobs(next(out) if tokens is not None else None, next(out) if entropy else None,
+                         next(out) if top else None, next(out) if top else None)

@@ -1,5 +1,6 @@
 """Float64 definitions of the language-model operators and their gradients
-(layer norm, gated scan, the scan layer's recurrence, logit shaping): plain
+(layer norm, gated scan, the scan layer's recurrence, logit shaping, token embedding, log
+probabilities, attention with decay): plain
 numpy, one step after the other, the yardstick of the kernels' tests."""
 import numpy as np
 
@@ -127,3 +128,104 @@ def process_logits(logits, tokens=None, lengths=None, prompt_lengths=None, rep=1
         if allowed is not None:
             x[i] = np.where(np.broadcast_to(allowed, (B, V))[i], x[i], -np.inf)
     return x
+
+
+def embed_tokens(ids, weight, scale=1.0):
+    """scale * weight[ids], zeros for ids outside the table."""
+    w, ids = np.asarray(weight, np.float64), np.asarray(ids)
+    y = np.zeros(ids.shape + (w.shape[1],))
+    ok = (ids >= 0) & (ids < w.shape[0])
+    y[ok] = scale * w[ids[ok]]
+    return y
+
+
+def embed_tokens_backward(ids, dy, vocab, scale=1.0, padding_idx=None):
+    """dweight of sum(dy * embed_tokens)."""
+    dy = np.asarray(dy, np.float64)
+    dw = np.zeros((vocab, dy.shape[-1]))
+    for i, g in zip(np.asarray(ids).reshape(-1), dy.reshape(-1, dy.shape[-1])):
+        if 0 <= i < vocab and i != padding_idx:
+            dw[i] += scale * g
+    return dw
+
+
+def token_logprobs(logits, tokens=None, top=0, ignore_index=-100):
+    """Row by row (logprobs, entropy, top_logprobs, top_tokens): of equal logits the lower token first, NaN above all."""
+    x = np.asarray(logits, np.float64)
+    N, V = x.shape
+    lp, ent = np.zeros(N), np.zeros(N)
+    top_lp, top_id = np.zeros((N, top)), np.zeros((N, top), np.int64)
+    for i in range(N):
+        if np.isnan(x[i]).any() or (x[i] == np.inf).any():
+            logp = np.full(V, np.nan)
+            ent[i] = np.nan
+        elif (x[i] == -np.inf).all():
+            logp = np.full(V, -np.inf)
+        else:
+            m = x[i].max()
+            logp = (x[i] - m) - np.log(np.exp(x[i] - m).sum())
+            live = logp > -np.inf
+            ent[i] = -(np.exp(logp[live]) * logp[live]).sum()
+        key = np.where(np.isnan(x[i]), np.inf, x[i])
+        order = np.lexsort((np.arange(V), -key, ~np.isnan(x[i])))[:top]
+        top_id[i], top_lp[i] = order, logp[order]
+        if tokens is not None and tokens[i] != ignore_index:
+            lp[i] = logp[tokens[i]] if 0 <= tokens[i] < V else np.nan
+    return lp, ent, top_lp, top_id
+
+
+def token_logprobs_backward(logits, tokens, top_tokens, g_lp, g_ent, g_top, ignore_index=-100):
+    """dlogits of sum(g_lp logprobs) + sum(g_ent entropy) + sum(g_top top_logprobs); each g may be None."""
+    x = np.asarray(logits, np.float64)
+    N, V = x.shape
+    dx = np.zeros((N, V))
+    for i in range(N):
+        if (x[i] == -np.inf).all():
+            continue
+        m = x[i].max()
+        logp = (x[i] - m) - np.log(np.exp(x[i] - m).sum())
+        p = np.exp(logp)
+        pairs = [] if g_lp is None or tokens[i] == ignore_index else [(tokens[i], g_lp[i])]
+        pairs += [] if g_top is None else list(zip(top_tokens[i], g_top[i]))
+        for t, g in pairs:
+            dx[i] -= g * p
+            dx[i, t] += g
+        if g_ent is not None:
+            live = p > 0
+            H = -(p[live] * logp[live]).sum()
+            dx[i, live] -= g_ent[i] * p[live] * (logp[live] + H)
+    return dx
+
+
+def decay_attention(q, k, v, decay, state=None, lengths=None, scale=1.0):
+    """S_t = decay S_{t-1} + k_t v_t^T, o_t = scale q_t S_t on [B, L, H, .]; returns (o, last state)."""
+    q, k, v, decay = (np.asarray(t, np.float64) for t in (q, k, v, decay))
+    B, L, H, K = q.shape
+    S = np.zeros((B, H, K, v.shape[3])) if state is None else np.array(state, np.float64)
+    o = np.zeros(v.shape)
+    for b in range(B):
+        for t in range(L if lengths is None else min(max(int(lengths[b]), 0), L)):
+            S[b] = decay[:, None, None] * S[b] + k[b, t][:, :, None] * v[b, t][:, None, :]
+            o[b, t] = scale * np.einsum("hk,hkv->hv", q[b, t], S[b])
+    return o, S
+
+
+def decay_attention_backward(q, k, v, decay, state, lengths, scale, do, dlast=None):
+    """(dq, dk, dv, dstate) of sum(do * o) + sum(dlast * last state)."""
+    q, k, v, decay = (np.asarray(t, np.float64) for t in (q, k, v, decay))
+    B, L, H, K = q.shape
+    S = np.zeros((B, H, K, v.shape[3])) if state is None else np.array(state, np.float64)
+    R = np.zeros_like(S) if dlast is None else np.array(dlast, np.float64)
+    do = np.zeros(v.shape) if do is None else np.asarray(do, np.float64)
+    dq, dk, dv = np.zeros(q.shape), np.zeros(k.shape), np.zeros(v.shape)
+    for b in range(B):
+        n = L if lengths is None else min(max(int(lengths[b]), 0), L)
+        for t in range(n):
+            S[b] = decay[:, None, None] * S[b] + k[b, t][:, :, None] * v[b, t][:, None, :]
+            dq[b, t] = scale * np.einsum("hv,hkv->hk", do[b, t], S[b])
+        for t in range(n - 1, -1, -1):
+            G = R[b] + scale * q[b, t][:, :, None] * do[b, t][:, None, :]
+            dk[b, t] = np.einsum("hkv,hv->hk", G, v[b, t])
+            dv[b, t] = np.einsum("hkv,hk->hv", G, k[b, t])
+            R[b] = decay[:, None, None] * G
+    return dq, dk, dv, R
