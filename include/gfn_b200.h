@@ -621,8 +621,11 @@ int gfn_token_logprobs_backward(const void* logits, long long logits_row_stride,
  * the state, and get zeros.  kdim, vdim up to 128.  A block of 64 tokens is
  * one step: NaN or infinity in k or v reaches that block's earlier outputs
  * too.  `workspace` of gfn_decay_attention_workspace_bytes() (on the current
- * device), 16-byte aligned, serves either pass.  Results repeat bit for bit. */
-long long gfn_decay_attention_workspace_bytes(int batch, int length, int heads, int kdim, int vdim);
+ * device; one for each pass), 16-byte aligned.  forward_workspace: the
+ * forward's, left as it was, for length above 1, or NULL (its states are worked
+ * out again).  Results repeat bit for bit. */
+long long gfn_decay_attention_workspace_bytes(int backward, int dtype, int batch, int length, int heads, int kdim,
+                                              int vdim);
 int gfn_decay_attention_forward(const void* q, const long long* q_strides, const void* k, const long long* k_strides,
                                 const void* v, const long long* v_strides, const float* decay, const float* state,
                                 const void* lengths, int lengths_are_64, int dtype, int batch, int length, int heads,
@@ -632,9 +635,9 @@ int gfn_decay_attention_backward(const void* q, const long long* q_strides, cons
                                  const void* v, const long long* v_strides, const void* d_o,
                                  const long long* do_strides, const float* decay, const float* state,
                                  const float* d_state_out, const void* lengths, int lengths_are_64, int dtype,
-                                 int batch, int length, int heads, int kdim, int vdim, float scale, void* dq, void* dk,
-                                 void* dv, float* d_state, void* workspace, long long workspace_bytes,
-                                 gfn_stream_t stream);
+                                 int batch, int length, int heads, int kdim, int vdim, float scale,
+                                 const void* forward_workspace, void* dq, void* dk, void* dv, float* d_state,
+                                 void* workspace, long long workspace_bytes, gfn_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * FunctionalEmbedding, mode 'binary', coord_dim 16, hidden 64, 2 hidden

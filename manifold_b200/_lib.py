@@ -90,11 +90,11 @@ _SIGS = {
     "gfn_token_embed_backward": [_p, _i, _ll, _p, _ll, _i, _i, _i, _f, _ll, _p, _p, _ll, _p],
     "gfn_token_logprobs_forward": [_p, _ll, _i, _ll, _i, _p, _ll, _i, _p, _p, _p, _p, _p, _p],
     "gfn_token_logprobs_backward": [_p, _ll, _i, _ll, _i, _p, _ll, _i, _p, _p, _p, _p, _p, _p, _p, _p],
-    "gfn_decay_attention_workspace_bytes": [_i, _i, _i, _i, _i],
+    "gfn_decay_attention_workspace_bytes": [_i, _i, _i, _i, _i, _i, _i],
     "gfn_decay_attention_forward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _p, _p, _p,
                                     _ll, _p],
     "gfn_decay_attention_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f,
-                                     _p, _p, _p, _p, _p, _ll, _p],
+                                     _p, _p, _p, _p, _p, _p, _ll, _p],
 }
 _RESTYPES = {
     "gfn_status_string": ctypes.c_char_p,

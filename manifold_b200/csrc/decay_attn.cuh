@@ -1,0 +1,775 @@
+// Linear attention with a decay for each head: a state S [K, V] per sequence
+// and head,
+//
+//   S_t = g S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
+//
+// the gated scan (gfn/scan.py:11-104) with a matrix for a state.  In blocks of
+// C tokens, i, j = 0 .. n - 1 within one and S the state before it:
+//
+//   O  = scale ((Q K^T) o M) V + scale diag(g^(i+1)) Q S,   M_ij = g^(i-j), j <= i
+//   S' = g^n S + (diag(g^(n-1-j)) K)^T V
+//
+// The gradients are the same pass with other operands: with do for q, v for k,
+// k for v and the transposed state it gives dq; from the last token to the
+// first, with the state's gradient R for S,
+//
+//   dv = pass(k, q, do; R),   dk = pass(v, do, q; R^T),
+//   R' = g (g^(n-1) R + scale sum of g^(n-1-j) q_j do_j^T)
+//
+// State, sums and powers of g are float32.  The products run on the tensor
+// cores with float32 accumulators; what is rounded for them:
+//   bfloat16: P = (Q K^T) o M and S as operands, to bfloat16, once each (the
+//     outputs are rounded to it too); the state's own update takes g^.. k in
+//     three bfloat16 pieces (24 bits), so that the state stays float32-exact.
+//   float16: operands as tf32, which holds float16 exactly and P and S to 11
+//     bits at float32's range (a float16 P or S could overflow); g^.. k in two
+//     tf32 pieces.
+//   float32: every operand in two tf32 pieces, three products (2^-22).
+#pragma once
+#include "decay_attn.h"
+#include "lm_host.h"
+#include "lm_ops.cuh"
+
+namespace gfn_attn {
+
+using namespace gfn;
+using namespace gfn_abi;
+
+GFN_DEV int length_of(const PassArgs& p, int b) {
+  if (!p.lengths) return p.L;
+  const long long n = p.lengths64 ? static_cast<const long long*>(p.lengths)[b] : static_cast<const int*>(p.lengths)[b];
+  return (int)(n < 0 ? 0 : n > p.L ? p.L : n);
+}
+
+GFN_DEV float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// log2 of a decay in [0, 1] (taken as the nearer end outside); 0 becomes a
+// finite number whose every multiple from one on is a power of 0.
+GFN_DEV float log2_decay(float g) {
+  g = g > 1.f ? 1.f : g < 0.f ? 0.f : g;
+  return g == 0.f ? -1e30f : log2f(g);
+}
+GFN_DEV float power(float lg, int n) { return exp2f(lg * (float)n); }
+
+// ---------------------------------------------------------------- fragments
+// Operands of one tensor-core step.  Lane l stands at g = l / 4, t = l % 4.
+// bfloat16: m16n8k16.  tf32: m16n8k8, where place t of the contraction is its
+// element 2 t and place t + 4 its element 2 t + 1 on both sides, so that two
+// neighbours are read at once and accumulators serve as operands as they are.
+template <typename T>
+struct Math {
+  static constexpr int KS = 8, PIECES = sizeof(T) == 4 ? 2 : 1;
+  using State = float;
+  static constexpr int PAD = sizeof(T) == 4 ? 4 : 8, STATE_PAD = 4;
+  struct A {
+    unsigned v[PIECES][4];
+  };
+  struct B {
+    unsigned v[PIECES][2];
+  };
+};
+template <>
+struct Math<__nv_bfloat16> {
+  static constexpr int KS = 16;
+  using State = __nv_bfloat16;
+  static constexpr int PAD = 8, STATE_PAD = 8;
+  struct A {
+    unsigned v[4];
+  };
+  struct B {
+    unsigned v[2];
+  };
+};
+
+GFN_DEV void mma_bf16(float (&c)[4], const unsigned (&a)[4], const unsigned (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+GFN_DEV void mma_tf32(float (&c)[4], const unsigned (&a)[4], const unsigned (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+GFN_DEV unsigned tf32(float v) {
+  unsigned r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+  return r;
+}
+template <int N>
+GFN_DEV void pieces(float v, unsigned (&r)[N]) {
+  r[0] = tf32(v);
+  if constexpr (N > 1) r[1] = tf32(v - __uint_as_float(r[0]));
+}
+
+template <int PA, int PB>
+GFN_DEV void mma_pieces(float (&c)[4], const unsigned (&a)[PA][4], const unsigned (&b)[PB][2]) {
+  if constexpr (PA > 1) mma_tf32(c, a[1], b[0]);
+  if constexpr (PB > 1) mma_tf32(c, a[0], b[1]);
+  mma_tf32(c, a[0], b[0]);
+}
+template <typename T>
+GFN_DEV void mma(float (&c)[4], const typename Math<T>::A& a, const typename Math<T>::B& b) {
+  if constexpr (Math<T>::KS == 16) mma_bf16(c, a.v, b.v);
+  else mma_pieces(c, a.v, b.v);
+}
+
+GFN_DEV void ldsm(unsigned& a, unsigned& b, unsigned& c, unsigned& d, const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(p)) : "memory");
+}
+GFN_DEV void ldsm_t(unsigned& a, unsigned& b, unsigned& c, unsigned& d, const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(p)) : "memory");
+}
+GFN_DEV float2 pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
+GFN_DEV float2 pair(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
+
+// A, 16 rows from p [row][k].
+template <typename T>
+GFN_DEV void load_a(typename Math<T>::A& f, const T* p, int ld, int lane) {
+  if constexpr (Math<T>::KS == 16) {
+    ldsm(f.v[0], f.v[1], f.v[2], f.v[3], p + ((lane & 7) + (lane & 8)) * ld + ((lane >> 4) << 3));
+  } else {
+    const T* q = p + (lane >> 2) * ld + 2 * (lane & 3);
+    const float2 x = pair(q), y = pair(q + 8 * ld);
+    const float w[4] = {x.x, y.x, x.y, y.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned r[Math<T>::PIECES];
+      pieces(w[i], r);
+#pragma unroll
+      for (int k = 0; k < Math<T>::PIECES; ++k) f.v[k][i] = r[k];
+    }
+  }
+}
+// Two neighbouring B of 8 columns each, from p [n][k].
+template <typename T, typename E>
+GFN_DEV void load_bn(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) {
+  if constexpr (Math<T>::KS == 16) {
+    ldsm(f[0].v[0], f[0].v[1], f[1].v[0], f[1].v[1], p + ((lane & 7) + ((lane >> 4) << 3)) * ld + (lane & 8));
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 x = pair(p + ((lane >> 2) + 8 * h) * ld + 2 * (lane & 3));
+      unsigned r[2][Math<T>::PIECES];
+      pieces(x.x, r[0]);
+      pieces(x.y, r[1]);
+#pragma unroll
+      for (int k = 0; k < Math<T>::PIECES; ++k) {
+        f[h].v[k][0] = r[0][k];
+        f[h].v[k][1] = r[1][k];
+      }
+    }
+  }
+}
+// The same from p [k][n].
+template <typename T, typename E>
+GFN_DEV void load_bk(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) {
+  if constexpr (Math<T>::KS == 16) {
+    ldsm_t(f[0].v[0], f[0].v[1], f[1].v[0], f[1].v[1], p + ((lane & 7) + (lane & 8)) * ld + ((lane >> 4) << 3));
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const E* q = p + 2 * (lane & 3) * ld + (lane >> 2) + 8 * h;
+      unsigned r[2][Math<T>::PIECES];
+      pieces(to_f(q[0]), r[0]);
+      pieces(to_f(q[ld]), r[1]);
+#pragma unroll
+      for (int k = 0; k < Math<T>::PIECES; ++k) {
+        f[h].v[k][0] = r[0][k];
+        f[h].v[k][1] = r[1][k];
+      }
+    }
+  }
+}
+
+GFN_DEV unsigned pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&v);
+}
+GFN_DEV float2 unpack_bf16(unsigned v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+
+// ------------------------------------------------------------------- blocks
+// Tokens per block, warps, and who holds what.  A warp has 16 rows of a
+// block's output and, of the state, 16 rows (a slab) of SN tiles of 8 columns.
+template <typename T, int DK, int DV>
+struct Shape {
+  static constexpr bool WIDE = DK > 64 || DV > 64;
+  static constexpr int W = WIDE ? 8 : 4, THREADS = 32 * W;
+  static constexpr int C = sizeof(T) == 4 && (DK > 32 || DV > 32) ? 32 : 64;
+  static constexpr int LDK = DK + Math<T>::PAD, LDV = DV + Math<T>::PAD, LS = DV + Math<T>::STATE_PAD;
+  static constexpr int ROWS = C / 16, SPLIT = W / ROWS;
+  static constexpr int SLABS = DK / 16, SN = DV / 8 / (W / SLABS);
+  static constexpr int TK = C * LDK, TV = C * LDV;  // elements of an operand
+  static constexpr int STATE_BYTES = DK * LS * (int)sizeof(typename Math<T>::State);
+  static constexpr int stage(int kind) { return kind == STATE ? TK + TV : kind == OUTPUT ? 2 * TK + TV : 2 * TK + 2 * TV; }
+  // the state's operand form twice where that fits: one barrier per block instead of two
+  static constexpr int buffers(int kind) {
+    return kind == STATE ? 0 : 2 * stage(kind) * (int)sizeof(T) + 2 * STATE_BYTES + 8 * C <= 227 * 1024 ? 2 : 1;
+  }
+  static constexpr int bytes(int kind) {
+    return 2 * stage(kind) * (int)sizeof(T) + buffers(kind) * STATE_BYTES + 8 * C;
+  }
+  static constexpr int resident(int kind) {
+    const int fit = 228 * 1024 / (bytes(kind) + 1024), most = WIDE ? 1 : kind == STATE ? 4 : kind == PAIR && sizeof(T) < 4 ? 2 : 3;
+    return fit < most ? fit : most;
+  }
+};
+
+// Brings rows 0 .. n - 1 of a block into shared memory, zeros behind them; row
+// r is the r-th token from `at` on (BACK: from there to the front).  Columns
+// from `dim` on were zeroed once and stay so.
+template <typename T, int D, int LD, int C, int THREADS, bool BACK>
+GFN_DEV void fetch(T* dst, const View& v, int b, int h, int dim, int at, int n, int vec) {
+  const T* src = static_cast<const T*>(v.p) + b * v.sb + h * v.sh + at * v.sl;
+  if (vec) {
+    constexpr int PER = 16 / sizeof(T), LANES = D / PER, STEP = THREADS / LANES;
+    const int col = (threadIdx.x % LANES) * PER, r0 = threadIdx.x / LANES;
+    if (col >= dim) return;
+    const T* from = src + col + (BACK ? -r0 : r0) * v.sl;
+    const long long step = (BACK ? -STEP : STEP) * v.sl;
+    const uint32_t to = smem_u32(dst + r0 * LD + col);
+#pragma unroll
+    for (int i = 0; i < C / STEP; ++i) {
+      const bool live = r0 + i * STEP < n;  // others are filled with zeros: 0 bytes are read
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * STEP * LD * (int)sizeof(T)),
+                   "l"(live ? from : static_cast<const T*>(v.p)), "r"(live ? 16 : 0)
+                   : "memory");
+      from += step;
+    }
+  } else {
+    for (int i = threadIdx.x; i < C * D; i += THREADS) {
+      const int r = i / D, col = i % D;
+      if (col < dim) dst[r * LD + col] = r < n ? src[(BACK ? -r : r) * v.sl + col] : from_f<T>(0.f);
+    }
+  }
+}
+
+// Powers of g that a thread applies to its scores, g^(i-j) s_in: on the two
+// tiles that the diagonal crosses, on the one before them, and from tile to
+// tile further back.
+struct Decay {
+  float diag[2][4], first[4], g8;
+  GFN_DEV Decay(float lg, float s_in) {
+    const int lane = threadIdx.x & 31, gap = (lane >> 2) - 2 * (lane & 3);
+    g8 = exp2_fast(8.f * lg);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = gap + 8 * (e >> 1) - (e & 1);
+      diag[0][e] = d < 0 ? 0.f : s_in * exp2_fast((float)d * lg);
+      diag[1][e] = d < 8 ? 0.f : s_in * exp2_fast((float)(d - 8) * lg);
+      first[e] = s_in * exp2_fast((float)(d + 8) * lg);
+    }
+  }
+};
+
+// One warp's 16 rows of a block's output: ON tiles of 8 columns from col0.
+// rows, keys [C][LDA] with kd of their columns in use, values [C][LDB]; st: the
+// state, seen from this product as [k][n] or (NMAJOR) [n][k].
+template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR>
+GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
+                    int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
+  using M = Math<T>;
+  const int lane = threadIdx.x & 31;
+  float s[C / 8][4];
+#pragma unroll
+  for (int i = 0; i < C / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < ON; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < DA; k += M::KS) {
+    if (k >= kd) continue;
+    typename M::A a;
+    load_a<T>(a, rows + rt * 16 * LDA + k, LDA, lane);
+#pragma unroll
+    for (int i = 0; i < ON; i += 2) {
+      const int col = col0 + i * 8;
+      if (col >= nd) continue;
+      typename M::B b[2];
+      if (NMAJOR) load_bn<T>(b, st + col * LS + k, LS, lane);
+      else load_bk<T>(b, st + k * LS + col, LS, lane);
+      mma<T>(o[i], a, b[0]);
+      mma<T>(o[i + 1], a, b[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < C / 16; ++i) {
+      if (i > rt) continue;  // keys behind the rows
+      typename M::B b[2];
+      load_bn<T>(b, keys + i * 16 * LDA + k, LDA, lane);
+      mma<T>(s[2 * i], a, b[0]);
+      mma<T>(s[2 * i + 1], a, b[1]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ON; ++i) {
+    o[i][0] *= w0;
+    o[i][1] *= w0;
+    o[i][2] *= w1;
+    o[i][3] *= w1;
+  }
+  F2 f0 = f2(g.first[0], g.first[1]), f1 = f2(g.first[2], g.first[3]);
+  const F2 g8 = f2(g.g8);
+#pragma unroll
+  for (int i = C / 8 - 1; i >= 0; --i) {
+    const int off = 2 * rt - i;  // -1, 0: the diagonal's tiles
+    if (off < -1) continue;
+    if (off > 0) {
+      split(f2(s[i][0], s[i][1]) * f0, s[i][0], s[i][1]);
+      split(f2(s[i][2], s[i][3]) * f1, s[i][2], s[i][3]);
+      f0 = f0 * g8;
+      f1 = f1 * g8;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = off == 0 ? g.diag[0][e] : g.diag[1][e];
+        s[i][e] = w == 0.f ? 0.f : s[i][e] * w;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < C / 16; ++i) {
+    if (i > rt) continue;
+#pragma unroll
+    for (int q = 0; q < 16 / M::KS; ++q) {
+      typename M::A a;
+      if constexpr (M::KS == 16) {
+        a.v[0] = pack_bf16(s[2 * i][0], s[2 * i][1]);
+        a.v[1] = pack_bf16(s[2 * i][2], s[2 * i][3]);
+        a.v[2] = pack_bf16(s[2 * i + 1][0], s[2 * i + 1][1]);
+        a.v[3] = pack_bf16(s[2 * i + 1][2], s[2 * i + 1][3]);
+      } else {
+        const float w[4] = {s[2 * i + q][0], s[2 * i + q][2], s[2 * i + q][1], s[2 * i + q][3]};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          unsigned r[M::PIECES];
+          pieces(w[e], r);
+#pragma unroll
+          for (int z = 0; z < M::PIECES; ++z) a.v[z][e] = r[z];
+        }
+      }
+      const T* v = values + (16 * i + M::KS * q) * LDB + col0;
+#pragma unroll
+      for (int n = 0; n < ON; n += 2) {
+        if (col0 + n * 8 >= nd) continue;
+        typename M::B b[2];
+        load_bk<T>(b, v + n * 8, LDB, lane);
+        mma<T>(o[n], a, b[0]);
+        mma<T>(o[n + 1], a, b[1]);
+      }
+    }
+  }
+}
+
+// Two values in three bfloat16 pieces each, which add up to them exactly.
+GFN_DEV void split3(float x, float y, unsigned& hi, unsigned& mid, unsigned& lo) {
+  auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
+  auto both = [](float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); };
+  hi = both(x, y);
+  x -= cut(x);
+  y -= cut(y);
+  mid = both(x, y);
+  lo = both(x - cut(x), y - cut(y));
+}
+
+// st = gn st + (diag(wt) keys)^T values for one warp's 16 rows (from m0) and N
+// tiles of columns (from n0) of the state.  The products of a block are summed
+// by themselves and then added, since the tensor cores cut where float32
+// addition rounds: over a long sequence that would drift.
+template <typename T, int C, int LDK, int LDV, int N>
+GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const float* wt, float gn, int m0, int n0, int nd) {
+  using M = Math<T>;
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  constexpr int AT = N < 8 ? N : 8;  // tiles at a time
+#pragma unroll
+  for (int at = 0; at < N; at += AT) {
+    if (n0 + at * 8 >= nd) continue;
+    float add[AT][4];
+#pragma unroll
+    for (int n = 0; n < AT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add[n][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < C; k += M::KS) {
+      const T* vals = values + k * LDV + n0 + at * 8;
+      if constexpr (M::KS == 16) {
+        unsigned raw[4], a[3][4];
+        ldsm_t(raw[0], raw[1], raw[2], raw[3], keys + (k + (lane & 7) + ((lane >> 4) << 3)) * LDK + m0 + (lane & 8));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float* w = wt + k + 2 * t + 8 * (e >> 1);
+          const float2 x = unpack_bf16(raw[e]);
+          split3(x.x * w[0], x.y * w[1], a[0][e], a[1][e], a[2][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < AT; n += 2) {
+          if (n0 + (at + n) * 8 >= nd) continue;
+          typename M::B b[2];
+          load_bk<T>(b, vals + n * 8, LDV, lane);
+#pragma unroll
+          for (int z = 2; z >= 0; --z) {
+            mma_bf16(add[n], a[z], b[0].v);
+            mma_bf16(add[n + 1], a[z], b[1].v);
+          }
+        }
+      } else {
+        unsigned a[2][4];
+        const T* q = keys + (k + 2 * t) * LDK + m0 + (lane >> 2);
+        const float w0 = wt[k + 2 * t], w1 = wt[k + 2 * t + 1];
+        const float x[4] = {to_f(q[0]) * w0, to_f(q[8]) * w0, to_f(q[LDK]) * w1, to_f(q[LDK + 8]) * w1};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          unsigned r[2];
+          pieces(x[e], r);
+          a[0][e] = r[0];
+          a[1][e] = r[1];
+        }
+#pragma unroll
+        for (int n = 0; n < AT; n += 2) {
+          if (n0 + (at + n) * 8 >= nd) continue;
+          typename M::B b[2];
+          load_bk<T>(b, vals + n * 8, LDV, lane);
+          mma_pieces(add[n], a, b[0].v);
+          mma_pieces(add[n + 1], a, b[1].v);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < AT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[at + n][e] = fmaf(st[at + n][e], gn, add[n][e]);
+  }
+}
+
+// Writes a warp's rows.  16-bit: lanes 2 i and 2 i + 1 trade a half of two
+// neighbouring tiles, so that four lanes write 32 bytes in a row.
+template <typename T, int ON, bool BACK>
+GFN_DEV void emit(void* out, const float (&o)[ON][4], const PassArgs& p, int b, int h, int dim, int at, int n, int rt, int col0) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = rt * 16 + (lane >> 2) + 8 * half;
+    T* row = static_cast<T*>(out) + (((long long)b * p.L + (BACK ? at - r : at + r)) * p.H + h) * dim;
+    if (sizeof(T) == 2 && dim % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < ON; i += 2) {
+        unsigned w[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const T two[2] = {from_f<T>(o[i + z][2 * half]), from_f<T>(o[i + z][2 * half + 1])};
+          w[z] = *reinterpret_cast<const unsigned*>(two);
+        }
+        const unsigned other = __shfl_xor_sync(0xffffffffu, t & 1 ? w[0] : w[1], 1);
+        const int col = col0 + (i + (t & 1)) * 8 + 2 * (t & 2);
+        if (r < n && col < dim) *reinterpret_cast<uint2*>(row + col) = t & 1 ? make_uint2(other, w[1]) : make_uint2(w[0], other);
+      }
+      continue;
+    }
+    if (r >= n) continue;
+#pragma unroll
+    for (int i = 0; i < ON; ++i) {
+      const int col = col0 + i * 8 + 2 * t;
+      const float lo = o[i][2 * half], hi = o[i][2 * half + 1];
+      if (sizeof(T) == 4 && dim % 2 == 0) {
+        if (col < dim) *reinterpret_cast<float2*>(row + col) = make_float2(lo, hi);
+      } else {
+        if (col < dim) row[col] = from_f<T>(lo);
+        if (col + 1 < dim) row[col + 1] = from_f<T>(hi);
+      }
+    }
+  }
+}
+
+// One thread block walks the blocks of C tokens of one segment of a sequence
+// and head, the state in registers (float32), the next block's operands on
+// their way.  OUTPUT: rows a, keys b, values c.  STATE: keys b, values c.
+// PAIR: with a = q, b = k, c = v, d = do, the outputs dv (rows b, keys a,
+// values d) and dk (rows c, keys d, values a) of the state's gradient.
+template <typename T, int DK, int DV, bool BACK, int KIND>
+__global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::resident(KIND)) attn_kernel(const PassArgs p) {
+  using S = Shape<T, DK, DV>;
+  using M = Math<T>;
+  using Op = typename M::State;
+  constexpr int STAGE = S::stage(KIND), BUFS = S::buffers(KIND);
+  extern __shared__ __align__(128) char attn_shared[];
+  T* stage = reinterpret_cast<T*>(attn_shared);
+  Op* st_op = reinterpret_cast<Op*>(stage + 2 * STAGE);
+  float* wt = reinterpret_cast<float*>(attn_shared + 2 * STAGE * sizeof(T) + BUFS * S::STATE_BYTES);  // [2 C]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int seg = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int len = length_of(p, b);
+  const int from = seg * p.seg_len, to = min(from + p.seg_len, len);
+  const float lg = log2_decay(p.decay[h]);
+  // the state's place of this warp
+  const int m0 = (warp % S::SLABS) * 16, n0 = (warp / S::SLABS) * S::SN * 8;
+  const bool holds = m0 < p.KD && n0 < p.VD;
+  float st[S::SN][4];
+  const long long mat = (long long)p.KD * p.VD, bh = (long long)b * p.H + h;
+  const float* init = KIND == STATE ? nullptr : p.segs ? p.segs + (bh * p.segments + seg) * mat : p.state ? p.state + bh * mat : nullptr;
+  const long long sr = p.segs ? p.segs_sr : p.sr, sc = p.segs ? p.segs_sc : p.sc;
+#pragma unroll
+  for (int i = 0; i < S::SN; ++i) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = m0 + (lane >> 2) + 8 * (e >> 1), col = n0 + i * 8 + 2 * (lane & 3) + (e & 1);
+      st[i][e] = init && row < p.KD && col < p.VD ? init[row * sr + col * sc] : 0.f;
+    }
+  }
+  {
+    uint4* z = reinterpret_cast<uint4*>(attn_shared);
+    for (int i = threadIdx.x; i < (int)((2 * STAGE * sizeof(T) + BUFS * S::STATE_BYTES) / 16); i += S::THREADS)
+      z[i] = make_uint4(0, 0, 0, 0);
+    // place C - 1 - e holds g^e (back: g^(e+1)); rows behind a short block take zeros
+    for (int i = threadIdx.x; i < 2 * S::C; i += S::THREADS)
+      wt[i] = i < S::C ? p.s_update * power(lg, S::C - 1 - i + (BACK ? 1 : 0)) : 0.f;
+  }
+  __syncthreads();
+  auto bring = [&](int c, T* dst) {
+    const int done = c * S::C, n = min(S::C, to - from - done), at = BACK ? to - 1 - done : from + done;
+    auto keys = [&](T* d, const View& v) { fetch<T, DK, S::LDK, S::C, S::THREADS, BACK>(d, v, b, h, p.KD, at, n, p.vec); };
+    auto vals = [&](T* d, const View& v) { fetch<T, DV, S::LDV, S::C, S::THREADS, BACK>(d, v, b, h, p.VD, at, n, p.vec); };
+    if (KIND == OUTPUT) {
+      keys(dst, p.a);
+      keys(dst + S::TK, p.b);
+      vals(dst + 2 * S::TK, p.c);
+    } else if (KIND == STATE) {
+      keys(dst, p.b);
+      vals(dst + S::TK, p.c);
+    } else {
+      keys(dst, p.a);
+      keys(dst + S::TK, p.b);
+      vals(dst + 2 * S::TK, p.c);
+      vals(dst + 2 * S::TK + S::TV, p.d);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto lay_out = [&](Op* q) {  // the state as the products take it
+    if (KIND == STATE || !holds) return;
+    q += (m0 + (lane >> 2)) * S::LS + n0 + 2 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < S::SN; ++i) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if constexpr (M::KS == 16)
+          *reinterpret_cast<unsigned*>(q + 8 * half * S::LS + i * 8) = pack_bf16(st[i][2 * half], st[i][2 * half + 1]);
+        else
+          *reinterpret_cast<float2*>(q + 8 * half * S::LS + i * 8) = make_float2(st[i][2 * half], st[i][2 * half + 1]);
+      }
+    }
+  };
+  const int blocks = to > from ? (to - from + S::C - 1) / S::C : 0;
+  if (blocks) bring(0, stage);
+  lay_out(st_op);
+  const int rt = warp % S::ROWS, part = warp / S::ROWS;
+  const Decay decay(lg, p.s_in);
+  // forward: row i takes g^(i+1) of the state; back: g^i, as the state's
+  // gradient arrives with that factor in it
+  const int r0 = rt * 16 + (lane >> 2) + (BACK ? 0 : 1);
+  const float w0 = p.s_state * power(lg, r0), w1 = p.s_state * power(lg, r0 + 8);
+  for (int c = 0; c < blocks; ++c) {
+    const T* cur = stage + (c & 1) * STAGE;
+    const Op* op = st_op + (BUFS == 2 ? (c & 1) * DK * S::LS : 0);
+    const int done = c * S::C, n = min(S::C, to - from - done), at = BACK ? to - 1 - done : from + done;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // and with it everyone has left the other stage
+    if (c + 1 < blocks) bring(c + 1, stage + ((c + 1) & 1) * STAGE);
+    if constexpr (KIND != STATE) {
+      constexpr int OV = DV / 8 / S::SPLIT;
+      float o[OV][4];
+      const int col0 = part * OV * 8;
+      if (col0 < p.VD) {
+        if constexpr (KIND == OUTPUT)
+          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false>(o, cur, cur + S::TK, cur + 2 * S::TK, op, rt, col0, p.KD, p.VD,
+                                                               decay, w0, w1);
+        else
+          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false>(o, cur + S::TK, cur, cur + 2 * S::TK + S::TV, op, rt, col0, p.KD,
+                                                               p.VD, decay, w0, w1);
+        emit<T, OV, BACK>(p.o, o, p, b, h, p.VD, at, n, rt, col0);
+      }
+    }
+    if constexpr (KIND == PAIR) {
+      constexpr int OK = DK / 8 / S::SPLIT;
+      float o[OK][4];
+      const int col0 = part * OK * 8;
+      if (col0 < p.KD) {
+        attend<T, S::C, DV, S::LDV, S::LDK, S::LS, OK, true>(o, cur + 2 * S::TK, cur + 2 * S::TK + S::TV, cur, op, rt, col0, p.VD,
+                                                            p.KD, decay, w0, w1);
+        emit<T, OK, BACK>(p.o2, o, p, b, h, p.KD, at, n, rt, col0);
+      }
+    }
+    const T* uk = KIND == OUTPUT ? cur + S::TK : cur;
+    const T* uv = KIND == OUTPUT ? cur + 2 * S::TK : KIND == STATE ? cur + S::TK : cur + 2 * S::TK + S::TV;
+    if (holds) update<T, S::C, S::LDK, S::LDV, S::SN>(st, uk, uv, wt + S::C - n, power(lg, n), m0, n0, p.VD);
+    if (BUFS == 1) __syncthreads();
+    if (BUFS > 0) lay_out(st_op + (BUFS == 2 ? ((c + 1) & 1) * DK * S::LS : 0));
+  }
+  // tokens behind the sequence: zeros
+  if (KIND != STATE && len < p.L) {
+    const int z0 = max(from, len), z1 = min(from + p.seg_len, p.L);
+    for (int pass = 0; pass < (KIND == PAIR ? 2 : 1); ++pass) {
+      const int dim = pass ? p.KD : p.VD;
+      T* y = static_cast<T*>(pass ? p.o2 : p.o);
+      for (long long i = threadIdx.x; i < (long long)(z1 - z0) * dim; i += S::THREADS)
+        y[(((long long)b * p.L + z0 + i / dim) * p.H + h) * dim + i % dim] = from_f<T>(0.f);
+    }
+  }
+  float* out = KIND == STATE ? p.segs + (bh * p.segments + seg) * mat : p.segs ? nullptr : p.state_out ? p.state_out + bh * mat : nullptr;
+  if (out) {
+#pragma unroll
+    for (int i = 0; i < S::SN; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = m0 + (lane >> 2) + 8 * (e >> 1), col = n0 + i * 8 + 2 * (lane & 3) + (e & 1);
+        if (row < p.KD && col < p.VD) out[row * p.VD + col] = st[i][e];
+      }
+  }
+}
+
+// The states before each segment, from what each segment adds; in place.  Up to
+// JOIN segments' parts are on their way at once.
+template <bool BACK>
+__global__ void __launch_bounds__(256) attn_join_kernel(const PassArgs p) {
+  constexpr int JOIN = 16;
+  const int mat = p.KD * p.VD, i = blockIdx.x * 256 + threadIdx.x;
+  const long long bh = blockIdx.y + (long long)gridDim.y * blockIdx.z;
+  if (i >= mat || bh >= (long long)p.B * p.H) return;
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H), len = length_of(p, b);
+  const float lg = log2_decay(p.decay[h]);
+  const int row = i / p.VD, col = i % p.VD;
+  float s = p.state ? p.state[bh * mat + row * p.sr + col * p.sc] : 0.f;
+  float* q = p.segs + bh * p.segments * mat + i;
+  const float whole = power(lg, p.seg_len);
+  for (int k0 = 0; k0 < p.segments; k0 += JOIN) {
+    float add[JOIN];
+#pragma unroll
+    for (int u = 0; u < JOIN; ++u) {
+      const int k = BACK ? p.segments - 1 - k0 - u : k0 + u;
+      add[u] = k0 + u < p.segments ? q[(long long)k * mat] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < JOIN; ++u) {
+      if (k0 + u >= p.segments) continue;
+      const int k = BACK ? p.segments - 1 - k0 - u : k0 + u;
+      const int n = min(max(len - k * p.seg_len, 0), p.seg_len);
+      q[(long long)k * mat] = s;
+      s = fmaf(n == p.seg_len ? whole : power(lg, n), s, add[u]);
+    }
+  }
+  if (p.state_out) p.state_out[bh * mat + i] = s;
+}
+
+// One token: the state is read, moved on and written once.  A thread owns VEC
+// columns of every RG-th row.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) attn_step_kernel(const PassArgs p) {
+  __shared__ float q[128], k[128], sum[256 * VEC];
+  const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
+  const long long mat = (long long)p.KD * p.VD, bh = (long long)b * p.H + h;
+  const bool live = length_of(p, b) > 0;
+  const float gam = fminf(fmaxf(p.decay[h], 0.f), 1.f), g = p.decay[h] != p.decay[h] ? p.decay[h] : gam;
+  auto at = [&](const View& v) { return static_cast<const T*>(v.p) + b * v.sb + h * v.sh; };
+  const int cols = p.VD / VEC, groups = 256 / cols, mine = threadIdx.x % cols, group = threadIdx.x / cols;
+  if (threadIdx.x < p.KD) {
+    q[threadIdx.x] = live ? to_f(at(p.a)[threadIdx.x]) * p.s_state : 0.f;
+    k[threadIdx.x] = live ? to_f(at(p.b)[threadIdx.x]) : 0.f;
+  }
+  float v[VEC], acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    v[e] = live ? to_f(at(p.c)[mine * VEC + e]) : 0.f;
+    acc[e] = 0.f;
+  }
+  __syncthreads();
+  struct alignas(4 * VEC) Cells {
+    float c[VEC];
+  };
+  if (group < groups) {
+#pragma unroll 4
+    for (int r = group; r < p.KD; r += groups) {
+      Cells s = {};
+      if (p.state) s = *reinterpret_cast<const Cells*>(p.state + bh * mat + (long long)r * p.VD + mine * VEC);
+      if (live) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s.c[e] = fmaf(g, s.c[e], k[r] * v[e]);
+          acc[e] = fmaf(q[r], s.c[e], acc[e]);
+        }
+      }
+      if (p.state_out) *reinterpret_cast<Cells*>(p.state_out + bh * mat + (long long)r * p.VD + mine * VEC) = s;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sum[threadIdx.x * VEC + e] = acc[e];
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.VD; c += 256) {
+    float t = 0.f;
+    for (int r = 0; r < groups; ++r) t += sum[(r * cols + c / VEC) * VEC + c % VEC];
+    static_cast<T*>(p.o)[bh * p.VD + c] = from_f<T>(t);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+template <typename T, int DK, int DV, bool BACK, int KIND>
+int attn_run(const PassArgs& p, cudaStream_t s) {
+  using S = Shape<T, DK, DV>;
+  static std::atomic<unsigned long long> done;
+  const int bytes = S::bytes(KIND);
+  const int st = shared_limit(attn_kernel<T, DK, DV, BACK, KIND>, bytes, &done, "attn_kernel");
+  if (st != GFN_OK) return st;
+  attn_kernel<T, DK, DV, BACK, KIND><<<dim3(p.segments, p.H, p.B), S::THREADS, bytes, s>>>(p);
+  return launch_status("attn_kernel");
+}
+
+template <typename T, int DK, int DV, bool BACK, int KIND>
+int attn_pass(PassArgs p, bool known, cudaStream_t s) {
+  if (p.segments == 1) p.segs = nullptr;
+  else if (!known) {
+    PassArgs w = p;
+    if (KIND == PAIR) {  // the state's rows are q's, its columns do's
+      w.b = p.a;
+      w.c = p.d;
+    }
+    int st = attn_run<T, DK, DV, BACK, STATE>(w, s);
+    if (st != GFN_OK) return st;
+    const int bh = p.B * p.H, y = bh < 32768 ? bh : 32768;
+    attn_join_kernel<BACK><<<dim3((unsigned)((p.KD * p.VD + 255) / 256), y, (bh + y - 1) / y), 256, 0, s>>>(w);
+    if ((st = launch_status("attn_join_kernel")) != GFN_OK) return st;
+  }
+  return attn_run<T, DK, DV, BACK, KIND>(p, s);
+}
+
+template <typename T, bool BACK, int KIND>
+int attn_dims(const PassArgs& p, bool known, cudaStream_t s) {
+  const Dims d = padded(p.KD, p.VD);
+  if (d.k == 32) return attn_pass<T, 32, 32, BACK, KIND>(p, known, s);
+  if (d.k == 64 && d.v == 64) return attn_pass<T, 64, 64, BACK, KIND>(p, known, s);
+  if (d.k == 64) return attn_pass<T, 64, 128, BACK, KIND>(p, known, s);
+  if (d.v == 64) return attn_pass<T, 128, 64, BACK, KIND>(p, known, s);
+  return attn_pass<T, 128, 128, BACK, KIND>(p, known, s);
+}
+
+template <typename T>
+int attn_step(const PassArgs& p, cudaStream_t s) {
+  const unsigned blocks = (unsigned)(p.B * p.H);
+  const bool vec = p.VD % 4 == 0 && (!p.state || aligned16(p.state)) && (!p.state_out || aligned16(p.state_out));
+  if (vec) attn_step_kernel<T, 4><<<blocks, 256, 0, s>>>(p);
+  else attn_step_kernel<T, 1><<<blocks, 256, 0, s>>>(p);
+  return launch_status("attn_step_kernel");
+}
+
+template <typename T>
+int attn_resident(Kind kind, int kd, int vd) {
+  const Dims d = padded(kd, vd);
+  if (d.k == 32) return Shape<T, 32, 32>::resident(kind);
+  if (d.k == 64) return d.v == 64 ? Shape<T, 64, 64>::resident(kind) : Shape<T, 64, 128>::resident(kind);
+  return d.v == 64 ? Shape<T, 128, 64>::resident(kind) : Shape<T, 128, 128>::resident(kind);
+}
+
+}  // namespace gfn_attn

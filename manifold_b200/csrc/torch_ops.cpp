@@ -510,15 +510,15 @@ struct AttnShape {
         H(extent(q.size(2), "decay_attention")), K(extent(q.size(3), "decay_attention")),
         V(extent(v.size(3), "decay_attention")) {}
   Tensor state(const Tensor& q) const { return fresh(q, {B, H, K, V}, at::kFloat); }
-  Tensor workspace(const Tensor& q, long long* n) const {
-    *n = api.gfn_decay_attention_workspace_bytes(B, L, H, K, V);
+  Tensor workspace(const Tensor& q, bool backward, long long* n) const {
+    *n = api.gfn_decay_attention_workspace_bytes(backward, code_of(q), B, L, H, K, V);
     if (*n < 0) throw Failure(std::string("decay_attention: ") + api.gfn_last_error_message());
     return *n ? fresh(q, {*n}, at::kByte) : Tensor();
   }
 };
 
 Tensor attn_run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& state,
-                const Tensor& lengths, double scale, Tensor* last) {
+                const Tensor& lengths, double scale, Tensor* last, Tensor* kept) {
   at::AutoDispatchBelowADInplaceOrView plain;
   const Launch on(q);
   const AttnShape s(q, v);
@@ -527,7 +527,8 @@ Tensor attn_run(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
   Tensor o = fresh(v, {s.B, s.L, s.H, s.V}, v.scalar_type());
   if (last) *last = s.state(q);
   long long n = 0;
-  const Tensor ws = s.workspace(q, &n);
+  const Tensor ws = s.workspace(q, false, &n);
+  if (kept && s.L > 1) *kept = ws;
   check(api.gfn_decay_attention_forward(hq.p(), hq.strides, hk.p(), hk.strides, hv.p(), hv.strides, fptr(decay),
                                         fptr(start), ptr(lengths), lengths.defined() && lengths.scalar_type() == at::kLong,
                                         code_of(q), s.B, s.L, s.H, s.K, s.V, (float)scale, ptr(o),
@@ -541,9 +542,9 @@ struct AttnNode : torch::autograd::Function<AttnNode> {
                                const Tensor& decay, const Maybe& start, const Maybe& lens, double scale,
                                bool want_last) {
     const Tensor state = start.value_or(Tensor()), lengths = lens.value_or(Tensor());
-    Tensor last;
-    Tensor o = attn_run(q, k, v, decay, state, lengths, scale, want_last ? &last : nullptr);
-    ctx->save_for_backward({q, k, v, decay, state, lengths});
+    Tensor last, states;
+    Tensor o = attn_run(q, k, v, decay, state, lengths, scale, want_last ? &last : nullptr, &states);
+    ctx->save_for_backward({q, k, v, decay, state, lengths, states});
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
     return want_last ? variable_list{o, last} : variable_list{o};
@@ -572,12 +573,12 @@ struct AttnNode : torch::autograd::Function<AttnNode> {
       // inputs are numbered without the absent ones
       if (state.defined() && ctx->needs_input_grad(4)) ds = s.state(q);
       long long n = 0;
-      const Tensor ws = s.workspace(q, &n);
+      const Tensor ws = s.workspace(q, true, &n);
       check(api.gfn_decay_attention_backward(hq.p(), hq.strides, hk.p(), hk.strides, hv.p(), hv.strides, ho.p(),
                                              ho.strides, fptr(decay), fptr(start), fptr(gl), ptr(lengths),
                                              lengths.defined() && lengths.scalar_type() == at::kLong, code_of(q), s.B,
-                                             s.L, s.H, s.K, s.V, (float)ctx->saved_data["scale"].toDouble(), ptr(dq),
-                                             ptr(dk), ptr(dv), fptr(ds), ptr(ws), n, on.stream),
+                                             s.L, s.H, s.K, s.V, (float)ctx->saved_data["scale"].toDouble(),
+                                             ptr(saved[6]), ptr(dq), ptr(dk), ptr(dv), fptr(ds), ptr(ws), n, on.stream),
             "gfn_decay_attention_backward");
     }
     return first_order({dq, dk, dv, Tensor(), ds, Tensor(), Tensor(), Tensor()}, grads, recording);
@@ -764,7 +765,7 @@ PyObject* py_decay_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
       Unlocked u;
       if (train) out = AttnNode::apply(q, k, val, decay, maybe(state), maybe(lengths), scale, want_last);
       else {
-        Tensor last, o = attn_run(q, k, val, decay, state, lengths, scale, want_last ? &last : nullptr);
+        Tensor last, o = attn_run(q, k, val, decay, state, lengths, scale, want_last ? &last : nullptr, nullptr);
         out = want_last ? variable_list{o, last} : variable_list{o};
       }
     }
