@@ -46,6 +46,10 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
+template <typename T> struct Two { using type = float2; };
+template <> struct Two<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct Two<__half> { using type = __half2; };
+
 GFN_DEV float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -104,12 +108,74 @@ GFN_DEV void lp_merge(float& m, float& s, float& u, float m2, float s2, float u2
   m = mn;
 }
 
+// The largest of a group; NaN does not count.
+template <typename T, int VEC>
+GFN_DEV float group_max(const Pack<T, VEC>& p) {
+  if constexpr (sizeof(T) == 4) {
+    float m = p.v[0];
+#pragma unroll
+    for (int e = 1; e < VEC; ++e) m = fmaxf(m, p.v[e]);
+    return m;
+  } else {
+    using T2 = typename Two<T>::type;
+    const T2* h = reinterpret_cast<const T2*>(&p);
+    T2 m = h[0];
+#pragma unroll
+    for (int e = 1; e < VEC / 2; ++e) m = __hmax2(m, h[e]);
+    return fmaxf(to_f(m.x), to_f(m.y));
+  }
+}
+
+// Adds N groups (g, g + THREADS, ...) to a thread's running maximum m, its
+// group gi, s = sum e^(x-m) and u = sum e^(x-m) (x - m).  The difference is taken
+// before the factor log2 e: in one fused step it would be off by up to half a
+// unit of |m| log2 e, and a row's only token would not have probability 1.
+template <typename T, int VEC, int N, bool ENT, bool TOP>
+GFN_DEV void lp_add(const Pack<T, VEC> (&raw)[N], int g, float& m, float& s, float& u, int& gi) {
+  float mn = m;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float gm = group_max<T, VEC>(raw[k]);
+    if (TOP && gm > mn) gi = g + k * LP_THREADS;
+    mn = fmaxf(mn, gm);
+  }
+  const float base = mn == -INFINITY ? 0.f : mn, c = exp2_fast((m - base) * LP_LOG2E);
+  if (ENT) u = c * (u + (m == -INFINITY ? 0.f : m - base) * s);
+  m = mn;
+  F2 s2 = f2(s * c, 0.f), u2 = f2(u, 0.f);
+  const F2 nb = f2(-base), l2 = f2(LP_LOG2E);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+      F2 d = f2(to_f(raw[k].v[e]), to_f(raw[k].v[e + 1])) + nb;
+      float lo, hi;
+      if (ENT) {
+        split(d, lo, hi);
+        d = f2(max_nan(lo, LP_LOW), max_nan(hi, LP_LOW));
+      }
+      split(d * l2, lo, hi);
+      const F2 ex = f2(exp2_fast(lo), exp2_fast(hi));
+      s2 = s2 + ex;
+      if (ENT) u2 = fma2(ex, d, u2);
+    }
+  }
+  float a, b;
+  split(s2, a, b);
+  s = a + b;
+  if (ENT) {
+    split(u2, a, b);
+    u = a + b;
+  }
+}
+
 struct LpShared {
   float3 warp[LP_WARPS];
   float3 part[LP_CLUSTER];                       // of every block of the row, in the first one
   unsigned long long quads[LP_QUADS];
   unsigned long long tau;
-  int count;
+  int count, holding;
+  unsigned short holders[LP_THREADS];
   unsigned long long best[LP_WARPS];
   unsigned long long cand[LP_CAP];
   unsigned long long list[LP_CLUSTER * LP_TOP];  // every block's alternatives, in the first one
@@ -134,6 +200,7 @@ GFN_DEV void lp_top(LpShared& sh, const LpRow<T>& row, int g0, int g1, int top, 
   if ((lane & 3) == 0) sh.quads[tid >> 2] = q;
   if (tid == 0) {
     sh.count = 0;
+    sh.holding = 0;
     sh.tau = 0;
   }
   __syncthreads();
@@ -146,18 +213,34 @@ GFN_DEV void lp_top(LpShared& sh, const LpRow<T>& row, int g0, int g1, int top, 
   }
   __syncthreads();
   const unsigned long long tau = sh.tau;
-  if (!odd && mine && high >= tau) {
-    for (int g = g0 + tid; g < g1; g += LP_THREADS) {
-      const Pack<T, VEC> p = row.load(g);
+  // The threads that may hold one of them, and their groups shared out to all:
+  // a thread reading its own again (the first form) kept every warp busy with
+  // a few lanes (4099 x 50257 bfloat16, 8 alternatives: 290 us against 99).
+  if (!odd && mine && high >= tau) sh.holders[atomicAdd(&sh.holding, 1)] = (unsigned short)tid;
+  __syncthreads();
+  const int per = (g1 - g0 + LP_THREADS - 1) / LP_THREADS, visits = sh.holding * per;
+  const float floor = key_value(tau);  // -inf, or 0 as a key, lets every logit through
+  for (int v = tid; v < visits; v += LP_THREADS) {
+    const int g = g0 + sh.holders[v / per] + (v % per) * LP_THREADS;
+    if (g >= g1) continue;
+    const Pack<T, VEC> p = row.load(g);
+    float f[VEC], gm = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const int i = g * VEC + e;
-        if (i < row.phase || i >= row.end) continue;
-        const unsigned long long k = rank_key(to_f(p.v[e]), (unsigned)(i - row.phase));
-        if (k < tau) continue;
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < LP_CAP) sh.cand[at] = k;
-      }
+    for (int e = 0; e < VEC; ++e) {
+      f[e] = to_f(p.v[e]);
+      gm = fmaxf(gm, f[e]);
+    }
+    if (tau && gm < floor) continue;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int j = g * VEC + e - row.phase;
+      if (j < 0 || j >= row.end - row.phase) continue;
+      // of logits of -inf, the first 64 tokens hold enough: fewer than `top` are above
+      if (f[e] == -INFINITY && j >= 2 * LP_TOP) continue;
+      const unsigned long long k = rank_key(f[e], (unsigned)j);
+      if (k < tau) continue;
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < LP_CAP) sh.cand[at] = k;
     }
   }
   __syncthreads();
@@ -206,7 +289,7 @@ GFN_DEV void lp_top(LpShared& sh, const LpRow<T>& row, int g0, int g1, int top, 
 
 template <typename T, bool ENT, bool TOP, bool SHARED_ROW>
 __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(const LpArgs p) {
-  constexpr int VEC = LpRow<T>::VEC, UNROLL = 4;
+  constexpr int VEC = LpRow<T>::VEC, UNROLL = 32 / VEC;
   __shared__ LpShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int parts = SHARED_ROW ? gridDim.y : 1, part = SHARED_ROW ? blockIdx.y : 0;  // a cluster along y
@@ -227,55 +310,18 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(const LpArgs p) {
   }
   float m = -INFINITY, s = 0.f, u = 0.f;
   int gi = g0 + tid;
-  for (int g = g0 + tid; g < g1; g += LP_THREADS * UNROLL) {
-    Pack<T, VEC> raw[UNROLL];
+  for (int g = gi; g < g1;) {
+    const int last = g + (UNROLL - 1) * LP_THREADS;
+    if (last < g1 && row.whole(g) && row.whole(last)) {
+      Pack<T, VEC> raw[UNROLL];
 #pragma unroll
-    for (int k = 0; k < UNROLL; ++k) {
-      if (g + k * LP_THREADS < g1) raw[k] = row.load(g + k * LP_THREADS);
-      else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) raw[k].v[e] = from_f<T>(-INFINITY);
-      }
-    }
-    float f[UNROLL][VEC], mn = m;
-#pragma unroll
-    for (int k = 0; k < UNROLL; ++k) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) f[k][e] = to_f(raw[k].v[e]);
-      float gm = f[k][0];
-#pragma unroll
-      for (int e = 1; e < VEC; ++e) gm = fmaxf(gm, f[k][e]);
-      if (TOP && gm > mn) gi = g + k * LP_THREADS;
-      mn = fmaxf(mn, gm);
-    }
-    const float base = mn == -INFINITY ? 0.f : mn, c = exp2_fast((m - base) * LP_LOG2E);
-    if (ENT) u = c * (u + (m == -INFINITY ? 0.f : m - base) * s);
-    s *= c;
-    m = mn;
-    F2 s2 = f2(s, 0.f), u2 = f2(u, 0.f);
-    const F2 nb = f2(-base), l2 = f2(LP_LOG2E);
-#pragma unroll
-    for (int k = 0; k < UNROLL; ++k) {
-#pragma unroll
-      for (int e = 0; e < VEC; e += 2) {
-        F2 d = f2(f[k][e], f[k][e + 1]) + nb;
-        float lo, hi;
-        if (ENT) {
-          split(d, lo, hi);
-          d = f2(max_nan(lo, LP_LOW), max_nan(hi, LP_LOW));
-        }
-        split(d * l2, lo, hi);
-        const F2 ex = f2(exp2_fast(lo), exp2_fast(hi));
-        s2 = s2 + ex;
-        if (ENT) u2 = fma2(ex, d, u2);
-      }
-    }
-    float a, b;
-    split(s2, a, b);
-    s = a + b;
-    if (ENT) {
-      split(u2, a, b);
-      u = a + b;
+      for (int k = 0; k < UNROLL; ++k) raw[k] = *reinterpret_cast<const Pack<T, VEC>*>(row.base + (long long)(g + k * LP_THREADS) * VEC);
+      lp_add<T, VEC, UNROLL, ENT, TOP>(raw, g, m, s, u, gi);
+      g += UNROLL * LP_THREADS;
+    } else {
+      const Pack<T, VEC> raw[1] = {row.load(g)};
+      lp_add<T, VEC, 1, ENT, TOP>(raw, g, m, s, u, gi);
+      g += LP_THREADS;
     }
   }
   float bm = m, bs = s, bu = u;
@@ -357,10 +403,11 @@ int lp_launch(const LpArgs& p, cudaStream_t s) {
   const int st = sm_count(&sms);
   if (st != GFN_OK) return st;
   // Few rows: up to eight blocks share one, as long as each has 8 KB to read
-  // and there are not four blocks per SM yet.
+  // and there are not two blocks per SM yet
+  // (256 x 50257 bfloat16: four blocks a row 29 us, two PARTS2).
   int parts = 1;
   const long long bytes = (long long)p.V * sizeof(T);
-  while (parts < LP_CLUSTER && p.rows * parts < 4LL * sms && bytes / (2 * parts) >= 8192) parts *= 2;
+  while (parts < LP_CLUSTER && p.rows * parts < 2LL * sms && bytes / (2 * parts) >= 8192) parts *= 2;
   if (parts == 1) {
     logprob_kernel<T, ENT, TOP, false><<<(unsigned)p.rows, LP_THREADS, 0, s>>>(p);
     return launch_status("logprob_kernel");
@@ -400,6 +447,13 @@ struct LpGradArgs {
   long long xs, rows, ignore;
   int V, top, blocks;  // blocks per row
 };
+
+GFN_DEV void store_two(float* p, float a, float b) {
+  p[0] = a;
+  p[1] = b;
+}
+GFN_DEV void store_two(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+GFN_DEV void store_two(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
 
 // A block owns THREADS * UNROLL groups of one row.  The part that every
 // element has, p_j (A + B d_j), is written in one go; then the block puts
@@ -447,22 +501,37 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_grad_kernel(const LpGradAr
   const float ge = ENT && !empty ? p.g_ent[r] : 0.f;
   const float A = ENT ? -total - ge * ((empty ? 0.f : p.ent[r]) - (empty ? 0.f : st.y)) : -total, B = -ge;
   const float nz = -st.y * LP_LOG2E;
-  auto grad = [&](float v) {
-    float d = v - st.x;
-    if (ENT) d = max_nan(d, LP_LOW);
-    const float pj = exp2_fast(fmaf(d, LP_LOG2E, nz));
-    return pj * (ENT ? fmaf(B, d, A) : A);
+  auto grad = [&](float lo, float hi, float& a, float& b) {
+    F2 d = f2(lo, hi) + f2(-st.x);
+    if (ENT) {
+      split(d, lo, hi);
+      d = f2(max_nan(lo, LP_LOW), max_nan(hi, LP_LOW));
+    }
+    split(fma2(d, f2(LP_LOG2E), f2(nz)), lo, hi);
+    split(f2(exp2_fast(lo), exp2_fast(hi)) * (ENT ? fma2(f2(B), d, f2(A)) : f2(A)), a, b);
+  };
+  auto grad1 = [&](float v) {
+    float a, b;
+    grad(v, v, a, b);
+    return a;
   };
 #pragma unroll
   for (int k = 0; k < UNROLL; ++k) {
     const int i = start + (k * LP_THREADS + tid) * VEC;
     if (i >= phase && i + VEC <= end) {
       Pack<T, VEC> o;
+      if constexpr (VEC == 1) o.v[0] = from_f<T>(grad1(to_f(raw[k].v[0])));
+      else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(grad(to_f(raw[k].v[e])));
+        for (int e = 0; e < VEC; e += 2) {
+          float a, b;
+          grad(to_f(raw[k].v[e]), to_f(raw[k].v[e + 1]), a, b);
+          store_two(&o.v[e], a, b);
+        }
+      }
       *reinterpret_cast<Pack<T, VEC>*>(dx - phase + i) = o;
     } else {
-      for (int j = max(i, phase); j < min(i + VEC, end); ++j) dx[j - phase] = from_f<T>(grad(to_f(x[j - phase])));
+      for (int j = max(i, phase); j < min(i + VEC, end); ++j) dx[j - phase] = from_f<T>(grad1(to_f(x[j - phase])));
     }
   }
   __syncthreads();
@@ -475,7 +544,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_grad_kernel(const LpGradAr
       if (i < tid) return;  // the first of the same token writes
       sum += g[i];
     }
-    dx[j] = from_f<T>(grad(to_f(x[j])) + sum);
+    dx[j] = from_f<T>(grad1(to_f(x[j])) + sum);
   }
 }
 

@@ -10,9 +10,12 @@
 // every run.  Sums are float32 and are rounded once.
 #include "lm_host.h"
 #include "lm_ops.cuh"
+#include "umma.cuh"
 
 using namespace gfn;
 using namespace gfn_abi;
+using umma::gdc_launch_dependents;
+using umma::gdc_wait;
 
 namespace {
 
@@ -139,16 +142,18 @@ int embed_forward(EmbedArgs p, cudaStream_t s) {
 // The sort: digits of up to 9 bits, least significant first.  A tile of
 // tokens is ranked by a block; where it writes a digit follows from the counts
 // of every digit in every tile, which the kernel before left in global memory.
-constexpr int SORT_THREADS = 256, SORT_WARPS = 8, SORT_ITEMS = 8, SORT_SUB = SORT_THREADS * SORT_ITEMS;
+// A key and its token travel as one 64-bit word.
+constexpr int SORT_THREADS = 256, SORT_WARPS = 8;
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILES = 256;
+constexpr int SORT_ITEMS = 4, SORT_SUB = SORT_THREADS * SORT_ITEMS;      // tokens of a thread, of a tile's part
+constexpr int SORT_ALONE = 8, SORT_ONE = SORT_THREADS * SORT_ALONE;      // where one block sorts them all
 // Tokens (in sorted order) that one group of threads sums.
 constexpr int SUM_RUN = 32, SUM_THREADS = 128, SUM_AHEAD = 8;
 
 struct SortArgs {
   const void* ids;
-  unsigned* keys[2];
-  unsigned* pos[2];
-  unsigned* counts;  // [passes][tiles][SORT_BINS]
+  uint2* sorted[2];  // (key, token)
+  unsigned* counts;  // [passes][tiles][bins]
   void* dw;
   long long dw_bytes;
   long long padding;
@@ -189,17 +194,20 @@ GFN_DEV void zero_stage(const SortArgs& p, int first, int stage, int stages) {
 
 // The counts of the first digit, and zeros for those of the later ones.
 __global__ void __launch_bounds__(SORT_THREADS) embed_count_kernel(const SortArgs p) {
+  gdc_launch_dependents();
+  gdc_wait();
   if ((int)blockIdx.x >= p.tiles) return zero_stage(p, p.tiles, 0, p.passes + 1);
   __shared__ unsigned bins[SORT_BINS];
-  for (int i = threadIdx.x; i < SORT_BINS; i += SORT_THREADS) bins[i] = 0;
+  const int n_bins = 1 << p.bits;
+  for (int i = threadIdx.x; i < n_bins; i += SORT_THREADS) bins[i] = 0;
   __syncthreads();
   const long long from = (long long)blockIdx.x * p.subs * SORT_SUB, to = min(from + (long long)p.subs * SORT_SUB, (long long)p.N);
-  const unsigned mask = (1u << p.bits) - 1;
+  const unsigned mask = n_bins - 1;
   for (long long n = from + threadIdx.x; n < to; n += SORT_THREADS) atomicAdd(&bins[sort_key(p, n, true) & mask], 1u);
   __syncthreads();
-  for (int i = threadIdx.x; i < SORT_BINS; i += SORT_THREADS) {
-    p.counts[(long long)blockIdx.x * SORT_BINS + i] = bins[i];
-    for (int q = 1; q < p.passes; ++q) p.counts[((long long)q * p.tiles + blockIdx.x) * SORT_BINS + i] = 0;
+  for (int i = threadIdx.x; i < n_bins; i += SORT_THREADS) {
+    p.counts[(long long)blockIdx.x * n_bins + i] = bins[i];
+    for (int q = 1; q < p.passes; ++q) p.counts[((long long)q * p.tiles + blockIdx.x) * n_bins + i] = 0;
   }
 }
 
@@ -221,38 +229,41 @@ GFN_DEV void scan_bins(SortShared& sh, const unsigned (&v)[2], unsigned (&out)[2
   if (lane == 31) sh.sums[warp] = inc;
   __syncthreads();
   unsigned before = 0;
-  for (int w = 0; w < warp; ++w) before += sh.sums[w];
+#pragma unroll
+  for (int w = 0; w < SORT_WARPS; ++w) before += w < warp ? sh.sums[w] : 0u;
   out[0] = before + inc - s;
   out[1] = out[0] + v[0];
   __syncthreads();
 }
 
-// Ranks SORT_SUB tokens from `from` on (below `to`) by the digit of their key
-// at `shift` and hands (key, position, place) of each to `put`; sh.next moves on.
-template <class Key, class Put>
-GFN_DEV void rank_part(SortShared& sh, long long from, long long to, unsigned shift, unsigned mask, Key key, Put put) {
+// Ranks THREADS * ITEMS tokens from `from` on (below `to`), given by `item`, by
+// the digit of their key at `shift`, and hands each with its place to `put`;
+// sh.next moves on.
+template <int ITEMS, class Item, class Put>
+GFN_DEV void rank_part(SortShared& sh, long long from, long long to, unsigned shift, unsigned mask, Item item, Put put) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < SORT_WARPS * SORT_BINS; i += SORT_THREADS) (&sh.warp[0][0])[i] = 0;
-  __syncthreads();
-  unsigned k[SORT_ITEMS], ps[SORT_ITEMS], rank[SORT_ITEMS];
+  uint2 k[ITEMS];
+  unsigned rank[ITEMS];
 #pragma unroll
-  for (int r = 0; r < SORT_ITEMS; ++r) {
-    const long long n = from + (warp * SORT_ITEMS + r) * 32 + lane;
-    k[r] = ps[r] = 0;
-    if (n < to) key(n, k[r], ps[r]);
+  for (int r = 0; r < ITEMS; ++r) {
+    const long long n = from + (warp * ITEMS + r) * 32 + lane;
+    k[r] = n < to ? item(n) : make_uint2(0u, 0u);
   }
+  for (int w = 0; w < SORT_WARPS; ++w)
+    for (int i = threadIdx.x; i <= (int)mask; i += SORT_THREADS) sh.warp[w][i] = 0;
+  __syncthreads();
 #pragma unroll
-  for (int r = 0; r < SORT_ITEMS; ++r) {
-    const long long n = from + (warp * SORT_ITEMS + r) * 32 + lane;
-    const unsigned d = n < to ? (k[r] >> shift) & mask : ~0u;
+  for (int r = 0; r < ITEMS; ++r) {
+    const bool live = from + (warp * ITEMS + r) * 32 + lane < to;
+    const unsigned d = live ? (k[r].x >> shift) & mask : ~0u;
     const unsigned same = __match_any_sync(0xffffffffu, d), before = __popc(same & ((1u << lane) - 1));
-    if (n < to) rank[r] = sh.warp[warp][d] + before;
+    rank[r] = live ? sh.warp[warp][d] + before : 0u;
     __syncwarp();
-    if (n < to && before == 0) sh.warp[warp][d] += __popc(same);
+    if (live && before == 0) sh.warp[warp][d] += __popc(same);
     __syncwarp();
   }
   __syncthreads();
-  for (int b = threadIdx.x; b < SORT_BINS; b += SORT_THREADS) {
+  for (int b = threadIdx.x; b <= (int)mask; b += SORT_THREADS) {
     unsigned at = sh.next[b];
 #pragma unroll
     for (int w = 0; w < SORT_WARPS; ++w) {
@@ -264,94 +275,81 @@ GFN_DEV void rank_part(SortShared& sh, long long from, long long to, unsigned sh
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < SORT_ITEMS; ++r) {
-    const long long n = from + (warp * SORT_ITEMS + r) * 32 + lane;
-    if (n < to) put(k[r], ps[r], sh.warp[warp][(k[r] >> shift) & mask] + rank[r]);
-  }
+  for (int r = 0; r < ITEMS; ++r)
+    if (from + (warp * ITEMS + r) * 32 + lane < to) put(k[r], sh.warp[warp][(k[r].x >> shift) & mask] + rank[r]);
   __syncthreads();
 }
 
 // One digit of the sort.  The counts of the next digit are collected on the way.
 __global__ void __launch_bounds__(SORT_THREADS) embed_rank_kernel(const SortArgs p, int pass) {
+  gdc_launch_dependents();
+  gdc_wait();
   if ((int)blockIdx.x >= p.tiles) return zero_stage(p, p.tiles, pass + 1, p.passes + 1);
   __shared__ SortShared sh;
-  const unsigned mask = (1u << p.bits) - 1, shift = pass * p.bits;
-  const unsigned* counts = p.counts + (long long)pass * p.tiles * SORT_BINS;
+  const int n_bins = 1 << p.bits;
+  const unsigned mask = n_bins - 1, shift = pass * p.bits;
+  const unsigned* counts = p.counts + (long long)pass * p.tiles * n_bins;
   unsigned total[2] = {0, 0}, before[2] = {0, 0}, start[2];
-#pragma unroll 8
-  for (int t = 0; t < p.tiles; ++t) {
-    const uint2 c = reinterpret_cast<const uint2*>(counts + (long long)t * SORT_BINS)[threadIdx.x];
-    total[0] += c.x;
-    total[1] += c.y;
-    if (t < (int)blockIdx.x) {
-      before[0] += c.x;
-      before[1] += c.y;
+  if ((int)threadIdx.x < n_bins / 2) {
+#pragma unroll 16
+    for (int t = 0; t < p.tiles; ++t) {
+      const uint2 c = reinterpret_cast<const uint2*>(counts + (long long)t * n_bins)[threadIdx.x];
+      total[0] += c.x;
+      total[1] += c.y;
+      if (t < (int)blockIdx.x) {
+        before[0] += c.x;
+        before[1] += c.y;
+      }
     }
   }
   scan_bins(sh, total, start);
   sh.next[2 * threadIdx.x] = start[0] + before[0];
   sh.next[2 * threadIdx.x + 1] = start[1] + before[1];
-  __syncthreads();
   const long long from = (long long)blockIdx.x * p.subs * SORT_SUB, to = min(from + (long long)p.subs * SORT_SUB, (long long)p.N);
-  const unsigned *ki = p.keys[(pass + 1) & 1], *pi = p.pos[(pass + 1) & 1];
-  unsigned *ko = p.keys[pass & 1], *po = p.pos[pass & 1];
-  unsigned* following = pass + 1 < p.passes ? p.counts + (long long)(pass + 1) * p.tiles * SORT_BINS : nullptr;
+  const uint2* in = pass & 1 ? p.sorted[0] : p.sorted[1];
+  uint2* out = pass & 1 ? p.sorted[1] : p.sorted[0];
+  unsigned* following = pass + 1 < p.passes ? p.counts + (long long)(pass + 1) * p.tiles * n_bins : nullptr;
   for (long long at = from; at < to; at += SORT_SUB)
-    rank_part(sh, at, to, shift, mask,
-              [&](long long n, unsigned& k, unsigned& ps) {
-                if (pass == 0) {
-                  k = sort_key(p, n, false);
-                  ps = (unsigned)n;
-                } else {
-                  k = ki[n];
-                  ps = pi[n];
-                }
-              },
-              [&](unsigned k, unsigned ps, unsigned place) {
-                ko[place] = k;
-                po[place] = ps;
-                if (following) atomicAdd(&following[(place / (p.subs * SORT_SUB)) * SORT_BINS + ((k >> (shift + p.bits)) & mask)], 1u);
-              });
+    rank_part<SORT_ITEMS>(
+        sh, at, to, shift, mask,
+        [&](long long n) { return pass == 0 ? make_uint2(sort_key(p, n, false), (unsigned)n) : in[n]; },
+        [&](uint2 k, unsigned place) {
+          out[place] = k;
+          if (following) atomicAdd(&following[(place / (p.subs * SORT_SUB)) * n_bins + ((k.x >> (shift + p.bits)) & mask)], 1u);
+        });
 }
 
-// The whole sort of up to SORT_SUB tokens by one block; the others fill zeros.
+// The whole sort of up to SORT_ONE tokens by one block; the others fill zeros.
 __global__ void __launch_bounds__(SORT_THREADS) embed_sort_kernel(const SortArgs p) {
+  gdc_launch_dependents();
+  gdc_wait();
   if (blockIdx.x >= 1) return zero_stage(p, 1, 0, 1);
   __shared__ SortShared sh;
-  __shared__ unsigned keys[SORT_SUB], pos[SORT_SUB];
-  const unsigned mask = (1u << p.bits) - 1;
-  for (int n = threadIdx.x; n < p.N; n += SORT_THREADS) {
-    keys[n] = sort_key(p, n, true);
-    pos[n] = n;
-  }
+  __shared__ uint2 items[SORT_ONE];
+  const int n_bins = 1 << p.bits;
+  const unsigned mask = n_bins - 1;
+  for (int n = threadIdx.x; n < p.N; n += SORT_THREADS) items[n] = make_uint2(sort_key(p, n, true), n);
+  uint2* out = (p.passes - 1) & 1 ? p.sorted[1] : p.sorted[0];
   for (int pass = 0; pass < p.passes; ++pass) {
     const unsigned shift = pass * p.bits;
     for (int i = threadIdx.x; i < SORT_BINS; i += SORT_THREADS) sh.next[i] = 0;
     __syncthreads();
-    for (int n = threadIdx.x; n < p.N; n += SORT_THREADS) atomicAdd(&sh.next[(keys[n] >> shift) & mask], 1u);
+    for (int n = threadIdx.x; n < p.N; n += SORT_THREADS) atomicAdd(&sh.next[(items[n].x >> shift) & mask], 1u);
     __syncthreads();
     const unsigned v[2] = {sh.next[2 * threadIdx.x], sh.next[2 * threadIdx.x + 1]};
     unsigned start[2];
     scan_bins(sh, v, start);
     sh.next[2 * threadIdx.x] = start[0];
     sh.next[2 * threadIdx.x + 1] = start[1];
-    __syncthreads();
     const bool last = pass == p.passes - 1;
-    rank_part(sh, 0, p.N, shift, mask,
-              [&](long long n, unsigned& k, unsigned& ps) {
-                k = keys[n];
-                ps = pos[n];
-              },
-              [&](unsigned k, unsigned ps, unsigned place) {  // every thread has read its own by now
-                (last ? p.keys[(p.passes - 1) & 1] : keys)[place] = k;
-                (last ? p.pos[(p.passes - 1) & 1] : pos)[place] = ps;
-              });
+    rank_part<SORT_ALONE>(
+        sh, 0, p.N, shift, mask, [&](long long n) { return items[n]; },
+        [&](uint2 k, unsigned place) { (last ? out : items)[place] = k; });  // every thread has read its own by now
   }
 }
 
 struct SumArgs {
-  const unsigned* keys;
-  const unsigned* pos;
+  const uint2* sorted;  // (key, token)
   const void* dy;
   void* dw;
   float* part;  // [runs][2][D]: what a run's first and last row have of a row that goes on in the neighbour
@@ -366,6 +364,8 @@ struct SumArgs {
 // and go to `part`.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const SumArgs p) {
+  gdc_launch_dependents();
+  gdc_wait();
   extern __shared__ unsigned sum_shared[];
   unsigned* key = sum_shared + threadIdx.y * (2 * SUM_RUN + 2) + 1;  // key[-1] .. key[SUM_RUN]
   unsigned* pos = key + SUM_RUN + 1;
@@ -373,8 +373,9 @@ __global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const SumArgs p)
   const unsigned none = (unsigned)p.V;
   for (int i = (int)threadIdx.x - 1; i <= SUM_RUN; i += blockDim.x) {
     const long long n = from + i;
-    key[i] = n >= 0 && n < p.N ? p.keys[n] : n < 0 ? ~0u : none;
-    if (i >= 0 && i < SUM_RUN) pos[i] = n < p.N ? p.pos[n] : 0u;
+    const uint2 k = n >= 0 && n < p.N ? p.sorted[n] : make_uint2(n < 0 ? ~0u : none, 0u);
+    key[i] = k.x;
+    if (i >= 0 && i < SUM_RUN) pos[i] = k.y;
   }
   __syncthreads();
   const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
@@ -416,36 +417,71 @@ __global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const SumArgs p)
 }
 
 // Rows shared by several groups of SUM_RUN tokens: the group in which such a
-// row begins adds the parts, eight interleaved sums joined in a fixed order.  A
-// block looks at JOIN_RUNS groups and adds what begins there over JOIN_COLS
-// columns.
-constexpr int JOIN_RUNS = 8, JOIN_COLS = 128;
+// row begins adds the parts over JOIN_COLS columns.  A warp looks at one group
+// and adds a row of up to JOIN_SHORT parts by itself; longer ones are added by
+// the whole block, in eight interleaved sums.
+constexpr int JOIN_RUNS = 8, JOIN_COLS = 128, JOIN_SHORT = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * JOIN_RUNS) embed_join_kernel(const SumArgs p) {
+  gdc_wait();
+  constexpr int PER = JOIN_COLS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long runs = ((long long)p.N + SUM_RUN - 1) / SUM_RUN, base = (long long)blockIdx.x * JOIN_RUNS;
   __shared__ unsigned row[JOIN_RUNS];
   __shared__ long long stop[JOIN_RUNS];  // behind the last run whose first token is the row's
   __shared__ float sums[JOIN_RUNS][JOIN_COLS];
+  auto first_part = [&](long long run, int from, float (&acc)[PER]) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int col = from + lane + 32 * j;
+      acc[j] = col < p.D ? p.part[(run * 2 + 1) * p.D + col] : 0.f;
+    }
+  };
+  auto add_parts = [&](long long r, long long end, int step, int from, float (&acc)[PER]) {
+#pragma unroll 4
+    for (; r < end; r += step) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int col = from + lane + 32 * j;
+        if (col < p.D) acc[j] += p.part[r * 2 * p.D + col];
+      }
+    }
+  };
   {
     const long long run = base + warp, from = run * SUM_RUN, end = from + SUM_RUN;
     unsigned k = p.V;
     if (end < p.N) {
-      k = p.keys[end - 1];
-      if (p.keys[end] != k || (p.keys[from] == k && from > 0 && p.keys[from - 1] == k)) k = p.V;
+      k = p.sorted[end - 1].x;
+      const unsigned next = p.sorted[end].x, begin = p.sorted[from].x, before = from > 0 ? p.sorted[from - 1].x : ~0u;
+      if (next != k || (begin == k && before == k)) k = p.V;
     }
+    bool wide = false;
     if (k < (unsigned)p.V) {
       long long last = run + 1;
       for (;;) {
         const long long r = last + lane;
-        const int n = __popc(__ballot_sync(0xffffffffu, r < runs && p.keys[r * SUM_RUN] == k));  // sorted: they come first
+        const int n = __popc(__ballot_sync(0xffffffffu, r < runs && p.sorted[r * SUM_RUN].x == k));  // sorted: they come first
         last += n;
         if (n < 32) break;
       }
-      if (lane == 0) stop[warp] = last;
+      wide = last - run > JOIN_SHORT;
+      if (wide) {
+        if (lane == 0) stop[warp] = last;
+      } else {
+        for (int at = blockIdx.y * JOIN_COLS; at < p.D; at += gridDim.y * JOIN_COLS) {
+          float acc[PER];
+          first_part(run, at, acc);
+          add_parts(run + 1, last, 1, at, acc);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const int col = at + lane + 32 * j;
+            if (col < p.D) static_cast<T*>(p.dw)[(long long)k * p.D + col] = from_f<T>(acc[j] * p.scale);
+          }
+        }
+      }
     }
-    if (lane == 0) row[warp] = k;
+    if (lane == 0) row[warp] = wide ? k : (unsigned)p.V;
   }
   __syncthreads();
   for (int w = 0; w < JOIN_RUNS; ++w) {
@@ -453,22 +489,11 @@ __global__ void __launch_bounds__(32 * JOIN_RUNS) embed_join_kernel(const SumArg
     if (k >= (unsigned)p.V) continue;
     const long long run = base + w, last = stop[w];
     for (int from = blockIdx.y * JOIN_COLS; from < p.D; from += gridDim.y * JOIN_COLS) {
-      float acc[JOIN_COLS / 32];
+      float acc[PER] = {};
+      if (warp == 0) first_part(run, from, acc);
+      add_parts(run + 1 + warp, last, JOIN_RUNS, from, acc);
 #pragma unroll
-      for (int j = 0; j < JOIN_COLS / 32; ++j) {
-        const int col = from + lane + 32 * j;
-        acc[j] = warp == 0 && col < p.D ? p.part[(run * 2 + 1) * p.D + col] : 0.f;
-      }
-#pragma unroll 4
-      for (long long r = run + 1 + warp; r < last; r += JOIN_RUNS) {
-#pragma unroll
-        for (int j = 0; j < JOIN_COLS / 32; ++j) {
-          const int col = from + lane + 32 * j;
-          if (col < p.D) acc[j] += p.part[r * 2 * p.D + col];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < JOIN_COLS / 32; ++j) sums[warp][lane + 32 * j] = acc[j];
+      for (int j = 0; j < PER; ++j) sums[warp][lane + 32 * j] = acc[j];
       __syncthreads();
       if (threadIdx.x < JOIN_COLS && from + (int)threadIdx.x < p.D) {
         float t = sums[0][threadIdx.x];
@@ -484,7 +509,7 @@ __global__ void __launch_bounds__(32 * JOIN_RUNS) embed_join_kernel(const SumArg
 // How the tokens are divided and where the workspace holds what.
 struct Plan {
   int bits, passes, tiles, subs;
-  long long runs, keys, counts, part, bytes;
+  long long runs, items, counts, part, bytes;
 };
 Plan embed_plan(long long N, int V, int D) {
   Plan q = {};
@@ -498,11 +523,29 @@ Plan embed_plan(long long N, int V, int D) {
   q.tiles = (int)((parts + q.subs - 1) / q.subs);
   q.runs = (N + SUM_RUN - 1) / SUM_RUN;
   auto up = [](long long b) { return (b + 255) / 256 * 256; };
-  q.keys = up(4 * N);
-  q.counts = 4 * q.keys;
-  q.part = q.counts + (parts > 1 ? up(4LL * q.passes * q.tiles * SORT_BINS) : 0);
+  q.items = up(8 * N);
+  q.counts = 2 * q.items;
+  q.part = q.counts + up(4LL * q.passes * q.tiles << q.bits);
   q.bytes = q.part + up(8 * q.runs * D);
   return q;
+}
+
+// A launch that may start while the one before it on the stream ends: the
+// kernels wait for that one's results before they touch memory.
+template <class... Args, class... Given>
+int chain(void (*kernel)(Args...), dim3 grid, dim3 block, int shared, cudaStream_t s, const char* what, const Given&... given) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = (size_t)shared;
+  cfg.stream = s;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, given...);
+  return e == cudaSuccess ? GFN_OK : cuda_status(e, what);
 }
 
 template <typename T>
@@ -516,14 +559,12 @@ int embed_sum(const SumArgs& p, long long runs, cudaStream_t s) {
   const dim3 grid((unsigned)((runs + block.y - 1) / block.y), (unsigned)((need + lanes - 1) / lanes));
   if (grid.y > 65535) return fail(GFN_ERR_UNSUPPORTED, "token_embed backward: dim %d", p.D);
   const int shared = (int)block.y * (2 * SUM_RUN + 2) * 4;
-  if (vec) embed_sum_kernel<T, VEC><<<grid, block, shared, s>>>(p);
-  else embed_sum_kernel<T, 1><<<grid, block, shared, s>>>(p);
-  const int st = launch_status("embed_sum_kernel");
+  const int st = vec ? chain(embed_sum_kernel<T, VEC>, grid, block, shared, s, "embed_sum_kernel", p)
+                     : chain(embed_sum_kernel<T, 1>, grid, block, shared, s, "embed_sum_kernel", p);
   if (st != GFN_OK || runs < 2) return st;
   const int cols = (p.D + JOIN_COLS - 1) / JOIN_COLS;
   const dim3 joins((unsigned)((runs + JOIN_RUNS - 1) / JOIN_RUNS), (unsigned)(cols < 65535 ? cols : 65535));
-  embed_join_kernel<T><<<joins, 32 * JOIN_RUNS, 0, s>>>(p);
-  return launch_status("embed_join_kernel");
+  return chain(embed_join_kernel<T>, joins, 32 * JOIN_RUNS, 0, s, "embed_join_kernel", p);
 }
 
 }  // namespace
@@ -582,28 +623,24 @@ int gfn_token_embed_backward(const void* ids, int ids_are_64, long long tokens, 
   char* ws = static_cast<char*>(workspace);
   SortArgs a = {};
   a.ids = ids;
-  a.keys[0] = reinterpret_cast<unsigned*>(ws);
-  a.keys[1] = reinterpret_cast<unsigned*>(ws + q.keys);
-  a.pos[0] = reinterpret_cast<unsigned*>(ws + 2 * q.keys);
-  a.pos[1] = reinterpret_cast<unsigned*>(ws + 3 * q.keys);
+  a.sorted[0] = reinterpret_cast<uint2*>(ws);
+  a.sorted[1] = reinterpret_cast<uint2*>(ws + q.items);
   a.counts = reinterpret_cast<unsigned*>(ws + q.counts);
   a.dw = dweight; a.dw_bytes = dw_bytes; a.padding = padding_id;
   a.N = (int)tokens; a.V = vocab; a.wide = ids_are_64 != 0;
   a.tiles = q.tiles; a.subs = q.subs; a.bits = q.bits; a.passes = q.passes;
   const unsigned fill = (unsigned)(4 * sms);
-  if (tokens <= SORT_SUB) {
-    embed_sort_kernel<<<1 + fill, SORT_THREADS, 0, s>>>(a);
-    if ((st = launch_status("embed_sort_kernel")) != GFN_OK) return st;
+  if (tokens <= SORT_ONE) {
+    if ((st = chain(embed_sort_kernel, 1 + fill, SORT_THREADS, 0, s, "embed_sort_kernel", a)) != GFN_OK) return st;
   } else {
-    embed_count_kernel<<<(unsigned)q.tiles + fill, SORT_THREADS, 0, s>>>(a);
-    if ((st = launch_status("embed_count_kernel")) != GFN_OK) return st;
-    for (int pass = 0; pass < q.passes; ++pass) {
-      embed_rank_kernel<<<(unsigned)q.tiles + fill, SORT_THREADS, 0, s>>>(a, pass);
-      if ((st = launch_status("embed_rank_kernel")) != GFN_OK) return st;
-    }
+    if ((st = chain(embed_count_kernel, (unsigned)q.tiles + fill, SORT_THREADS, 0, s, "embed_count_kernel", a)) != GFN_OK)
+      return st;
+    for (int pass = 0; pass < q.passes; ++pass)
+      if ((st = chain(embed_rank_kernel, (unsigned)q.tiles + fill, SORT_THREADS, 0, s, "embed_rank_kernel", a, pass)) != GFN_OK)
+        return st;
   }
   SumArgs b = {};
-  b.keys = a.keys[(q.passes - 1) & 1]; b.pos = a.pos[(q.passes - 1) & 1];
+  b.sorted = a.sorted[(q.passes - 1) & 1];
   b.dy = dy; b.dw = dweight; b.part = reinterpret_cast<float*>(ws + q.part);
   b.ds = dy_row_stride; b.N = a.N; b.V = vocab; b.D = dim; b.scale = scale;
   if (dtype == GFN_F32) return embed_sum<float>(b, q.runs, s);
