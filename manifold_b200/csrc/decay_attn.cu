@@ -1,5 +1,7 @@
 // Linear attention with a decay for each head: the entry points, and how
 // sequences are cut.  The kernels are in decay_attn.cuh.
+#include <initializer_list>
+
 #include "decay_attn.h"
 #include "lm_host.h"
 
@@ -31,9 +33,16 @@ Cut cut(Kind kind, int dtype, int batch, int length, int heads, int kd, int vd, 
   return {(int)(per * SEG_UNIT), (int)((units + per - 1) / per)};
 }
 
-bool pieces16(const View& v, int dim, int size) {
-  const long long per = 16 / size;
-  return aligned16(v.p) && dim % per == 0 && v.sb % per == 0 && v.sl % per == 0 && v.sh % per == 0;
+// The largest piece, up to 16 bytes, that rows of `v` divide into and start on.
+int piece_of(const View& v, int dim, int size) {
+  unsigned long long all = reinterpret_cast<uintptr_t>(v.p) | 16ull;
+  for (const long long n : {(long long)dim, v.sb, v.sl, v.sh}) all |= (unsigned long long)(n < 0 ? -n : n) * size;
+  return (int)(all & (~all + 1));
+}
+int smallest(std::initializer_list<int> pieces) {
+  int n = 16;
+  for (const int q : pieces) n = q < n ? q : n;
+  return n;
 }
 
 int attn_check(const char* what, int dtype, int batch, int length, int heads, int kdim, int vdim, bool null) {
@@ -103,7 +112,7 @@ int gfn_decay_attention_forward(const void* q, const long long* q_strides, const
   if (!enough(workspace, workspace_bytes, c.floats(batch, heads, kdim, vdim)))
     return fail(GFN_ERR_INVALID, "decay_attention: a workspace of gfn_decay_attention_workspace_bytes is needed");
   const int size = dtype == GFN_F32 ? 4 : 2;
-  p.vec = pieces16(p.a, kdim, size) && pieces16(p.b, kdim, size) && pieces16(p.c, vdim, size);
+  p.piece = smallest({piece_of(p.a, kdim, size), piece_of(p.b, kdim, size), piece_of(p.c, vdim, size)});
   return dtype == GFN_F32 ? forward_f32(p, false, s) : dtype == GFN_BF16 ? forward_bf16(p, false, s) : forward_f16(p, false, s);
 }
 
@@ -125,7 +134,7 @@ int gfn_decay_attention_backward(const void* q, const long long* q_strides, cons
   PassArgs p = {};
   p.decay = decay; p.lengths = lengths; p.lengths64 = lengths_are_64; p.B = batch; p.L = length; p.H = heads;
   const int size = dtype == GFN_F32 ? 4 : 2;
-  p.vec = pieces16(vq, kdim, size) && pieces16(vk, kdim, size) && pieces16(vv, vdim, size) && pieces16(vo, vdim, size);
+  p.piece = smallest({piece_of(vq, kdim, size), piece_of(vk, kdim, size), piece_of(vv, vdim, size), piece_of(vo, vdim, size)});
   // dq, over the forward pass's segments: its states serve again, transposed
   const Cut cf = cut(OUTPUT, dtype, batch, length, heads, kdim, vdim, sms);
   const Cut cr = cut(PAIR, dtype, batch, length, heads, kdim, vdim, sms);

@@ -119,11 +119,11 @@ GFN_DEV void mma(float (&c)[4], const typename Math<T>::A& a, const typename Mat
 
 GFN_DEV void ldsm(unsigned& a, unsigned& b, unsigned& c, unsigned& d, const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(p)) : "memory");
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(p)));
 }
 GFN_DEV void ldsm_t(unsigned& a, unsigned& b, unsigned& c, unsigned& d, const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(p)) : "memory");
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(p)));
 }
 GFN_DEV float2 pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
 GFN_DEV float2 pair(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
@@ -207,44 +207,75 @@ struct Shape {
   static constexpr int TK = C * LDK, TV = C * LDV;  // elements of an operand
   static constexpr int STATE_BYTES = DK * LS * (int)sizeof(typename Math<T>::State);
   static constexpr int stage(int kind) { return kind == STATE ? TK + TV : kind == OUTPUT ? 2 * TK + TV : 2 * TK + 2 * TV; }
-  // the state's operand form twice where that fits: one barrier per block instead of two
+  // thread blocks of an SM that registers allow
+  static constexpr int most(int kind) {
+    return WIDE ? (DK + DV < 256 ? 2 : 1) : kind == STATE ? 4 : kind == PAIR && sizeof(T) < 4 ? 2 : 3;
+  }
+  static constexpr int need(int kind, int stages, int buffers) {
+    return stages * stage(kind) * (int)sizeof(T) + buffers * STATE_BYTES + 8 * C;
+  }
+  static constexpr int fit(int kind, int stages, int buffers) {
+    const int n = 228 * 1024 / (need(kind, stages, buffers) + 1024);
+    return n < most(kind) ? n : most(kind);
+  }
+  // Operands of two blocks of tokens (one on its way) unless one alone lets an
+  // SM hold more thread blocks; the state's operand form twice where that costs
+  // none: then a block of tokens takes one barrier instead of two.
+  static constexpr int stages(int kind) { return kind == STATE || fit(kind, 2, 1) >= fit(kind, 1, 1) ? 2 : 1; }
   static constexpr int buffers(int kind) {
-    return kind == STATE ? 0 : 2 * stage(kind) * (int)sizeof(T) + 2 * STATE_BYTES + 8 * C <= 227 * 1024 ? 2 : 1;
+    return kind == STATE ? 0 : stages(kind) == 2 && fit(kind, 2, 2) >= fit(kind, 2, 1) ? 2 : 1;
   }
-  static constexpr int bytes(int kind) {
-    return 2 * stage(kind) * (int)sizeof(T) + buffers(kind) * STATE_BYTES + 8 * C;
-  }
-  static constexpr int resident(int kind) {
-    const int fit = 228 * 1024 / (bytes(kind) + 1024), most = WIDE ? 1 : kind == STATE ? 4 : kind == PAIR && sizeof(T) < 4 ? 2 : 3;
-    return fit < most ? fit : most;
-  }
+  static constexpr int bytes(int kind) { return need(kind, stages(kind), buffers(kind)); }
+  static constexpr int resident(int kind) { return fit(kind, stages(kind), buffers(kind)); }
 };
 
 // Brings rows 0 .. n - 1 of a block into shared memory, zeros behind them; row
 // r is the r-th token from `at` on (BACK: from there to the front).  Columns
 // from `dim` on were zeroed once and stay so.
-template <typename T, int D, int LD, int C, int THREADS, bool BACK>
-GFN_DEV void fetch(T* dst, const View& v, int b, int h, int dim, int at, int n, int vec) {
-  const T* src = static_cast<const T*>(v.p) + b * v.sb + h * v.sh + at * v.sl;
-  if (vec) {
-    constexpr int PER = 16 / sizeof(T), LANES = D / PER, STEP = THREADS / LANES;
-    const int col = (threadIdx.x % LANES) * PER, r0 = threadIdx.x / LANES;
-    if (col >= dim) return;
-    const T* from = src + col + (BACK ? -r0 : r0) * v.sl;
-    const long long step = (BACK ? -STEP : STEP) * v.sl;
-    const uint32_t to = smem_u32(dst + r0 * LD + col);
+template <int BYTES>
+GFN_DEV void copy_async(uint32_t to, const void* from, int read) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(read) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(read) : "memory");
+}
+template <typename T, int D, int LD, int C, int THREADS, bool BACK, int BYTES>
+GFN_DEV void fetch_pieces(T* dst, const T* src, const void* any, long long sl, int dim, int n) {
+  constexpr int PER = BYTES / sizeof(T), ROW = D / PER, LANES = ROW < THREADS ? ROW : THREADS, STEP = THREADS / LANES;
+  const int col = (threadIdx.x % LANES) * PER, r0 = threadIdx.x / LANES;
+  if (col >= dim) return;
+  const T* from = src + col + (BACK ? -r0 : r0) * sl;
+  const long long step = (BACK ? -STEP : STEP) * sl;
+  const uint32_t to = smem_u32(dst + r0 * LD + col);
 #pragma unroll
-    for (int i = 0; i < C / STEP; ++i) {
-      const bool live = r0 + i * STEP < n;  // others are filled with zeros: 0 bytes are read
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * STEP * LD * (int)sizeof(T)),
-                   "l"(live ? from : static_cast<const T*>(v.p)), "r"(live ? 16 : 0)
-                   : "memory");
-      from += step;
-    }
-  } else {
-    for (int i = threadIdx.x; i < C * D; i += THREADS) {
-      const int r = i / D, col = i % D;
-      if (col < dim) dst[r * LD + col] = r < n ? src[(BACK ? -r : r) * v.sl + col] : from_f<T>(0.f);
+  for (int i = 0; i < C / STEP; ++i) {
+    const bool live = r0 + i * STEP < n;  // others are filled with zeros: 0 bytes are read
+    copy_async<BYTES>(to + i * STEP * LD * (int)sizeof(T), live ? from : any, live ? BYTES : 0);
+    from += step;
+  }
+}
+template <typename T, int D, int LD, int C, int THREADS, bool BACK, bool FULL>
+GFN_DEV void fetch(T* dst, const View& v, int b, int h, int dim, int at, int n, int piece) {
+  const T* src = static_cast<const T*>(v.p) + b * v.sb + h * v.sh + at * v.sl;
+  if (FULL || piece == 16) fetch_pieces<T, D, LD, C, THREADS, BACK, 16>(dst, src, v.p, v.sl, dim, n);
+  else if (piece == 8) fetch_pieces<T, D, LD, C, THREADS, BACK, 8>(dst, src, v.p, v.sl, dim, n);
+  else if (piece == 4) fetch_pieces<T, D, LD, C, THREADS, BACK, 4>(dst, src, v.p, v.sl, dim, n);
+  else {  // 16-bit elements at odd places
+    constexpr int AHEAD = 8, COUNT = C * D / THREADS;
+    static_assert(COUNT % AHEAD == 0, "");
+#pragma unroll 1
+    for (int i0 = 0; i0 < COUNT; i0 += AHEAD) {
+      T e[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = (i0 + u) * THREADS + threadIdx.x, r = i / D, col = i % D;
+        e[u] = col < dim && r < n ? src[(BACK ? -r : r) * v.sl + col] : from_f<T>(0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = (i0 + u) * THREADS + threadIdx.x, r = i / D, col = i % D;
+        if (col < dim) dst[r * LD + col] = e[u];
+      }
     }
   }
 }
@@ -267,12 +298,100 @@ struct Decay {
   }
 };
 
+// attend (see attend_tf32) for bfloat16: the keys' tiles of 16 one after the other, from
+// the diagonal back, so that eight scores are in registers instead of a row of
+// them and no branch stands within a tile.
+template <int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
+GFN_DEV void attend_bf16(float (&o)[ON][4], const __nv_bfloat16* rows, const __nv_bfloat16* keys, const __nv_bfloat16* values,
+                         const __nv_bfloat16* st, int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
+  using T = __nv_bfloat16;
+  using M = Math<T>;
+  constexpr int KN = DA / 16;
+  const int lane = threadIdx.x & 31;
+  M::A a[KN];
+#pragma unroll
+  for (int k = 0; k < KN; ++k) load_a<T>(a[k], rows + rt * 16 * LDA + k * 16, LDA, lane);
+#pragma unroll
+  for (int i = 0; i < ON; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < KN; ++k) {
+    if (!FULL && k * 16 >= kd) continue;
+#pragma unroll
+    for (int i = 0; i < ON; i += 2) {
+      const int col = col0 + i * 8;
+      if (!FULL && col >= nd) continue;
+      M::B b[2];
+      if (NMAJOR) load_bn<T>(b, st + col * LS + k * 16, LS, lane);
+      else load_bk<T>(b, st + k * 16 * LS + col, LS, lane);
+      mma<T>(o[i], a[k], b[0]);
+      mma<T>(o[i + 1], a[k], b[1]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ON; ++i) {
+    o[i][0] *= w0;
+    o[i][1] *= w0;
+    o[i][2] *= w1;
+    o[i][3] *= w1;
+  }
+  auto scores = [&](int i, float (&s)[2][4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KN; ++k) {
+      if (!FULL && k * 16 >= kd) continue;
+      M::B b[2];
+      load_bn<T>(b, keys + i * 16 * LDA + k * 16, LDA, lane);
+      mma<T>(s[0], a[k], b[0]);
+      mma<T>(s[1], a[k], b[1]);
+    }
+  };
+  auto add = [&](int i, const float (&s)[2][4]) {
+    M::A p;
+    p.v[0] = pack_bf16(s[0][0], s[0][1]);
+    p.v[1] = pack_bf16(s[0][2], s[0][3]);
+    p.v[2] = pack_bf16(s[1][0], s[1][1]);
+    p.v[3] = pack_bf16(s[1][2], s[1][3]);
+#pragma unroll
+    for (int n = 0; n < ON; n += 2) {
+      if (!FULL && col0 + n * 8 >= nd) continue;
+      M::B b[2];
+      load_bk<T>(b, values + i * 16 * LDB + col0 + n * 8, LDB, lane);
+      mma<T>(o[n], p, b[0]);
+      mma<T>(o[n + 1], p, b[1]);
+    }
+  };
+  float s[2][4];
+  scores(rt, s);
+#pragma unroll
+  for (int z = 0; z < 2; ++z)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[z][e] = g.diag[z][e] == 0.f ? 0.f : s[z][e] * g.diag[z][e];
+  add(rt, s);
+  F2 f0 = f2(g.first[0], g.first[1]), f1 = f2(g.first[2], g.first[3]);
+  const F2 g8 = f2(g.g8);
+#pragma unroll 2
+  for (int i = rt - 1; i >= 0; --i) {
+    scores(i, s);
+#pragma unroll
+    for (int z = 1; z >= 0; --z) {
+      split(f2(s[z][0], s[z][1]) * f0, s[z][0], s[z][1]);
+      split(f2(s[z][2], s[z][3]) * f1, s[z][2], s[z][3]);
+      f0 = f0 * g8;
+      f1 = f1 * g8;
+    }
+    add(i, s);
+  }
+}
+
 // One warp's 16 rows of a block's output: ON tiles of 8 columns from col0.
 // rows, keys [C][LDA] with kd of their columns in use, values [C][LDB]; st: the
 // state, seen from this product as [k][n] or (NMAJOR) [n][k].
-template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR>
-GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
-                    int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
+template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
+GFN_DEV void attend_tf32(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
+                         int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
   using M = Math<T>;
   const int lane = threadIdx.x & 31;
   float s[C / 8][4];
@@ -286,13 +405,13 @@ GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* va
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 #pragma unroll
   for (int k = 0; k < DA; k += M::KS) {
-    if (k >= kd) continue;
+    if (!FULL && k >= kd) continue;
     typename M::A a;
     load_a<T>(a, rows + rt * 16 * LDA + k, LDA, lane);
 #pragma unroll
     for (int i = 0; i < ON; i += 2) {
       const int col = col0 + i * 8;
-      if (col >= nd) continue;
+      if (!FULL && col >= nd) continue;
       typename M::B b[2];
       if (NMAJOR) load_bn<T>(b, st + col * LS + k, LS, lane);
       else load_bk<T>(b, st + k * LS + col, LS, lane);
@@ -358,7 +477,7 @@ GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* va
       const T* v = values + (16 * i + M::KS * q) * LDB + col0;
 #pragma unroll
       for (int n = 0; n < ON; n += 2) {
-        if (col0 + n * 8 >= nd) continue;
+        if (!FULL && col0 + n * 8 >= nd) continue;
         typename M::B b[2];
         load_bk<T>(b, v + n * 8, LDB, lane);
         mma<T>(o[n], a, b[0]);
@@ -368,29 +487,42 @@ GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* va
   }
 }
 
-// Two values in three bfloat16 pieces each, which add up to them exactly.
-GFN_DEV void split3(float x, float y, unsigned& hi, unsigned& mid, unsigned& lo) {
-  auto cut = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
+template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
+GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
+                    int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
+  if constexpr (Math<T>::KS == 16)
+    attend_bf16<DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
+  else
+    attend_tf32<T, C, DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
+}
+
+// Two values in three bfloat16 pieces each (cut, not rounded), which add up to
+// them exactly.
+GFN_DEV void split3(F2 v, unsigned& hi, unsigned& mid, unsigned& lo) {
+  auto cut = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); };
   auto both = [](float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); };
+  float x, y;
+  split(v, x, y);
   hi = both(x, y);
-  x -= cut(x);
-  y -= cut(y);
+  v = v + f2(-cut(x), -cut(y));
+  split(v, x, y);
   mid = both(x, y);
-  lo = both(x - cut(x), y - cut(y));
+  split(v + f2(-cut(x), -cut(y)), x, y);
+  lo = both(x, y);
 }
 
 // st = gn st + (diag(wt) keys)^T values for one warp's 16 rows (from m0) and N
 // tiles of columns (from n0) of the state.  The products of a block are summed
 // by themselves and then added, since the tensor cores cut where float32
 // addition rounds: over a long sequence that would drift.
-template <typename T, int C, int LDK, int LDV, int N>
+template <typename T, int C, int LDK, int LDV, int N, bool FULL>
 GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const float* wt, float gn, int m0, int n0, int nd) {
   using M = Math<T>;
   const int lane = threadIdx.x & 31, t = lane & 3;
   constexpr int AT = N < 8 ? N : 8;  // tiles at a time
 #pragma unroll
   for (int at = 0; at < N; at += AT) {
-    if (n0 + at * 8 >= nd) continue;
+    if (!FULL && n0 + at * 8 >= nd) continue;
     float add[AT][4];
 #pragma unroll
     for (int n = 0; n < AT; ++n)
@@ -406,11 +538,11 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
         for (int e = 0; e < 4; ++e) {
           const float* w = wt + k + 2 * t + 8 * (e >> 1);
           const float2 x = unpack_bf16(raw[e]);
-          split3(x.x * w[0], x.y * w[1], a[0][e], a[1][e], a[2][e]);
+          split3(f2(x.x, x.y) * f2(w[0], w[1]), a[0][e], a[1][e], a[2][e]);
         }
 #pragma unroll
         for (int n = 0; n < AT; n += 2) {
-          if (n0 + (at + n) * 8 >= nd) continue;
+          if (!FULL && n0 + (at + n) * 8 >= nd) continue;
           typename M::B b[2];
           load_bk<T>(b, vals + n * 8, LDV, lane);
 #pragma unroll
@@ -433,7 +565,7 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
         }
 #pragma unroll
         for (int n = 0; n < AT; n += 2) {
-          if (n0 + (at + n) * 8 >= nd) continue;
+          if (!FULL && n0 + (at + n) * 8 >= nd) continue;
           typename M::B b[2];
           load_bk<T>(b, vals + n * 8, LDV, lane);
           mma_pieces(add[n], a, b[0].v);
@@ -492,16 +624,16 @@ GFN_DEV void emit(void* out, const float (&o)[ON][4], const PassArgs& p, int b, 
 // their way.  OUTPUT: rows a, keys b, values c.  STATE: keys b, values c.
 // PAIR: with a = q, b = k, c = v, d = do, the outputs dv (rows b, keys a,
 // values d) and dk (rows c, keys d, values a) of the state's gradient.
-template <typename T, int DK, int DV, bool BACK, int KIND>
+template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL>
 __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::resident(KIND)) attn_kernel(const PassArgs p) {
   using S = Shape<T, DK, DV>;
   using M = Math<T>;
   using Op = typename M::State;
-  constexpr int STAGE = S::stage(KIND), BUFS = S::buffers(KIND);
+  constexpr int STAGE = S::stage(KIND), BUFS = S::buffers(KIND), STAGES = S::stages(KIND);
   extern __shared__ __align__(128) char attn_shared[];
   T* stage = reinterpret_cast<T*>(attn_shared);
-  Op* st_op = reinterpret_cast<Op*>(stage + 2 * STAGE);
-  float* wt = reinterpret_cast<float*>(attn_shared + 2 * STAGE * sizeof(T) + BUFS * S::STATE_BYTES);  // [2 C]
+  Op* st_op = reinterpret_cast<Op*>(stage + STAGES * STAGE);
+  float* wt = reinterpret_cast<float*>(attn_shared + STAGES * STAGE * sizeof(T) + BUFS * S::STATE_BYTES);  // [2 C]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int seg = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int len = length_of(p, b);
@@ -509,7 +641,7 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
   const float lg = log2_decay(p.decay[h]);
   // the state's place of this warp
   const int m0 = (warp % S::SLABS) * 16, n0 = (warp / S::SLABS) * S::SN * 8;
-  const bool holds = m0 < p.KD && n0 < p.VD;
+  const bool holds = FULL || (m0 < p.KD && n0 < p.VD);
   float st[S::SN][4];
   const long long mat = (long long)p.KD * p.VD, bh = (long long)b * p.H + h;
   const float* init = KIND == STATE ? nullptr : p.segs ? p.segs + (bh * p.segments + seg) * mat : p.state ? p.state + bh * mat : nullptr;
@@ -524,7 +656,7 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
   }
   {
     uint4* z = reinterpret_cast<uint4*>(attn_shared);
-    for (int i = threadIdx.x; i < (int)((2 * STAGE * sizeof(T) + BUFS * S::STATE_BYTES) / 16); i += S::THREADS)
+    for (int i = threadIdx.x; i < (int)((STAGES * STAGE * sizeof(T) + BUFS * S::STATE_BYTES) / 16); i += S::THREADS)
       z[i] = make_uint4(0, 0, 0, 0);
     // place C - 1 - e holds g^e (back: g^(e+1)); rows behind a short block take zeros
     for (int i = threadIdx.x; i < 2 * S::C; i += S::THREADS)
@@ -533,8 +665,8 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
   __syncthreads();
   auto bring = [&](int c, T* dst) {
     const int done = c * S::C, n = min(S::C, to - from - done), at = BACK ? to - 1 - done : from + done;
-    auto keys = [&](T* d, const View& v) { fetch<T, DK, S::LDK, S::C, S::THREADS, BACK>(d, v, b, h, p.KD, at, n, p.vec); };
-    auto vals = [&](T* d, const View& v) { fetch<T, DV, S::LDV, S::C, S::THREADS, BACK>(d, v, b, h, p.VD, at, n, p.vec); };
+    auto keys = [&](T* d, const View& v) { fetch<T, DK, S::LDK, S::C, S::THREADS, BACK, FULL>(d, v, b, h, p.KD, at, n, p.piece); };
+    auto vals = [&](T* d, const View& v) { fetch<T, DV, S::LDV, S::C, S::THREADS, BACK, FULL>(d, v, b, h, p.VD, at, n, p.piece); };
     if (KIND == OUTPUT) {
       keys(dst, p.a);
       keys(dst + S::TK, p.b);
@@ -569,27 +701,38 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
   lay_out(st_op);
   const int rt = warp % S::ROWS, part = warp / S::ROWS;
   const Decay decay(lg, p.s_in);
+  const float whole = power(lg, S::C);
   // forward: row i takes g^(i+1) of the state; back: g^i, as the state's
   // gradient arrives with that factor in it
   const int r0 = rt * 16 + (lane >> 2) + (BACK ? 0 : 1);
   const float w0 = p.s_state * power(lg, r0), w1 = p.s_state * power(lg, r0 + 8);
   for (int c = 0; c < blocks; ++c) {
-    const T* cur = stage + (c & 1) * STAGE;
+    const T* cur = stage + (STAGES == 2 ? (c & 1) * STAGE : 0);
     const Op* op = st_op + (BUFS == 2 ? (c & 1) * DK * S::LS : 0);
     const int done = c * S::C, n = min(S::C, to - from - done), at = BACK ? to - 1 - done : from + done;
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // and with it everyone has left the other stage
-    if (c + 1 < blocks) bring(c + 1, stage + ((c + 1) & 1) * STAGE);
+    if (STAGES == 2 && c + 1 < blocks) bring(c + 1, stage + ((c + 1) & 1) * STAGE);
+    auto move_on = [&] {
+      const T* uk = KIND == OUTPUT ? cur + S::TK : cur;
+      const T* uv = KIND == OUTPUT ? cur + 2 * S::TK : KIND == STATE ? cur + S::TK : cur + 2 * S::TK + S::TV;
+      const float gn = n == S::C ? whole : power(lg, n);
+      if (holds) update<T, S::C, S::LDK, S::LDV, S::SN, FULL>(st, uk, uv, wt + S::C - n, gn, m0, n0, p.VD);
+    };
+    if (BUFS == 2) {  // the next block's state, beside the outputs of this one
+      move_on();
+      lay_out(st_op + ((c + 1) & 1) * DK * S::LS);
+    }
     if constexpr (KIND != STATE) {
       constexpr int OV = DV / 8 / S::SPLIT;
       float o[OV][4];
       const int col0 = part * OV * 8;
-      if (col0 < p.VD) {
+      if (FULL || col0 < p.VD) {
         if constexpr (KIND == OUTPUT)
-          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false>(o, cur, cur + S::TK, cur + 2 * S::TK, op, rt, col0, p.KD, p.VD,
+          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false, FULL>(o, cur, cur + S::TK, cur + 2 * S::TK, op, rt, col0, p.KD, p.VD,
                                                                decay, w0, w1);
         else
-          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false>(o, cur + S::TK, cur, cur + 2 * S::TK + S::TV, op, rt, col0, p.KD,
+          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false, FULL>(o, cur + S::TK, cur, cur + 2 * S::TK + S::TV, op, rt, col0, p.KD,
                                                                p.VD, decay, w0, w1);
         emit<T, OV, BACK>(p.o, o, p, b, h, p.VD, at, n, rt, col0);
       }
@@ -598,17 +741,18 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
       constexpr int OK = DK / 8 / S::SPLIT;
       float o[OK][4];
       const int col0 = part * OK * 8;
-      if (col0 < p.KD) {
-        attend<T, S::C, DV, S::LDV, S::LDK, S::LS, OK, true>(o, cur + 2 * S::TK, cur + 2 * S::TK + S::TV, cur, op, rt, col0, p.VD,
+      if (FULL || col0 < p.KD) {
+        attend<T, S::C, DV, S::LDV, S::LDK, S::LS, OK, true, FULL>(o, cur + 2 * S::TK, cur + 2 * S::TK + S::TV, cur, op, rt, col0, p.VD,
                                                             p.KD, decay, w0, w1);
         emit<T, OK, BACK>(p.o2, o, p, b, h, p.KD, at, n, rt, col0);
       }
     }
-    const T* uk = KIND == OUTPUT ? cur + S::TK : cur;
-    const T* uv = KIND == OUTPUT ? cur + 2 * S::TK : KIND == STATE ? cur + S::TK : cur + 2 * S::TK + S::TV;
-    if (holds) update<T, S::C, S::LDK, S::LDV, S::SN>(st, uk, uv, wt + S::C - n, power(lg, n), m0, n0, p.VD);
-    if (BUFS == 1) __syncthreads();
-    if (BUFS > 0) lay_out(st_op + (BUFS == 2 ? ((c + 1) & 1) * DK * S::LS : 0));
+    if (BUFS < 2) move_on();
+    if (BUFS == 1) {
+      __syncthreads();
+      if (STAGES == 1 && c + 1 < blocks) bring(c + 1, stage);
+      lay_out(st_op);
+    }
   }
   // tokens behind the sequence: zeros
   if (KIND != STATE && len < p.L) {
@@ -666,17 +810,36 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const PassArgs p) {
 }
 
 // One token: the state is read, moved on and written once.  A thread owns VEC
-// columns of every RG-th row.
+// columns of every `groups`-th row, and AT rows are on their way at once, the
+// first ones beside the token's q, k and v.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) attn_step_kernel(const PassArgs p) {
+  constexpr int AT = 4;
   __shared__ float q[128], k[128], sum[256 * VEC];
+  struct alignas(4 * VEC) Cells {
+    float c[VEC];
+  };
   const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
   const long long mat = (long long)p.KD * p.VD, bh = (long long)b * p.H + h;
-  const bool live = length_of(p, b) > 0;
-  const float gam = fminf(fmaxf(p.decay[h], 0.f), 1.f), g = p.decay[h] != p.decay[h] ? p.decay[h] : gam;
-  auto at = [&](const View& v) { return static_cast<const T*>(v.p) + b * v.sb + h * v.sh; };
   const int cols = p.VD / VEC, groups = 256 / cols, mine = threadIdx.x % cols, group = threadIdx.x / cols;
-  if (threadIdx.x < p.KD) {
+  const int rows = group < groups ? p.KD : 0;  // the last threads may be left over
+  const float* in = p.state ? p.state + bh * mat + mine * VEC : nullptr;
+  float* out = p.state_out ? p.state_out + bh * mat + mine * VEC : nullptr;
+  Cells s[AT];
+  auto read = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < AT; ++u) {
+      const int r = r0 + u * groups;
+      s[u] = {};
+      if (in && r < rows) s[u] = *reinterpret_cast<const Cells*>(in + r * p.VD);
+    }
+  };
+  read(group);
+  const bool live = length_of(p, b) > 0;
+  float g = p.decay[h];
+  g = g > 1.f ? 1.f : g < 0.f ? 0.f : g;
+  auto at = [&](const View& v) { return static_cast<const T*>(v.p) + b * v.sb + h * v.sh; };
+  if ((int)threadIdx.x < p.KD) {
     q[threadIdx.x] = live ? to_f(at(p.a)[threadIdx.x]) * p.s_state : 0.f;
     k[threadIdx.x] = live ? to_f(at(p.b)[threadIdx.x]) : 0.f;
   }
@@ -687,22 +850,20 @@ __global__ void __launch_bounds__(256) attn_step_kernel(const PassArgs p) {
     acc[e] = 0.f;
   }
   __syncthreads();
-  struct alignas(4 * VEC) Cells {
-    float c[VEC];
-  };
-  if (group < groups) {
-#pragma unroll 4
-    for (int r = group; r < p.KD; r += groups) {
-      Cells s = {};
-      if (p.state) s = *reinterpret_cast<const Cells*>(p.state + bh * mat + (long long)r * p.VD + mine * VEC);
+  for (int r0 = group; r0 < rows; r0 += AT * groups) {
+    if (r0 != group) read(r0);
+#pragma unroll
+    for (int u = 0; u < AT; ++u) {
+      const int r = r0 + u * groups;
+      if (r >= rows) continue;
       if (live) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          s.c[e] = fmaf(g, s.c[e], k[r] * v[e]);
-          acc[e] = fmaf(q[r], s.c[e], acc[e]);
+          s[u].c[e] = fmaf(g, s[u].c[e], k[r] * v[e]);
+          acc[e] = fmaf(q[r], s[u].c[e], acc[e]);
         }
       }
-      if (p.state_out) *reinterpret_cast<Cells*>(p.state_out + bh * mat + (long long)r * p.VD + mine * VEC) = s;
+      if (out) *reinterpret_cast<Cells*>(out + r * p.VD) = s[u];
     }
   }
 #pragma unroll
@@ -710,21 +871,28 @@ __global__ void __launch_bounds__(256) attn_step_kernel(const PassArgs p) {
   __syncthreads();
   for (int c = threadIdx.x; c < p.VD; c += 256) {
     float t = 0.f;
-    for (int r = 0; r < groups; ++r) t += sum[(r * cols + c / VEC) * VEC + c % VEC];
+#pragma unroll 8
+    for (int r = 0; r < groups; ++r) t += sum[r * p.VD + c];
     static_cast<T*>(p.o)[bh * p.VD + c] = from_f<T>(t);
   }
 }
 
 // ------------------------------------------------------------------ launches
-template <typename T, int DK, int DV, bool BACK, int KIND>
-int attn_run(const PassArgs& p, cudaStream_t s) {
+// FULL: heads as wide as the kernel, and all operands in 16-byte pieces.
+template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL>
+int attn_launch(const PassArgs& p, cudaStream_t s) {
   using S = Shape<T, DK, DV>;
   static std::atomic<unsigned long long> done;
   const int bytes = S::bytes(KIND);
-  const int st = shared_limit(attn_kernel<T, DK, DV, BACK, KIND>, bytes, &done, "attn_kernel");
+  const int st = shared_limit(attn_kernel<T, DK, DV, BACK, KIND, FULL>, bytes, &done, "attn_kernel");
   if (st != GFN_OK) return st;
-  attn_kernel<T, DK, DV, BACK, KIND><<<dim3(p.segments, p.H, p.B), S::THREADS, bytes, s>>>(p);
+  attn_kernel<T, DK, DV, BACK, KIND, FULL><<<dim3(p.segments, p.H, p.B), S::THREADS, bytes, s>>>(p);
   return launch_status("attn_kernel");
+}
+template <typename T, int DK, int DV, bool BACK, int KIND>
+int attn_run(const PassArgs& p, cudaStream_t s) {
+  return p.piece == 16 && p.KD == DK && p.VD == DV ? attn_launch<T, DK, DV, BACK, KIND, true>(p, s)
+                                           : attn_launch<T, DK, DV, BACK, KIND, false>(p, s);
 }
 
 template <typename T, int DK, int DV, bool BACK, int KIND>

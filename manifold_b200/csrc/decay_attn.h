@@ -26,7 +26,7 @@ struct PassArgs {
   long long sr, sc;     // strides of the state's rows and columns
   int seg_len, segments;
   float s_in, s_state, s_update;  // factors of the products within a block, with the state, and of the state's update
-  int vec;              // operands arrive in 16-byte pieces
+  int piece;            // operands arrive in pieces of so many bytes (16, 8, 4), or by single 16-bit elements (2)
 };
 
 // What a launch does: a segment's output, its part of the state alone, or the
