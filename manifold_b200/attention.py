@@ -1,8 +1,6 @@
 """Linear attention with a decay for each head: the gated scan's recurrence
 (scan.py, gfn/scan.py:11-104) with a matrix for a state.  CUDA tensors only."""
-import torch
-
-from ._lib import GfnError, dtype_code, same_device, torch_ops
+from ._lib import torch_ops
 
 
 def decay_attention(q, k, v, decay, state=None, return_state=False, lengths=None, scale=1.0):
@@ -27,37 +25,4 @@ def decay_attention(q, k, v, decay, state=None, return_state=False, lengths=None
     (not where they are kept).  Tokens are taken in blocks of up to 64, so that a
     NaN or infinity in k or v reaches the outputs of its block's earlier tokens too.
     """
-    same_device("decay_attention", q, k, v, decay, state, lengths)
-    dtype_code(q, "q")
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:3] != q.shape[:3]:
-        raise GfnError("decay_attention: q, k must be [batch, length, heads, kdim] and v [batch, length, heads, vdim], "
-                       f"got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise GfnError(f"decay_attention: q is {q.dtype}, k {k.dtype}, v {v.dtype}")
-    B, L, H, K = q.shape
-    V = v.shape[3]
-    if not 0 < K <= 128 or not 0 < V <= 128:
-        raise GfnError(f"decay_attention: head dims from 1 to 128 are implemented, got {K}, {V}")
-    if decay.dtype != torch.float32 or decay.shape != (H,):
-        raise GfnError(f"decay_attention: decay must be float32 [{H}], got {decay.dtype} {tuple(decay.shape)}")
-    grad = torch.is_grad_enabled()
-    if grad and decay.requires_grad:
-        raise GfnError("decay_attention is not differentiable in decay: pass decay.detach()")
-    if not decay.is_contiguous():
-        decay = decay.contiguous()
-    wants = q.requires_grad or k.requires_grad or v.requires_grad
-    if state is not None:
-        if state.dtype != torch.float32 or state.shape != (B, H, K, V):
-            raise GfnError(f"decay_attention: state must be float32 {(B, H, K, V)}, got {state.dtype} "
-                           f"{tuple(state.shape)}")
-        wants = wants or state.requires_grad
-    if lengths is not None:
-        if lengths.shape != (B,) or (lengths.dtype != torch.int64 and lengths.dtype != torch.int32):
-            raise GfnError(f"decay_attention: lengths must be int64 or int32 [{B}], got {lengths.dtype} "
-                           f"{tuple(lengths.shape)}")
-        if not lengths.is_contiguous():
-            lengths = lengths.contiguous()
-    if isinstance(scale, torch.Tensor):
-        raise GfnError("decay_attention: scale must be a number")
-    out = torch_ops().decay_attention(q, k, v, decay, state, lengths, scale, return_state, wants and grad)
-    return out if return_state else out[0]
+    return torch_ops().decay_attention(q, k, v, decay, state, lengths, scale, return_state)

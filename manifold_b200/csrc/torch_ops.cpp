@@ -5,8 +5,8 @@
 // ctypes and a Python autograd Function took 10.8 us forward and, trained,
 // 104 us, of which the hand-over to the engine's thread and back is 45; here a
 // call takes 7 and a small training step 65 to 80.
-// Arguments arrive checked (norm.py, scan.py, cuda/ops.py, sampling.py,
-// embeddings.py, attention.py); the
+// Arguments arrive checked (norm.py, scan.py, cuda/ops.py, sampling.py) or
+// are checked here (the embedding, log probabilities, the attention); the
 // entry points of the C ABI are handed over by bind(), so that one library is
 // loaded whoever calls.
 #include <Python.h>
@@ -615,7 +615,7 @@ bool flag_arg(PyObject* o) { return PyObject_IsTrue(o) == 1; }
 PyObject* tuple_of(const variable_list& ts) {
   PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
   if (!r) throw python_error();
-  for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(r, (Py_ssize_t)i, THPVariable_Wrap(ts[i]));
+  for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(r, (Py_ssize_t)i, THPVariable_Wrap(ts[i]));  // undefined: None
   return r;
 }
 
@@ -719,57 +719,149 @@ PyObject* py_process_logits(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-// embed_tokens(ids, weight, scale, padding, train) -> y
+// The three calls below check their arguments here: in Python that took as
+// long as the rest of a small call (a token of decay_attention took 10.0 us a call, 7.4 here).
+std::string text(const Tensor& t) {
+  std::string r = std::string(c10::toString(t.scalar_type())) + " (";
+  for (int64_t i = 0; i < t.dim(); ++i) r += (i ? ", " : "") + std::to_string(t.size(i));
+  return r + ")";
+}
+
+// Every operand on the first one's CUDA device; that one's type is one of the three.
+void operands(const char* what, const char* first_name, const Tensor& first, std::initializer_list<const Tensor*> others) {
+  if (!first.defined()) throw Failure(std::string(what) + ": " + first_name + " must be a tensor");
+  for (const Tensor* t : others)
+    if (t->defined() && !t->is_cuda())
+      throw Failure("manifold_b200 runs on CUDA tensors only (no CPU path); got a " + t->device().str() + " tensor");
+  if (!first.is_cuda())
+    throw Failure("manifold_b200 runs on CUDA tensors only (no CPU path); got a " + first.device().str() + " tensor");
+  for (const Tensor* t : others)
+    if (t->defined() && t->device() != first.device())
+      throw Failure(std::string(what) + ": operands on " + first.device().str() + " and " + t->device().str());
+  const at::ScalarType s = first.scalar_type();
+  if (s != at::kFloat && s != at::kBFloat16 && s != at::kHalf)
+    throw Failure(std::string(first_name) + " must be float32, bfloat16 or float16, got " + c10::toString(s));
+}
+
+bool whole_numbers(const Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
+
+double factor_arg(PyObject* o, const char* what) {
+  if (THPVariable_Check(o)) throw Failure(std::string(what) + ": scale must be a number (multiply by a tensor afterwards)");
+  return number_arg(o);
+}
+
+// embed_tokens(ids, weight, scale, padding_idx or None) -> y
 PyObject* py_embed_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded(n, 5, [&] {
+  return guarded(n, 4, [&] {
     const Tensor ids = tensor_arg(v[0]), w = tensor_arg(v[1]);
-    const double scale = number_arg(v[2]);
-    const int64_t padding = integer_arg(v[3]);
-    const bool train = flag_arg(v[4]);
+    operands("embed_tokens", "weight", w, {&ids});
+    if (!ids.defined() || !whole_numbers(ids))
+      throw Failure("embed_tokens: ids must be int64 or int32" + (ids.defined() ? ", got " + text(ids) : std::string()));
+    if (w.dim() != 2 || w.size(0) < 1 || w.size(1) < 1)
+      throw Failure("embed_tokens: weight must be [vocab, dim], got " + text(w));
+    const double scale = factor_arg(v[2], "embed_tokens");
+    int64_t padding = -1;
+    if (v[3] != Py_None) {
+      const int64_t given = integer_arg(v[3]);
+      padding = given < 0 ? given + w.size(0) : given;
+      if (padding < 0 || padding >= w.size(0))
+        throw Failure("embed_tokens: padding_idx " + std::to_string(given) + " outside a vocabulary of " + std::to_string(w.size(0)));
+    }
     Tensor y;
     {
       Unlocked u;
-      y = train ? EmbedNode::apply(ids, w, scale, padding) : embed_run(ids, w, scale);
+      y = w.requires_grad() && at::GradMode::is_enabled() ? EmbedNode::apply(ids, w, scale, padding) : embed_run(ids, w, scale);
     }
     return THPVariable_Wrap(y);
   });
 }
 
-// token_logprobs(x, tokens, top, entropy, ignore_index, train) -> those of (logprobs, entropy, top_logprobs, top_tokens)
-// that are asked for
+// token_logprobs(x, tokens, top, entropy, ignore_index) -> (logprobs, entropy, top_logprobs, top_tokens), each or None
 PyObject* py_token_logprobs(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded(n, 6, [&] {
+  return guarded(n, 5, [&] {
     const Tensor x = tensor_arg(v[0]), tokens = tensor_arg(v[1]);
     const int64_t top = integer_arg(v[2]), ignore = integer_arg(v[4]);
-    const bool entropy = flag_arg(v[3]), train = flag_arg(v[5]);
-    variable_list out;
+    const bool entropy = flag_arg(v[3]);
+    operands("token_logprobs", "logits", x, {&tokens});
+    if (x.dim() < 1 || x.size(-1) < 1) throw Failure("token_logprobs: logits must be [..., vocab], got " + text(x));
+    const int64_t most = x.size(-1) < 32 ? x.size(-1) : 32;
+    if (top < 0 || top > most)
+      throw Failure("token_logprobs: top must be 0 to " + std::to_string(most) + ", got " + std::to_string(top));
+    if (tokens.defined()) {
+      if (!whole_numbers(tokens) || tokens.sizes() != x.sizes().slice(0, x.dim() - 1))
+        throw Failure("token_logprobs: tokens must be int64 or int32 of the logits' leading shape, got " + text(tokens) +
+                      " for logits " + text(x));
+    } else if (!top && !entropy) {
+      throw Failure("token_logprobs: nothing asked for (tokens, top or entropy)");
+    }
+    Tensor r[4];
     {
       Unlocked u;
-      const Tensor t = whole(tokens);
-      out = train ? LogprobNode::apply(x, maybe(t), top, entropy, ignore)
-                  : logprob_run(x, t, top, entropy, ignore, false).outputs();
+      const Tensor t = tokens.defined() && tokens.scalar_type() != at::kLong ? tokens.to(at::kLong) : whole(tokens);
+      if (x.requires_grad() && at::GradMode::is_enabled()) {
+        const variable_list out = LogprobNode::apply(x, maybe(t), top, entropy, ignore);
+        size_t at = 0;
+        if (t.defined()) r[0] = out[at++];
+        if (entropy) r[1] = out[at++];
+        if (top) {
+          r[2] = out[at++];
+          r[3] = out[at++];
+        }
+      } else {
+        const Probs o = logprob_run(x, t, top, entropy, ignore, false);
+        r[0] = o.lp;
+        r[1] = o.ent;
+        r[2] = o.top_lp;
+        r[3] = o.top_id;
+      }
     }
-    return tuple_of(out);
+    return tuple_of({r[0], r[1], r[2], r[3]});
   });
 }
 
-// decay_attention(q, k, v, decay, state, lengths, scale, want_last, train) -> (o,) or (o, last)
+// decay_attention(q, k, v, decay, state, lengths, scale, want_last) -> o or (o, last)
 PyObject* py_decay_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded(n, 9, [&] {
-    const Tensor q = tensor_arg(v[0]), k = tensor_arg(v[1]), val = tensor_arg(v[2]), decay = tensor_arg(v[3]),
-                 state = tensor_arg(v[4]), lengths = tensor_arg(v[5]);
-    const double scale = number_arg(v[6]);
-    const bool want_last = flag_arg(v[7]), train = flag_arg(v[8]);
-    variable_list out;
+  return guarded(n, 8, [&] {
+    const Tensor q = tensor_arg(v[0]), k = tensor_arg(v[1]), val = tensor_arg(v[2]), state = tensor_arg(v[4]),
+                 lengths = tensor_arg(v[5]);
+    Tensor decay = tensor_arg(v[3]);
+    operands("decay_attention", "q", q, {&k, &val, &decay, &state, &lengths});
+    if (!k.defined() || !val.defined() || !decay.defined()) throw Failure("decay_attention: k, v and decay must be tensors");
+    if (q.dim() != 4 || k.sizes() != q.sizes() || val.dim() != 4 || val.sizes().slice(0, 3) != q.sizes().slice(0, 3))
+      throw Failure("decay_attention: q, k must be [batch, length, heads, kdim] and v [batch, length, heads, vdim], got " +
+                    text(q) + ", " + text(k) + ", " + text(val));
+    if (k.scalar_type() != q.scalar_type() || val.scalar_type() != q.scalar_type())
+      throw Failure("decay_attention: q is " + text(q) + ", k " + text(k) + ", v " + text(val));
+    const int64_t B = q.size(0), H = q.size(2), K = q.size(3), V = val.size(3);
+    if (K < 1 || K > 128 || V < 1 || V > 128)
+      throw Failure("decay_attention: head dims from 1 to 128 are implemented, got " + std::to_string(K) + ", " + std::to_string(V));
+    if (decay.scalar_type() != at::kFloat || decay.dim() != 1 || decay.size(0) != H)
+      throw Failure("decay_attention: decay must be float32 [" + std::to_string(H) + "], got " + text(decay));
+    const bool grad = at::GradMode::is_enabled();
+    if (grad && decay.requires_grad())
+      throw Failure("decay_attention is not differentiable in decay: pass decay.detach()");
+    if (state.defined() && (state.scalar_type() != at::kFloat || state.sizes() != at::IntArrayRef({B, H, K, V})))
+      throw Failure("decay_attention: state must be float32 [batch, heads, kdim, vdim], got " + text(state) + " for q " +
+                    text(q) + ", v " + text(val));
+    if (lengths.defined() && (!whole_numbers(lengths) || lengths.dim() != 1 || lengths.size(0) != B))
+      throw Failure("decay_attention: lengths must be int64 or int32 [" + std::to_string(B) + "], got " + text(lengths));
+    const double scale = factor_arg(v[6], "decay_attention");
+    const bool want_last = flag_arg(v[7]);
+    const bool train = grad && (q.requires_grad() || k.requires_grad() || val.requires_grad() ||
+                                (state.defined() && state.requires_grad()));
+    Tensor o, last;
     {
       Unlocked u;
-      if (train) out = AttnNode::apply(q, k, val, decay, maybe(state), maybe(lengths), scale, want_last);
-      else {
-        Tensor last, o = attn_run(q, k, val, decay, state, lengths, scale, want_last ? &last : nullptr, nullptr);
-        out = want_last ? variable_list{o, last} : variable_list{o};
+      const Tensor d = whole(decay), l = whole(lengths);
+      if (train) {
+        const variable_list out = AttnNode::apply(q, k, val, d, maybe(state), maybe(l), scale, want_last);
+        o = out[0];
+        if (want_last) last = out[1];
+      } else {
+        o = attn_run(q, k, val, d, state, l, scale, want_last ? &last : nullptr, nullptr);
       }
     }
-    return tuple_of(out);
+    return want_last ? tuple_of({o, last}) : THPVariable_Wrap(o);
   });
 }
 

@@ -10,7 +10,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from ._lib import GfnError, dtype_code, require_cuda, same_device, torch_ops
+from ._lib import GfnError, require_cuda, torch_ops
 from .cuda import ops
 
 
@@ -25,20 +25,7 @@ def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
     token outside the vocabulary gives a row of zeros, takes no part in the
     gradient and sets a device error bit (gfn.cuda.ops.device_error).
     """
-    same_device("embed_tokens", weight, ids)
-    dtype_code(weight, "weight")
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise GfnError(f"embed_tokens: weight must be [vocab, dim], got {tuple(weight.shape)}")
-    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
-        raise GfnError(f"embed_tokens: ids must be int64 or int32, got {ids.dtype}")
-    if isinstance(scale, torch.Tensor):
-        raise GfnError("embed_tokens: scale must be a number (multiply by a tensor afterwards)")
-    pad = -1
-    if padding_idx is not None:
-        pad = padding_idx if padding_idx >= 0 else padding_idx + weight.shape[0]
-        if not 0 <= pad < weight.shape[0]:
-            raise GfnError(f"embed_tokens: padding_idx {padding_idx} outside a vocabulary of {weight.shape[0]}")
-    return torch_ops().embed_tokens(ids, weight, scale, pad, weight.requires_grad and torch.is_grad_enabled())
+    return torch_ops().embed_tokens(ids, weight, scale, padding_idx)
 
 
 class Embedding(nn.Embedding):

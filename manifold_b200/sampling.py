@@ -138,21 +138,4 @@ def token_logprobs(logits, tokens=None, top=0, entropy=False, ignore_index=-100)
     zeros; one with NaN or +inf gives NaN.  Differentiable (once) in the logits,
     through every float result.
     """
-    same_device("token_logprobs", logits, tokens)
-    dtype_code(logits, "logits")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise GfnError(f"token_logprobs: logits must be [..., vocab], got {tuple(logits.shape)}")
-    if not isinstance(top, int) or not 0 <= top <= min(32, logits.shape[-1]):
-        raise GfnError(f"token_logprobs: top must be 0 to {min(32, logits.shape[-1])}, got {top}")
-    if tokens is not None:
-        if tokens.shape != logits.shape[:-1] or (tokens.dtype != torch.int64 and tokens.dtype != torch.int32):
-            raise GfnError(f"token_logprobs: tokens must be int64 {tuple(logits.shape[:-1])}, got {tokens.dtype} "
-                           f"{tuple(tokens.shape)}")
-        if tokens.dtype != torch.int64:
-            tokens = tokens.to(torch.int64)
-    elif not top and not entropy:
-        raise GfnError("token_logprobs: nothing asked for (tokens, top or entropy)")
-    out = iter(torch_ops().token_logprobs(logits, tokens, top, entropy, ignore_index,
-                                          logits.requires_grad and torch.is_grad_enabled()))
-    return TokenLogprobs(next(out) if tokens is not None else None, next(out) if entropy else None,
-                         next(out) if top else None, next(out) if top else None)
+    return TokenLogprobs(*torch_ops().token_logprobs(logits, tokens, top, entropy, ignore_index))
