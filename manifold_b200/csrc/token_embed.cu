@@ -10,12 +10,9 @@
 // every run.  Sums are float32 and are rounded once.
 #include "lm_host.h"
 #include "lm_ops.cuh"
-#include "umma.cuh"
 
 using namespace gfn;
 using namespace gfn_abi;
-using umma::gdc_launch_dependents;
-using umma::gdc_wait;
 
 namespace {
 
@@ -48,78 +45,138 @@ struct EmbedArgs {
   const void* ids;
   const void* w;
   void* y;
-  long long N, ws, total;  // tokens, row stride of the table, groups of y
+  long long N, ws, total;  // tokens, row stride of the table, items of all rows
   int V, D, wide;
   float scale;
-  Divisor per_row;  // groups per row (VECLOAD), else elements per row
+  Divisor per_row;  // groups or other items of a row
 };
 
-// y in groups of VEC elements, 16 bytes where y starts on 16 bytes.  With
-// VECLOAD the rows of table and y are whole groups; otherwise a group may lie
-// across two rows and its elements are fetched one by one.
-template <typename T, int VEC, bool VECLOAD>
+// The 16 bytes at address `at`, which is a multiple of the element's size only,
+// out of the two aligned ones that hold them.
+GFN_DEV uint4 cut_out(uintptr_t at, const uint4& lo, const uint4& hi) {
+  unsigned w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = at & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = at & 4 ? w[i + 1] : w[i];
+  const unsigned sh = (unsigned)(at & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
+                    __funnelshift_r(w[3], w[4], sh));
+}
+
+// y in groups of VEC elements, which rows of table and y are made of (16 bytes
+// where they are; else elements).
+template <typename T, int VEC>
 __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(const EmbedArgs p) {
   constexpr int TILE = EMBED_THREADS * EMBED_GROUPS;
   const long long first = (long long)blockIdx.x * TILE;
   const T* w = static_cast<const T*>(p.w);
-  if constexpr (VECLOAD) {
-    const long long row0 = first / p.per_row.d;
-    const unsigned rem = (unsigned)(first - row0 * p.per_row.d);
-    const T* src[EMBED_GROUPS];
-    Pack<T, VEC> v[EMBED_GROUPS];
+  const long long row0 = first / p.per_row.d;
+  const unsigned rem = (unsigned)(first - row0 * p.per_row.d);
+  const T* src[EMBED_GROUPS];
+  Pack<T, VEC> v[EMBED_GROUPS];
 #pragma unroll
-    for (int u = 0; u < EMBED_GROUPS; ++u) {
-      const unsigned at = threadIdx.x + u * EMBED_THREADS, off = rem + at, r = quotient(off, p.per_row);
-      src[u] = nullptr;
-      if (first + at < p.total) {
-        const long long id = id_at(p.ids, p.wide, row0 + r);
-        if ((unsigned long long)id < (unsigned)p.V) src[u] = w + id * p.ws + (long long)(off - r * p.per_row.d) * VEC;
-        else gfn_flag_error(kDevErrBadToken);
-      }
+  for (int u = 0; u < EMBED_GROUPS; ++u) {
+    const unsigned at = threadIdx.x + u * EMBED_THREADS, off = rem + at, r = quotient(off, p.per_row);
+    src[u] = nullptr;
+    if (first + at < p.total) {
+      const long long id = id_at(p.ids, p.wide, row0 + r);
+      if ((unsigned long long)id < (unsigned)p.V) src[u] = w + id * p.ws + (long long)(off - r * p.per_row.d) * VEC;
+      else gfn_flag_error(kDevErrBadToken);
     }
+  }
 #pragma unroll
-    for (int u = 0; u < EMBED_GROUPS; ++u)
-      if (src[u]) v[u] = *reinterpret_cast<const Pack<T, VEC>*>(src[u]);
+  for (int u = 0; u < EMBED_GROUPS; ++u)
+    if (src[u]) v[u] = *reinterpret_cast<const Pack<T, VEC>*>(src[u]);
 #pragma unroll
-    for (int u = 0; u < EMBED_GROUPS; ++u) {
-      const long long g = first + threadIdx.x + u * EMBED_THREADS;
-      if (g >= p.total) continue;
-      Pack<T, VEC> o;
+  for (int u = 0; u < EMBED_GROUPS; ++u) {
+    const long long g = first + threadIdx.x + u * EMBED_THREADS;
+    if (g >= p.total) continue;
+    Pack<T, VEC> o;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(src[u] ? to_f(v[u].v[e]) * p.scale : 0.f);
-      reinterpret_cast<Pack<T, VEC>*>(p.y)[g] = o;
+    for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(src[u] ? to_f(v[u].v[e]) * p.scale : 0.f);
+    reinterpret_cast<Pack<T, VEC>*>(p.y)[g] = o;
+  }
+}
+
+// Rows off 16 bytes, y on them.  A row is 2 VEC single elements (those before
+// its first and behind its last whole 16 bytes of y, some of them none) and
+// the groups between, each cut out of two loads.  20011 x 1001 bfloat16: 24 us,
+// against 27 where groups over the rows' ends were fetched by elements in a loop
+// (33 with the rest of them sped up as here).
+template <typename T>
+__global__ void __launch_bounds__(EMBED_THREADS) embed_across_kernel(const EmbedArgs p) {
+  constexpr int TILE = EMBED_THREADS * EMBED_GROUPS, VEC = 16 / sizeof(T);
+  const long long first = (long long)blockIdx.x * TILE;
+  const T* w = static_cast<const T*>(p.w);
+  const uintptr_t begin = reinterpret_cast<uintptr_t>(w), end = reinterpret_cast<uintptr_t>(w + (p.V - 1) * p.ws + p.D);
+  const long long row0 = first / p.per_row.d;
+  const unsigned rem = (unsigned)(first - row0 * p.per_row.d);
+  const T* src[EMBED_GROUPS];
+  int col[EMBED_GROUPS], width[EMBED_GROUPS];  // width: 0 nothing, 1 an element, VEC a group
+  uint4 lo[EMBED_GROUPS], hi[EMBED_GROUPS];
+  T one[EMBED_GROUPS];
+#pragma unroll
+  for (int u = 0; u < EMBED_GROUPS; ++u) {
+    const unsigned at = threadIdx.x + u * EMBED_THREADS, r = quotient(rem + at, p.per_row);
+    const int i = (int)(rem + at - r * p.per_row.d);
+    const int head = (int)((VEC - (unsigned long long)(row0 + r) * (unsigned)p.D % VEC) % VEC);
+    const int groups = (p.D - head) / VEC, behind = head + groups * VEC;
+    width[u] = 0;
+    src[u] = nullptr;
+    if (first + at >= p.total) continue;
+    if (i < VEC) {
+      col[u] = i;
+      width[u] = i < head;
+    } else if (i < 2 * VEC) {
+      col[u] = behind + i - VEC;
+      width[u] = col[u] < p.D;
+    } else {
+      col[u] = head + (i - 2 * VEC) * VEC;
+      width[u] = i - 2 * VEC < groups ? VEC : 0;
     }
-  } else {
-    const long long all = p.N * p.D;
-    const long long row0 = first * VEC / p.D;
-    const unsigned rem = (unsigned)(first * VEC - row0 * p.D);
+    if (!width[u]) continue;
+    const long long id = id_at(p.ids, p.wide, row0 + r);
+    if ((unsigned long long)id < (unsigned)p.V) src[u] = w + id * p.ws + col[u];
+    else gfn_flag_error(kDevErrBadToken);
+  }
+  auto within = [&](int u) {
+    const uintptr_t q = reinterpret_cast<uintptr_t>(src[u]) & ~(uintptr_t)15;
+    return q >= begin && q + 32 <= end;
+  };
 #pragma unroll
-    for (int u = 0; u < EMBED_GROUPS; ++u) {
-      const unsigned at = threadIdx.x + u * EMBED_THREADS;
-      const long long e0 = (first + at) * VEC;
-      if (e0 >= all) continue;
-      unsigned r = quotient(rem + at * VEC, p.per_row), c = rem + at * VEC - r * (unsigned)p.D;
-      const T* src = nullptr;
-      Pack<T, VEC> o;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (c == (unsigned)p.D) {
-          c = 0;
-          ++r;
-        }
-        if ((e == 0 || c == 0) && e0 + e < all) {
-          const long long id = id_at(p.ids, p.wide, row0 + r);
-          src = (unsigned long long)id < (unsigned)p.V ? w + id * p.ws : nullptr;
-          if (!src) gfn_flag_error(kDevErrBadToken);
-        }
-        o.v[e] = from_f<T>(src && e0 + e < all ? to_f(src[c]) * p.scale : 0.f);
-        ++c;
-      }
-      T* y = static_cast<T*>(p.y) + e0;
-      if (VEC > 1 && e0 + VEC <= all) *reinterpret_cast<Pack<T, VEC>*>(y) = o;
-      else
-        for (int e = 0; e < VEC && e0 + e < all; ++e) y[e] = o.v[e];
+  for (int u = 0; u < EMBED_GROUPS; ++u) {
+    if (!src[u]) continue;
+    if (width[u] == 1) one[u] = *src[u];
+    else if (within(u)) {
+      const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src[u]) & ~(uintptr_t)15);
+      lo[u] = q[0];
+      hi[u] = q[1];
     }
+  }
+#pragma unroll
+  for (int u = 0; u < EMBED_GROUPS; ++u) {
+    if (!width[u]) continue;
+    const unsigned at = threadIdx.x + u * EMBED_THREADS;
+    T* y = static_cast<T*>(p.y) + (row0 + quotient(rem + at, p.per_row)) * p.D + col[u];
+    if (width[u] == 1) {
+      *y = from_f<T>(src[u] ? to_f(one[u]) * p.scale : 0.f);
+      continue;
+    }
+    Pack<T, VEC> o;
+    if (!src[u]) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(0.f);
+    } else if (within(u)) {
+      const uint4 bits = cut_out(reinterpret_cast<uintptr_t>(src[u]), lo[u], hi[u]);
+      const T* v = reinterpret_cast<const T*>(&bits);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(to_f(v[e]) * p.scale);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(to_f(src[u][e]) * p.scale);
+    }
+    *reinterpret_cast<Pack<T, VEC>*>(y) = o;
   }
 }
 
@@ -127,14 +184,15 @@ template <typename T>
 int embed_forward(EmbedArgs p, cudaStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
   const bool rows = aligned16(p.w) && aligned16(p.y) && p.D % VEC == 0 && p.ws % VEC == 0;
-  const int vec = aligned16(p.y) ? VEC : 1;
-  p.total = (p.N * p.D + vec - 1) / vec;
-  p.per_row = divisor((unsigned)(rows ? p.D / VEC : p.D));
+  const bool across = !rows && aligned16(p.y) && p.D >= 8 * VEC;  // shorter rows are mostly ends
+  const int items = rows ? p.D / VEC : across ? 2 * VEC + p.D / VEC : p.D;
+  p.total = p.N * items;
+  p.per_row = divisor((unsigned)items);
   const long long blocks = (p.total + EMBED_THREADS * EMBED_GROUPS - 1) / (EMBED_THREADS * EMBED_GROUPS);
   if (blocks > 0x7fffffffLL) return fail(GFN_ERR_UNSUPPORTED, "embed: %lld x %d elements", p.N, p.D);
-  if (rows) embed_kernel<T, VEC, true><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
-  else if (vec > 1) embed_kernel<T, VEC, false><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
-  else embed_kernel<T, 1, false><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
+  if (rows) embed_kernel<T, VEC><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
+  else if (across) embed_across_kernel<T><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
+  else embed_kernel<T, 1><<<(unsigned)blocks, EMBED_THREADS, 0, s>>>(p);
   return launch_status("embed_kernel");
 }
 
@@ -148,7 +206,8 @@ constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILES = 256;
 constexpr int SORT_ITEMS = 4, SORT_SUB = SORT_THREADS * SORT_ITEMS;      // tokens of a thread, of a tile's part
 constexpr int SORT_ALONE = 8, SORT_ONE = SORT_THREADS * SORT_ALONE;      // where one block sorts them all
 // Tokens (in sorted order) that one group of threads sums.
-constexpr int SUM_RUN = 32, SUM_THREADS = 128, SUM_AHEAD = 8;
+constexpr int SUM_RUN = 32, SUM_THREADS = 128, SUM_AHEAD = 8, SUM_WORDS = 4 * SUM_RUN + 2;
+constexpr int SUM_COLS = 4;  // columns of a thread where rows are not whole groups of 16 bytes
 
 struct SortArgs {
   const void* ids;
@@ -194,8 +253,6 @@ GFN_DEV void zero_stage(const SortArgs& p, int first, int stage, int stages) {
 
 // The counts of the first digit, and zeros for those of the later ones.
 __global__ void __launch_bounds__(SORT_THREADS) embed_count_kernel(const SortArgs p) {
-  gdc_launch_dependents();
-  gdc_wait();
   if ((int)blockIdx.x >= p.tiles) return zero_stage(p, p.tiles, 0, p.passes + 1);
   __shared__ unsigned bins[SORT_BINS];
   const int n_bins = 1 << p.bits;
@@ -282,8 +339,6 @@ GFN_DEV void rank_part(SortShared& sh, long long from, long long to, unsigned sh
 
 // One digit of the sort.  The counts of the next digit are collected on the way.
 __global__ void __launch_bounds__(SORT_THREADS) embed_rank_kernel(const SortArgs p, int pass) {
-  gdc_launch_dependents();
-  gdc_wait();
   if ((int)blockIdx.x >= p.tiles) return zero_stage(p, p.tiles, pass + 1, p.passes + 1);
   __shared__ SortShared sh;
   const int n_bins = 1 << p.bits;
@@ -321,8 +376,6 @@ __global__ void __launch_bounds__(SORT_THREADS) embed_rank_kernel(const SortArgs
 
 // The whole sort of up to SORT_ONE tokens by one block; the others fill zeros.
 __global__ void __launch_bounds__(SORT_THREADS) embed_sort_kernel(const SortArgs p) {
-  gdc_launch_dependents();
-  gdc_wait();
   if (blockIdx.x >= 1) return zero_stage(p, 1, 0, 1);
   __shared__ SortShared sh;
   __shared__ uint2 items[SORT_ONE];
@@ -358,73 +411,105 @@ struct SumArgs {
   float scale;
 };
 
-// A group of blockDim.x threads sums SUM_RUN sorted tokens over the columns
-// of its threads, VEC each.  Rows of the table whose tokens lie within are
-// written; the first and the last may be shared with the neighbouring groups
-// and go to `part`.
-template <typename T, int VEC>
+// A group of blockDim.x threads sums SUM_RUN sorted tokens (a run) over the
+// columns of its threads, VEC each.  A row of the table whose tokens begin in
+// one run and end in the next belongs to the first.  Longer ones leave a part
+// for each run in `part`: [0] of a run's first row, [1] of its last.
+template <typename T, int VEC, int COLS>
 __global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const SumArgs p) {
-  gdc_launch_dependents();
-  gdc_wait();
   extern __shared__ unsigned sum_shared[];
-  unsigned* key = sum_shared + threadIdx.y * (2 * SUM_RUN + 2) + 1;  // key[-1] .. key[SUM_RUN]
-  unsigned* pos = key + SUM_RUN + 1;
+  unsigned* key = sum_shared + threadIdx.y * SUM_WORDS + 1;  // key[-1] .. key[2 SUM_RUN]
+  unsigned* pos = key + 2 * SUM_RUN + 1;
   const long long run = (long long)blockIdx.x * blockDim.y + threadIdx.y, from = run * SUM_RUN;
   const unsigned none = (unsigned)p.V;
-  for (int i = (int)threadIdx.x - 1; i <= SUM_RUN; i += blockDim.x) {
+  for (int i = (int)threadIdx.x - 1; i <= 2 * SUM_RUN; i += blockDim.x) {
     const long long n = from + i;
     const uint2 k = n >= 0 && n < p.N ? p.sorted[n] : make_uint2(n < 0 ? ~0u : none, 0u);
     key[i] = k.x;
-    if (i >= 0 && i < SUM_RUN) pos[i] = k.y;
+    if (i >= 0 && i < 2 * SUM_RUN) pos[i] = k.y;
   }
+  const unsigned far = from > SUM_RUN && from < p.N ? p.sorted[from - SUM_RUN - 1].x : ~0u;  // the last key before the run before
   __syncthreads();
-  const int col = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-  if (col >= p.D || key[0] >= none) return;
-  const T* dy = static_cast<const T*>(p.dy) + col;
-  float acc[VEC];
+  // COLS groups of VEC columns, blockDim.x groups apart
+  const int first = (blockIdx.y * blockDim.x * COLS + threadIdx.x) * VEC, gap = blockDim.x * VEC;
+  if (first >= p.D || key[0] >= none) return;
+  const T* dy = static_cast<const T*>(p.dy) + first;
+  float acc[COLS][VEC];
+  auto clear = [&] {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[c][e] = 0.f;
+  };
+  clear();
+  // the first row, where it began before: the run before has it if it ends here and began there
   bool open = key[0] == key[-1];
+  const bool skip = open && far != key[0] && key[SUM_RUN] != key[0];
+  const unsigned skipped = skip ? key[0] : ~0u;
+  // the last row, where it goes on: this run has it if it began here and ends in the next
+  const unsigned final = key[SUM_RUN - 1];
+  const bool goes_on = final < none && key[SUM_RUN] == final, began = key[0] != final || !open;
+  const bool whole = goes_on && began && key[2 * SUM_RUN] != final;
+  const int end = whole ? 2 * SUM_RUN : SUM_RUN;
   auto store = [&](float* dst) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) dst[e] = acc[e];
-  };
-  for (int i0 = 0; i0 < SUM_RUN; i0 += SUM_AHEAD) {
-    Pack<T, VEC> v[SUM_AHEAD];
+    for (int c = 0; c < COLS; ++c) {
+      if (first + c * gap >= p.D) continue;
 #pragma unroll
-    for (int i = 0; i < SUM_AHEAD; ++i)
-      if (key[i0 + i] < none) v[i] = *reinterpret_cast<const Pack<T, VEC>*>(dy + (long long)pos[i0 + i] * p.ds);
+      for (int e = 0; e < VEC; ++e) dst[first + c * gap + e] = acc[c][e];
+    }
+  };
+  for (int i0 = 0; i0 < end; i0 += SUM_AHEAD) {
+    if (i0 >= SUM_RUN && key[i0] != final) break;
+    Pack<T, VEC> v[SUM_AHEAD][COLS];
 #pragma unroll
     for (int i = 0; i < SUM_AHEAD; ++i) {
       const unsigned k = key[i0 + i];
-      if (k >= none) return;
+      if (k < none && k != skipped && (i0 < SUM_RUN || k == final)) {
+        const T* row = dy + (long long)pos[i0 + i] * p.ds;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] += to_f(v[i].v[e]);
+        for (int c = 0; c < COLS; ++c)
+          if (first + c * gap < p.D) v[i][c] = *reinterpret_cast<const Pack<T, VEC>*>(row + c * gap);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < SUM_AHEAD; ++i) {
+      const unsigned k = key[i0 + i];
+      if (k >= none || (i0 >= SUM_RUN && k != final)) return;
+      if (k == skipped) {
+        open = false;
+        continue;
+      }
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[c][e] += to_f(v[i][c].v[e]);
       if (key[i0 + i + 1] == k) continue;
-      if (open) store(p.part + run * 2 * p.D + col);
+      if (open) store(p.part + run * 2 * p.D);
       else {
-        Pack<T, VEC> o;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(acc[e] * p.scale);
-        *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(p.dw) + (long long)k * p.D + col) = o;
+        for (int c = 0; c < COLS; ++c) {
+          if (first + c * gap >= p.D) continue;
+          Pack<T, VEC> o;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(acc[c][e] * p.scale);
+          *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(p.dw) + (long long)k * p.D + first + c * gap) = o;
+        }
       }
       open = false;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+      clear();
     }
   }
-  if (key[SUM_RUN] == key[SUM_RUN - 1]) store(p.part + (run * 2 + (open ? 0 : 1)) * p.D + col);
+  if (goes_on && !whole) store(p.part + (run * 2 + (open ? 0 : 1)) * p.D);
 }
 
-// Rows shared by several groups of SUM_RUN tokens: the group in which such a
-// row begins adds the parts over JOIN_COLS columns.  A warp looks at one group
-// and adds a row of up to JOIN_SHORT parts by itself; longer ones are added by
+// Rows of more than two runs: the run in which such a row begins adds the
+// parts over JOIN_COLS columns.  A warp looks at one run and adds a row of up to JOIN_SHORT parts by itself; longer ones are added by
 // the whole block, in eight interleaved sums.
-constexpr int JOIN_RUNS = 8, JOIN_COLS = 128, JOIN_SHORT = 8;
+constexpr int JOIN_RUNS = 8, JOIN_COLS = 128, JOIN_SHORT = 8, JOIN_AHEAD = 10;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * JOIN_RUNS) embed_join_kernel(const SumArgs p) {
-  gdc_wait();
   constexpr int PER = JOIN_COLS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long runs = ((long long)p.N + SUM_RUN - 1) / SUM_RUN, base = (long long)blockIdx.x * JOIN_RUNS;
@@ -439,31 +524,41 @@ __global__ void __launch_bounds__(32 * JOIN_RUNS) embed_join_kernel(const SumArg
     }
   };
   auto add_parts = [&](long long r, long long end, int step, int from, float (&acc)[PER]) {
-#pragma unroll 4
-    for (; r < end; r += step) {
+    for (; r < end; r += JOIN_AHEAD * step) {
+      float v[JOIN_AHEAD][PER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int col = from + lane + 32 * j;
-        if (col < p.D) acc[j] += p.part[r * 2 * p.D + col];
-      }
+      for (int u = 0; u < JOIN_AHEAD; ++u)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const int col = from + lane + 32 * j;
+          v[u][j] = r + u * step < end && col < p.D ? p.part[(r + u * step) * 2 * p.D + col] : 0.f;
+        }
+#pragma unroll
+      for (int u = 0; u < JOIN_AHEAD; ++u)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) acc[j] += v[u][j];
     }
   };
   {
     const long long run = base + warp, from = run * SUM_RUN, end = from + SUM_RUN;
     unsigned k = p.V;
-    if (end < p.N) {
-      k = p.sorted[end - 1].x;
+    if (end + SUM_RUN < p.N) {
+      k = p.sorted[end + SUM_RUN].x;
+      const unsigned own = p.sorted[end - 1].x;
       const unsigned next = p.sorted[end].x, begin = p.sorted[from].x, before = from > 0 ? p.sorted[from - 1].x : ~0u;
-      if (next != k || (begin == k && before == k)) k = p.V;
+      if (own != k || next != k || (begin == k && before == k)) k = p.V;
     }
     bool wide = false;
     if (k < (unsigned)p.V) {
+      // the first run that does not begin with k (sorted: those that do come first), by steps of 32 runs, then of one
       long long last = run + 1;
-      for (;;) {
-        const long long r = last + lane;
-        const int n = __popc(__ballot_sync(0xffffffffu, r < runs && p.sorted[r * SUM_RUN].x == k));  // sorted: they come first
-        last += n;
-        if (n < 32) break;
+      for (int step = 32; step; step = step == 32 ? 1 : 0) {
+        for (;;) {
+          const long long r = last + (step == 32 ? 31 + 32 * lane : lane);
+          const int n = __popc(__ballot_sync(0xffffffffu, r < runs && p.sorted[r * SUM_RUN].x == k));
+          last += n * step;
+          if (n < 32) break;
+        }
       }
       wide = last - run > JOIN_SHORT;
       if (wide) {
@@ -530,41 +625,25 @@ Plan embed_plan(long long N, int V, int D) {
   return q;
 }
 
-// A launch that may start while the one before it on the stream ends: the
-// kernels wait for that one's results before they touch memory.
-template <class... Args, class... Given>
-int chain(void (*kernel)(Args...), dim3 grid, dim3 block, int shared, cudaStream_t s, const char* what, const Given&... given) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = (size_t)shared;
-  cfg.stream = s;
-  cudaLaunchAttribute at = {};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, given...);
-  return e == cudaSuccess ? GFN_OK : cuda_status(e, what);
-}
-
 template <typename T>
 int embed_sum(const SumArgs& p, long long runs, cudaStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
   const bool vec = aligned16(p.dy) && aligned16(p.dw) && p.D % VEC == 0 && (p.N == 1 || p.ds % VEC == 0);
-  const int per = vec ? VEC : 1, need = (p.D + per - 1) / per;
+  const int per = vec ? VEC : SUM_COLS, need = (p.D + per - 1) / per;
   int lanes = 8;
   while (lanes < SUM_THREADS && lanes < need) lanes *= 2;
   const dim3 block((unsigned)lanes, (unsigned)(SUM_THREADS / lanes));
   const dim3 grid((unsigned)((runs + block.y - 1) / block.y), (unsigned)((need + lanes - 1) / lanes));
   if (grid.y > 65535) return fail(GFN_ERR_UNSUPPORTED, "token_embed backward: dim %d", p.D);
-  const int shared = (int)block.y * (2 * SUM_RUN + 2) * 4;
-  const int st = vec ? chain(embed_sum_kernel<T, VEC>, grid, block, shared, s, "embed_sum_kernel", p)
-                     : chain(embed_sum_kernel<T, 1>, grid, block, shared, s, "embed_sum_kernel", p);
-  if (st != GFN_OK || runs < 2) return st;
+  const int shared = (int)block.y * SUM_WORDS * 4;
+  if (vec) embed_sum_kernel<T, VEC, 1><<<grid, block, shared, s>>>(p);
+  else embed_sum_kernel<T, 1, SUM_COLS><<<grid, block, shared, s>>>(p);
+  const int st = launch_status("embed_sum_kernel");
+  if (st != GFN_OK || runs < 3) return st;
   const int cols = (p.D + JOIN_COLS - 1) / JOIN_COLS;
   const dim3 joins((unsigned)((runs + JOIN_RUNS - 1) / JOIN_RUNS), (unsigned)(cols < 65535 ? cols : 65535));
-  return chain(embed_join_kernel<T>, joins, 32 * JOIN_RUNS, 0, s, "embed_join_kernel", p);
+  embed_join_kernel<T><<<joins, 32 * JOIN_RUNS, 0, s>>>(p);
+  return launch_status("embed_join_kernel");
 }
 
 }  // namespace
@@ -631,13 +710,15 @@ int gfn_token_embed_backward(const void* ids, int ids_are_64, long long tokens, 
   a.tiles = q.tiles; a.subs = q.subs; a.bits = q.bits; a.passes = q.passes;
   const unsigned fill = (unsigned)(4 * sms);
   if (tokens <= SORT_ONE) {
-    if ((st = chain(embed_sort_kernel, 1 + fill, SORT_THREADS, 0, s, "embed_sort_kernel", a)) != GFN_OK) return st;
+    embed_sort_kernel<<<1 + fill, SORT_THREADS, 0, s>>>(a);
+    if ((st = launch_status("embed_sort_kernel")) != GFN_OK) return st;
   } else {
-    if ((st = chain(embed_count_kernel, (unsigned)q.tiles + fill, SORT_THREADS, 0, s, "embed_count_kernel", a)) != GFN_OK)
-      return st;
-    for (int pass = 0; pass < q.passes; ++pass)
-      if ((st = chain(embed_rank_kernel, (unsigned)q.tiles + fill, SORT_THREADS, 0, s, "embed_rank_kernel", a, pass)) != GFN_OK)
-        return st;
+    embed_count_kernel<<<(unsigned)q.tiles + fill, SORT_THREADS, 0, s>>>(a);
+    if ((st = launch_status("embed_count_kernel")) != GFN_OK) return st;
+    for (int pass = 0; pass < q.passes; ++pass) {
+      embed_rank_kernel<<<(unsigned)q.tiles + fill, SORT_THREADS, 0, s>>>(a, pass);
+      if ((st = launch_status("embed_rank_kernel")) != GFN_OK) return st;
+    }
   }
   SumArgs b = {};
   b.sorted = a.sorted[(q.passes - 1) & 1];

@@ -133,7 +133,7 @@ class Manifold(nn.Module):
             return force_manual
         if isinstance(self.embedding, FunctionalEmbedding):
             return self.embedding(input_ids, out_dtype=self.force_dtype)
-        if self.library_embedding and isinstance(self.embedding, nn.Embedding):
+        if getattr(self, "library_embedding", False) and isinstance(self.embedding, nn.Embedding):
             return embed_tokens(input_ids, self.embedding.weight, padding_idx=self.embedding.padding_idx)
         return self.embedding(input_ids)
 
