@@ -26,6 +26,8 @@
 //     tf32 pieces.
 //   float32: every operand in two tf32 pieces, three products (2^-22).
 #pragma once
+#include <type_traits>
+
 #include "decay_attn.h"
 #include "lm_host.h"
 #include "lm_ops.cuh"
@@ -56,14 +58,16 @@ GFN_DEV float power(float lg, int n) { return exp2f(lg * (float)n); }
 
 // ---------------------------------------------------------------- fragments
 // Operands of one tensor-core step.  Lane l stands at g = l / 4, t = l % 4.
-// bfloat16: m16n8k16.  tf32: m16n8k8, where place t of the contraction is its
-// element 2 t and place t + 4 its element 2 t + 1 on both sides, so that two
-// neighbours are read at once and accumulators serve as operands as they are.
+// 16-bit types: m16n8k16, pairs of neighbours of the contraction in a register.
+// tf32: m16n8k8, where place t of the contraction is its element 2 t and place
+// t + 4 its element 2 t + 1 on both sides, so that two neighbours are read at
+// once, accumulators serve as operands as they are, and a 16-bit step's
+// registers hold two tf32 steps.
 template <typename T>
-struct Math {
-  static constexpr int KS = 8, PIECES = sizeof(T) == 4 ? 2 : 1;
+struct Math {  // float32
+  static constexpr int KS = 8, PIECES = 2;
   using State = float;
-  static constexpr int PAD = sizeof(T) == 4 ? 4 : 8, STATE_PAD = 4;
+  static constexpr int PAD = 4, STATE_PAD = 4;
   struct A {
     unsigned v[PIECES][4];
   };
@@ -71,11 +75,8 @@ struct Math {
     unsigned v[PIECES][2];
   };
 };
-template <>
-struct Math<__nv_bfloat16> {
-  static constexpr int KS = 16;
-  using State = __nv_bfloat16;
-  static constexpr int PAD = 8, STATE_PAD = 8;
+struct Math16 {
+  static constexpr int KS = 16, PAD = 8;
   struct A {
     unsigned v[4];
   };
@@ -83,9 +84,24 @@ struct Math<__nv_bfloat16> {
     unsigned v[2];
   };
 };
+template <>
+struct Math<__nv_bfloat16> : Math16 {
+  using State = __nv_bfloat16;
+  static constexpr int STATE_PAD = 8;
+};
+template <>
+struct Math<__half> : Math16 {
+  using State = float;  // tf32 values
+  static constexpr int STATE_PAD = 4;
+};
 
 GFN_DEV void mma_bf16(float (&c)[4], const unsigned (&a)[4], const unsigned (&b)[2]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+GFN_DEV void mma_f16(float (&c)[4], const unsigned (&a)[4], const unsigned (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
@@ -113,7 +129,8 @@ GFN_DEV void mma_pieces(float (&c)[4], const unsigned (&a)[PA][4], const unsigne
 }
 template <typename T>
 GFN_DEV void mma(float (&c)[4], const typename Math<T>::A& a, const typename Math<T>::B& b) {
-  if constexpr (Math<T>::KS == 16) mma_bf16(c, a.v, b.v);
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) mma_bf16(c, a.v, b.v);
+  else if constexpr (std::is_same_v<T, __half>) mma_f16(c, a.v, b.v);
   else mma_pieces(c, a.v, b.v);
 }
 
@@ -126,7 +143,6 @@ GFN_DEV void ldsm_t(unsigned& a, unsigned& b, unsigned& c, unsigned& d, const vo
                : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(smem_u32(p)));
 }
 GFN_DEV float2 pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
-GFN_DEV float2 pair(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
 
 // A, 16 rows from p [row][k].
 template <typename T>
@@ -186,6 +202,19 @@ GFN_DEV void load_bk(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) 
     }
   }
 }
+
+// Two float16 neighbours as tf32 (exact).
+GFN_DEV void unpack_f16(unsigned v, unsigned& lo, unsigned& hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  lo = __float_as_uint(f.x);
+  hi = __float_as_uint(f.y);
+}
+// Step q (0, 1) of eight of a 16-bit operand, as tf32.
+GFN_DEV void half_step(const Math16::A& f, int q, unsigned (&a)[4]) {
+  unpack_f16(f.v[2 * q], a[0], a[2]);
+  unpack_f16(f.v[2 * q + 1], a[1], a[3]);
+}
+GFN_DEV void half_step(const Math16::B& f, int q, unsigned (&b)[2]) { unpack_f16(f.v[q], b[0], b[1]); }
 
 GFN_DEV unsigned pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -298,17 +327,18 @@ struct Decay {
   }
 };
 
-// attend (see attend_tf32) for bfloat16: the keys' tiles of 16 one after the other, from
-// the diagonal back, so that eight scores are in registers instead of a row of
-// them and no branch stands within a tile.
-template <int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
-GFN_DEV void attend_bf16(float (&o)[ON][4], const __nv_bfloat16* rows, const __nv_bfloat16* keys, const __nv_bfloat16* values,
-                         const __nv_bfloat16* st, int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
-  using T = __nv_bfloat16;
+// attend (see attend_f32) for the 16-bit types: the keys' tiles of 16 one after
+// the other, from the diagonal back, so that eight scores are in registers
+// instead of a row of them and no branch stands within a tile.  float16 rows and
+// values meet state and scores as tf32.
+template <typename T, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
+GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
+                       int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
   using M = Math<T>;
+  constexpr bool HALF = std::is_same_v<T, __half>;
   constexpr int KN = DA / 16;
   const int lane = threadIdx.x & 31;
-  M::A a[KN];
+  typename M::A a[KN];
 #pragma unroll
   for (int k = 0; k < KN; ++k) load_a<T>(a[k], rows + rt * 16 * LDA + k * 16, LDA, lane);
 #pragma unroll
@@ -318,15 +348,37 @@ GFN_DEV void attend_bf16(float (&o)[ON][4], const __nv_bfloat16* rows, const __n
 #pragma unroll
   for (int k = 0; k < KN; ++k) {
     if (!FULL && k * 16 >= kd) continue;
+    if constexpr (HALF) {
 #pragma unroll
-    for (int i = 0; i < ON; i += 2) {
-      const int col = col0 + i * 8;
-      if (!FULL && col >= nd) continue;
-      M::B b[2];
-      if (NMAJOR) load_bn<T>(b, st + col * LS + k * 16, LS, lane);
-      else load_bk<T>(b, st + k * 16 * LS + col, LS, lane);
-      mma<T>(o[i], a[k], b[0]);
-      mma<T>(o[i + 1], a[k], b[1]);
+      for (int q = 0; q < 2; ++q) {
+        unsigned aq[4];
+        half_step(a[k], q, aq);
+#pragma unroll
+        for (int i = 0; i < ON; ++i) {
+          const int col = col0 + i * 8 + (lane >> 2), kk = k * 16 + q * 8 + 2 * (lane & 3);
+          unsigned b[2];
+          if (NMAJOR) {
+            const float2 x = pair(st + col * LS + kk);
+            b[0] = __float_as_uint(x.x);
+            b[1] = __float_as_uint(x.y);
+          } else {
+            b[0] = __float_as_uint(st[kk * LS + col]);
+            b[1] = __float_as_uint(st[(kk + 1) * LS + col]);
+          }
+          mma_tf32(o[i], aq, b);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < ON; i += 2) {
+        const int col = col0 + i * 8;
+        if (!FULL && col >= nd) continue;
+        typename M::B b[2];
+        if (NMAJOR) load_bn<T>(b, st + col * LS + k * 16, LS, lane);
+        else load_bk<T>(b, st + k * 16 * LS + col, LS, lane);
+        mma<T>(o[i], a[k], b[0]);
+        mma<T>(o[i + 1], a[k], b[1]);
+      }
     }
   }
 #pragma unroll
@@ -342,25 +394,47 @@ GFN_DEV void attend_bf16(float (&o)[ON][4], const __nv_bfloat16* rows, const __n
 #pragma unroll
     for (int k = 0; k < KN; ++k) {
       if (!FULL && k * 16 >= kd) continue;
-      M::B b[2];
+      typename M::B b[2];
       load_bn<T>(b, keys + i * 16 * LDA + k * 16, LDA, lane);
       mma<T>(s[0], a[k], b[0]);
       mma<T>(s[1], a[k], b[1]);
     }
   };
   auto add = [&](int i, const float (&s)[2][4]) {
-    M::A p;
-    p.v[0] = pack_bf16(s[0][0], s[0][1]);
-    p.v[1] = pack_bf16(s[0][2], s[0][3]);
-    p.v[2] = pack_bf16(s[1][0], s[1][1]);
-    p.v[3] = pack_bf16(s[1][2], s[1][3]);
+    typename M::A p;
+    unsigned pq[2][4];
+    if constexpr (HALF) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float w[4] = {s[q][0], s[q][2], s[q][1], s[q][3]};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pq[q][e] = tf32(w[e]);
+      }
+    } else {
+      p.v[0] = pack_bf16(s[0][0], s[0][1]);
+      p.v[1] = pack_bf16(s[0][2], s[0][3]);
+      p.v[2] = pack_bf16(s[1][0], s[1][1]);
+      p.v[3] = pack_bf16(s[1][2], s[1][3]);
+    }
 #pragma unroll
     for (int n = 0; n < ON; n += 2) {
       if (!FULL && col0 + n * 8 >= nd) continue;
-      M::B b[2];
+      typename M::B b[2];
       load_bk<T>(b, values + i * 16 * LDB + col0 + n * 8, LDB, lane);
-      mma<T>(o[n], p, b[0]);
-      mma<T>(o[n + 1], p, b[1]);
+      if constexpr (HALF) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            unsigned bq[2];
+            half_step(b[z], q, bq);
+            mma_tf32(o[n + z], pq[q], bq);
+          }
+        }
+      } else {
+        mma<T>(o[n], p, b[0]);
+        mma<T>(o[n + 1], p, b[1]);
+      }
     }
   };
   float s[2][4];
@@ -390,7 +464,7 @@ GFN_DEV void attend_bf16(float (&o)[ON][4], const __nv_bfloat16* rows, const __n
 // rows, keys [C][LDA] with kd of their columns in use, values [C][LDB]; st: the
 // state, seen from this product as [k][n] or (NMAJOR) [n][k].
 template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
-GFN_DEV void attend_tf32(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
+GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
                          int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
   using M = Math<T>;
   const int lane = threadIdx.x & 31;
@@ -459,20 +533,13 @@ GFN_DEV void attend_tf32(float (&o)[ON][4], const T* rows, const T* keys, const 
 #pragma unroll
     for (int q = 0; q < 16 / M::KS; ++q) {
       typename M::A a;
-      if constexpr (M::KS == 16) {
-        a.v[0] = pack_bf16(s[2 * i][0], s[2 * i][1]);
-        a.v[1] = pack_bf16(s[2 * i][2], s[2 * i][3]);
-        a.v[2] = pack_bf16(s[2 * i + 1][0], s[2 * i + 1][1]);
-        a.v[3] = pack_bf16(s[2 * i + 1][2], s[2 * i + 1][3]);
-      } else {
-        const float w[4] = {s[2 * i + q][0], s[2 * i + q][2], s[2 * i + q][1], s[2 * i + q][3]};
+      const float w[4] = {s[2 * i + q][0], s[2 * i + q][2], s[2 * i + q][1], s[2 * i + q][3]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          unsigned r[M::PIECES];
-          pieces(w[e], r);
+      for (int e = 0; e < 4; ++e) {
+        unsigned r[M::PIECES];
+        pieces(w[e], r);
 #pragma unroll
-          for (int z = 0; z < M::PIECES; ++z) a.v[z][e] = r[z];
-        }
+        for (int z = 0; z < M::PIECES; ++z) a.v[z][e] = r[z];
       }
       const T* v = values + (16 * i + M::KS * q) * LDB + col0;
 #pragma unroll
@@ -491,9 +558,9 @@ template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJ
 GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
                     int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
   if constexpr (Math<T>::KS == 16)
-    attend_bf16<DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
+    attend_16<T, DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
   else
-    attend_tf32<T, C, DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
+    attend_f32<T, C, DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
 }
 
 // Two values in three bfloat16 pieces each (cut, not rounded), which add up to
@@ -531,7 +598,40 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
 #pragma unroll
     for (int k = 0; k < C; k += M::KS) {
       const T* vals = values + k * LDV + n0 + at * 8;
-      if constexpr (M::KS == 16) {
+      if constexpr (std::is_same_v<T, __half>) {
+        unsigned raw[4], a[2][2][4];  // step, piece
+        ldsm_t(raw[0], raw[1], raw[2], raw[3], keys + (k + (lane & 7) + ((lane >> 4) << 3)) * LDK + m0 + (lane & 8));
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float w0 = wt[k + 8 * q + 2 * t], w1 = wt[k + 8 * q + 2 * t + 1];
+          unsigned x[4];
+          unpack_f16(raw[2 * q], x[0], x[2]);
+          unpack_f16(raw[2 * q + 1], x[1], x[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            unsigned r[2];
+            pieces(__uint_as_float(x[e]) * (e < 2 ? w0 : w1), r);
+            a[q][0][e] = r[0];
+            a[q][1][e] = r[1];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < AT; n += 2) {
+          if (!FULL && n0 + (at + n) * 8 >= nd) continue;
+          typename M::B b[2];
+          load_bk<T>(b, vals + n * 8, LDV, lane);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              unsigned bq[2];
+              half_step(b[z], q, bq);
+              mma_tf32(add[n + z], a[q][1], bq);
+              mma_tf32(add[n + z], a[q][0], bq);
+            }
+          }
+        }
+      } else if constexpr (M::KS == 16) {
         unsigned raw[4], a[3][4];
         ldsm_t(raw[0], raw[1], raw[2], raw[3], keys + (k + (lane & 7) + ((lane >> 4) << 3)) * LDK + m0 + (lane & 8));
 #pragma unroll
@@ -689,10 +789,11 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
     for (int i = 0; i < S::SN; ++i) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        if constexpr (M::KS == 16)
-          *reinterpret_cast<unsigned*>(q + 8 * half * S::LS + i * 8) = pack_bf16(st[i][2 * half], st[i][2 * half + 1]);
-        else
-          *reinterpret_cast<float2*>(q + 8 * half * S::LS + i * 8) = make_float2(st[i][2 * half], st[i][2 * half + 1]);
+        const float x = st[i][2 * half], y = st[i][2 * half + 1];
+        Op* at = q + 8 * half * S::LS + i * 8;
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) *reinterpret_cast<unsigned*>(at) = pack_bf16(x, y);
+        else if constexpr (std::is_same_v<T, __half>) *reinterpret_cast<uint2*>(at) = make_uint2(tf32(x), tf32(y));
+        else *reinterpret_cast<float2*>(at) = make_float2(x, y);
       }
     }
   };
