@@ -331,11 +331,17 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(const LpArgs p) {
              __shfl_xor_sync(0xffffffffu, bu, o));
   if (lane == 0) sh.warp[warp] = make_float3(bm, bs, bu);
   __syncthreads();
-  bm = sh.warp[0].x;
-  bs = sh.warp[0].y;
-  bu = sh.warp[0].z;
+  bm = sh.warp[lane % LP_WARPS].x;
+  bs = sh.warp[lane % LP_WARPS].y;
+  bu = sh.warp[lane % LP_WARPS].z;
 #pragma unroll
-  for (int w = 1; w < LP_WARPS; ++w) lp_merge(bm, bs, bu, sh.warp[w].x, sh.warp[w].y, sh.warp[w].z);
+  for (int o = LP_WARPS / 2; o; o >>= 1)
+    lp_merge(bm, bs, bu, __shfl_xor_sync(0xffffffffu, bm, o), __shfl_xor_sync(0xffffffffu, bs, o),
+             __shfl_xor_sync(0xffffffffu, bu, o));
+  // the same bits for every thread: lanes merge in different orders
+  bm = __shfl_sync(0xffffffffu, bm, 0);
+  bs = __shfl_sync(0xffffffffu, bs, 0);
+  bu = __shfl_sync(0xffffffffu, bu, 0);
   // the first block runs by now, so that its shared memory can be written
   if (SHARED_ROW) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   if (TOP) {
@@ -404,7 +410,7 @@ int lp_launch(const LpArgs& p, cudaStream_t s) {
   if (st != GFN_OK) return st;
   // Few rows: up to eight blocks share one, as long as each has 8 KB to read
   // and there are not two blocks per SM yet
-  // (256 x 50257 bfloat16: four blocks a row 29 us, two PARTS2).
+  // (256 x 50257 bfloat16: four blocks a row 29 us, two 20).
   int parts = 1;
   const long long bytes = (long long)p.V * sizeof(T);
   while (parts < LP_CLUSTER && p.rows * parts < 2LL * sms && bytes / (2 * parts) >= 8192) parts *= 2;

@@ -221,6 +221,15 @@ def test_given_tokens_ignored_and_outside():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 300, 2000])
+def test_a_given_token_among_the_alternatives_has_the_same_bits(N):
+    x, _ = _case(N, 3001, torch.float32)
+    r = gfn.token_logprobs(x, x.argmax(-1), top=3)
+    assert torch.equal(r.logprobs, r.top_logprobs[:, 0]) and torch.equal(r.top_tokens[:, 0], x.argmax(-1))
+    assert (r.top_logprobs <= 0).all()
+
+
+@pytest.mark.gpu
 def test_generate_with_logprobs():
     torch.manual_seed(0)
     m = gfn.Manifold(vocab_size=17, dim=16, depth=1, heads=2, use_scan=True).to(DEV)
