@@ -618,9 +618,9 @@ int gfn_token_logprobs_backward(const void* logits, long long logits_row_stride,
  * [batch][heads][kdim][vdim] float or NULL (zero / not wanted).  lengths
  * [batch] int64 (lengths_are_64) or int32, or NULL (all `length`; clamped to
  * [0, length]): tokens behind a sequence's length are not read, do not reach
- * the state, and get zeros.  kdim, vdim up to 128.  A block of 64 tokens is
- * one step: NaN or infinity in k or v reaches that block's earlier outputs
- * too.  `workspace` of gfn_decay_attention_workspace_bytes() (on the current
+ * the state, and get zeros.  kdim, vdim up to 128.  Tokens are
+ * taken in tiles of 16: NaN or infinity in k or v reaches the outputs of up to
+ * 15 tokens before it too (in q or d_o the gradients of 15 behind it).  `workspace` of gfn_decay_attention_workspace_bytes() (on the current
  * device; one for each pass), 16-byte aligned.  forward_workspace: the
  * forward's, left as it was, for length above 1, or NULL (its states are worked
  * out again).  Results repeat bit for bit. */

@@ -103,7 +103,8 @@ struct LpRow {
 GFN_DEV void lp_merge(float& m, float& s, float& u, float m2, float s2, float u2) {
   const float mn = fmaxf(m, m2), base = mn == -INFINITY ? 0.f : mn;
   const float c1 = exp2_fast((m - base) * LP_LOG2E), c2 = exp2_fast((m2 - base) * LP_LOG2E);
-  u = c1 * (u + (m == -INFINITY ? 0.f : m - base) * s) + c2 * (u2 + (m2 == -INFINITY ? 0.f : m2 - base) * s2);
+  // far maxima count as LP_LOW away: their factor is 0, and their distance times a sum could be infinite
+  u = c1 * (u + fmaxf(m - base, LP_LOW) * s) + c2 * (u2 + fmaxf(m2 - base, LP_LOW) * s2);
   s = c1 * s + c2 * s2;
   m = mn;
 }
@@ -140,7 +141,7 @@ GFN_DEV void lp_add(const Pack<T, VEC> (&raw)[N], int g, float& m, float& s, flo
     mn = fmaxf(mn, gm);
   }
   const float base = mn == -INFINITY ? 0.f : mn, c = exp2_fast((m - base) * LP_LOG2E);
-  if (ENT) u = c * (u + (m == -INFINITY ? 0.f : m - base) * s);
+  if (ENT) u = c * (u + fmaxf(m - base, LP_LOW) * s);
   m = mn;
   F2 s2 = f2(s * c, 0.f), u2 = f2(u, 0.f);
   const F2 nb = f2(-base), l2 = f2(LP_LOG2E);

@@ -498,7 +498,7 @@ struct Heads {
   Tensor t;
   long long strides[3];
   explicit Heads(const Tensor& u) : t(u.is_contiguous() || u.stride(3) == 1 || u.size(3) == 1 ? u : u.contiguous()) {
-    for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
+    for (int i = 0; i < 3; ++i) strides[i] = t.size(i) > 1 ? t.stride(i) : 0;  // one element: its stride says nothing
   }
   const void* p() const { return ptr(t); }
 };

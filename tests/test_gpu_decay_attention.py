@@ -123,6 +123,37 @@ def test_padded_batches(L, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_how_far_a_bad_token_reaches(bad, dtype):
+    """Up to 15 tokens against the order of the pass, one sequence, one head."""
+    q, k, v, decay, st, _ = _case(2, 300, 2, 24, 40, dtype)
+    do = torch.randn(v.shape, generator=torch.Generator().manual_seed(3)).to(dtype).to(DEV)
+
+    def both(*ts):
+        leaves = [t.clone().requires_grad_(True) for t in ts]
+        o = gfn.decay_attention(*leaves, decay, state=st)
+        return (o, *torch.autograd.grad(o, leaves, do))
+    want = both(q, k, v)
+    for i in range(3):
+        for t in (70, 127, 128, 200):
+            ts = [q.clone(), k.clone(), v.clone()]
+            ts[i][1, t, 1] = bad
+            got = both(*ts)
+            for a, b in zip(got, want):
+                assert torch.equal(a[0], b[0]) and torch.equal(a[1, :, 0], b[1, :, 0])  # other sequences, other heads
+            early, late = slice(0, t - 15), slice(t + 16, None)
+            if i == 0:  # q: its own output; dk and dv before it, and up to 15 tokens behind
+                assert torch.equal(got[0][1, :t], want[0][1, :t]) and torch.equal(got[0][1, t + 1:], want[0][1, t + 1:])
+                for g, w in zip(got[2:], want[2:]):
+                    assert torch.equal(g[1, late], w[1, late])
+                assert torch.equal(got[1], want[1])
+            else:  # k, v: outputs from the token on, and up to 15 before
+                assert torch.equal(got[0][1, early], want[0][1, early])
+                assert not torch.isfinite(got[0][1, t, 1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_decays_from_0_to_1(dtype):
     q, k, v, _, st, _ = _case(1, 150, 6, 16, 24, dtype)
     decay = torch.tensor([0.0, 1e-30, 1e-3, 0.5, 1 - 2.0 ** -20, 1.0], device=DEV)
@@ -240,3 +271,36 @@ def test_repeats_bit_for_bit():
     for _ in range(3):
         for a, b in zip(first, once()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_far_apart_tokens_and_offsets_past_32_bits(dtype):
+    """Views whose batch or token stride passes 2^31 elements, in and behind the same allocation."""
+    size = 2 if dtype != torch.float32 else 4
+    base = torch.zeros(2 ** 31 // 2 * 3, device=DEV, dtype=dtype)  # 2^31 elements lie between the first and the last third
+    q, k, v, decay, st, _ = _case(3, 5, 2, 16, 16, dtype)
+    far = lambda t, at: base.as_strided(t.shape, (2 ** 30 + 8 * size, 64, 16, 1), at).copy_(t)  # noqa: E731
+    a, b, c = far(q, 0), far(k, 1024), far(v, 2048)
+    o, last = gfn.decay_attention(q, k, v, decay, state=st, return_state=True)
+    o2, last2 = gfn.decay_attention(a, b, c, decay, state=st, return_state=True)
+    assert torch.equal(o, o2) and torch.equal(last, last2)
+    del base, a, b, c
+
+
+@pytest.mark.gpu
+def test_a_million_tokens():
+    """One long sequence: the state behind 2^20 tokens against float64 sums (a decay of 1 adds them all)."""
+    n = 2 ** 20 + 37
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q, k, v = (torch.randn(1, n, 1, 8, device=DEV, generator=g).bfloat16() for _ in range(3))
+    for gam in (1.0, 1 - 2.0 ** -10):
+        decay = torch.tensor([gam], device=DEV)
+        o, last = gfn.decay_attention(q, k, v, decay, return_state=True)
+        w = gam ** torch.arange(n - 1, -1, -1, device=DEV, dtype=torch.float64)
+        want = torch.einsum("t,tk,tv->kv", w, k[0, :, 0].double(), v[0, :, 0].double())
+        big = torch.einsum("t,tk,tv->kv", w, k[0, :, 0].double().abs(), v[0, :, 0].double().abs())
+        assert ((last[0, 0] - want).abs() <= 2.0 ** -18 * big).all()
+        tail = (q[0, -1, 0].double() @ want)
+        bound = 2.0 ** -8 * (q[0, -1, 0].double().abs() @ want.abs()) + 2.0 ** -8 * tail.abs() + 2.0 ** -8 * 64 * 8 * 16
+        assert ((o[0, -1, 0] - tail).abs() <= bound).all()

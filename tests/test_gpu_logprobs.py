@@ -29,6 +29,9 @@ def _np(t):
 def _close(got, want, tol):
     assert got.shape == want.shape
     assert np.array_equal(np.isnan(got), np.isnan(want))
+    # the results are float32: lowest - highest = -6.8e38 is -inf there (rounding to nearest goes to
+    # infinity from (2 - 2^-24) 2^127 = 3.4028236e38 on)
+    want = np.where(np.abs(want) >= (2 - 2.0 ** -24) * 2.0 ** 127, np.copysign(np.inf, want), want)
     inf = np.isinf(want)
     assert np.array_equal(got[inf], want[inf])
     ok = ~(inf | np.isnan(want))
@@ -162,6 +165,23 @@ def test_logits_of_any_size():
     x[:, 3] = 65504.0
     x[1, 4] = -65504.0
     _check(x, t, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [3, 700])
+def test_masks_of_the_types_lowest_value(N, dtype):
+    """A mask of finfo.min instead of -inf: probability 0 beside others, and a uniform row where it is all there is."""
+    V, low = 1003, torch.finfo(dtype).min
+    x, t = _case(N, V, dtype)
+    x[0] = low
+    x[1, 5:] = low
+    x[2, ::2] = torch.finfo(dtype).max
+    x[2, 1::2] = low
+    t[1] = 3
+    r, d = _check(x, t, 7)
+    assert abs(r.entropy[0].item() - np.log(V)) < 1e-5 and r.top_tokens[0].tolist() == list(range(7))
+    assert r.top_tokens[1].tolist()[5:] == [5, 6] and torch.isfinite(d).all()
 
 
 @pytest.mark.gpu
