@@ -877,11 +877,10 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
   }
 }
 
-// The states before each segment, from what each segment adds; in place.  Up to
-// JOIN segments' parts are on their way at once.
-template <bool BACK>
+// The states before each segment, from what each segment adds; in place.  JOIN
+// segments' parts are on their way at once.
+template <bool BACK, int JOIN>
 __global__ void __launch_bounds__(256) attn_join_kernel(const PassArgs p) {
-  constexpr int JOIN = 16;
   const int mat = p.KD * p.VD, i = blockIdx.x * 256 + threadIdx.x;
   const long long bh = blockIdx.y + (long long)gridDim.y * blockIdx.z;
   if (i >= mat || bh >= (long long)p.B * p.H) return;
@@ -908,6 +907,62 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const PassArgs p) {
     }
   }
   if (p.state_out) p.state_out[bh * mat + i] = s;
+}
+
+// The same for many segments of few heads: a warp has 32 cells of the state over
+// an eighth of the segments, whose maps s -> g^n s + add are composed, handed on
+// and then applied one by one.
+template <bool BACK>
+__global__ void __launch_bounds__(256) attn_join_long_kernel(const PassArgs p) {
+  constexpr int PARTS = 8, AHEAD = 8;
+  __shared__ float sums[PARTS][32], gains[PARTS];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int mat = p.KD * p.VD, i = blockIdx.x * 32 + lane;
+  const long long bh = blockIdx.y + (long long)gridDim.y * blockIdx.z;
+  if (bh >= (long long)p.B * p.H) return;
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H), len = length_of(p, b);
+  const float lg = log2_decay(p.decay[h]), whole = power(lg, p.seg_len);
+  const bool live = i < mat;
+  float* q = p.segs + bh * p.segments * mat + i;
+  auto place = [&](int k) { return BACK ? p.segments - 1 - k : k; };
+  auto tokens = [&](int k) { return min(max(len - place(k) * p.seg_len, 0), p.seg_len); };
+  auto gain = [&](int k) {
+    const int n = tokens(k);
+    return n == p.seg_len ? whole : power(lg, n);
+  };
+  const int per = (p.segments + PARTS - 1) / PARTS, from = min(part * per, p.segments), to = min(from + per, p.segments);
+  float add[AHEAD], s = 0.f, g = 1.f;
+  auto read = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) add[u] = live && k0 + u < to ? q[(long long)place(k0 + u) * mat] : 0.f;
+  };
+  for (int k0 = from; k0 < to; k0 += AHEAD) {
+    read(k0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (k0 + u >= to) continue;
+      const float w = gain(k0 + u);
+      s = fmaf(w, s, add[u]);
+      g *= w;
+    }
+  }
+  sums[part][lane] = s;
+  if (lane == 0) gains[part] = g;
+  __syncthreads();
+  if (!live) return;
+  const int row = i / p.VD, col = i % p.VD;
+  s = p.state ? p.state[bh * mat + row * p.sr + col * p.sc] : 0.f;
+  for (int r = 0; r < part; ++r) s = fmaf(gains[r], s, sums[r][lane]);
+  for (int k0 = from; k0 < to; k0 += AHEAD) {
+    if (per > AHEAD) read(k0);  // a single batch is still there
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (k0 + u >= to) continue;
+      q[(long long)place(k0 + u) * mat] = s;
+      s = fmaf(gain(k0 + u), s, add[u]);
+    }
+  }
+  if (part == PARTS - 1 && p.state_out) p.state_out[bh * mat + i] = s;
 }
 
 // One token: the state is read, moved on and written once.  A thread owns VEC
@@ -1008,7 +1063,15 @@ int attn_pass(PassArgs p, bool known, cudaStream_t s) {
     int st = attn_run<T, DK, DV, BACK, STATE>(w, s);
     if (st != GFN_OK) return st;
     const int bh = p.B * p.H, y = bh < 32768 ? bh : 32768;
-    attn_join_kernel<BACK><<<dim3((unsigned)((p.KD * p.VD + 255) / 256), y, (bh + y - 1) / y), 256, 0, s>>>(w);
+    // one head, 342 segments of 64 x 64: 22 us by one thread a cell, 12 by eight;
+    // 40 heads, 3 segments of 128 x 128: 97 by eight, by one 20 with 4 parts
+    // under way and 43 with 32; 8 heads, 54 segments: 7.5 with 16, 6.3 with 32
+    const bool many = p.segments > 96;
+    const dim3 grid((unsigned)((p.KD * p.VD + (many ? 31 : 255)) / (many ? 32 : 256)), y, (bh + y - 1) / y);
+    if (many) attn_join_long_kernel<BACK><<<grid, 256, 0, s>>>(w);
+    else if (p.segments <= 4) attn_join_kernel<BACK, 4><<<grid, 256, 0, s>>>(w);
+    else if (p.segments <= 16) attn_join_kernel<BACK, 16><<<grid, 256, 0, s>>>(w);
+    else attn_join_kernel<BACK, 32><<<grid, 256, 0, s>>>(w);
     if ((st = launch_status("attn_join_kernel")) != GFN_OK) return st;
   }
   return attn_run<T, DK, DV, BACK, KIND>(p, s);

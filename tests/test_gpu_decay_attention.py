@@ -89,7 +89,8 @@ def test_outputs_state_and_gradients(B, L, H, K, V, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("B,L,H,K,V", [(1, 1100, 2, 64, 64), (3, 700, 1, 20, 24), (1, 1030, 1, 128, 96), (2, 2500, 2, 32, 16)])
+@pytest.mark.parametrize("B,L,H,K,V", [(1, 1100, 2, 64, 64), (3, 700, 1, 20, 24), (1, 1030, 1, 128, 96), (2, 2500, 2, 32, 16),
+                                       (1, 16000, 1, 24, 9)])
 def test_sequences_cut_into_segments(B, L, H, K, V, dtype):
     q, k, v, decay, st, lengths = _case(B, L, H, K, V, dtype, seed=L, ragged=True)
     _run(q, k, v, decay, st, None, K ** -0.5)
