@@ -258,9 +258,6 @@ struct Shape {
   static constexpr int resident(int kind) { return fit(kind, stages(kind), buffers(kind)); }
 };
 
-// Brings rows 0 .. n - 1 of a block into shared memory, zeros behind them; row
-// r is the r-th token from `at` on (BACK: from there to the front).  Columns
-// from `dim` on were zeroed once and stay so.
 template <int BYTES>
 GFN_DEV void copy_async(uint32_t to, const void* from, int read) {
   if constexpr (BYTES == 16)
@@ -283,6 +280,9 @@ GFN_DEV void fetch_pieces(T* dst, const T* src, const void* any, long long sl, i
     from += step;
   }
 }
+// Brings rows 0 .. n - 1 of a block into shared memory, zeros behind them; row
+// r is the r-th token from `at` on (BACK: from there to the front).  Columns
+// from `dim` on were zeroed once and stay so.
 template <typename T, int D, int LD, int C, int THREADS, bool BACK, bool FULL>
 GFN_DEV void fetch(T* dst, const View& v, int b, int h, int dim, int at, int n, int piece) {
   const T* src = static_cast<const T*>(v.p) + b * v.sb + h * v.sh + at * v.sl;

@@ -217,7 +217,9 @@ GFN_DEV void lp_top(LpShared& sh, const LpRow<T>& row, int g0, int g1, int top, 
   // The threads that may hold one of them, and their groups shared out to all:
   // a thread reading its own again (the first form) kept every warp busy with
   // a few lanes (4099 x 50257 bfloat16, 8 alternatives: 290 us against 99).
-  if (!odd && mine && high >= tau) sh.holders[atomicAdd(&sh.holding, 1)] = (unsigned short)tid;
+  // Of logits of -inf, the first 64 tokens hold enough: fewer than `top` are above.
+  if (!odd && mine && high >= tau && (m > -INFINITY || lo < 2 * LP_TOP))
+    sh.holders[atomicAdd(&sh.holding, 1)] = (unsigned short)tid;
   __syncthreads();
   const int per = (g1 - g0 + LP_THREADS - 1) / LP_THREADS, visits = sh.holding * per;
   const float floor = key_value(tau);  // -inf, or 0 as a key, lets every logit through
@@ -236,7 +238,6 @@ GFN_DEV void lp_top(LpShared& sh, const LpRow<T>& row, int g0, int g1, int top, 
     for (int e = 0; e < VEC; ++e) {
       const int j = g * VEC + e - row.phase;
       if (j < 0 || j >= row.end - row.phase) continue;
-      // of logits of -inf, the first 64 tokens hold enough: fewer than `top` are above
       if (f[e] == -INFINITY && j >= 2 * LP_TOP) continue;
       const unsigned long long k = rank_key(f[e], (unsigned)j);
       if (k < tau) continue;

@@ -133,9 +133,13 @@ class Manifold(nn.Module):
             return force_manual
         if isinstance(self.embedding, FunctionalEmbedding):
             return self.embedding(input_ids, out_dtype=self.force_dtype)
-        if getattr(self, "library_embedding", False) and isinstance(self.embedding, nn.Embedding):
+        if getattr(self, "library_embedding", False) and self._plain_table():
             return embed_tokens(input_ids, self.embedding.weight, padding_idx=self.embedding.padding_idx)
         return self.embedding(input_ids)
+
+    def _plain_table(self):
+        """Whether a token's force is its row of the embedding's weight (not scaled, as gfn.Embedding can)."""
+        return isinstance(self.embedding, nn.Embedding) and getattr(self.embedding, "scale", 1.0) == 1.0
 
     def _apply_readout(self, out):
         """The readout: nn.Linear through the split-fp16 tensor-core GEMMs
@@ -173,7 +177,7 @@ class Manifold(nn.Module):
             x, v = state
         mask = attention_mask
         base_dt = self.layers[0].base_dt
-        if force_manual is None and isinstance(self.embedding, nn.Embedding):
+        if force_manual is None and self._plain_table():
             x_seq, v_seq, xf, vf = seq(x, v, packed, meta, base_dt, ids=input_ids,
                                        table=self.embedding.weight, mask=mask, want_v_seq=want_v_seq)
             forces = None

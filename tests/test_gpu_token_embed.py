@@ -166,3 +166,22 @@ def test_the_library_embedding_of_a_model():
         n = torch.bincount(ids.flatten(), minlength=40).max().item()
         big = grads[0].abs().max().item()
         assert (grads[1] - grads[0]).abs().max().item() <= 4 * (n + 4) * 2.0 ** -24 * n * big
+
+
+@pytest.mark.gpu
+def test_a_model_with_a_scaled_embedding():
+    """A gfn.Embedding with a factor in a model's place: the fused lookup, which knows no factor, is not taken."""
+    for scan in (False, True):
+        torch.manual_seed(0)
+        model = gfn.Manifold(vocab_size=40, dim=32, depth=1, heads=2, rank=4, use_scan=scan,
+                             integrator_type="leapfrog", base_dt=0.1).to(DEV)
+        ids = _ids(60, 40).view(2, 30)
+        scaled = gfn.Embedding(40, 32, scale=3.0).to(DEV)
+        with torch.no_grad():
+            scaled.weight.copy_(model.embedding.weight)
+            want = model(force_manual=3.0 * model.embedding(ids))[0]
+            model.embedding = scaled
+            for on in (False, True):
+                model.use_library_embedding(on)
+                # the products of 3 and the weights round once on either side
+                assert torch.equal(model(ids)[0], want)
