@@ -569,8 +569,8 @@ int gfn_process_logits(const void* logits, long long logits_row_stride, int dtyp
  * contiguous.  A token outside [0, vocab) gives a row of zeros, takes no part
  * in the gradient and sets GFN_DEVERR_BAD_TOKEN.  The backward writes every
  * row of dweight [vocab][dim] (contiguous, of `dtype`); tokens equal to
- * padding_id (-1: none) take no part.  Sums are float32 in the order of the
- * tokens, rounded once; results repeat bit for bit.  Its workspace of
+ * padding_id (-1: none) take no part.  Sums are float32 in a fixed order,
+ * rounded once; results repeat bit for bit.  Its workspace of
  * gfn_token_embed_backward_workspace_bytes() (negative: too large) is 16-byte
  * aligned.  16-byte aligned rows take 128-bit accesses. */
 int gfn_token_embed_forward(const void* ids, int ids_are_64, long long tokens, const void* weight,

@@ -6,8 +6,13 @@
 // (the reference's nn.Embedding, gfn/model.py:52-66, whose gradient it leaves
 // to torch).  Both are bound by HBM.  The gradient sorts the tokens by id, a
 // stable radix sort, so that every row of the table has one owner that sums
-// its tokens in the order of the sequence: no float atomics, the same bits on
-// every run.  Sums are float32 and are rounded once.
+// its tokens in a fixed order (that of the sequence; rows of more than two runs
+// of 32 tokens by parts): no float atomics, the same bits on every run.  Sums are
+// float32 and are rounded once.
+//
+// Kernels, us, on one B200: 65536 tokens of 50257 x 1024 bfloat16 looked up 34
+// (185 MB, 5.4 TB/s); 65536 of 32000 x 512 float32, lookup 30 (4.4 TB/s written),
+// gradient 66: sort and 65 MB of zeros 26, sums 32 (134 MB read), joins 8.
 #include "lm_host.h"
 #include "lm_ops.cuh"
 
@@ -200,7 +205,10 @@ int embed_forward(EmbedArgs p, cudaStream_t s) {
 // The sort: digits of up to 9 bits, least significant first.  A tile of
 // tokens is ranked by a block; where it writes a digit follows from the counts
 // of every digit in every tile, which the kernel before left in global memory.
-// A key and its token travel as one 64-bit word.
+// A key and its token travel as one 64-bit word.  Three launches of 7 to 10 us
+// (65536 tokens, 17% issue) are latency: counts of 64 tiles, eight barriers,
+// scattered stores.  One cluster of eight blocks that keeps all in shared memory
+// took 33 us for the same, since eight SMs then do all the ranking.
 constexpr int SORT_THREADS = 256, SORT_WARPS = 8;
 constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_TILES = 256;
 constexpr int SORT_ITEMS = 4, SORT_SUB = SORT_THREADS * SORT_ITEMS;      // tokens of a thread, of a tile's part
@@ -414,7 +422,10 @@ struct SumArgs {
 // A group of blockDim.x threads sums SUM_RUN sorted tokens (a run) over the
 // columns of its threads, VEC each.  A row of the table whose tokens begin in
 // one run and end in the next belongs to the first.  Longer ones leave a part
-// for each run in `part`: [0] of a run's first row, [1] of its last.
+// for each run in `part`: [0] of a run's first row, [1] of its last.  Eight tokens'
+// rows are on their way at once.  65536 x 512 float32: 29 to 32 us, 63% of DRAM's
+// rate; 20011 x 1001 bfloat16 24 us, by single elements, four columns a thread (30
+// with one: the work on keys and places is shared by the columns).
 template <typename T, int VEC, int COLS>
 __global__ void __launch_bounds__(SUM_THREADS) embed_sum_kernel(const SumArgs p) {
   extern __shared__ unsigned sum_shared[];

@@ -20,8 +20,8 @@ def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
     ids: int64 or int32 of any shape.  weight [vocab, dim]: float32, bfloat16 or
     float16; rows of a wider table are read in place.  scale: a number.
     Differentiable (once) in weight: the rows of every token are summed in
-    float32, in the order of the tokens (the tokens are sorted; no atomics), so
-    results repeat bit for bit; tokens equal to padding_idx take no part.  A
+    float32 in a fixed order (the tokens are sorted; no atomics), so that results
+    repeat bit for bit; tokens equal to padding_idx take no part.  A
     token outside the vocabulary gives a row of zeros, takes no part in the
     gradient and sets a device error bit (gfn.cuda.ops.device_error).
     """

@@ -255,8 +255,7 @@ class Manifold(nn.Module):
     def use_library_embedding(self, on=True):
         """Look the tokens up, and sum their rows' gradient, on the library's
         kernels instead of torch's nn.Embedding (embed_tokens: the same values;
-        the gradient's sums run in the order of the tokens and repeat bit for
-        bit).  Returns the model."""
+        the gradient's sums run in a fixed order and repeat bit for bit).  Returns the model."""
         self.library_embedding = bool(on)
         return self
 
