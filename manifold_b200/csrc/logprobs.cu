@@ -499,11 +499,15 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_grad_kernel(const LpGradAr
   T* dx = static_cast<T*>(p.dx) + r * p.V;
   const int phase = VEC > 1 ? (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % VEC) : 0, end = p.V + phase;
   const int start = block * RUN;
+  // places are counted from `start`: the last block's would pass 2^31 behind the longest rows
+  const int front = phase - start, left = end - start;
+  const T* from = x - phase + start;
+  T* to = dx - phase + start;
   Pack<T, VEC> raw[UNROLL];
 #pragma unroll
   for (int k = 0; k < UNROLL; ++k) {
-    const int i = start + (k * LP_THREADS + tid) * VEC;
-    if (i >= phase && i + VEC <= end) raw[k] = *reinterpret_cast<const Pack<T, VEC>*>(x - phase + i);
+    const int i = (k * LP_THREADS + tid) * VEC;
+    if (i >= front && i + VEC <= left) raw[k] = *reinterpret_cast<const Pack<T, VEC>*>(from + i);
   }
   const float2 st = p.stats[r];
   const bool empty = st.y == INFINITY;
@@ -546,8 +550,8 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_grad_kernel(const LpGradAr
   };
 #pragma unroll
   for (int k = 0; k < UNROLL; ++k) {
-    const int i = start + (k * LP_THREADS + tid) * VEC;
-    if (i >= phase && i + VEC <= end) {
+    const int i = (k * LP_THREADS + tid) * VEC;
+    if (i >= front && i + VEC <= left) {
       Pack<T, VEC> o;
       if constexpr (VEC == 1) o.v[0] = from_f<T>(grad1(to_f(raw[k].v[0])));
       else {
@@ -558,15 +562,16 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_grad_kernel(const LpGradAr
           store_two(&o.v[e], a, b);
         }
       }
-      *reinterpret_cast<Pack<T, VEC>*>(dx - phase + i) = o;
+      *reinterpret_cast<Pack<T, VEC>*>(to + i) = o;
     } else {
-      for (int j = max(i, phase); j < min(i + VEC, end); ++j) dx[j - phase] = from_f<T>(grad1(to_f(x[j - phase])));
+      for (int j = max(i, front); j < min(i + VEC, left); ++j) to[j] = from_f<T>(grad1(to_f(from[j])));
     }
   }
   __syncthreads();
   if (tid <= p.top && id[tid] >= 0 && id[tid] < p.V) {
     const long long j = id[tid];
-    if (j + phase < start || j + phase >= start + RUN) return;
+    const long long at = j + phase - start;
+    if (at < 0 || at >= RUN) return;
     float sum = 0.f;
     for (int i = 0; i <= p.top; ++i) {
       if (id[i] != j) continue;
