@@ -35,6 +35,18 @@ class Embedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, embeddings, freeze=True, padding_idx=None, *, scale=1.0):
+        """A module on the table `embeddings` [vocab, dim], which it shares; freeze: the table is not trained."""
+        if embeddings.dim() != 2:
+            raise GfnError(f"Embedding.from_pretrained: embeddings must be [vocab, dim], got {tuple(embeddings.shape)}")
+        module = cls(*embeddings.shape, padding_idx=padding_idx, scale=scale, device="meta", dtype=embeddings.dtype)
+        module.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return module
+
+    def extra_repr(self):
+        return super().extra_repr() + ("" if self.scale == 1.0 else f", scale={self.scale}")
+
     def forward(self, input_ids):
         return embed_tokens(input_ids, self.weight, self.scale, self.padding_idx)
 
