@@ -133,13 +133,23 @@ class Manifold(nn.Module):
             return force_manual
         if isinstance(self.embedding, FunctionalEmbedding):
             return self.embedding(input_ids, out_dtype=self.force_dtype)
-        if getattr(self, "library_embedding", False) and self._plain_table():
+        if getattr(self, "library_embedding", False) and self._library_takes_embedding():
             return embed_tokens(input_ids, self.embedding.weight, padding_idx=self.embedding.padding_idx)
         return self.embedding(input_ids)
 
     def _plain_table(self):
         """Whether a token's force is its row of the embedding's weight (not scaled, as gfn.Embedding can)."""
         return isinstance(self.embedding, nn.Embedding) and getattr(self.embedding, "scale", 1.0) == 1.0
+
+    def _library_takes_embedding(self):
+        """Whether embed_tokens does all that calling the embedding would: a bare nn.Embedding, without hooks or options."""
+        e = self.embedding
+        everywhere = torch.nn.modules.module
+        return (self._plain_table() and getattr(e.forward, "__func__", None) is nn.Embedding.forward
+                and not (e.max_norm is not None or e.scale_grad_by_freq or e.sparse)
+                and not (e._forward_hooks or e._forward_pre_hooks or e._backward_hooks or e._backward_pre_hooks)
+                and not (everywhere._global_forward_hooks or everywhere._global_forward_pre_hooks
+                         or everywhere._global_backward_hooks or everywhere._global_backward_pre_hooks))
 
     def _apply_readout(self, out):
         """The readout: nn.Linear through the split-fp16 tensor-core GEMMs
@@ -255,7 +265,9 @@ class Manifold(nn.Module):
     def use_library_embedding(self, on=True):
         """Look the tokens up, and sum their rows' gradient, on the library's
         kernels instead of torch's nn.Embedding (embed_tokens: the same values;
-        the gradient's sums run in a fixed order and repeat bit for bit).  Returns the model."""
+        the gradient's sums run in a fixed order and repeat bit for bit).  An
+        embedding with hooks, with max_norm, scale_grad_by_freq or sparse, or with a
+        forward of its own is called as the module it is.  Returns the model."""
         self.library_embedding = bool(on)
         return self
 
