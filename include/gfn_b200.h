@@ -618,9 +618,8 @@ int gfn_token_logprobs_backward(const void* logits, long long logits_row_stride,
  * [batch][heads][kdim][vdim] float or NULL (zero / not wanted).  lengths
  * [batch] int64 (lengths_are_64) or int32, or NULL (all `length`; clamped to
  * [0, length]): tokens behind a sequence's length are not read, do not reach
- * the state, and get zeros.  kdim, vdim up to 128.  Tokens are taken in tiles
- * of 16: NaN or infinity in k or v reaches the outputs of up to 15 tokens
- * before it too (in q or d_o the gradients of up to 15 behind it).  `workspace`
+ * the state, and get zeros.  kdim, vdim up to 128.  NaN or infinity reaches what
+ * the recurrence takes it to and nothing else.  `workspace`
  * of gfn_decay_attention_workspace_bytes() (on the current device; one for each
  * pass), 16-byte aligned.  forward_workspace: the forward's, left as it was, for
  * length above 1, or NULL (its states are worked out again).  Results repeat bit

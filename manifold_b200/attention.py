@@ -22,8 +22,7 @@ def decay_attention(q, k, v, decay, state=None, return_state=False, lengths=None
     The state is float32 throughout.  Products run on the tensor cores: float32
     operands in two tf32 pieces each (2^-22), float16 ones exactly, and of bfloat16
     ones the scores and the state are rounded to bfloat16 where they are multiplied
-    (not where they are kept).  Tokens are taken in tiles of 16, so that a NaN or
-    infinity in k or v reaches the outputs of up to 15 tokens before it too (and one
-    in q or a gradient the gradients of up to 15 tokens behind it).
+    (not where they are kept).  A NaN or an infinity reaches what the recurrence takes
+    it to and nothing else (a sequence with one is passed over twice).
     """
     return torch_ops().decay_attention(q, k, v, decay, state, lengths, scale, return_state)

@@ -323,8 +323,10 @@ GFN_DEV void fetch(T* dst, const View& v, int b, int h, int dim, int at, int n, 
 // tile further back.
 struct Decay {
   float diag[2][4], first[4], g8;
+  int gap;  // the first score's row less its key
   GFN_DEV Decay(float lg, float s_in) {
-    const int lane = threadIdx.x & 31, gap = (lane >> 2) - 2 * (lane & 3);
+    const int lane = threadIdx.x & 31;
+    gap = (lane >> 2) - 2 * (lane & 3);
     g8 = exp2_fast(8.f * lg);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -334,13 +336,55 @@ struct Decay {
       first[e] = s_in * exp2_fast((float)(d + 8) * lg);
     }
   }
+  // Score e of the diagonal's tile z (keys 8 z .. 8 z + 7): 0 where the key
+  // stands behind the row, whatever it holds.
+  GFN_DEV float masked(float s, int z, int e) const {
+    return gap + 8 * (e >> 1) - (e & 1) - 8 * z < 0 ? 0.f : s * diag[z][e];
+  }
 };
+
+// Whether N tiles of 16 rows and 8 columns hold NaN or an infinity.
+template <typename T, int N>
+GFN_DEV bool tiles_are_bad(const T* p, int ld, int lane) {
+  float t = 0.f;
+#pragma unroll 1
+  for (int i = lane; i < 16 * 8 * N; i += 32) t = fmaf(to_f(p[i / (8 * N) * ld + i % (8 * N)]), 0.f, t);
+  return __any_sync(0xffffffffu, t != 0.f);
+}
+// o += s times the values of the diagonal's tile, each row with the keys up to
+// its own.  The tensor cores multiply the keys behind a row too, by scores of 0,
+// which makes NaN of a NaN or an infinity there.
+template <typename T, int N>
+GFN_DEV void add_up_to_diagonal(float (&o)[N][4], const float (&s)[2][4], const T* values, int ld, int lane) {
+#pragma unroll 1
+  for (int j = 0; j < 16; ++j) {
+    float w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float even = j & 8 ? s[1][2 * h] : s[0][2 * h], odd = j & 8 ? s[1][2 * h + 1] : s[0][2 * h + 1];
+      w[h] = __shfl_sync(0xffffffffu, j & 1 ? odd : even, (lane & 28) | ((j & 7) >> 1));
+    }
+    const T* v = values + j * ld + 2 * (lane & 3);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float lo = to_f(v[n * 8]), hi = to_f(v[n * 8 + 1]);
+      if (j <= lane >> 2) {
+        o[n][0] = fmaf(w[0], lo, o[n][0]);
+        o[n][1] = fmaf(w[0], hi, o[n][1]);
+      }
+      if (j <= (lane >> 2) + 8) {
+        o[n][2] = fmaf(w[1], lo, o[n][2]);
+        o[n][3] = fmaf(w[1], hi, o[n][3]);
+      }
+    }
+  }
+}
 
 // attend (see attend_f32) for the 16-bit types: the keys' tiles of 16 one after
 // the other, from the diagonal back, so that eight scores are in registers
 // instead of a row of them and no branch stands within a tile.  float16 rows and
 // values meet state and scores as tf32.
-template <typename T, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
+template <typename T, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL, bool CARE>
 GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
                        int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
   using M = Math<T>;
@@ -451,8 +495,10 @@ GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T*
 #pragma unroll
   for (int z = 0; z < 2; ++z)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[z][e] = g.diag[z][e] == 0.f ? 0.f : s[z][e] * g.diag[z][e];
-  add(rt, s);
+    for (int e = 0; e < 4; ++e) s[z][e] = g.masked(s[z][e], z, e);
+  const T* own = values + rt * 16 * LDB + col0;
+  if (CARE && tiles_are_bad<T, ON>(own, LDB, lane)) add_up_to_diagonal<T, ON>(o, s, own, LDB, lane);
+  else add(rt, s);
   F2 f0 = f2(g.first[0], g.first[1]), f1 = f2(g.first[2], g.first[3]);
   const F2 g8 = f2(g.g8);
 #pragma unroll 2
@@ -472,7 +518,7 @@ GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T*
 // One warp's 16 rows of a block's output: ON tiles of 8 columns from col0.
 // rows, keys [C][LDA] with kd of their columns in use, values [C][LDB]; st: the
 // state, seen from this product as [k][n] or (NMAJOR) [n][k].
-template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
+template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL, bool CARE>
 GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
                          int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
   using M = Math<T>;
@@ -530,15 +576,20 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
       f1 = f1 * g8;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float w = off == 0 ? g.diag[0][e] : g.diag[1][e];
-        s[i][e] = w == 0.f ? 0.f : s[i][e] * w;
-      }
+      for (int e = 0; e < 4; ++e) s[i][e] = off == 0 ? g.masked(s[i][e], 0, e) : g.masked(s[i][e], 1, e);
     }
   }
+  const T* own = values + rt * 16 * LDB + col0;
+  const bool bad = CARE && tiles_are_bad<T, ON>(own, LDB, lane);
 #pragma unroll
   for (int i = 0; i < C / 16; ++i) {
     if (i > rt) continue;
+    if (bad && i == rt) {
+      const float d[2][4] = {{s[2 * i][0], s[2 * i][1], s[2 * i][2], s[2 * i][3]},
+                             {s[2 * i + 1][0], s[2 * i + 1][1], s[2 * i + 1][2], s[2 * i + 1][3]}};
+      add_up_to_diagonal<T, ON>(o, d, own, LDB, lane);
+      continue;
+    }
 #pragma unroll
     for (int q = 0; q < 16 / M::KS; ++q) {
       typename M::A a;
@@ -563,13 +614,13 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
   }
 }
 
-template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL>
+template <typename T, int C, int DA, int LDA, int LDB, int LS, int ON, bool NMAJOR, bool FULL, bool CARE>
 GFN_DEV void attend(float (&o)[ON][4], const T* rows, const T* keys, const T* values, const typename Math<T>::State* st,
                     int rt, int col0, int kd, int nd, const Decay& g, float w0, float w1) {
   if constexpr (Math<T>::KS == 16)
-    attend_16<T, DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
+    attend_16<T, DA, LDA, LDB, LS, ON, NMAJOR, FULL, CARE>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
   else
-    attend_f32<T, C, DA, LDA, LDB, LS, ON, NMAJOR, FULL>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
+    attend_f32<T, C, DA, LDA, LDB, LS, ON, NMAJOR, FULL, CARE>(o, rows, keys, values, st, rt, col0, kd, nd, g, w0, w1);
 }
 
 // Two values in three bfloat16 pieces each (cut, not rounded), which add up to
@@ -735,8 +786,9 @@ GFN_DEV void emit(void* out, const float (&o)[ON][4], const PassArgs& p, int b, 
 // values d) and dk (rows c, keys d, values a) of the state's gradient.  dv and dk in
 // one launch share the operands and the state: 32 x 2048 x 8 heads of 64 in bfloat16
 // 149 us, where the outputs alone take 103 (256 thread blocks: two an SM, or one).
-template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL>
-__global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::resident(KIND)) attn_kernel(const PassArgs p) {
+// Returns whether the segment is to be walked again with CARE.
+template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL, bool CARE>
+GFN_DEV bool attn_walk(const PassArgs& p) {
   using S = Shape<T, DK, DV>;
   using M = Math<T>;
   using Op = typename M::State;
@@ -757,14 +809,14 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
   const long long mat = (long long)p.KD * p.VD, bh = (long long)b * p.H + h;
   const float* init = KIND == STATE ? nullptr : p.segs ? p.segs + (bh * p.segments + seg) * mat : p.state ? p.state + bh * mat : nullptr;
   const long long sr = p.segs ? p.segs_sr : p.sr, sc = p.segs ? p.segs_sc : p.sc;
+  auto before = [&](int i, int e) {
+    const int row = m0 + (lane >> 2) + 8 * (e >> 1), col = n0 + i * 8 + 2 * (lane & 3) + (e & 1);
+    return init && row < p.KD && col < p.VD ? init[row * sr + col * sc] : 0.f;
+  };
 #pragma unroll
-  for (int i = 0; i < S::SN; ++i) {
+  for (int i = 0; i < S::SN; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = m0 + (lane >> 2) + 8 * (e >> 1), col = n0 + i * 8 + 2 * (lane & 3) + (e & 1);
-      st[i][e] = init && row < p.KD && col < p.VD ? init[row * sr + col * sc] : 0.f;
-    }
-  }
+    for (int e = 0; e < 4; ++e) st[i][e] = before(i, e);
   {
     uint4* z = reinterpret_cast<uint4*>(attn_shared);
     for (int i = threadIdx.x; i < (int)((STAGES * STAGE * sizeof(T) + BUFS * S::STATE_BYTES) / 16); i += S::THREADS)
@@ -809,8 +861,6 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
     }
   };
   const int blocks = to > from ? (to - from + S::C - 1) / S::C : 0;
-  if (blocks) bring(0, stage);
-  lay_out(st_op);
   const int rt = warp % S::ROWS, part = warp / S::ROWS;
   const Decay decay(lg, p.s_in);
   const float whole = power(lg, S::C);
@@ -818,6 +868,17 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
   // gradient arrives with that factor in it
   const int r0 = rt * 16 + (lane >> 2) + (BACK ? 0 : 1);
   const float w0 = p.s_state * power(lg, r0), w1 = p.s_state * power(lg, r0 + 8);
+  // Whether the state holds NaN or an infinity: one that a token brings stays there.
+  auto turned_bad = [&] {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < S::SN; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t = fmaf(st[i][e], 0.f, t);
+    return t != 0.f;
+  };
+  if (blocks) bring(0, stage);
+  lay_out(st_op);
   for (int c = 0; c < blocks; ++c) {
     const T* cur = stage + (STAGES == 2 ? (c & 1) * STAGE : 0);
     const Op* op = st_op + (BUFS == 2 ? (c & 1) * DK * S::LS : 0);
@@ -841,10 +902,10 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
       const int col0 = part * OV * 8;
       if (FULL || col0 < p.VD) {
         if constexpr (KIND == OUTPUT)
-          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false, FULL>(o, cur, cur + S::TK, cur + 2 * S::TK, op, rt, col0, p.KD, p.VD,
+          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false, FULL, CARE>(o, cur, cur + S::TK, cur + 2 * S::TK, op, rt, col0, p.KD, p.VD,
                                                                decay, w0, w1);
         else
-          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false, FULL>(o, cur + S::TK, cur, cur + 2 * S::TK + S::TV, op, rt, col0, p.KD,
+          attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false, FULL, CARE>(o, cur + S::TK, cur, cur + 2 * S::TK + S::TV, op, rt, col0, p.KD,
                                                                p.VD, decay, w0, w1);
         emit<T, OV, BACK>(p.o, o, p, b, h, p.VD, at, n, rt, col0);
       }
@@ -854,7 +915,7 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
       float o[OK][4];
       const int col0 = part * OK * 8;
       if (FULL || col0 < p.KD) {
-        attend<T, S::C, DV, S::LDV, S::LDK, S::LS, OK, true, FULL>(o, cur + 2 * S::TK, cur + 2 * S::TK + S::TV, cur, op, rt, col0, p.VD,
+        attend<T, S::C, DV, S::LDV, S::LDK, S::LS, OK, true, FULL, CARE>(o, cur + 2 * S::TK, cur + 2 * S::TK + S::TV, cur, op, rt, col0, p.VD,
                                                             p.KD, decay, w0, w1);
         emit<T, OK, BACK>(p.o2, o, p, b, h, p.KD, at, n, rt, col0);
       }
@@ -866,6 +927,7 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
       lay_out(st_op);
     }
   }
+  if (!CARE && KIND != STATE && __syncthreads_or(turned_bad())) return true;
   // tokens behind the sequence: zeros
   if (KIND != STATE && len < p.L) {
     const int z0 = max(from, len), z1 = min(from + p.seg_len, p.L);
@@ -886,6 +948,21 @@ __global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::r
         if (row < p.KD && col < p.VD) out[row * p.VD + col] = st[i][e];
       }
   }
+  return false;
+}
+
+// Segments of finite tokens are walked once.  Others are walked again, by code of
+// its own, so that care (see add_up_to_diagonal) costs next to nothing on the way:
+// 32 x 2048 x 8 heads of 64 in bfloat16, trained, 351 us with and without it; asking
+// in the walk which infinities the state came with took 397.
+template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL>
+__device__ __noinline__ void attn_walk_again(const PassArgs& p) {
+  attn_walk<T, DK, DV, BACK, KIND, FULL, true>(p);
+}
+template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL>
+__global__ void __launch_bounds__(Shape<T, DK, DV>::THREADS, Shape<T, DK, DV>::resident(KIND))
+    attn_kernel(const __grid_constant__ PassArgs p) {
+  if (attn_walk<T, DK, DV, BACK, KIND, FULL, false>(p)) attn_walk_again<T, DK, DV, BACK, KIND, FULL>(p);
 }
 
 // The states before each segment, from what each segment adds; in place.  JOIN
