@@ -638,12 +638,45 @@ GFN_DEV void split3(F2 v, unsigned& hi, unsigned& mid, unsigned& lo) {
   lo = both(x, y);
 }
 
+// Those of a block's sums that came out as NaN once more, term by term: the
+// pieces of a product make NaN of an infinity (inf - inf, 0 x inf) that the
+// product alone leaves one.  faded: the factor of an infinity whose own has become 0.
+template <typename T, int C, int LDK, int LDV, int N>
+GFN_DEV void add_again(float (&add)[N][4], const T* keys, const T* values, const float* wt, float faded, int m0, int n0) {
+  const int lane = threadIdx.x & 31;
+  float s[4 * N];
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i) s[i] = add[i / 4][i % 4];
+#pragma unroll 1
+  for (int i = 0; i < 4 * N; ++i) {
+    if (!isnan(s[i])) continue;
+    const T* k = keys + m0 + (lane >> 2) + (i & 2) * 4;
+    const T* v = values + n0 + (i >> 2) * 8 + 2 * (lane & 3) + (i & 1);
+    float sum = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < C && !isnan(sum); ++j) {
+      const float x = to_f(k[j * LDK]), y = to_f(v[j * LDV]), w = wt[j];
+      sum += isfinite(x) && isfinite(y) ? x * w * y : x * y * (w == 0.f ? faded : w);
+    }
+    s[i] = sum;
+  }
+#pragma unroll
+  for (int i = 0; i < 4 * N; ++i) add[i / 4][i % 4] = s[i];
+}
+
+// w s + add for a power w of the decay; an infinity stays one while the decay is
+// above 0 (lasts), even if w is below float32's range.
+GFN_DEV float carried(float s, float w, float add, bool lasts) {
+  return w == 0.f && lasts && isinf(s) ? s + add : fmaf(w, s, add);
+}
+
 // st = gn st + (diag(wt) keys)^T values for one warp's 16 rows (from m0) and N
 // tiles of columns (from n0) of the state.  The products of a block are summed
 // by themselves and then added, since the tensor cores cut where float32
 // addition rounds: over a long sequence that would drift.
-template <typename T, int C, int LDK, int LDV, int N, bool FULL>
-GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const float* wt, float gn, int m0, int n0, int nd) {
+template <typename T, int C, int LDK, int LDV, int N, bool FULL, bool CARE>
+GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const float* wt, float gn, int m0, int n0, int nd,
+                    float faded, bool lasts) {
   using M = Math<T>;
   const int lane = threadIdx.x & 31, t = lane & 3;
   constexpr int AT = N < 8 ? N : 8;  // tiles at a time
@@ -733,10 +766,12 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
         }
       }
     }
+    if (CARE) add_again<T, C, LDK, LDV, AT>(add, keys, values, wt, faded, m0, n0 + at * 8);
 #pragma unroll
     for (int n = 0; n < AT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st[at + n][e] = fmaf(st[at + n][e], gn, add[n][e]);
+      for (int e = 0; e < 4; ++e)
+        st[at + n][e] = CARE ? carried(st[at + n][e], gn, add[n][e], lasts) : fmaf(st[at + n][e], gn, add[n][e]);
   }
 }
 
@@ -802,6 +837,7 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
   const int len = length_of(p, b);
   const int from = seg * p.seg_len, to = min(from + p.seg_len, len);
   const float lg = log2_decay(p.decay[h]);
+  const bool lasts = p.decay[h] > 0.f;
   // the state's place of this warp
   const int m0 = (warp % S::SLABS) * 16, n0 = (warp / S::SLABS) * S::SN * 8;
   const bool holds = FULL || (m0 < p.KD && n0 < p.VD);
@@ -890,7 +926,7 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
       const T* uk = KIND == OUTPUT ? cur + S::TK : cur;
       const T* uv = KIND == OUTPUT ? cur + 2 * S::TK : KIND == STATE ? cur + S::TK : cur + 2 * S::TK + S::TV;
       const float gn = n == S::C ? whole : power(lg, n);
-      if (holds) update<T, S::C, S::LDK, S::LDV, S::SN, FULL>(st, uk, uv, wt + S::C - n, gn, m0, n0, p.VD);
+      if (holds) update<T, S::C, S::LDK, S::LDV, S::SN, FULL, CARE>(st, uk, uv, wt + S::C - n, gn, m0, n0, p.VD, lasts ? p.s_update : 0.f, lasts);
     };
     if (BUFS == 2) {  // the next block's state, beside the outputs of this one
       move_on();
@@ -927,7 +963,7 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
       lay_out(st_op);
     }
   }
-  if (!CARE && KIND != STATE && __syncthreads_or(turned_bad())) return true;
+  if (!CARE && __syncthreads_or(turned_bad())) return true;
   // tokens behind the sequence: zeros
   if (KIND != STATE && len < p.L) {
     const int z0 = max(from, len), z1 = min(from + p.seg_len, p.L);
@@ -952,7 +988,7 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
 }
 
 // Segments of finite tokens are walked once.  Others are walked again, by code of
-// its own, so that care (see add_up_to_diagonal) costs next to nothing on the way:
+// its own, so that care (see add_up_to_diagonal, add_again) costs next to nothing on the way:
 // 32 x 2048 x 8 heads of 64 in bfloat16, trained, 351 us with and without it; asking
 // in the walk which infinities the state came with took 397.
 template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL>
@@ -974,6 +1010,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const PassArgs p) {
   if (i >= mat || bh >= (long long)p.B * p.H) return;
   const int b = (int)(bh / p.H), h = (int)(bh % p.H), len = length_of(p, b);
   const float lg = log2_decay(p.decay[h]);
+  const bool lasts = p.decay[h] > 0.f;
   const int row = i / p.VD, col = i % p.VD;
   float s = p.state ? p.state[bh * mat + row * p.sr + col * p.sc] : 0.f;
   float* q = p.segs + bh * p.segments * mat + i;
@@ -991,7 +1028,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const PassArgs p) {
       const int k = BACK ? p.segments - 1 - k0 - u : k0 + u;
       const int n = min(max(len - k * p.seg_len, 0), p.seg_len);
       q[(long long)k * mat] = s;
-      s = fmaf(n == p.seg_len ? whole : power(lg, n), s, add[u]);
+      s = carried(s, n == p.seg_len ? whole : power(lg, n), add[u], lasts);
     }
   }
   if (p.state_out) p.state_out[bh * mat + i] = s;
@@ -1010,6 +1047,7 @@ __global__ void __launch_bounds__(256) attn_join_long_kernel(const PassArgs p) {
   if (bh >= (long long)p.B * p.H) return;
   const int b = (int)(bh / p.H), h = (int)(bh % p.H), len = length_of(p, b);
   const float lg = log2_decay(p.decay[h]), whole = power(lg, p.seg_len);
+  const bool lasts = p.decay[h] > 0.f;
   const bool live = i < mat;
   float* q = p.segs + bh * p.segments * mat + i;
   auto place = [&](int k) { return BACK ? p.segments - 1 - k : k; };
@@ -1030,7 +1068,7 @@ __global__ void __launch_bounds__(256) attn_join_long_kernel(const PassArgs p) {
     for (int u = 0; u < AHEAD; ++u) {
       if (k0 + u >= to) continue;
       const float w = gain(k0 + u);
-      s = fmaf(w, s, add[u]);
+      s = carried(s, w, add[u], lasts);
       g *= w;
     }
   }
@@ -1040,14 +1078,14 @@ __global__ void __launch_bounds__(256) attn_join_long_kernel(const PassArgs p) {
   if (!live) return;
   const int row = i / p.VD, col = i % p.VD;
   s = p.state ? p.state[bh * mat + row * p.sr + col * p.sc] : 0.f;
-  for (int r = 0; r < part; ++r) s = fmaf(gains[r], s, sums[r][lane]);
+  for (int r = 0; r < part; ++r) s = carried(s, gains[r], sums[r][lane], lasts);
   for (int k0 = from; k0 < to; k0 += AHEAD) {
     if (per > AHEAD) read(k0);  // a single batch is still there
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (k0 + u >= to) continue;
       q[(long long)place(k0 + u) * mat] = s;
-      s = fmaf(gain(k0 + u), s, add[u]);
+      s = carried(s, gain(k0 + u), add[u], lasts);
     }
   }
   if (part == PARTS - 1 && p.state_out) p.state_out[bh * mat + i] = s;

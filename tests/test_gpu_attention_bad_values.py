@@ -24,14 +24,17 @@ def _np(t):
     return None if t is None else t.detach().double().cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
 
 
-def _reach(name, got, want, tol):
-    """Finite where the definition is, and close there."""
+def _reach(name, got, want, tol, signs=False):
+    """Finite where the definition is, and close there; signs: the same infinities and NaN elsewhere too."""
     assert got.shape == want.shape, name
     fine = np.isfinite(want)
     wrong = np.isfinite(got) != fine
     assert not wrong.any(), (name, int(wrong.sum()), np.argwhere(wrong)[0])
     bad = ~(np.abs(got - want)[fine] <= tol[fine])
     assert not bad.any(), (name, int(bad.sum()), np.abs(got - want)[fine][bad].max())
+    if signs:
+        other = ~fine & ~((got == want) | (np.isnan(got) & np.isnan(want)))
+        assert not other.any(), (name, int(other.sum()), got[other][0], want[other][0])
 
 
 def _check(ts, clean, decay, st, lengths, scale, do, dl, what):
@@ -50,10 +53,10 @@ def _check(ts, clean, decay, st, lengths, scale, do, dl, what):
         bo, bs = O.decay_attention(*m, _np(lengths), scale)
         bg = O.decay_attention_backward(*m, _np(lengths), scale, d, np.abs(_np(dl)))
         _reach(what + ": o", _np(o), wo, uo * np.abs(wo) + op * bo + 2.0 ** -24)
-        _reach(what + ": state", _np(last), ws, 2.0 ** -18 * bs)
+        _reach(what + ": state", _np(last), ws, 2.0 ** -18 * bs, signs=True)
         for name, g, w, b in zip(("dq", "dk", "dv"), grads, wg, bg):
             _reach(what + ": " + name, _np(g), w, uo * np.abs(w) + op * b + 2.0 ** -24)
-        _reach(what + ": dstate", _np(grads[3]), wg[3], 2.0 ** -18 * bg[3])
+        _reach(what + ": dstate", _np(grads[3]), wg[3], 2.0 ** -18 * bg[3], signs=True)
 
 
 def _case(B, L, H, K, V, dtype, seed=0):
