@@ -123,9 +123,13 @@ GFN_DEV unsigned tf32(float v) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
   return r;
 }
-template <int N>
+// WIDE: the first piece stops at tf32's largest number.  Values between that and
+// float32's largest, as finfo.max is, round to infinity otherwise and leave
+// inf - inf; but everywhere this conversion costs 10 to 16% of a float32 pass.
+template <bool WIDE, int N>
 GFN_DEV void pieces(float v, unsigned (&r)[N]) {
-  r[0] = tf32(v);
+  if constexpr (WIDE) asm("cvt.rna.satfinite.tf32.f32 %0, %1;" : "=r"(r[0]) : "f"(v));
+  else r[0] = tf32(v);
   if constexpr (N > 1) r[1] = tf32(v - __uint_as_float(r[0]));
 }
 
@@ -153,7 +157,7 @@ GFN_DEV void ldsm_t(unsigned& a, unsigned& b, unsigned& c, unsigned& d, const vo
 GFN_DEV float2 pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
 
 // A, 16 rows from p [row][k].
-template <typename T>
+template <typename T, bool CARE>
 GFN_DEV void load_a(typename Math<T>::A& f, const T* p, int ld, int lane) {
   if constexpr (Math<T>::KS == 16) {
     ldsm(f.v[0], f.v[1], f.v[2], f.v[3], p + ((lane & 7) + (lane & 8)) * ld + ((lane >> 4) << 3));
@@ -164,14 +168,14 @@ GFN_DEV void load_a(typename Math<T>::A& f, const T* p, int ld, int lane) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       unsigned r[Math<T>::PIECES];
-      pieces(w[i], r);
+      pieces<CARE>(w[i], r);
 #pragma unroll
       for (int k = 0; k < Math<T>::PIECES; ++k) f.v[k][i] = r[k];
     }
   }
 }
 // Two neighbouring B of 8 columns each, from p [n][k].
-template <typename T, typename E>
+template <typename T, bool CARE, typename E>
 GFN_DEV void load_bn(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) {
   if constexpr (Math<T>::KS == 16) {
     ldsm(f[0].v[0], f[0].v[1], f[1].v[0], f[1].v[1], p + ((lane & 7) + ((lane >> 4) << 3)) * ld + (lane & 8));
@@ -180,8 +184,8 @@ GFN_DEV void load_bn(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) 
     for (int h = 0; h < 2; ++h) {
       const float2 x = pair(p + ((lane >> 2) + 8 * h) * ld + 2 * (lane & 3));
       unsigned r[2][Math<T>::PIECES];
-      pieces(x.x, r[0]);
-      pieces(x.y, r[1]);
+      pieces<CARE>(x.x, r[0]);
+      pieces<CARE>(x.y, r[1]);
 #pragma unroll
       for (int k = 0; k < Math<T>::PIECES; ++k) {
         f[h].v[k][0] = r[0][k];
@@ -191,7 +195,7 @@ GFN_DEV void load_bn(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) 
   }
 }
 // The same from p [k][n].
-template <typename T, typename E>
+template <typename T, bool CARE, typename E>
 GFN_DEV void load_bk(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) {
   if constexpr (Math<T>::KS == 16) {
     ldsm_t(f[0].v[0], f[0].v[1], f[1].v[0], f[1].v[1], p + ((lane & 7) + (lane & 8)) * ld + ((lane >> 4) << 3));
@@ -200,8 +204,8 @@ GFN_DEV void load_bk(typename Math<T>::B (&f)[2], const E* p, int ld, int lane) 
     for (int h = 0; h < 2; ++h) {
       const E* q = p + 2 * (lane & 3) * ld + (lane >> 2) + 8 * h;
       unsigned r[2][Math<T>::PIECES];
-      pieces(to_f(q[0]), r[0]);
-      pieces(to_f(q[ld]), r[1]);
+      pieces<CARE>(to_f(q[0]), r[0]);
+      pieces<CARE>(to_f(q[ld]), r[1]);
 #pragma unroll
       for (int k = 0; k < Math<T>::PIECES; ++k) {
         f[h].v[k][0] = r[0][k];
@@ -393,7 +397,7 @@ GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T*
   const int lane = threadIdx.x & 31;
   typename M::A a[KN];
 #pragma unroll
-  for (int k = 0; k < KN; ++k) load_a<T>(a[k], rows + rt * 16 * LDA + k * 16, LDA, lane);
+  for (int k = 0; k < KN; ++k) load_a<T, CARE>(a[k], rows + rt * 16 * LDA + k * 16, LDA, lane);
 #pragma unroll
   for (int i = 0; i < ON; ++i)
 #pragma unroll
@@ -427,8 +431,8 @@ GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T*
         const int col = col0 + i * 8;
         if (!FULL && col >= nd) continue;
         typename M::B b[2];
-        if (NMAJOR) load_bn<T>(b, st + col * LS + k * 16, LS, lane);
-        else load_bk<T>(b, st + k * 16 * LS + col, LS, lane);
+        if (NMAJOR) load_bn<T, CARE>(b, st + col * LS + k * 16, LS, lane);
+        else load_bk<T, CARE>(b, st + k * 16 * LS + col, LS, lane);
         mma<T>(o[i], a[k], b[0]);
         mma<T>(o[i + 1], a[k], b[1]);
       }
@@ -448,7 +452,7 @@ GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T*
     for (int k = 0; k < KN; ++k) {
       if (!FULL && k * 16 >= kd) continue;
       typename M::B b[2];
-      load_bn<T>(b, keys + i * 16 * LDA + k * 16, LDA, lane);
+      load_bn<T, CARE>(b, keys + i * 16 * LDA + k * 16, LDA, lane);
       mma<T>(s[0], a[k], b[0]);
       mma<T>(s[1], a[k], b[1]);
     }
@@ -473,7 +477,7 @@ GFN_DEV void attend_16(float (&o)[ON][4], const T* rows, const T* keys, const T*
     for (int n = 0; n < ON; n += 2) {
       if (!FULL && col0 + n * 8 >= nd) continue;
       typename M::B b[2];
-      load_bk<T>(b, values + i * 16 * LDB + col0 + n * 8, LDB, lane);
+      load_bk<T, CARE>(b, values + i * 16 * LDB + col0 + n * 8, LDB, lane);
       if constexpr (HALF) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -536,14 +540,14 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
   for (int k = 0; k < DA; k += M::KS) {
     if (!FULL && k >= kd) continue;
     typename M::A a;
-    load_a<T>(a, rows + rt * 16 * LDA + k, LDA, lane);
+    load_a<T, CARE>(a, rows + rt * 16 * LDA + k, LDA, lane);
 #pragma unroll
     for (int i = 0; i < ON; i += 2) {
       const int col = col0 + i * 8;
       if (!FULL && col >= nd) continue;
       typename M::B b[2];
-      if (NMAJOR) load_bn<T>(b, st + col * LS + k, LS, lane);
-      else load_bk<T>(b, st + k * LS + col, LS, lane);
+      if (NMAJOR) load_bn<T, CARE>(b, st + col * LS + k, LS, lane);
+      else load_bk<T, CARE>(b, st + k * LS + col, LS, lane);
       mma<T>(o[i], a, b[0]);
       mma<T>(o[i + 1], a, b[1]);
     }
@@ -551,7 +555,7 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
     for (int i = 0; i < C / 16; ++i) {
       if (i > rt) continue;  // keys behind the rows
       typename M::B b[2];
-      load_bn<T>(b, keys + i * 16 * LDA + k, LDA, lane);
+      load_bn<T, CARE>(b, keys + i * 16 * LDA + k, LDA, lane);
       mma<T>(s[2 * i], a, b[0]);
       mma<T>(s[2 * i + 1], a, b[1]);
     }
@@ -597,7 +601,7 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         unsigned r[M::PIECES];
-        pieces(w[e], r);
+        pieces<CARE>(w[e], r);
 #pragma unroll
         for (int z = 0; z < M::PIECES; ++z) a.v[z][e] = r[z];
       }
@@ -606,7 +610,7 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
       for (int n = 0; n < ON; n += 2) {
         if (!FULL && col0 + n * 8 >= nd) continue;
         typename M::B b[2];
-        load_bk<T>(b, v + n * 8, LDB, lane);
+        load_bk<T, CARE>(b, v + n * 8, LDB, lane);
         mma<T>(o[n], a, b[0]);
         mma<T>(o[n + 1], a, b[1]);
       }
@@ -703,7 +707,7 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             unsigned r[2];
-            pieces(__uint_as_float(x[e]) * (e < 2 ? w0 : w1), r);
+            pieces<CARE>(__uint_as_float(x[e]) * (e < 2 ? w0 : w1), r);
             a[q][0][e] = r[0];
             a[q][1][e] = r[1];
           }
@@ -712,7 +716,7 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
         for (int n = 0; n < AT; n += 2) {
           if (!FULL && n0 + (at + n) * 8 >= nd) continue;
           typename M::B b[2];
-          load_bk<T>(b, vals + n * 8, LDV, lane);
+          load_bk<T, CARE>(b, vals + n * 8, LDV, lane);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -737,7 +741,7 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
         for (int n = 0; n < AT; n += 2) {
           if (!FULL && n0 + (at + n) * 8 >= nd) continue;
           typename M::B b[2];
-          load_bk<T>(b, vals + n * 8, LDV, lane);
+          load_bk<T, CARE>(b, vals + n * 8, LDV, lane);
 #pragma unroll
           for (int z = 2; z >= 0; --z) {
             mma_bf16(add[n], a[z], b[0].v);
@@ -752,7 +756,7 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           unsigned r[2];
-          pieces(x[e], r);
+          pieces<CARE>(x[e], r);
           a[0][e] = r[0];
           a[1][e] = r[1];
         }
@@ -760,7 +764,7 @@ GFN_DEV void update(float (&st)[N][4], const T* keys, const T* values, const flo
         for (int n = 0; n < AT; n += 2) {
           if (!FULL && n0 + (at + n) * 8 >= nd) continue;
           typename M::B b[2];
-          load_bk<T>(b, vals + n * 8, LDV, lane);
+          load_bk<T, CARE>(b, vals + n * 8, LDV, lane);
           mma_pieces(add[n], a, b[0].v);
           mma_pieces(add[n + 1], a, b[1].v);
         }
@@ -904,9 +908,18 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
   // gradient arrives with that factor in it
   const int r0 = rt * 16 + (lane >> 2) + (BACK ? 0 : 1);
   const float w0 = p.s_state * power(lg, r0), w1 = p.s_state * power(lg, r0 + 8);
-  // Whether the state holds NaN or an infinity: one that a token brings stays there.
+  constexpr bool WATCH = !CARE && sizeof(T) == 4;
+  float watch = 0.f;  // turns NaN
+  auto note = [&](const auto& o) {
+#pragma unroll
+    for (const auto& tile : o)
+#pragma unroll
+      for (const float x : tile) watch = fmaf(x, 0.f, watch);
+  };
+  // Whether the state holds NaN or an infinity: one that a token brings stays
+  // there.  float32 outputs are watched too, for operands beyond tf32's range.
   auto turned_bad = [&] {
-    float t = 0.f;
+    float t = watch;
 #pragma unroll
     for (int i = 0; i < S::SN; ++i)
 #pragma unroll
@@ -943,6 +956,7 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
         else
           attend<T, S::C, DK, S::LDK, S::LDV, S::LS, OV, false, FULL, CARE>(o, cur + S::TK, cur, cur + 2 * S::TK + S::TV, op, rt, col0, p.KD,
                                                                p.VD, decay, w0, w1);
+        if (WATCH) note(o);
         emit<T, OV, BACK>(p.o, o, p, b, h, p.VD, at, n, rt, col0);
       }
     }
@@ -953,6 +967,7 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
       if (FULL || col0 < p.KD) {
         attend<T, S::C, DV, S::LDV, S::LDK, S::LS, OK, true, FULL, CARE>(o, cur + 2 * S::TK, cur + 2 * S::TK + S::TV, cur, op, rt, col0, p.VD,
                                                             p.KD, decay, w0, w1);
+        if (WATCH) note(o);
         emit<T, OK, BACK>(p.o2, o, p, b, h, p.KD, at, n, rt, col0);
       }
     }

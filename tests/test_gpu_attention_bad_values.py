@@ -46,7 +46,8 @@ def _check(ts, clean, decay, st, lengths, scale, do, dl, what):
     uo, op = UO[dt], OPERAND[dt]
     n = [_np(t) for t in (*ts, decay, st)]
     m = [np.abs(_np(t)) for t in (*clean, decay, st)]
-    d = np.nan_to_num(np.abs(_np(do)), nan=1.0, posinf=1.0, neginf=1.0)
+    d = np.abs(_np(do))
+    d[~np.isfinite(d)] = 1.0
     with np.errstate(invalid="ignore", over="ignore"):
         wo, ws = O.decay_attention(*n, _np(lengths), scale)
         wg = O.decay_attention_backward(*n, _np(lengths), scale, _np(do), _np(dl))
@@ -118,3 +119,18 @@ def test_bad_states(dtype):
         bad[0, 1, 3, 4], bad[1, 0, 5, 6], d[1, 1, 7, 8], d[0, 0, 9, 10] = NAN, INF, -INF, NAN
         _check((q, k, v), (q, k, v), decay, bad, None, 0.2, do, dl, "state of %d" % L)
         _check((q, k, v), (q, k, v), decay, st, None, 0.2, do, d, "gradient of %d" % L)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L,K,V", [(140, 24, 32), (90, 64, 64), (600, 16, 24)])
+def test_the_largest_finite_values(L, K, V, dtype):
+    """finfo.min and finfo.max are values like others where scores, sums (before the factor) and results are in range."""
+    q, k, v, decay, st, do, dl = _case(5, L, 2, K, V, dtype, seed=L)
+    # all others below 1: 3.4e38 times one above (v d_o is a score of dq) is no float32, nor 65504 times one a float16
+    q, k, v, st, do, dl = q * 2.0 ** -12, k * 2.0 ** -6, *(t * 2.0 ** -4 for t in (v, st, do, dl))
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    v[0, 20, 1, 3], v[1, 70, 0, 4], q[2, 50, 1, 5] = low, high, low
+    k[3, 61, 0, 2], v[3, 61, 0] = high, v[3, 61, 0] * 2.0 ** -10
+    do[4, 33, 1, 7] = high
+    _check((q, k, v), (q, k, v), decay, st, None, 2.0 ** -8, do, dl, "largest")
