@@ -301,8 +301,8 @@ GFN_DEV void fetch(T* dst, const View& v, int b, int h, int dim, int at, int n, 
   const T* src = static_cast<const T*>(v.p) + b * v.sb + h * v.sh + at * v.sl;
   if (FULL || piece == 16) fetch_pieces<T, D, LD, C, THREADS, BACK, 16>(dst, src, v.p, v.sl, dim, n);
   else if (piece == 8) fetch_pieces<T, D, LD, C, THREADS, BACK, 8>(dst, src, v.p, v.sl, dim, n);
-  else if (piece == 4) fetch_pieces<T, D, LD, C, THREADS, BACK, 4>(dst, src, v.p, v.sl, dim, n);
-  else {  // 16-bit elements at odd places
+  else if (sizeof(T) == 4 || piece == 4) fetch_pieces<T, D, LD, C, THREADS, BACK, 4>(dst, src, v.p, v.sl, dim, n);
+  else if constexpr (sizeof(T) == 2) {  // elements at odd places
     constexpr int AHEAD = 8, COUNT = C * D / THREADS;
     static_assert(COUNT % AHEAD == 0, "");
 #pragma unroll 1
@@ -1095,7 +1095,7 @@ __global__ void __launch_bounds__(256) attn_join_long_kernel(const PassArgs p) {
   s = p.state ? p.state[bh * mat + row * p.sr + col * p.sc] : 0.f;
   for (int r = 0; r < part; ++r) s = carried(s, gains[r], sums[r][lane], lasts);
   for (int k0 = from; k0 < to; k0 += AHEAD) {
-    if (per > AHEAD) read(k0);  // a single batch is still there
+    read(k0);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (k0 + u >= to) continue;

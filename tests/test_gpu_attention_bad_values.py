@@ -46,6 +46,7 @@ def _check(ts, clean, decay, st, lengths, scale, do, dl, what):
     uo, op = UO[dt], OPERAND[dt]
     n = [_np(t) for t in (*ts, decay, st)]
     m = [np.abs(_np(t)) for t in (*clean, decay, st)]
+    m[4][~np.isfinite(m[4])] = 1.0
     d = np.abs(_np(do))
     d[~np.isfinite(d)] = 1.0
     with np.errstate(invalid="ignore", over="ignore"):
@@ -119,6 +120,17 @@ def test_bad_states(dtype):
         bad[0, 1, 3, 4], bad[1, 0, 5, 6], d[1, 1, 7, 8], d[0, 0, 9, 10] = NAN, INF, -INF, NAN
         _check((q, k, v), (q, k, v), decay, bad, None, 0.2, do, dl, "state of %d" % L)
         _check((q, k, v), (q, k, v), decay, st, None, 0.2, do, d, "gradient of %d" % L)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_bad_values_in_a_sequence_of_many_segments(dtype):
+    """125 segments, whose parts are joined by eight warps."""
+    q, k, v, _, st, do, dl = _case(2, 16000, 2, 8, 8, dtype)
+    decay = torch.tensor([0.1, 0.99], device=DEV)
+    ts, s0 = [q.clone(), k.clone(), v.clone()], st.clone()
+    ts[1][0, 9000, :, 1], ts[2][0, 12345, 0, 2], s0[0, 1, 5, 6], s0[1, 0, 3, 3] = INF, NAN, -INF, INF
+    _check(ts, (q, k, v), decay, s0, None, 0.3, do, dl, "many")
 
 
 @pytest.mark.gpu
