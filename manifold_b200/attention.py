@@ -20,9 +20,10 @@ def decay_attention(q, k, v, decay, state=None, return_state=False, lengths=None
     (once) in q, k, v and state.
 
     The state is float32 throughout.  Products run on the tensor cores: float32
-    operands in two tf32 pieces each (2^-22), float16 ones exactly, and of bfloat16
-    ones the scores and the state are rounded to bfloat16 where they are multiplied
-    (not where they are kept).  A NaN or an infinity reaches what the recurrence takes
-    it to and nothing else (a sequence with one is passed over twice).
+    operands in two tf32 pieces each (2^-22); of bfloat16 ones the scores and the state
+    are rounded to bfloat16 where they are multiplied (not where they are kept), of
+    float16 ones to tf32's 11 bits; the operands themselves are exact.  A NaN or an
+    infinity reaches what the recurrence takes it to and nothing else; a sequence with
+    one takes three to four times as long, with many up to 20 times.
     """
     return torch_ops().decay_attention(q, k, v, decay, state, lengths, scale, return_state)

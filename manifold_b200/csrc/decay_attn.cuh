@@ -139,6 +139,15 @@ GFN_DEV void mma_pieces(float (&c)[4], const unsigned (&a)[PA][4], const unsigne
   if constexpr (PB > 1) mma_tf32(c, a[0], b[1]);
   mma_tf32(c, a[0], b[0]);
 }
+// c += a b with the products of a step summed by themselves first: the tensor
+// cores cut where float32 addition rounds, three times a step, and over an output's
+// steps that adds up (40 x 72 heads: error 1.3e-6, so 7.8e-7; 443 -> 453 us trained).
+GFN_DEV void mma_apart(float (&c)[4], const unsigned (&a)[2][4], const unsigned (&b)[2][2]) {
+  float d[4] = {};
+  mma_pieces(d, a, b);
+  split(f2(c[0], c[1]) + f2(d[0], d[1]), c[0], c[1]);
+  split(f2(c[2], c[3]) + f2(d[2], d[3]), c[2], c[3]);
+}
 template <typename T>
 GFN_DEV void mma(float (&c)[4], const typename Math<T>::A& a, const typename Math<T>::B& b) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>) mma_bf16(c, a.v, b.v);
@@ -548,8 +557,8 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
       typename M::B b[2];
       if (NMAJOR) load_bn<T, CARE>(b, st + col * LS + k, LS, lane);
       else load_bk<T, CARE>(b, st + k * LS + col, LS, lane);
-      mma<T>(o[i], a, b[0]);
-      mma<T>(o[i + 1], a, b[1]);
+      mma_apart(o[i], a.v, b[0].v);
+      mma_apart(o[i + 1], a.v, b[1].v);
     }
 #pragma unroll
     for (int i = 0; i < C / 16; ++i) {
@@ -611,8 +620,8 @@ GFN_DEV void attend_f32(float (&o)[ON][4], const T* rows, const T* keys, const T
         if (!FULL && col0 + n * 8 >= nd) continue;
         typename M::B b[2];
         load_bk<T, CARE>(b, v + n * 8, LDB, lane);
-        mma<T>(o[n], a, b[0]);
-        mma<T>(o[n + 1], a, b[1]);
+        mma_apart(o[n], a.v, b[0].v);
+        mma_apart(o[n + 1], a.v, b[1].v);
       }
     }
   }
