@@ -146,3 +146,32 @@ def test_the_largest_finite_values(L, K, V, dtype):
     k[3, 61, 0, 2], v[3, 61, 0] = high, v[3, 61, 0] * 2.0 ** -10
     do[4, 33, 1, 7] = high
     _check((q, k, v), (q, k, v), decay, st, None, 2.0 ** -8, do, dl, "largest")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_bad_values_in_a_replayed_graph(dtype):
+    """A captured training step meets a NaN and an infinity in one replay and none in the next."""
+    q, k, v, decay, _, do, _ = _case(2, 1500, 3, 64, 64, dtype)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def step(ts):
+        o = gfn.decay_attention(*ts, decay)
+        return (o, *torch.autograd.grad(o, ts, do))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step([t.detach().clone().requires_grad_(True) for t in leaves])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(leaves)
+    for bad in (False, True, False):
+        with torch.no_grad():
+            k[0, 700, 1, 3] = NAN if bad else 1.0
+            v[1, 10, 2, 5] = INF if bad else 1.0
+        graph.replay()
+        want = step([t.detach().clone().requires_grad_(True) for t in leaves])
+        for a, b in zip(outs, want):
+            assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+        assert torch.isfinite(outs[0]).all().item() != bad
