@@ -20,7 +20,7 @@ def decay_attention(q, k, v, decay, state=None, return_state=False, lengths=None
     (once) in q, k, v and state.
 
     The state is float32 throughout.  Products run on the tensor cores: float32
-    operands in two tf32 pieces each (2^-22); of bfloat16 ones the scores and the state
+    operands in two tf32 pieces each (2^-22 a product, results to 1e-6); of bfloat16 ones the scores and the state
     are rounded to bfloat16 where they are multiplied (not where they are kept), of
     float16 ones to tf32's 11 bits; the operands themselves are exact.  A NaN or an
     infinity reaches what the recurrence takes it to and nothing else; a sequence with

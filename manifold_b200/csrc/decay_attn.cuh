@@ -25,12 +25,14 @@
 //     bits at float32's range (a float16 P or S could overflow); g^.. k in two
 //     tf32 pieces.
 //   float32: every operand in two tf32 pieces, three products (2^-22).
+// The scores' powers of g come from ex2.approx (2^-22 relative, 0 below 2^-126),
+// which is below what the operands lose.
 //
 // Why mma.sync: scores are masked, g^.. applied and the result multiplied again
 // without leaving the registers, and so is k where it is split.  Through tensor
 // memory those steps would keep about 70% of today's issue slots.  1 x 65536 x 8
-// heads of 64 in bfloat16: outputs 84 us (tensor pipe 52%, issue 40%, 12 warps an
-// SM), segments' states 46 (57%, 36%), their join 6; the bytes would take 41.  What
+// heads of 64 in bfloat16: outputs 86 us (tensor pipe 50%, issue 39%, 12 warps an
+// SM), segments' states 46 (56%, 36%), their join 7; the bytes would take 41.  What
 // is left is latency between the steps of a block of tokens.  Larger tiles a warp
 // do better than more warps: 8 warps of half the columns took 108 us for the outputs.
 #pragma once
@@ -258,7 +260,8 @@ struct Shape {
   static constexpr int STATE_BYTES = DK * LS * (int)sizeof(typename Math<T>::State);
   static constexpr int stage(int kind) { return kind == STATE ? TK + TV : kind == OUTPUT ? 2 * TK + TV : 2 * TK + 2 * TV; }
   // thread blocks of an SM that registers allow (heads up to 32: four instead of
-  // three, 4 x 6000 x 4 heads of 32 trained in bfloat16 66 us of kernels to 62)
+  // three, 4 x 6000 x 4 heads of 32 trained in bfloat16 66 us of kernels to 62; 65 since
+  // segments end with a look for bad values)
   static constexpr int most(int kind) {
     return WIDE ? (DK + DV < 256 ? 2 : 1) : kind == STATE || DK == 32 ? 4 : kind == PAIR && sizeof(T) < 4 ? 2 : 3;
   }
@@ -833,7 +836,7 @@ GFN_DEV void emit(void* out, const float (&o)[ON][4], const PassArgs& p, int b, 
 // PAIR: with a = q, b = k, c = v, d = do, the outputs dv (rows b, keys a,
 // values d) and dk (rows c, keys d, values a) of the state's gradient.  dv and dk in
 // one launch share the operands and the state: 32 x 2048 x 8 heads of 64 in bfloat16
-// 149 us, where the outputs alone take 103 (256 thread blocks: two an SM, or one).
+// 145 us, where the outputs alone take 106 (256 thread blocks: two an SM, or one).
 // Returns whether the segment is to be walked again with CARE.
 template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL, bool CARE>
 GFN_DEV bool attn_walk(const PassArgs& p) {
@@ -1013,7 +1016,7 @@ GFN_DEV bool attn_walk(const PassArgs& p) {
 
 // Segments of finite tokens are walked once.  Others are walked again, by code of
 // its own, so that care (see add_up_to_diagonal, add_again) costs next to nothing on the way:
-// 32 x 2048 x 8 heads of 64 in bfloat16, trained, 351 us with and without it; asking
+// 32 x 2048 x 8 heads of 64 in bfloat16, trained, 353 us, and 351 without it; asking
 // in the walk which infinities the state came with took 397.
 template <typename T, int DK, int DV, bool BACK, int KIND, bool FULL>
 __device__ __noinline__ void attn_walk_again(const PassArgs& p) {
